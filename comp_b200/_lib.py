@@ -17,6 +17,24 @@ P = ctypes.c_void_p
 I64 = ctypes.c_int64
 INT = ctypes.c_int
 
+
+
+class KVCacheDesc(ctypes.Structure):
+    """b2q_kv_cache (include/comp_b200.h)."""
+
+    _fields_ = [("kq", P), ("ks", P), ("vq", P), ("vs", P), ("pages", I64), ("heads", ctypes.c_int32),
+                ("page", ctypes.c_int32), ("dim", ctypes.c_int32), ("fmt", ctypes.c_int32)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """b2q_attention_args (include/comp_b200.h)."""
+
+    _fields_ = [*[(n, P) for n in ("q", "out", "lse", "table", "lens", "cu_q", "prefix", "starts", "slopes")],
+                *[(n, I64) for n in ("q_st", "q_sh", "T", "batch", "table_stride", "table_pages", "max_q", "max_len")],
+                *[(n, ctypes.c_int32) for n in ("q_heads", "dtype", "window")],
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/comp_b200.h declares
 SIGNATURES = {
     "b2q_version": (ctypes.c_char_p, []),
@@ -41,6 +59,10 @@ SIGNATURES = {
     "b2q_quant_gemv_ws": (INT, [INT, P, I64, P, P, I64, P, P, P, I64, I64, I64, P, ctypes.c_size_t, P]),
     "b2q_gemv_allgather": (INT, [INT, P, I64, P, P, I64, P, P, P, I64, P, P, I64, I64, I64, I64, I64, INT, INT,
                                  ctypes.c_longlong, P]),
+    "b2q_kv_write": (INT, [P, INT, P, I64, I64, P, I64, I64, P, I64, P]),
+    "b2q_kv_read": (INT, [P, INT, P, P, P, I64, P]),
+    "b2q_attention_workspace_size": (ctypes.c_size_t, [P, P]),
+    "b2q_attention": (INT, [P, P, P, ctypes.c_size_t, P]),
     "b2q_set_tuning": (INT, [INT, INT, INT]),
     "b2q_set_pipeline": (INT, [INT, INT]),
     "b2q_set_warps": (INT, [INT]),

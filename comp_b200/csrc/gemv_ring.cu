@@ -1,5 +1,6 @@
 // Instantiations of the TMA-ring GEMV kernels (see gemv_kernels.cuh), and the device error word they write.
 #include "gemv_kernels.cuh"
+#include "kv_internal.h"
 
 namespace b2q {
 
@@ -57,6 +58,13 @@ extern "C" int b2q_device_error(int* code, int clear) {
     const int zero = 0;
     e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_device_error: %s", cudaGetErrorString(e));
+  }
+  // the words of the KV cache's and the attention's translation units; the first that is set is reported
+  for (auto read : {kv_cache_error, kv_attention_q4_error, kv_attention_q8_error}) {
+    int word = 0;
+    const int rc = read(&word, clear);
+    if (rc) return rc;
+    if (!*code) *code = word;
   }
   return B2Q_OK;
 }

@@ -1,0 +1,42 @@
+// Host-side internals shared by the KV cache and attention translation units: argument checks, the parameter block of
+// the attention kernels and the launchers that the dispatcher picks from.
+#pragma once
+
+#include "b2q_internal.h"
+
+namespace b2q {
+
+constexpr int kErrSlot = 2;  // device error word: a slot beyond the cache
+constexpr int kErrPage = 3;  // device error word: a token whose page is outside the table or the cache
+
+inline int kv_row_bytes(const b2q_kv_cache& c) { return c.fmt == B2Q_FMT_Q4_0 ? c.dim / 2 : c.dim; }
+inline int dtype_size(int dtype) { return dtype == B2Q_DTYPE_F32 ? 4 : 2; }
+
+// The checks of a cache descriptor that every entry point makes (kv_cache.cu).
+int check_kv_cache(const char* who, const b2q_kv_cache* c);
+
+struct AttnParams {
+  const void* q;
+  void* out;
+  float* lse;
+  const uint8_t *kq, *vq;
+  const uint16_t *ks, *vs;
+  const int32_t *table, *lens, *cu_q, *prefix, *starts;
+  const float* slopes;
+  float* part_o;   // [T * q_heads][splits][dim] partial outputs (not divided), when the keys are split
+  float2* part_m;  // [T * q_heads][splits] their reference exponent and sum
+  int64_t q_st, q_sh, T, table_stride, pages;
+  int table_pages, batch, q_heads, heads, group, page_shift, splits, row_tiles, window, dtype;
+  float scale, softcap;
+};
+
+// A device error word lives in each translation unit whose kernels set one; b2q_device_error reads them all.
+int kv_cache_error(int* code, int clear);
+int kv_attention_q4_error(int* code, int clear);
+int kv_attention_q8_error(int* code, int clear);
+
+// Decode kernels by format: `rows` is 8 or 16 query rows a tile.
+int launch_attention_q4(const AttnParams& p, int dim, int rows, cudaStream_t stream);
+int launch_attention_q8(const AttnParams& p, int dim, int rows, cudaStream_t stream);
+
+}  // namespace b2q

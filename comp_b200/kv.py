@@ -1,0 +1,216 @@
+"""Quantized KV cache and the attention that reads it (an extension beyond the reference, which has no attention).
+
+A `KVCache` holds paged keys and values as ggml blocks (q4_0: 4.5 bits a value, q8_0: 8.5 bits). `kv_write` quantizes
+tokens into it, `kv_read` gives back the values that it stands for, and `attention` runs queries against it: single
+tokens (decode), a few tokens a sequence (drafts) or prompt chunks, with capped scores, a bias by distance, sliding
+windows, prefix and document masks. The kernels are this package's own, through the C-ABI (include/comp_b200.h, where
+the layouts and formulas stand); like comp_b200.host the functions take CUDA tensors only, run on the current stream of
+their device, and raise TypeError / ValueError / RuntimeError on what they do not take.
+
+    cache = kv.KVCache("q4_0", pages=4096, page_size=64, heads=8, head_dim=128)
+    kv.kv_write(cache, k, v, slots)                     # k, v [T][8][128]; slots int64 [T] = page * page_size + offset
+    out = kv.attention(q, cache, table, lens)           # q [B][32][128]; table int32 [B][pages]; lens int32 [B]
+"""
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .host import FMT_ID, _need_cuda, _on, _stream
+
+FORMATS = ("q4_0", "q8_0")
+HEAD_DIMS = (64, 96, 128, 256)
+BLOCK_BYTES = {"q4_0": 16, "q8_0": 32}
+DTYPE_ID = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _fmt(fmt):
+    if fmt not in FORMATS:
+        raise ValueError(f"unknown cache format {fmt!r}: expected one of {FORMATS}")
+    return fmt
+
+
+class KVCache:
+    """Planes of a paged cache: quants uint8 [pages][heads][page_size][row bytes] and scales int16 (f16 bits)
+    [pages][heads][page_size][head_dim / 32], for keys (kq, ks) and values (vq, vs)."""
+
+    def __init__(self, fmt, pages, page_size, heads, head_dim, device="cuda"):
+        _fmt(fmt)
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"KVCache: head_dim {head_dim} not in {HEAD_DIMS}")
+        nb = head_dim // 32
+        shape = (pages, heads, page_size)
+        planes = [torch.zeros((*shape, n), dtype=dt, device=device) for _ in "kv"
+                  for n, dt in ((nb * BLOCK_BYTES[fmt], torch.uint8), (nb, torch.int16))]
+        self._set(fmt, *planes)
+
+    @classmethod
+    def from_planes(cls, fmt, kq, ks, vq, vs):
+        """A cache on planes that the caller owns (contiguous, 16-byte aligned)."""
+        self = cls.__new__(cls)
+        self._set(_fmt(fmt), kq, ks, vq, vs)
+        return self
+
+    def _set(self, fmt, kq, ks, vq, vs):
+        dev = _need_cuda("KVCache", kq, ks, vq, vs)
+        if ks.dim() != 4:
+            raise ValueError(f"KVCache: scales must be [pages][heads][page_size][head_dim/32], got {tuple(ks.shape)}")
+        nb = ks.shape[3]
+        for t, name, dtype, last in ((kq, "kq", torch.uint8, nb * BLOCK_BYTES[fmt]), (ks, "ks", torch.int16, nb),
+                                     (vq, "vq", torch.uint8, nb * BLOCK_BYTES[fmt]), (vs, "vs", torch.int16, nb)):
+            if t.dtype != dtype:
+                raise TypeError(f"KVCache: {name}: dtype {t.dtype}, expected {dtype}")
+            if tuple(t.shape) != (*ks.shape[:3], last):
+                raise ValueError(f"KVCache: {name}: shape {tuple(t.shape)}, expected {(*ks.shape[:3], last)}")
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"KVCache: {name} must be contiguous and 16-byte aligned")
+        pages, heads, page = ks.shape[:3]
+        if nb * 32 not in HEAD_DIMS:
+            raise ValueError(f"KVCache: head_dim {nb * 32} not in {HEAD_DIMS}")
+        if page < 16 or page > 65536 or page & (page - 1):
+            raise ValueError(f"KVCache: page_size {page} is not a power of two from 16 to 65536")
+        if heads < 1 or heads > 4096:
+            raise ValueError(f"KVCache: {heads} heads (1..4096)")
+        self.fmt, self.kq, self.ks, self.vq, self.vs = fmt, kq, ks, vq, vs
+        self.pages, self.heads, self.page_size, self.head_dim, self.device = pages, heads, page, nb * 32, dev
+        self._desc = _lib.KVCacheDesc(kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr(), pages, heads, page,
+                                      nb * 32, FMT_ID[fmt])
+        self._ref = ctypes.addressof(self._desc)
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.kq, self.ks, self.vq, self.vs))
+
+
+def _dtype_id(name, t):
+    if t.dtype not in DTYPE_ID:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected float32, float16 or bfloat16")
+    return DTYPE_ID[t.dtype]
+
+
+def _slots(name, cache, slots):
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise TypeError(f"{name}: slots must be a 1-D int64 tensor, got {slots.dtype} {tuple(slots.shape)}")
+    return slots if slots.is_contiguous() else slots.contiguous()
+
+
+def _heads_aligned(t):
+    """t with a contiguous last axis, a 16-byte aligned base and strides of whole 16 bytes (a copy only when needed)."""
+    size = t.element_size()
+    if t.stride(2) != 1 or t.data_ptr() % 16 or t.stride(0) * size % 16 or t.stride(1) * size % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def kv_write(cache, k, v, slots):
+    """Quantizes k and v [T][heads][head_dim] (f32, f16 or bf16; any token and head strides) into the slots int64 [T] of
+    the cache (page * page_size + offset). Negative slots are skipped (padding tokens). The blocks are ggml's, bit for
+    bit (quantize_row_q4_0 / q8_0 of the value widened to f32); a 16-bit caller needs no cast."""
+    dev = _need_cuda("kv_write", cache.kq, k, v, slots)
+    shape = (slots.shape[0], cache.heads, cache.head_dim)
+    did = _dtype_id("kv_write: k", k)
+    if v.dtype != k.dtype:
+        raise TypeError(f"kv_write: k is {k.dtype}, v is {v.dtype}")
+    if k.shape != shape or v.shape != shape:
+        raise ValueError(f"kv_write: k {tuple(k.shape)} and v {tuple(v.shape)}, expected {shape}")
+    slots = _slots("kv_write", cache, slots)
+    k, v = _heads_aligned(k), _heads_aligned(v)
+    ks, vs = k.stride(), v.stride()
+    with _on(dev):
+        _lib.call("b2q_kv_write", cache._ref, did, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                  slots.data_ptr(), shape[0], _stream(dev))
+
+
+def kv_read(cache, slots, dtype=torch.float32):
+    """-> (k, v) [T][heads][head_dim] of `dtype`: the values that the slots int64 [T] hold (f16 scale times quant, rounded
+    once). Negative slots give zeros."""
+    dev = _need_cuda("kv_read", cache.kq, slots)
+    if dtype not in DTYPE_ID:
+        raise TypeError(f"kv_read: dtype {dtype}, expected float32, float16 or bfloat16")
+    slots = _slots("kv_read", cache, slots)
+    shape = (slots.shape[0], cache.heads, cache.head_dim)
+    k = torch.empty(shape, dtype=dtype, device=dev)
+    v = torch.empty(shape, dtype=dtype, device=dev)
+    with _on(dev):
+        _lib.call("b2q_kv_read", cache._ref, DTYPE_ID[dtype], k.data_ptr(), v.data_ptr(), slots.data_ptr(), shape[0],
+                  _stream(dev))
+    return k, v
+
+
+def _index(t, name, shape, dev, dtype=torch.int32):
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"attention: {name}: dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"attention: {name}: shape {tuple(t.shape)}, expected {shape}")
+    if t.device != dev:
+        raise RuntimeError(f"comp_b200.attention: {name} must be on {dev}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_len=None, softcap=0.0, window=0,
+              slopes=None, prefix=None, starts=None, out=None, return_lse=False, workspace=None):
+    """Attention of query tokens q [T][q_heads][head_dim] (f32, f16 or bf16) over the cache -> out of the same shape and
+    type (and lse f32 [T][q_heads] when return_lse).
+
+    table: int32 [B][P], the pages of each sequence; lens: int32 [B], its tokens in the cache, the query tokens' own
+    among them. cu_q: int32 [B + 1], where each sequence's query tokens begin in q (default: one token each, T == B); the
+    last one is at position lens - 1. q head h reads KV head h // (q_heads // heads). scale: default head_dim ** -0.5.
+
+    softcap > 0: scores s -> softcap * tanh(s / softcap); slopes f32 [q_heads]: minus slopes[h] times the distance of
+    query and key. A query at p sees the keys max(starts, p - window + 1) <= j < min(lens, max(p + 1, prefix)): window
+    (0: none) slides, prefix int32 [B] keys are seen by every query, starts int32 [T] is the first key of a query's
+    document. A query that sees no key gives zeros (lse -inf).
+
+    max_q / max_len: the most query tokens of a sequence and the longest length, where the caller knows them (default:
+    T, or 1 without cu_q, and what the table can hold): max_q must not be less than what cu_q has, max_len only plans
+    the work. workspace: a CUDA byte tensor of attention_workspace_size(...) bytes (allocated here when None). out: a
+    contiguous tensor for the result."""
+    dev = _need_cuda("attention", q, cache.kq, table, lens)
+    did = _dtype_id("attention: q", q)
+    if q.dim() != 3 or q.shape[2] != cache.head_dim:
+        raise ValueError(f"attention: q {tuple(q.shape)}, expected [T][q_heads][{cache.head_dim}]")
+    T, heads, dim = q.shape
+    if heads == 0 or heads % cache.heads:
+        raise ValueError(f"attention: {heads} query heads over {cache.heads} KV heads")
+    if table.dtype != torch.int32 or table.dim() != 2:
+        raise TypeError(f"attention: table must be a 2-D int32 tensor, got {table.dtype} {tuple(table.shape)}")
+    B, P = table.shape
+    if P and table.stride(1) != 1:
+        table = table.contiguous()
+    lens = _index(lens, "lens", (B,), dev)
+    if cu_q is None:
+        if T != B:
+            raise ValueError(f"attention: {T} query tokens for {B} sequences need cu_q")
+        max_q = 1
+    else:
+        cu_q = _index(cu_q, "cu_q", (B + 1,), dev)
+        max_q = T if max_q is None else max_q
+    prefix = _index(prefix, "prefix", (B,), dev)
+    starts = _index(starts, "starts", (T,), dev)
+    slopes = _index(slopes, "slopes", (heads,), dev, torch.float32)
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((T, heads, dim), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"attention: out must be a contiguous {q.dtype} {tuple(q.shape)} tensor on {dev}")
+    lse = torch.empty((T, heads), dtype=torch.float32, device=dev) if return_lse else None
+    args = _lib.AttentionArgs(q.data_ptr(), out.data_ptr(), _ptr(lse), table.data_ptr(), lens.data_ptr(), _ptr(cu_q),
+                              _ptr(prefix), _ptr(starts), _ptr(slopes), q.stride(0), q.stride(1), T, B,
+                              table.stride(0) if P else 0, P, max_q, P * cache.page_size if max_len is None else max_len,
+                              heads, did, window, dim**-0.5 if scale is None else scale, softcap)
+    ref = ctypes.addressof(args)
+    with _on(dev):
+        need = _lib.load().b2q_attention_workspace_size(cache._ref, ref)
+        if need and workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.call("b2q_attention", cache._ref, ref, workspace.data_ptr() if need else None,
+                  workspace.numel() * workspace.element_size() if need else 0, _stream(dev))
+    return (out, lse) if return_lse else out

@@ -275,6 +275,93 @@ int b2q_gemv_allgather(int fmt, const uint8_t* wq, int64_t ldwq, const int16_t* 
                        int32_t* status, int64_t row0, int64_t n_local, int64_t N_total, int64_t K, int64_t M,
                        int rank, int nranks, long long spin_limit, b2q_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Quantized KV cache (extension: COMP has no counterpart): paged planes of ggml blocks, written from and read back to
+ * f32 / f16 / bf16 values, and the attention that reads them.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+#define B2Q_DTYPE_F32 0
+#define B2Q_DTYPE_F16 1
+#define B2Q_DTYPE_BF16 2
+
+/*
+ * A paged cache of keys and values: per plane quants u8 [pages][heads][page][row] and scales [pages][heads][page]
+ * [dim/32] (f16 bits), one f16 scale per 32 values. fmt B2Q_FMT_Q4_0 (row = dim/2, value = d * (nibble - 8)) or
+ * B2Q_FMT_Q8_0 (row = dim, value = d * (byte - 128): ggml's int8 plus 128). A row holds the quant bytes of ggml's
+ * blocks, seen as [dim/32 blocks][U][unit bytes] and stored as [U][dim/32][unit]: U = 4 for keys, 8 for values (unit
+ * j of a block then lies next to unit j of the row's other blocks, which is what one lane of the attention's matrix
+ * instructions needs from a row). dim 64, 96, 128 or 256; page a power of two from 16 to 65536; planes 16-byte aligned.
+ * A slot is page * `page` + offset.
+ */
+typedef struct {
+  uint8_t* kq;
+  int16_t* ks;
+  uint8_t* vq;
+  int16_t* vs;
+  int64_t pages;
+  int32_t heads, page, dim, fmt;
+} b2q_kv_cache;
+
+/*
+ * Quantizes keys and values [T][heads][dim] (dtype B2Q_DTYPE_*, element strides k_st / v_st per token and k_sh / v_sh
+ * per head, the last axis contiguous) into the slots int64 [T] of the cache. Negative slots are skipped; a slot beyond
+ * the cache is skipped and sets the device error word to 2 (b2q_device_error); if a slot is given twice, which token
+ * stays is not defined. Blocks are ggml's, bit for bit, in f32 steps from the value widened to f32:
+ *   q4_0: m = the value of largest magnitude (first on ties), d = m / -8, q = min(15, trunc(x * (1/d) + 8.5));
+ *   q8_0: d = max|x| / 127, q = roundf(x * (1/d)); the scale kept is f16(d); d == 0 gives 1/d = 0.
+ * k and v must be aligned to 8 elements' width (16 bytes; strides a multiple of that). Asynchronous on `stream`.
+ */
+int b2q_kv_write(const b2q_kv_cache* cache, int dtype, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                 int64_t v_st, int64_t v_sh, const int64_t* slots, int64_t T, b2q_stream_t stream);
+
+/*
+ * The values of the slots int64 [T], as dtype, into k and v [T][heads][dim] (contiguous, 16-byte aligned; either may be
+ * NULL): one f32 product f16 scale * quant, rounded once. A negative slot gives zeros, and so does one beyond the cache
+ * (which sets the device error word to 2). Asynchronous on `stream`.
+ */
+int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const int64_t* slots, int64_t T,
+                b2q_stream_t stream);
+
+/*
+ * Attention of query tokens over the cache. Sequence b owns the cache tokens 0 .. lens[b]-1, token j in page
+ * table[b * table_stride + j / page]; its queries are the tokens cu_q[b] .. cu_q[b+1]-1 of q (cu_q NULL: one each, T ==
+ * batch), the last of its n queries at position lens[b]-1: query i is at p = lens[b] - n + i. Head h reads KV head
+ * h / (q_heads / heads). For every query and head
+ *   s_j = scale * q.k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);  slopes: s_j -= slopes[h] * |p - j|
+ *   over the visible keys  max(starts[t], window ? p - window + 1 : 0) <= j < min(lens[b], max(p + 1, prefix[b])),
+ *   out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j).
+ * A row that sees no key gives out = 0 and lse = -inf. starts (per query token: the first key of its document) and
+ * prefix (per sequence: keys that every query sees) are int32, slopes f32 [q_heads]; each may be NULL. scale > 0.
+ * Scores, softmax sums and outputs are held in f32.
+ * max_q: at least the most queries of a sequence (0: max_q = T); max_len: at least the longest lens, used to plan the
+ * split of the keys only. Tokens beyond the table or in pages outside the cache read as masked, and set the device
+ * error word to 3. out [T][q_heads][dim] contiguous, of q's dtype; lse f32 [T][q_heads] or NULL. Rows of q beyond
+ * cu_q[batch] are left unwritten. q: element strides per token and head, last axis contiguous, any alignment.
+ */
+typedef struct {
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu_q;
+  const int32_t* prefix;
+  const int32_t* starts;
+  const float* slopes;
+  int64_t q_st, q_sh;
+  int64_t T, batch, table_stride, table_pages, max_q, max_len;
+  int32_t q_heads, dtype, window;
+  float scale, softcap;
+} b2q_attention_args;
+
+/* Device workspace bytes b2q_attention needs for these arguments (partial results of split keys; 0: none). */
+size_t b2q_attention_workspace_size(const b2q_kv_cache* cache, const b2q_attention_args* args);
+
+/* Runs it. workspace: device memory, 16-byte aligned, of at least that many bytes; calls that may overlap on the GPU
+ * need a workspace each. Asynchronous on `stream`. */
+int b2q_attention(const b2q_kv_cache* cache, const b2q_attention_args* args, void* workspace, size_t workspace_bytes,
+                  b2q_stream_t stream);
+
 /* Benchmark/tuning hook (process-wide): force rows per group (1, 2, 4), chunks per thread and grid size of the
  * GEMV schedule; 0 restores the planner's choice. Results do not depend on it (except the f32 summation order). */
 int b2q_set_tuning(int rows_per_group, int chunks_per_thread, int grid);
@@ -312,8 +399,9 @@ int b2q_set_gemm_schedule(int schedule);
 int b2q_set_cluster(int ctas);
 
 
-/* Reads (and with clear != 0 resets) the library's device error word: nonzero if a kernel's bounded wait on an
- * mbarrier gave up (the kernel then returned early; its outputs are invalid). Synchronizes with the device. */
+/* Reads (and with clear != 0 resets) the library's device error word: 1 if a kernel's bounded wait on an mbarrier gave
+ * up (the kernel then returned early; its outputs are invalid), 2 if a KV cache slot was beyond its cache, 3 if an
+ * attention call met a token without a valid page. Synchronizes with the device. */
 int b2q_device_error(int* code, int clear);
 
 /* CUDA IPC helpers for the multi-GPU path. b2q_ipc_get_handle exports the allocation containing dev_ptr as a 64-byte
