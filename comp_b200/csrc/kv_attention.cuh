@@ -16,9 +16,10 @@
 // A weight matrix leaves the first product with keys along the lanes' rows and enters the second with keys along their
 // pairs: one 8x8 transpose in registers each.
 //
-// What bounds it: the cache's bytes. Every warp is on its own: it owns every W-th stage of 32 or 64 keys of its CTA's
-// share, copied by its own ring of bulk copies (at most 64 keys: four contiguous pieces a page), and joins the others
-// once at the end through shared memory. With few rows the keys are split over CTAs, and a second kernel joins those.
+// What bounds it: the cache's bytes. Every warp is on its own: it owns every W-th stage of 16 to 64 keys of its CTA's
+// share, copied by its own ring of bulk copies (contiguous pieces of a page), and joins the others
+// once at the end of a tile through shared memory. The CTAs fill the GPU once and take equal shares of all stages of
+// all sequences, heads and row tiles, whatever their lengths; tiles that cross shares are joined by a second kernel.
 #pragma once
 
 #include <climits>
@@ -36,50 +37,56 @@ constexpr float kNoRef = -1e30f;  // reference exponent of a row that has seen n
 
 template <int FMT, int NB>
 struct KvTile {
-  static constexpr int kRow = NB * (FMT == 0 ? 16 : 32);           // quant bytes of a token's row
-  static constexpr int kTokens = kRow * 64 * 2 > 10240 ? 32 : 64;  // tokens a stage
+  static constexpr int kRow = NB * (FMT == 0 ? 16 : 32);  // quant bytes of a token's row
+  // tokens a stage: at most 9216 bytes, so that 12 warps with two stages each fill an SM
+  static constexpr int kTokens = kRow <= 32 ? 128 : (kRow <= 64 ? 64 : (kRow <= 128 ? 32 : 16));
   static constexpr int kQuants = kTokens * kRow, kScales = kTokens * NB * 2;
   static constexpr int kStage = 2 * (kQuants + kScales);
   static constexpr int kWarps = 4;
-  // ring stages a warp: at most 111 KB a CTA, two CTAs an SM (one for q8_0 rows of 256)
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 2;
   static constexpr int kRing = kStage * kStages * kWarps;
 };
+
+// CTAs an SM: as many as their registers and rings leave room for.
+template <int FMT, int NB, int NT, int PARTS>
+constexpr int kv_ctas_per_sm() {
+  return NB == 8 || NT == 2 || PARTS == 2 ? 2 : 3;
+}
 
 // Row r of a 16-token tile is this token: chosen so that both the key loads (lanes of two rows side by side) and the
 // value loads (lanes of four tokens side by side) spread over the shared-memory banks.
 __device__ __forceinline__ int tile_token(int r) { return (r & 1) ? ((r >> 1) ^ 1) + 4 : (r >> 1); }
 
-// NB consecutive 32-bit words.
-template <int NB>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[NB]) {
-  if constexpr (NB % 4 == 0) {
+// N consecutive 32-bit words of shared memory.
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < NB; i += 4) {
-      const uint4 v = lds_v4(addr + 4 * i);
+    for (int i = 0; i < N; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(at + 4 * i);
       w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
     }
-  } else if constexpr (NB % 2 == 0) {
+  } else if constexpr (N % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < NB; i += 2) {
-      const uint2 v = lds_v2(addr + 4 * i);
+    for (int i = 0; i < N; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(at + 4 * i);
       w[i] = v.x, w[i + 1] = v.y;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) w[i] = lds_u32(addr + 4 * i);
+    for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint32_t*>(at + 4 * i);
   }
 }
 
-// NB consecutive 16-bit words, two to a register (the last register's high half is unused when NB is odd).
-template <int NB>
-__device__ __forceinline__ void lds_halves(uint32_t addr, uint32_t (&w)[(NB + 1) / 2]) {
-  if constexpr (NB % 2 == 0) {
-    lds_words<NB / 2>(addr, w);
+// N consecutive 16-bit words, two to a register (the last register's high half is unused when N is odd).
+template <int N>
+__device__ __forceinline__ void lds_halves(const uint8_t* at, uint32_t (&w)[(N + 1) / 2]) {
+  if constexpr (N % 2 == 0) {
+    lds_words<N / 2>(at, w);
   } else {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const uint32_t h = lds_u16(addr + 2 * i);
+    for (int i = 0; i < N; ++i) {
+      const uint32_t h = *reinterpret_cast<const uint16_t*>(at + 2 * i);
       w[i / 2] = (i & 1) ? (w[i / 2] | h << 16) : h;
     }
   }
@@ -87,18 +94,34 @@ __device__ __forceinline__ void lds_halves(uint32_t addr, uint32_t (&w)[(NB + 1)
 
 // The NB f16 scales of a token.
 template <int NB>
-__device__ __forceinline__ void lds_scales(uint32_t addr, float (&d)[NB]) {
+__device__ __forceinline__ void lds_scales(const uint8_t* at, float (&d)[NB]) {
   uint32_t w[(NB + 1) / 2];
-  lds_halves<NB>(addr, w);
+  lds_halves<NB>(at, w);
 #pragma unroll
-  for (int b = 0; b < NB; ++b) d[b] = f16_bits_to_f32((uint16_t)(w[b / 2] >> (16 * (b & 1))));
+  for (int b = 0; b < NB; ++b) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w[b / 2]);
+    d[b] = (b & 1) ? __high2float(h) : __low2float(h);
+  }
 }
 
-__device__ __forceinline__ float load_elt(const void* p, int64_t i, int dtype) {
-  if (dtype == B2Q_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == B2Q_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// 4 values at p (of type dtype, p counted in elements), 4-element aligned.
+__device__ __forceinline__ void load4_as(const void* p, int64_t i, int dtype, float (&v)[4]) {
+  if (dtype == B2Q_DTYPE_F32)
+    load4(static_cast<const float*>(p) + i, v);
+  else if (dtype == B2Q_DTYPE_F16)
+    load4(static_cast<const __half*>(p) + i, v);
+  else
+    load4(static_cast<const __nv_bfloat16*>(p) + i, v);
 }
+__device__ __forceinline__ void store4_as(void* p, int64_t i, int dtype, float a, float b, float c, float d) {
+  if (dtype == B2Q_DTYPE_F32)
+    store4(static_cast<float*>(p) + i, a, b, c, d);
+  else if (dtype == B2Q_DTYPE_F16)
+    store4(static_cast<__half*>(p) + i, a, b, c, d);
+  else
+    store4(static_cast<__nv_bfloat16*>(p) + i, a, b, c, d);
+}
+
 __device__ __forceinline__ void store_elt(void* p, int64_t i, int dtype, float v) {
   if (dtype == B2Q_DTYPE_F32)
     static_cast<float*>(p)[i] = v;
@@ -116,520 +139,761 @@ __device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
   return copysignf(cap * (z < 0.25f ? poly : far), x);
 }
 
-// The query token and head of row r of sequence b's rows for KV head h, and its visible keys.
-struct QueryRow {
-  int64_t token;
-  int head, pos, lo, hi;
+// Position and visible keys [lo, hi) of query i of sequence b.
+struct QuerySpan {
+  int pos, lo, hi;
 };
-__device__ __forceinline__ QueryRow query_row(const AttnParams& p, int b, int h, int r, int64_t q0, int n, int len) {
-  QueryRow s;
-  const int i = r / p.group;
-  s.head = h * p.group + (r - i * p.group);
-  s.token = q0 + i;
+__device__ __forceinline__ QuerySpan query_span(const AttnParams& p, int b, int i, int64_t q0, int n, int len) {
+  QuerySpan s;
   s.pos = len - n + i;
   s.hi = s.pos + 1;
   if (p.prefix) s.hi = max(s.hi, p.prefix[b]);
   s.hi = max(0, min(s.hi, len));
-  s.lo = p.starts ? max(0, p.starts[s.token]) : 0;
+  s.lo = p.starts ? max(0, p.starts[q0 + i]) : 0;
   if (p.window > 0) s.lo = max(s.lo, s.pos - p.window + 1);
   return s;
 }
 
+// Sequence b's query tokens (held within q whatever cu_q says) and length (within its table).
+struct Sequence {
+  int64_t q0;
+  int n, len;
+};
+__device__ __forceinline__ Sequence sequence(const AttnParams& p, int b) {
+  Sequence s = {b, 1, 0};
+  if (p.cu_q) {
+    s.q0 = max((int64_t)0, min((int64_t)p.cu_q[b], p.T));
+    s.n = (int)(min((int64_t)p.cu_q[b + 1], p.T) - s.q0);
+  }
+  s.len = max(0, min(p.lens[b], p.table_pages << p.page_shift));
+  return s;
+}
+
+// What beginning a tile costs a CTA, in stages of its share (measured: 6 us against 0.8 us a stage): without it, a share
+// of many short tiles takes far longer than one long run (decode of 64 sequences of 100 to 8192 tokens).
+constexpr int kTileCost = 8;
+
+// The stages that hold the visible keys of row tile rt of sequence b: `count` is 0 for a tile without rows and at least 1
+// for any other, so that a tile that sees nothing is somebody's work too.
+struct Span {
+  int first, count;
+};
+template <int STG, int R>
+__device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
+  const Sequence q = sequence(p, b);
+  if (rt * R >= q.n * p.group) return {0, 0};
+  int i0 = 0, i1 = 0;
+  if (p.cu_q) i0 = rt * R / p.group, i1 = min(q.n - 1, (rt * R + R - 1) / p.group);
+  int lo = INT_MAX, hi = 0;
+  if (!p.starts) {  // both ends grow with the position
+    lo = query_span(p, b, i0, q.q0, q.n, q.len).lo, hi = query_span(p, b, i1, q.q0, q.n, q.len).hi;
+  } else {
+    for (int i = i0; i <= i1; ++i) {
+      const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
+      if (s.lo < s.hi) lo = min(lo, s.lo), hi = max(hi, s.hi);
+    }
+  }
+  if (lo >= hi) return {0, 1};
+  return {lo / STG, (hi + STG - 1) / STG - lo / STG};
+}
+
+__device__ __forceinline__ int tile_units(Span s) { return s.count ? s.count + kTileCost : 0; }
+
 // FMT 0 (q4_0) or 2 (q8_0), NB blocks a head, NT tiles of 8 query rows, PARTS f16 parts of queries and weights.
 template <int FMT, int NB, int NT, int PARTS>
-__global__ void __launch_bounds__(128) attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) attention_kernel(const AttnParams p) {
   using C = KvTile<FMT, NB>;
-  constexpr int D = NB * 32, W = C::kWarps, STG = C::kTokens, SUB = STG / 16, R = NT * 8;
+  constexpr int D = NB * 32, W = C::kWarps, S = C::kStages, STG = C::kTokens, SUB = STG / 16, R = NT * 8;
+  constexpr bool SIGNED = PARTS == 2;  // quants enter the products with their offset taken off
   constexpr float kOff = FMT == 0 ? 8.f : 128.f;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t bars[W * C::kStages];
-  __shared__ int s_lo[R], s_hi[R], s_pos[R];
-  __shared__ float s_slope[R];
+  // the start values of a block's sum as a whole accumulator (4 registers a block and row tile) where registers allow,
+  // else added after the product
+  constexpr bool QUAD = NB * NT <= 4;
+  constexpr int UN = SUB % 2 == 0 && NB * NT <= 4 && PARTS == 1 ? 2 : 1;
+  extern __shared__ __align__(128) uint8_t smem[];  // [stage][warp] ring; the last stage holds the queries at first
+  __shared__ uint64_t bars[W * S];
+  __shared__ int s_lo[R], s_hi[R], s_pos[R], s_out[R], s_top[R], s_entry, s_head, s_skip;
+  __shared__ float s_slope[R], s_rowf[R];
+  __shared__ int64_t s_scan[W];
+  __shared__ uint32_t s_off[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  int task = blockIdx.x;
-  const int split = task % p.splits;
-  task /= p.splits;
-  const int rt = task % p.row_tiles;
-  task /= p.row_tiles;
-  const int h = task % p.heads, b = task / p.heads;
-
-  const uint32_t my_bars = smem_addr(&bars[warp * C::kStages]);
-  const uint32_t ring = smem_addr(smem) + warp * C::kStages * C::kStage;
+  const uint32_t my_bars = smem_addr(&bars[warp * S]);
+  const uint32_t ring = smem_addr(smem) + warp * C::kStage;
   if (lane == 0) {
-    for (int s = 0; s < C::kStages; ++s) mbar_init(my_bars + 8 * s, 1);
+    for (int s = 0; s < S; ++s) mbar_init(my_bars + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x < 8) s_off[threadIdx.x] = threadIdx.x < 4 ? 0x80088008u : 0x80808080u;
   pdl_wait_then_trigger();
 
-  // the sequence's query tokens, held within q whatever cu_q says
-  const int64_t q0 = p.cu_q ? max((int64_t)0, min((int64_t)p.cu_q[b], p.T)) : b;
-  const int n = p.cu_q ? (int)(min((int64_t)p.cu_q[b + 1], p.T) - q0) : 1;
-  const int rows = n * p.group - rt * R;  // rows from this tile on
-  if (rows <= 0) return;
-  const int len = max(0, min(p.lens[b], p.table_pages << p.page_shift));
-  if (p.lens[b] > len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
-
-  // visible keys of the tile's rows: their union is read, their intersection needs no mask
-  if (threadIdx.x < R) {
-    const int r = threadIdx.x;
-    const bool there = r < rows;
-    const QueryRow s = query_row(p, b, h, rt * R + (there ? r : 0), q0, n, len);
-    s_lo[r] = s.lo;
-    s_hi[r] = there ? s.hi : 0;
-    s_pos[r] = s.pos;
-    s_slope[r] = p.slopes ? p.slopes[s.head] * kLog2e : 0.f;
+  // ---------------------------------------------------------------- the plan: every CTA an equal share of all stages
+  // entries (sequence, row tile) have their stages, after kTileCost units without any, once a KV head; a CTA's share is
+  // [pos, end) of their run
+  const int entries = p.batch * p.row_tiles;
+  int64_t per, pos, end;
+  {
+    const int chunk = (entries + 127) / 128, e0 = min(entries, (int)threadIdx.x * chunk), e1 = min(entries, e0 + chunk);
+    int64_t mine = 0;
+    for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
+    mine *= p.heads;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) s_scan[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < warp) upto += s_scan[w];
+      total += s_scan[w];
+    }
+    // a share is at least a stage for each warp
+    if (total < (int64_t)1 << 31)
+      per = max((int)((uint32_t)(total + gridDim.x - 1) / gridDim.x), W);
+    else
+      per = (total + gridDim.x - 1) / gridDim.x;
+    pos = per * blockIdx.x;
+    end = min(total, pos + per);
+    if (pos >= end) {
+      if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
+      return;
+    }
+    if (pos >= upto - mine && pos < upto) {
+      int64_t off = pos - (upto - mine);
+      for (int e = e0; e < e1; ++e) {
+        const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
+        if (off < (int64_t)count * p.heads) {
+          int h = 0;
+          while (off >= count) off -= count, ++h;
+          s_entry = e, s_head = h, s_skip = (int)off;
+          break;
+        }
+        off -= (int64_t)count * p.heads;
+      }
+    }
   }
   __syncthreads();
-  int first = INT_MAX, last = 0, all_lo = 0, all_hi = INT_MAX;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (r >= rows) continue;
-    const int lo = s_lo[r], hi = s_hi[r];
-    if (lo < hi) first = min(first, lo), last = max(last, hi);
-    all_lo = max(all_lo, lo), all_hi = min(all_hi, hi);
-  }
-  first = min(first, last) / STG;
-  const int stages = (last + STG - 1) / STG - first;  // of the whole tile
-  const int begin = first + (int)((int64_t)stages * split / p.splits);
-  const int end = first + (int)((int64_t)stages * (split + 1) / p.splits);
+  int entry = s_entry, h = s_head, skip = s_skip;
+  AttnJoin join = {-1, 0, 0, 0, 0};
 
-  // ---------------------------------------------------------------- the ring: lane i copies piece i / 4, plane i % 4
   const uint64_t pol = evict_first_policy();
   const int page = 1 << p.page_shift;
   const int piece = min(page, STG), pieces = STG / piece;
-  const int32_t* table = p.table + (int64_t)b * p.table_stride;
-  const int my_piece = lane >> 2, plane = lane & 3;
-  // the page of this lane's piece of a stage, or -1
-  auto page_of = [&](int stage) -> int {
-    const int tok = stage * STG + my_piece * piece;
-    if (stage >= end || my_piece >= pieces || tok >= last) return -1;
-    const int id = table[tok >> p.page_shift];
-    if (id < 0 || id >= p.pages) {
-      atomicCAS(&g_device_error, 0, kErrPage);
-      return -1;
-    }
-    return id;
-  };
-  auto issue = [&](int stage, int slot, int id) {
-    const int bytes = plane < 2 ? piece * C::kRow : piece * NB * 2;
-    int total = id >= 0 ? bytes : 0;
+  const int my_piece = lane >> 2, plane = lane & 3;  // the ring: lane i copies plane i % 4 of piece i / 4
+  const int copy_row = plane < 2 ? C::kRow : NB * 2, copy_bytes = piece * copy_row;
+  const uint32_t copy_to = ring + (plane & 1) * (plane < 2 ? C::kQuants : C::kScales) + (plane < 2 ? 0 : 2 * C::kQuants) +
+                           my_piece * copy_bytes;
+  const uint8_t* copy_from = plane == 0   ? p.kq
+                             : plane == 1 ? p.vq
+                             : plane == 2 ? reinterpret_cast<const uint8_t*>(p.ks)
+                                          : reinterpret_cast<const uint8_t*>(p.vs);
+  const bool special = p.softcap > 0.f || p.slopes != nullptr;
+  const int tokA = tile_token(g);  // key rows g and g + 8 of a tile: tokA, tokA + 8
+  const int vtok0 = tile_token(2 * t), vtok1 = tile_token(2 * t + 1);
+  // The offsets as operands. Read from shared memory, and as volatile: from constants the compiler would make their eight
+  // registers anew for every product (measured: 32 moves of the 350 instructions of a 16-key step).
+  uint32_t off0[4], off1[4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const uint32_t bar = my_bars + 8 * slot;
-    if (lane == 0) mbar_expect_tx(bar, (uint32_t)total);
-    __syncwarp();
-    if (id >= 0) {
-      const int off = (stage * STG + my_piece * piece) & (page - 1);
-      const int64_t row = (((int64_t)id * p.heads + h) << p.page_shift) + off;
-      const uint32_t base = ring + slot * C::kStage;
-      if (plane == 0)
-        bulk_g2s(base + my_piece * bytes, p.kq + row * C::kRow, bytes, bar, pol);
-      else if (plane == 1)
-        bulk_g2s(base + C::kQuants + my_piece * bytes, p.vq + row * C::kRow, bytes, bar, pol);
-      else if (plane == 2)
-        bulk_g2s(base + 2 * C::kQuants + my_piece * bytes, p.ks + row * NB, bytes, bar, pol);
-      else
-        bulk_g2s(base + 2 * C::kQuants + C::kScales + my_piece * bytes, p.vs + row * NB, bytes, bar, pol);
-    }
-  };
-  // a page that cannot be read masks its tokens: the bits of a stage's good pieces (lane 4 * piece votes)
-  uint32_t good[C::kStages];
-  int ids = page_of(begin + warp);
-#pragma unroll
-  for (int s = 0; s < C::kStages; ++s) {
-    const int st = begin + warp + s * W;
-    good[s] = __ballot_sync(0xffffffffu, ids >= 0);
-    if (st < end) issue(st, s, ids);
-    ids = page_of(st + W);
+  for (int i = 0; i < 4; ++i) {
+    off1[i] = *const_cast<volatile uint32_t*>(&s_off[4 + i]);
+    off0[i] = FMT == 0 ? *const_cast<volatile uint32_t*>(&s_off[i]) : off1[i];
   }
+  uint32_t phases = 0;  // the parity of each stage's next completion
+  bool ok = true;
 
-  // ---------------------------------------------------------------- queries: B operands, row scales, start values
-  uint32_t qb[NT][NB][2][2][PARTS];
-  float start[NT][NB][2], rowf[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = rt * R + nt * 8 + g;
-    const bool there = nt * 8 + g < rows;
-    const int i = r / p.group;
-    const int64_t src = there ? (q0 + i) * p.q_st + (int64_t)(h * p.group + r - i * p.group) * p.q_sh : 0;
-    float v[NB][8], top = 0.f;
-#pragma unroll
-    for (int k = 0; k < NB; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = FMT == 0 ? 32 * k + 4 * t + (e & 3) + (e >> 2) * 16 : 32 * k + 8 * t + e;
-        v[k][e] = there ? load_elt(p.q, src + at, p.dtype) : 0.f;
-        top = fmaxf(top, fabsf(v[k][e]));
+  while (pos < end) {
+    // -------------------------------------------------------------- the next tile of the share: (b, rt, h), its rows
+    const int b = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - b * p.row_tiles;
+    const Span span = tile_span<STG, R>(p, b, rt);
+    if (h == p.heads || span.count == 0) {
+      ++entry, h = 0;
+      continue;
+    }
+    const int units = tile_units(span), take = (int)min((int64_t)(units - skip), end - pos);
+    // this share's stages of the tile: [from, to) of span.count
+    const int from = max(0, skip - kTileCost), to = max(0, skip + take - kTileCost);
+    if (to == from) {
+      pos += take, skip += take;
+      if (skip == units) skip = 0, ++h;
+      continue;
+    }
+    const Sequence q = sequence(p, b);
+    const int rows = q.n * p.group - rt * R;  // rows from this tile on (at least 1)
+    if (p.lens[b] > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
+    const int begin = span.first + from, stop = span.first + to;
+
+    const int32_t* table = p.table + (int64_t)b * p.table_stride;
+    // the page of this lane's piece of a stage, or -1
+    auto page_of = [&](int stage) -> int {
+      const int tok = stage * STG + my_piece * piece;
+      if (stage >= stop || my_piece >= pieces || tok >= q.len) return -1;
+      const int id = table[tok >> p.page_shift];
+      if (id < 0 || id >= p.pages) {
+        atomicCAS(&g_device_error, 0, kErrPage);
+        return -1;
       }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^(13 - e) for a largest magnitude in [2^e, 2^(e+1)); e bounded so that the factors stay normal numbers
-    const int e2 = max(-100, (int)(__float_as_uint(top) >> 23) - 127);
-    const float up = __uint_as_float((uint32_t)(127 + 13 - e2) << 23);
-    float f = __uint_as_float((uint32_t)(127 + e2 - 13) << 23) * p.scale * 0x1p24f;
-    if (p.softcap <= 0.f) f *= kLog2e;
+      return id;
+    };
+    auto issue = [&](int stage, int s, int id, uint32_t vote) {
+      const uint32_t bar = my_bars + 8 * s;
+      if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(vote) >> 2) * (uint32_t)(2 * piece * (C::kRow + NB * 2)));
+      __syncwarp();
+      if (id >= 0) {
+        const int off = (stage * STG + my_piece * piece) & (page - 1);
+        const int64_t row = (((int64_t)id * p.heads + h) << p.page_shift) + off;
+        bulk_g2s(copy_to + s * (W * C::kStage), copy_from + row * copy_row, copy_bytes, bar, pol);
+      }
+    };
+    // a page that cannot be read masks its tokens: the bits of a stage's good pieces (its lanes vote)
+    uint32_t good[S];
+    int ids[S];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
+    for (int i = 0; i < S; ++i) ids[i] = page_of(begin + warp + i * W);
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      good[i] = __ballot_sync(0xffffffffu, ids[i] >= 0);
+      if (i + 1 < S && begin + warp + i * W < stop) issue(begin + warp + i * W, i, ids[i], good[i]);
+    }
+
+    // -------------------------------------------------------------- queries: the tile's rows as B operands of f16
+    // A thread takes 8 values of a row at a time. Rows are scaled by a power of two; block sums give the start values.
+    // Operands lie in the ring's last stage as [part][row][block][t] 16-byte words, one for a lane's 4 registers.
+    uint4* sq = reinterpret_cast<uint4*>(smem + (S - 1) * W * C::kStage);
+    float* s_start = reinterpret_cast<float*>(sq + PARTS * R * NB * 4);  // [row][block]
+    static_assert(PARTS * R * NB * 4 * 16 + R * NB * 4 <= W * C::kStage, "queries in one stage of the ring");
+    constexpr int kItems = R * NB * 4, kPasses = (kItems + 127) / 128;
+    if (threadIdx.x < R) {
+      const int r = threadIdx.x, rr = rt * R + (r < rows ? r : 0);
+      const int i = p.cu_q ? rr / p.group : 0, head = h * p.group + (rr - i * p.group);
+      const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
+      s_lo[r] = s.lo, s_hi[r] = r < rows ? s.hi : 0, s_pos[r] = s.pos;
+      s_out[r] = (int)(q.q0 + i) * p.q_heads + head;
+      s_slope[r] = p.slopes ? p.slopes[head] * kLog2e : 0.f;
+      s_top[r] = 0;
+    }
+    __syncthreads();
+    float v[kPasses][8];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int item = i * 128 + threadIdx.x, r = item / (NB * 4), c = item - r * (NB * 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+      if (item < kItems && r < rows) {
+        const int tok = s_out[r] / p.q_heads, head = s_out[r] - tok * p.q_heads;
+        const int64_t src = (int64_t)tok * p.q_st + (int64_t)head * p.q_sh + c * 8;
+        load4_as(p.q, src, p.dtype, *reinterpret_cast<float(*)[4]>(&v[i][0]));
+        load4_as(p.q, src + 4, p.dtype, *reinterpret_cast<float(*)[4]>(&v[i][4]));
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[i][e]));
+        atomicMax(&s_top[r], __float_as_int(top));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int item = i * 128 + threadIdx.x, r = min(item / (NB * 4), R - 1), c = item - r * (NB * 4);
+      // 2^(13 - e) for a largest magnitude in [2^e, 2^(e+1)); e bounded so that the factors stay normal numbers
+      const int e2 = max(-100, (s_top[r] >> 23) - 127);
+      const float up = __int_as_float((127 + 13 - e2) << 23);
       float sum = 0.f;
+      uint32_t w[PARTS][4];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float x = v[k][e] * up;
-        if (PARTS == 1) x = __half2float(__float2half_rn(x));
-        sum += x;
-        v[k][e] = x;
+        v[i][e] *= up;
+        if (PARTS == 1) v[i][e] = __half2float(__float2half_rn(v[i][e]));
+        sum += v[i][e];
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      sum *= -kOff * 0x1p-24f;
-      start[nt][k][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-      start[nt][k][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      // (step, half): q4_0 values s and s + 2 of the low (high) nibbles; q8_0 values 4s + 2 half and the next
+      const int l = c & 3, k = c >> 2;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float lo = FMT == 0 ? v[k][hf * 4 + s] : v[k][s * 4 + hf * 2];
-          float hi = FMT == 0 ? v[k][hf * 4 + s + 2] : v[k][s * 4 + hf * 2 + 1];
-          if (FMT == 0 && hf) lo *= 0.0625f, hi *= 0.0625f;
-          const uint32_t w = pack_half2(lo, hi);
-          qb[nt][k][s][hf][0] = w;
-          if (PARTS == 2) {
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w));
-            qb[nt][k][s][hf][PARTS - 1] = pack_half2(lo - back.x, hi - back.y);
-          }
-        }
-    }
-    rowf[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);
-    rowf[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-  }
-
-  float o[NT][NB][2][4], ref[NT][2], sum[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    ref[nt][0] = ref[nt][1] = kNoRef;
-    sum[nt][0] = sum[nt][1] = 0.f;
-#pragma unroll
-    for (int k = 0; k < NB; ++k)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) o[nt][k][m][0] = o[nt][k][m][1] = o[nt][k][m][2] = o[nt][k][m][3] = 0.f;
-  }
-  const float inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
-  const int tokA = tile_token(g);                                // key rows g and g + 8 of a tile: tokA, tokA + 8
-  const int vtok0 = tile_token(2 * t), vtok1 = tile_token(2 * t + 1);
-
-  bool ok = true;
-  int slot = 0;
-  uint32_t parity = 0;
-  for (int st = begin + warp; st < end; st += W) {
-    if (!__all_sync(0xffffffffu, mbar_wait(my_bars + 8 * slot, parity, kWaitLimit))) {
-      ok = false;
-      break;
-    }
-    const uint32_t base = ring + slot * C::kStage;
-    const int j0 = st * STG;
-    uint32_t here = 0;
-#pragma unroll
-    for (int s = 0; s < C::kStages; ++s) here = s == slot ? good[s] : here;
-    const bool whole = j0 >= all_lo && j0 + STG <= all_hi && __popc(here) == 4 * pieces;
-
-    // ---- scores
-    float x[NT][SUB][4];
-    float dtop = 0.f;  // largest value scale of this lane's tokens
-    float dv[SUB][2][NB];
-#pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      float acc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-      const int rowA = u * 16 + tokA, rowB = rowA + 8;
-      float dA[NB], dB[NB];
-      lds_scales<NB>(base + 2 * C::kQuants + rowA * NB * 2, dA);
-      lds_scales<NB>(base + 2 * C::kQuants + rowB * NB * 2, dB);
-      constexpr int KW = FMT == 0 ? NB : 2 * NB;
-      uint32_t wA[KW], wB[KW];
-      lds_words<KW>(base + rowA * C::kRow + t * KW * 4, wA);
-      lds_words<KW>(base + rowB * C::kRow + t * KW * 4, wB);
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        uint32_t a[2][4];
-        if constexpr (FMT == 0) {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            a[s][0] = (wA[k] >> (8 * s)) & 0x000f000fu, a[s][1] = (wB[k] >> (8 * s)) & 0x000f000fu;
-            a[s][2] = (wA[k] >> (8 * s)) & 0x00f000f0u, a[s][3] = (wB[k] >> (8 * s)) & 0x00f000f0u;
-          }
-        } else {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            a[s][0] = __byte_perm(wA[2 * k + s], 0, 0x4140), a[s][1] = __byte_perm(wB[2 * k + s], 0, 0x4140);
-            a[s][2] = __byte_perm(wA[2 * k + s], 0, 0x4342), a[s][3] = __byte_perm(wB[2 * k + s], 0, 0x4342);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float c[4];
-          mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0][0][0], qb[nt][k][0][1][0], start[nt][k][0],
-                    start[nt][k][1], start[nt][k][0], start[nt][k][1]);
-          mma_16816(c, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][k][1][0][0], qb[nt][k][1][1][0]);
-          if constexpr (PARTS == 2) {
-            mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0][0][1], qb[nt][k][0][1][1]);
-            mma_16816(c, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][k][1][0][1], qb[nt][k][1][1][1]);
-          }
-          acc[nt][0] = fmaf(dA[k], c[0], acc[nt][0]);
-          acc[nt][1] = fmaf(dA[k], c[1], acc[nt][1]);
-          acc[nt][2] = fmaf(dB[k], c[2], acc[nt][2]);
-          acc[nt][3] = fmaf(dB[k], c[3], acc[nt][3]);
+      for (int j = 0; j < 4; ++j) {
+        // q4_0: values 0, 2 | 1, 3 of each run of 4, the nibbles of bits 4-7 and 12-15 a 16th; q8_0: runs of 2
+        float lo = FMT == 0 ? v[i][(j >> 1) * 4 + (j & 1)] : v[i][2 * j];
+        float hi = FMT == 0 ? v[i][(j >> 1) * 4 + (j & 1) + 2] : v[i][2 * j + 1];
+        if (FMT == 0 && l >= 2) lo *= 0.0625f, hi *= 0.0625f;
+        w[0][j] = pack_half2(lo, hi);
+        if constexpr (PARTS == 2) {
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[0][j]));
+          w[1][j] = pack_half2(lo - back.x, hi - back.y);
         }
       }
-      lds_scales<NB>(base + 2 * C::kQuants + C::kScales + rowA * NB * 2, dv[u][0]);
-      lds_scales<NB>(base + 2 * C::kQuants + C::kScales + rowB * NB * 2, dv[u][1]);
+      if (item < kItems) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int part = 0; part < PARTS; ++part) {
+          uint32_t* dst = reinterpret_cast<uint32_t*>(sq + (part * R + r) * NB * 4 + k * 4);
+          if constexpr (FMT == 0) {  // t = 2 (l % 2) + j / 2, register 2 (j % 2) + l / 2
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y = acc[nt][e] * rowf[nt][e & 1];
-          if (p.softcap > 0.f) y = soft_cap(y, p.softcap, inv_cap) * kLog2e;
-          x[nt][u][e] = y;
+            for (int j = 0; j < 4; ++j) dst[(2 * (l & 1) + (j >> 1)) * 4 + 2 * (j & 1) + (l >> 1)] = w[part][j];
+          } else {
+            sq[(part * R + r) * NB * 4 + k * 4 + l] = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
+          }
         }
-      if (p.slopes) {
+        if (l == 0) s_start[r * NB + k] = sum * (-kOff * 0x1p-24f);
+        if (c == 0) {
+          float f = __int_as_float((127 + e2 - 13) << 23) * p.scale * 0x1p24f;
+          if (p.softcap <= 0.f) f *= kLog2e;
+          s_rowf[r] = f;
+        }
+      }
+    }
+    __syncthreads();
+    uint4 qb[NT][NB][PARTS];
+    float start[NT][NB][QUAD ? 4 : 2], mul[NT][2];  // mul: scores to exponents of 2 (1 where they are that already)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) qb[nt][k][part] = sq[(part * R + nt * 8 + g) * NB * 4 + k * 4 + t];
+#pragma unroll
+        for (int c = 0; c < (QUAD ? 4 : 2); ++c)
+          start[nt][k][c] = SIGNED ? 0.f : s_start[(nt * 8 + 2 * t + (c & 1)) * NB + k];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) mul[nt][c] = special ? 1.f : s_rowf[nt * 8 + 2 * t + c];
+    }
+    int all_lo = 0, all_hi = INT_MAX;  // keys that every row sees: no mask
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r < rows) all_lo = max(all_lo, s_lo[r]), all_hi = min(all_hi, s_hi[r]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the operands are read before the last stage fills
+    __syncthreads();
+    int st = begin + warp;
+    if (st + (S - 1) * W < stop) issue(st + (S - 1) * W, S - 1, ids[S - 1], good[S - 1]);
+    int id = page_of(st + S * W);
+
+    float o[NT][NB][2][4], ref[NT][2], sum[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      ref[nt][0] = ref[nt][1] = kNoRef;
+      sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) o[nt][k][m][0] = o[nt][k][m][1] = o[nt][k][m][2] = o[nt][k][m][3] = 0.f;
+    }
+
+    int slot = 0;
+    for (; st < stop; st += W) {
+      if (!__all_sync(0xffffffffu, mbar_wait(my_bars + 8 * slot, (phases >> slot) & 1, kWaitLimit))) {
+        ok = false;
+        break;
+      }
+      phases ^= 1u << slot;
+      const uint8_t* base = smem + (slot * W + warp) * C::kStage;
+      const uint8_t* kscales = base + 2 * C::kQuants;
+      const uint8_t* vscales = kscales + C::kScales;
+      uint32_t here = 0;
+#pragma unroll
+      for (int s = 0; s < S; ++s) here = s == slot ? good[s] : here;
+      const bool whole = st * STG >= all_lo && st * STG + STG <= all_hi && __popc(here) == 4 * pieces;
+
+      // UN sub-tiles of 16 keys at a time: their chains of dependent instructions overlap
+#pragma unroll 1
+      for (int u0 = 0; u0 < SUB; u0 += UN) {
+        // ---- scores
+        float x[UN][NT][4];
+        float dA[UN][NB], dB[UN][NB];
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+          const int rowA = (u0 + i) * 16 + tokA;
+          lds_scales<NB>(kscales + rowA * NB * 2, dA[i]);
+          lds_scales<NB>(kscales + (rowA + 8) * NB * 2, dB[i]);
+          constexpr int KW = FMT == 0 ? NB : 2 * NB;
+          uint32_t wA[KW], wB[KW];
+          lds_words<KW>(base + rowA * C::kRow + t * KW * 4, wA);
+          lds_words<KW>(base + (rowA + 8) * C::kRow + t * KW * 4, wB);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) x[i][nt][0] = x[i][nt][1] = x[i][nt][2] = x[i][nt][3] = 0.f;
+#pragma unroll
+          for (int k = 0; k < NB; ++k) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              if constexpr (FMT == 0) {
+                a[s][0] = (wA[k] >> (8 * s)) & 0x000f000fu, a[s][1] = (wB[k] >> (8 * s)) & 0x000f000fu;
+                a[s][2] = (wA[k] >> (8 * s)) & 0x00f000f0u, a[s][3] = (wB[k] >> (8 * s)) & 0x00f000f0u;
+                if constexpr (SIGNED) {
+                  a[s][0] = add_half2(a[s][0], 0x80088008u), a[s][1] = add_half2(a[s][1], 0x80088008u);
+                  a[s][2] = add_half2(a[s][2], 0x80808080u), a[s][3] = add_half2(a[s][3], 0x80808080u);
+                }
+              } else {
+                a[s][0] = __byte_perm(wA[2 * k + s], 0, 0x4140), a[s][1] = __byte_perm(wB[2 * k + s], 0, 0x4140);
+                a[s][2] = __byte_perm(wA[2 * k + s], 0, 0x4342), a[s][3] = __byte_perm(wB[2 * k + s], 0, 0x4342);
+                if constexpr (SIGNED) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) a[s][j] = add_half2(a[s][j], 0x80808080u);
+                }
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float c[4];
+              if constexpr (QUAD && !SIGNED)
+                mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0].x, qb[nt][k][0].y, start[nt][k][0],
+                          start[nt][k][1], start[nt][k][2], start[nt][k][3]);
+              else
+                mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0].x, qb[nt][k][0].y, 0.f, 0.f, 0.f, 0.f);
+              mma_16816(c, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][k][0].z, qb[nt][k][0].w);
+              if constexpr (PARTS == 2) {
+                mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][1].x, qb[nt][k][1].y);
+                mma_16816(c, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][k][1].z, qb[nt][k][1].w);
+              }
+              if constexpr (!QUAD && !SIGNED) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] += start[nt][k][e & 1];
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[i][nt][e] = fmaf(e < 2 ? dA[i][k] : dB[i][k], c[e], x[i][nt][e]);
+            }
+          }
+          lds_scales<NB>(vscales + rowA * NB * 2, dA[i]);  // from here on the value scales of the lane's two tokens
+          lds_scales<NB>(vscales + (rowA + 8) * NB * 2, dB[i]);
+        }
+        if (special) {
+          const float inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+#pragma unroll
+          for (int i = 0; i < UN; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int r = nt * 8 + 2 * t + (e & 1), j = st * STG + (u0 + i) * 16 + tokA + (e >> 1) * 8;
+                float y = x[i][nt][e] * s_rowf[r];
+                if (p.softcap > 0.f) y = soft_cap(y, p.softcap, inv_cap) * kLog2e;
+                x[i][nt][e] = y - s_slope[r] * (float)abs(s_pos[r] - j);
+              }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < UN; ++i)
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              const int row = (u0 + i) * 16 + tokA + e2 * 8, j = st * STG + row;
+              const bool read = (here >> (4 * (row / piece))) & 1;  // its page was read
+              bool seen = false;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const int r = nt * 8 + 2 * t + c;
+                  if (!read || j < s_lo[r] || j >= s_hi[r])
+                    x[i][nt][e2 * 2 + c] = -INFINITY;
+                  else
+                    seen = true;
+                }
+              // the scales of a token that no row sees must not enter; one that is not finite would reach the rows that
+              // do not see it as 0 * d: it is taken off, and makes the rows that see it NaN
+              float most = 0.f;
+#pragma unroll
+              for (int k = 0; k < NB; ++k) most = most + fabsf(e2 ? dB[i][k] : dA[i][k]);
+              if (!seen || !(most < INFINITY)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int c = 0; c < 2; ++c)
+                    if (x[i][nt][e2 * 2 + c] != -INFINITY) x[i][nt][e2 * 2 + c] = NAN;
+#pragma unroll
+                for (int k = 0; k < NB; ++k) (e2 ? dB[i][k] : dA[i][k]) = 0.f;
+              }
+            }
+        }
+
+        // ---- reference exponents: raised only where a weight times a value scale could pass 2^15
+        // ceil(log2) of the lane's largest scale from its exponent bits, within 2^-30 (no scale) and 2^17 (an infinite
+        // one, which must not lower the weights of a row that does not see it)
+        float dtop = 0.f;
+#pragma unroll
+        for (int i = 0; i < UN; ++i)
+#pragma unroll
+          for (int k = 0; k < NB; ++k) dtop = fmaxf(dtop, fmaxf(fabsf(dA[i][k]), fabsf(dB[i][k])));
+        const float dlog = (float)(min(max((int)(__float_as_uint(dtop) >> 23), 97), 143) - 126);
+        bool raise = false;
+        float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = nt * 8 + 2 * t + (e & 1), j = j0 + rowA + (e >> 1) * 8;
-            x[nt][u][e] -= s_slope[r] * (float)abs(s_pos[r] - j);
-          }
-      }
-      if (!whole) {
+          for (int c = 0; c < 2; ++c) {
+            float m = fmaxf(x[0][nt][c], x[0][nt][2 + c]);
 #pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-          const int j = j0 + rowA + e2 * 8;
-          // pages that were not read, and tokens past the last: nothing of theirs may enter
-          const bool read = (here >> (4 * ((rowA + e2 * 8) / piece))) & 1;
+            for (int i = 1; i < UN; ++i) m = fmaxf(m, fmaxf(x[i][nt][c], x[i][nt][2 + c]));
+            top[nt][c] = fmaf(m, mul[nt][c], dlog);
+            raise |= top[nt][c] > ref[nt][c] + 15.f;
+          }
+        if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const int r = nt * 8 + 2 * t + c;
-              if (!read || j < s_lo[r] || j >= s_hi[r]) x[nt][u][e2 * 2 + c] = -INFINITY;
+              float m = top[nt][c] - 8.f;
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              if (m > ref[nt][c]) {
+                const float f = exp2_approx(ref[nt][c] - m);
+                ref[nt][c] = m;
+                sum[nt][c] *= f;
+#pragma unroll
+                for (int k = 0; k < NB; ++k)
+#pragma unroll
+                  for (int mt = 0; mt < 2; ++mt) o[nt][k][mt][c] *= f, o[nt][k][mt][2 + c] *= f;
+              }
             }
-          bool seen = false;
+        }
+
+        // ---- weights and values
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) seen |= x[nt][u][e2 * 2] != -INFINITY || x[nt][u][e2 * 2 + 1] != -INFINITY;
-          if (!seen) {
+        for (int i = 0; i < UN; ++i) {
+          float w[NT][4];
 #pragma unroll
-            for (int k = 0; k < NB; ++k) dv[u][e2][k] = 0.f;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[nt][e] = exp2_approx(fmaf(x[i][nt][e], mul[nt][e & 1], -ref[nt][e & 1]));
+              sum[nt][e & 1] += w[nt][e];
+            }
+          constexpr int VW = FMT == 0 ? (NB + 1) / 2 : NB;
+          uint32_t v[4][VW];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = (u0 + i) * 16 + (j & 1 ? vtok1 : vtok0) + (j & 2 ? 8 : 0);
+            const uint8_t* at = base + C::kQuants + row * C::kRow + g * NB * (FMT == 0 ? 2 : 4);
+            if constexpr (FMT == 0)
+              lds_halves<NB>(at, v[j]);
+            else
+              lds_words<NB>(at, v[j]);
+          }
+#pragma unroll
+          for (int k = 0; k < NB; ++k) {
+            uint32_t a[2][4];
+            if constexpr (FMT == 0) {
+              // the 16 bits of both tokens of a pair: values 2g, 16+2g, 2g+1, 17+2g in nibbles 0..3
+              const uint32_t lo = __byte_perm(v[0][k / 2], v[1][k / 2], (k & 1) ? 0x7632 : 0x5410);
+              const uint32_t hi = __byte_perm(v[2][k / 2], v[3][k / 2], (k & 1) ? 0x7632 : 0x5410);
+              a[0][0] = lo & 0x000f000fu, a[0][1] = (lo >> 8) & 0x000f000fu;
+              a[0][2] = hi & 0x000f000fu, a[0][3] = (hi >> 8) & 0x000f000fu;
+              a[1][0] = lo & 0x00f000f0u, a[1][1] = (lo >> 8) & 0x00f000f0u;
+              a[1][2] = hi & 0x00f000f0u, a[1][3] = (hi >> 8) & 0x00f000f0u;
+            } else {
+              // bytes i of both tokens of a pair: values 4g + i
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) {
+                const uint32_t lo = __byte_perm(v[0][k], v[1][k], mt ? 0x7362 : 0x5140);
+                const uint32_t hi = __byte_perm(v[2][k], v[3][k], mt ? 0x7362 : 0x5140);
+                a[mt][0] = __byte_perm(lo, 0, 0x4140), a[mt][1] = __byte_perm(lo, 0, 0x4342);
+                a[mt][2] = __byte_perm(hi, 0, 0x4140), a[mt][3] = __byte_perm(hi, 0, 0x4342);
+              }
+            }
+            if constexpr (SIGNED) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                a[0][j] = add_half2(a[0][j], FMT == 0 ? 0x80088008u : 0x80808080u);
+                a[1][j] = add_half2(a[1][j], 0x80808080u);
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = w[nt][e] * (e < 2 ? dA[i][k] : dB[i][k]);
+              const uint32_t p0 = pack_half2(y[0], y[1]), p1 = pack_half2(y[2], y[3]);
+              const uint32_t b0 = transpose_8x8(p0), b1 = transpose_8x8(p1);
+              if constexpr (PARTS == 1) {
+                // the offsets of these 16 keys, at once: the sum does not drift and cancel
+                mma_16816(o[nt][k][0], off0[0], off0[1], off0[2], off0[3], b0, b1);
+                mma_16816(o[nt][k][1], off1[0], off1[1], off1[2], off1[3], b0, b1);
+                mma_16816(o[nt][k][0], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
+                mma_16816(o[nt][k][1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
+              } else {
+                // the tensor cores cut their sums off (towards zero), which adds up over a long row: for f32 each
+                // tile's products are summed from zero and added to the row by rounded additions
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
+                const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
+                const uint32_t l0 = transpose_8x8(pack_half2(y[0] - f0.x, y[1] - f0.y));
+                const uint32_t l1 = transpose_8x8(pack_half2(y[2] - f1.x, y[3] - f1.y));
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                  float c[4];
+                  mma_16816(c, a[mt][0], a[mt][1], a[mt][2], a[mt][3], l0, l1, 0.f, 0.f, 0.f, 0.f);
+                  mma_16816(c, a[mt][0], a[mt][1], a[mt][2], a[mt][3], b0, b1);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[nt][k][mt][e] += c[e];
+                }
+              }
+            }
           }
         }
       }
+
+      // ---- the stage is read: refill it
+      __syncwarp();
+      const uint32_t vote = __ballot_sync(0xffffffffu, id >= 0);
 #pragma unroll
-      for (int k = 0; k < NB; ++k) dtop = fmaxf(dtop, fmaxf(fabsf(dv[u][0][k]), fabsf(dv[u][1][k])));
+      for (int s = 0; s < S; ++s)
+        if (s == slot) good[s] = vote;
+      if (st + S * W < stop) issue(st + S * W, slot, id, vote);
+      id = page_of(st + (S + 1) * W);
+      if (++slot == S) slot = 0;
     }
 
-    // ---- reference exponents: raised only where a weight times a value scale could pass 2^15
-    // ceil(log2) of the lane's largest scale from its exponent bits, within 2^-30 (no scale) and 2^17 (an infinite one,
-    // which must not lower the weights of a row that does not see it)
-    const float dlog = (float)(min(max((int)(__float_as_uint(dtop) >> 23), 97), 143) - 126);
-    bool raise = false;
-    float top[NT][2];
+    // -------------------------------------------------------------- join the warps (in the ring's memory: all is read)
+    if (__syncthreads_or(!ok)) break;
+    float* so = reinterpret_cast<float*>(smem);              // [W][R][D]
+    float2* sm = reinterpret_cast<float2*>(so + W * R * D);  // [W][R] reference, sum
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float m = -INFINITY;
+        float l = sum[nt][c];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int r = nt * 8 + 2 * t + c;
+        if (g == 0) sm[warp * R + r] = make_float2(ref[nt][c], l);
+        float* dst = so + (warp * R + r) * D + (FMT == 0 ? 2 : 4) * g;
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) m = fmaxf(m, fmaxf(x[nt][u][c], x[nt][u][2 + c]));
-        top[nt][c] = m + dlog;
-        raise |= top[nt][c] - ref[nt][c] > 15.f;
-      }
-    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float m = top[nt][c];
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-          if (m - 8.f > ref[nt][c]) {
-            const float f = exp2_approx(ref[nt][c] - (m - 8.f));
-            ref[nt][c] = m - 8.f;
-            sum[nt][c] *= f;
-#pragma unroll
-            for (int k = 0; k < NB; ++k)
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt) o[nt][k][mt][c] *= f, o[nt][k][mt][2 + c] *= f;
-          }
-        }
-    }
-
-    // ---- weights and values
-#pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      float w[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[nt][e] = exp2_approx(x[nt][u][e] - ref[nt][e & 1]);
-          sum[nt][e & 1] += w[nt][e];
-        }
-      constexpr int VW = FMT == 0 ? (NB + 1) / 2 : NB;
-      uint32_t v[4][VW];
-      const uint32_t vb = base + C::kQuants + u * 16 * C::kRow + g * NB * (FMT == 0 ? 2 : 4);
-      if constexpr (FMT == 0) {
-        lds_halves<NB>(vb + vtok0 * C::kRow, v[0]);
-        lds_halves<NB>(vb + vtok1 * C::kRow, v[1]);
-        lds_halves<NB>(vb + (vtok0 + 8) * C::kRow, v[2]);
-        lds_halves<NB>(vb + (vtok1 + 8) * C::kRow, v[3]);
-      } else {
-        lds_words<NB>(vb + vtok0 * C::kRow, v[0]);
-        lds_words<NB>(vb + vtok1 * C::kRow, v[1]);
-        lds_words<NB>(vb + (vtok0 + 8) * C::kRow, v[2]);
-        lds_words<NB>(vb + (vtok1 + 8) * C::kRow, v[3]);
-      }
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        uint32_t a[2][4];
-        if constexpr (FMT == 0) {
-          // the 16 bits of both tokens of a pair: values 2g, 16+2g, 2g+1, 17+2g in nibbles 0..3
-          const uint32_t lo = __byte_perm(v[0][k / 2], v[1][k / 2], (k & 1) ? 0x7632 : 0x5410);
-          const uint32_t hi = __byte_perm(v[2][k / 2], v[3][k / 2], (k & 1) ? 0x7632 : 0x5410);
-          a[0][0] = add_half2(lo & 0x000f000fu, 0x80088008u), a[0][1] = add_half2((lo >> 8) & 0x000f000fu, 0x80088008u);
-          a[0][2] = add_half2(hi & 0x000f000fu, 0x80088008u), a[0][3] = add_half2((hi >> 8) & 0x000f000fu, 0x80088008u);
-          a[1][0] = add_half2(lo & 0x00f000f0u, 0x80808080u), a[1][1] = add_half2((lo >> 8) & 0x00f000f0u, 0x80808080u);
-          a[1][2] = add_half2(hi & 0x00f000f0u, 0x80808080u), a[1][3] = add_half2((hi >> 8) & 0x00f000f0u, 0x80808080u);
-        } else {
-          // bytes i of both tokens of a pair: values 4g + i
+        for (int k = 0; k < NB; ++k)
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            const uint32_t lo = __byte_perm(v[0][k], v[1][k], mt ? 0x7362 : 0x5140);
-            const uint32_t hi = __byte_perm(v[2][k], v[3][k], mt ? 0x7362 : 0x5140);
-            a[mt][0] = add_half2(__byte_perm(lo, 0, 0x4140), 0x80808080u);
-            a[mt][1] = add_half2(__byte_perm(lo, 0, 0x4342), 0x80808080u);
-            a[mt][2] = add_half2(__byte_perm(hi, 0, 0x4140), 0x80808080u);
-            a[mt][3] = add_half2(__byte_perm(hi, 0, 0x4342), 0x80808080u);
+            const float f = FMT == 0 && mt ? 0x1p20f : 0x1p24f;  // the unit of the quants' bits
+            *reinterpret_cast<float2*>(dst + 32 * k + (FMT == 0 ? 16 : 2) * mt) =
+                make_float2(o[nt][k][mt][c] * f, o[nt][k][mt][2 + c] * f);
           }
-        }
+      }
+    __syncthreads();
+    const bool begun = from > 0, done = to == span.count;
+    const int part = 2 * (int)blockIdx.x + (begun ? 0 : 1);  // a share ends at most one tile and begins one at most
+    for (int i = threadIdx.x; i < min(rows, R) * (D / 4); i += 128) {
+      const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
+      float top = kNoRef, l = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float y[4];
+      for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w * R + r].x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = w[nt][e] * dv[u][e >> 1][k];
-          if (!whole) {  // a masked key's scale may be anything
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = x[nt][u][e] == -INFINITY ? 0.f : y[e];
-          }
-          const uint32_t p0 = pack_half2(y[0], y[1]), p1 = pack_half2(y[2], y[3]);
-          const uint32_t b0 = transpose_8x8(p0), b1 = transpose_8x8(p1);
-          mma_16816(o[nt][k][0], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
-          mma_16816(o[nt][k][1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
-          if constexpr (PARTS == 2) {
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&p0));
-            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
-            const uint32_t l0 = transpose_8x8(pack_half2(y[0] - f0.x, y[1] - f0.y));
-            const uint32_t l1 = transpose_8x8(pack_half2(y[2] - f1.x, y[3] - f1.y));
-            mma_16816(o[nt][k][0], a[0][0], a[0][1], a[0][2], a[0][3], l0, l1);
-            mma_16816(o[nt][k][1], a[1][0], a[1][1], a[1][2], a[1][3], l0, l1);
-          }
-        }
+      for (int w = 0; w < W; ++w) {
+        const float2 m = sm[w * R + r];
+        const float f = exp2_approx(m.x - top);
+        const float4 z = *reinterpret_cast<const float4*>(so + (w * R + r) * D + c);
+        l = fmaf(m.y, f, l);
+        y[0] = fmaf(z.x, f, y[0]), y[1] = fmaf(z.y, f, y[1]), y[2] = fmaf(z.z, f, y[2]), y[3] = fmaf(z.w, f, y[3]);
+      }
+      if (!begun && done) {
+        const float inv = l > 0.f || l != l ? __fdividef(1.f, l) : 0.f;
+        store4_as(p.out, (int64_t)s_out[r] * D + c, p.dtype, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        if (p.lse && c == 0) p.lse[s_out[r]] = (top + log2f(l)) * kLn2;
+      } else {
+        store4(p.part_o + ((int64_t)part * R + r) * D + c, y[0], y[1], y[2], y[3]);
+        if (c == 0) p.part_m[part * R + r] = make_float2(top, l);
       }
     }
+    if (begun && done && threadIdx.x == 0) {  // this CTA ends a tile that others began: the joining kernel's work
+      join.first = (int)((pos - skip + kTileCost) / per);
+      join.rows = min(rows, R), join.row0 = rt * R, join.head0 = h * p.group, join.q0 = (int)q.q0;
+    }
+    pos += take, skip += take;
+    if (skip == units) skip = 0, ++h;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // these reads and writes before the next copies
+    __syncthreads();
+  }
+  if (pos < end) {  // a wait gave up: no copy may be in flight when the CTA leaves
+    if (!ok && lane == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
+    for (int s = 0; s < S; ++s) {
+      mbar_wait(my_bars + 8 * s, 0, kWaitLimit);
+      mbar_wait(my_bars + 8 * s, 1, kWaitLimit);
+    }
+    join.first = -1;
+  }
+  if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
+}
 
-    // ---- the stage is read: refill it
-    __syncwarp();
-    const int next = st + C::kStages * W;
-    const uint32_t vote = __ballot_sync(0xffffffffu, ids >= 0);
+// Joins the parts of tiles that several CTAs worked on: one warp for each CTA that ended such a tile and each of its
+// rows, its lanes over the dimension. The CTA that began the tile left its second part, the others their first.
+template <int NB, int R>
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttnParams p, int ctas) {
+  constexpr int D = NB * 32;
+  pdl_wait_then_trigger();
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int cta = item / R, r = item - cta * R;
+  if (cta >= ctas) return;
+  const AttnJoin join = p.joins[cta];
+  if (join.first < 0 || r >= join.rows) return;
+  const int rr = join.row0 + r, qi = p.cu_q ? rr / p.group : 0;
+  const int64_t out_row = (int64_t)(join.q0 + qi) * p.q_heads + join.head0 + (rr - qi * p.group);
+  const int n = cta - join.first + 1;
+  auto part_of = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? 1 : 0)) * R + r; };
+  float top = kNoRef, l = 0.f, y[NB];
 #pragma unroll
-    for (int s = 0; s < C::kStages; ++s)
-      if (s == slot) good[s] = vote;
-    if (next < end) issue(next, slot, ids);
-    ids = page_of(next + W);
-    if (++slot == C::kStages) slot = 0, parity ^= 1;
-  }
-  if (!ok && lane == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
-
-  // ---------------------------------------------------------------- join the warps
-  // every copy that was issued has been waited for (a wait that gave up returns with its copies drained below)
-  if (!ok) {
-    for (int s = 0; s < C::kStages; ++s) mbar_wait(my_bars + 8 * s, 0, kWaitLimit), mbar_wait(my_bars + 8 * s, 1, kWaitLimit);
-  }
-  __syncthreads();  // the ring's memory is free
-  float* so = reinterpret_cast<float*>(smem);                    // [W][R][D]
-  float2* sm = reinterpret_cast<float2*>(so + W * R * D);        // [W][R] reference, sum
+  for (int i = 0; i < NB; ++i) y[i] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {  // 32 parts at a time: a lane holds the reference and sum of one
+    const int m = min(32, n - i0);
+    const float2 v = lane < m ? p.part_m[part_of(i0 + lane)] : make_float2(kNoRef, 0.f);
+    float now = fmaxf(top, v.x);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+    const float old = exp2_approx(top - now), f = lane < m ? exp2_approx(v.x - now) : 0.f;
+    float s = v.y * f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float l = sum[nt][c];
-      l += __shfl_xor_sync(0xffffffffu, l, 4);
-      l += __shfl_xor_sync(0xffffffffu, l, 8);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const int r = nt * 8 + 2 * t + c;
-      if (g == 0) sm[warp * R + r] = make_float2(ok ? ref[nt][c] : NAN, l);
-      float* dst = so + (warp * R + r) * D;
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    l = fmaf(l, old, s), top = now;
 #pragma unroll
-      for (int k = 0; k < NB; ++k)
+    for (int i = 0; i < NB; ++i) y[i] *= old;
+    constexpr int kOnce = NB <= 4 ? 16 : 8;  // loads of so many parts in flight
+    for (int j0 = 0; j0 < m; j0 += kOnce) {
+      float z[kOnce][NB];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const float f = FMT == 0 && mt ? 0x1p20f : 0x1p24f;  // the unit of the quants' bits
-          const int at = FMT == 0 ? 32 * k + 16 * mt + 2 * g : 32 * k + 4 * g + 2 * mt;
-          dst[at] = o[nt][k][mt][c] * f;
-          dst[at + 1] = o[nt][k][mt][2 + c] * f;
-        }
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < R * D; i += 128) {
-    const int r = i / D, c = i - r * D;
-    if (r >= rows) break;
-    float m = kNoRef;
-    bool bad = false;
+      for (int j = 0; j < kOnce; ++j)
 #pragma unroll
-    for (int w = 0; w < W; ++w) m = fmaxf(m, sm[w * R + r].x), bad |= isnan(sm[w * R + r].x);
-    float l = 0.f, y = 0.f;
+        for (int c = 0; c < NB; ++c) z[j][c] = j0 + j < m ? p.part_o[part_of(i0 + j0 + j) * D + c * 32 + lane] : 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float2 v = sm[w * R + r];
-      const float f = bad ? NAN : exp2_approx(v.x - m);
-      l += v.y * f;
-      y += so[(w * R + r) * D + c] * f;
-    }
-    const int rr = rt * R + r, qi = rr / p.group;
-    const int64_t out_row = (q0 + qi) * p.q_heads + h * p.group + (rr - qi * p.group);
-    if (p.splits == 1) {
-      store_elt(p.out, out_row * D + c, p.dtype, l > 0.f || l != l ? y / l : 0.f);
-      if (p.lse && c == 0) p.lse[out_row] = (m + log2f(l)) * kLn2;
-    } else {
-      p.part_o[(out_row * p.splits + split) * D + c] = y;
-      if (c == 0) p.part_m[out_row * p.splits + split] = make_float2(m, l);
+      for (int j = 0; j < kOnce; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j0 + j);  // 0 past the last part
+#pragma unroll
+        for (int c = 0; c < NB; ++c) y[c] = fmaf(z[j][c], fj, y[c]);
+      }
     }
   }
+  const float inv = l > 0.f || l != l ? __fdividef(1.f, l) : 0.f;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) store_elt(p.out, out_row * D + i * 32 + lane, p.dtype, y[i] * inv);
+  if (p.lse && lane == 0) p.lse[out_row] = (top + log2f(l)) * kLn2;
 }
 
 template <int FMT, int NB, int NT, int PARTS>
-static int launch_attention_as(const AttnParams& p, cudaStream_t stream) {
+static int launch_attention_as(const AttnParams& p, int sms, int64_t max_len, cudaStream_t stream) {
   using C = KvTile<FMT, NB>;
-  constexpr int kJoin = C::kWarps * NT * 8 * (NB * 32 + 2) * 4;
+  constexpr int kJoin = C::kWarps * NT * 8 * (NB * 32 + 2) * 4;  // the warps' results, in the ring's place
   constexpr int kSmem = C::kRing > kJoin ? C::kRing : kJoin;
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
   auto kernel = attention_kernel<FMT, NB, NT, PARTS>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
-  const int64_t ctas = (int64_t)p.batch * p.heads * p.row_tiles * p.splits;
+  static_assert(kv_ctas_per_sm<FMT, NB, NT, PARTS>() * (kSmem + 1024 + 1024) <= 228 * 1024, "shared memory of an SM");
+  const int64_t slots = (int64_t)sms * kv_ctas_per_sm<FMT, NB, NT, PARTS>();
+  // no more CTAs than there can be stages; max_len bounds the lengths from above
+  const int64_t most = (int64_t)p.batch * p.row_tiles * p.heads * ((max_len + C::kTokens - 1) / C::kTokens + 1);
+  const int64_t ctas = most < slots ? most : slots;
   launch_maybe_pdl(kernel, dim3((unsigned)ctas), dim3(128), kSmem, stream, p);
-  return after_launch("attention");
+  int rc = after_launch("attention");
+  if (rc) return rc;
+  const int64_t warps = ctas * NT * 8;
+  launch_maybe_pdl(attention_join_kernel<NB, NT * 8>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p, (int)ctas);
+  return after_launch("attention_join");
 }
 
 template <int FMT>
-static int launch_attention_fmt(const AttnParams& p, int dim, int rows, cudaStream_t stream) {
+static int launch_attention_fmt(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream) {
   const bool wide = p.dtype == B2Q_DTYPE_F32;
   auto by_rows = [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
     if constexpr (NB < 8)
       if (rows == 16)
-        return wide ? launch_attention_as<FMT, NB, 2, 2>(p, stream) : launch_attention_as<FMT, NB, 2, 1>(p, stream);
-    return wide ? launch_attention_as<FMT, NB, 1, 2>(p, stream) : launch_attention_as<FMT, NB, 1, 1>(p, stream);
+        return wide ? launch_attention_as<FMT, NB, 2, 2>(p, sms, max_len, stream) : launch_attention_as<FMT, NB, 2, 1>(p, sms, max_len, stream);
+    return wide ? launch_attention_as<FMT, NB, 1, 2>(p, sms, max_len, stream) : launch_attention_as<FMT, NB, 1, 1>(p, sms, max_len, stream);
   };
   switch (dim) {
     case 64: return by_rows(std::integral_constant<int, 2>{});

@@ -42,7 +42,7 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float
 // A[g][2t+8..], A[g+8][2t+8..]; B[2t..][g], B[2t+8..][g]; D/C [g][2t], [g][2t+1], [g+8][2t], [g+8][2t+1].
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, "
       "%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -56,7 +56,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 // Transpose of an 8x8 matrix of 16-bit values, lane (g, t) holding row g, columns 2t and 2t+1, before and after.
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -70,17 +70,12 @@ __device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 2^x and 1/x, 2 ulp (the hardware approximations).
+// 2^x, the hardware's approximation (2 ulp), results below 2^-126 as 0: the other form scales its argument for those
+// (three more instructions), which a softmax weight has no use for.
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-__device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
 }
 
 // Reads, and with `clear` resets, a translation unit's device error word.

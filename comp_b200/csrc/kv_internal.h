@@ -15,6 +15,12 @@ inline int dtype_size(int dtype) { return dtype == B2Q_DTYPE_F32 ? 4 : 2; }
 // The checks of a cache descriptor that every entry point makes (kv_cache.cu).
 int check_kv_cache(const char* who, const b2q_kv_cache* c);
 
+// A tile that several CTAs worked on, told by the CTA that ended it: the CTA that began it (-1: no such tile), the tile's
+// rows, its first row and head, and its sequence's first query token.
+struct AttnJoin {
+  int first, rows, row0, head0, q0;
+};
+
 struct AttnParams {
   const void* q;
   void* out;
@@ -23,10 +29,11 @@ struct AttnParams {
   const uint16_t *ks, *vs;
   const int32_t *table, *lens, *cu_q, *prefix, *starts;
   const float* slopes;
-  float* part_o;   // [T * q_heads][splits][dim] partial outputs (not divided), when the keys are split
-  float2* part_m;  // [T * q_heads][splits] their reference exponent and sum
+  float* part_o;    // [2 a CTA][rows of a tile][dim] outputs, not divided, of tiles that cross CTAs' shares
+  float2* part_m;   // [2 a CTA][rows of a tile] their reference exponent and sum
+  AttnJoin* joins;  // [CTAs]
   int64_t q_st, q_sh, T, table_stride, pages;
-  int table_pages, batch, q_heads, heads, group, page_shift, splits, row_tiles, window, dtype;
+  int table_pages, batch, q_heads, heads, group, page_shift, row_tiles, window, dtype;
   float scale, softcap;
 };
 
@@ -35,8 +42,9 @@ int kv_cache_error(int* code, int clear);
 int kv_attention_q4_error(int* code, int clear);
 int kv_attention_q8_error(int* code, int clear);
 
-// Decode kernels by format: `rows` is 8 or 16 query rows a tile.
-int launch_attention_q4(const AttnParams& p, int dim, int rows, cudaStream_t stream);
-int launch_attention_q8(const AttnParams& p, int dim, int rows, cudaStream_t stream);
+// Streaming kernels by format: `rows` is 8 or 16 query rows a tile, max_len bounds the lengths from above.
+int launch_attention_q4(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream);
+int launch_attention_q8(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream);
+constexpr int kMaxCtasPerSm = 4;
 
 }  // namespace b2q

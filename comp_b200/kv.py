@@ -195,8 +195,7 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     prefix = _index(prefix, "prefix", (B,), dev)
     starts = _index(starts, "starts", (T,), dev)
     slopes = _index(slopes, "slopes", (heads,), dev, torch.float32)
-    if q.stride(2) != 1:
-        q = q.contiguous()
+    q = _heads_aligned(q)
     if out is None:
         out = torch.empty((T, heads, dim), dtype=q.dtype, device=dev)
     elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev or not out.is_contiguous():

@@ -336,7 +336,8 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
  * max_q: at least the most queries of a sequence (0: max_q = T); max_len: at least the longest lens, used to plan the
  * split of the keys only. Tokens beyond the table or in pages outside the cache read as masked, and set the device
  * error word to 3. out [T][q_heads][dim] contiguous, of q's dtype; lse f32 [T][q_heads] or NULL. Rows of q beyond
- * cu_q[batch] are left unwritten. q: element strides per token and head, last axis contiguous, any alignment.
+ * cu_q[batch] are left unwritten. q: element strides per token and head, last axis
+ * contiguous, 16-byte aligned in base and strides.
  */
 typedef struct {
   const void* q;
@@ -354,7 +355,7 @@ typedef struct {
   float scale, softcap;
 } b2q_attention_args;
 
-/* Device workspace bytes b2q_attention needs for these arguments (partial results of split keys; 0: none). */
+/* Device workspace bytes b2q_attention needs for these arguments (partial results of keys that are split over the GPU). */
 size_t b2q_attention_workspace_size(const b2q_kv_cache* cache, const b2q_attention_args* args);
 
 /* Runs it. workspace: device memory, 16-byte aligned, of at least that many bytes; calls that may overlap on the GPU
