@@ -6,7 +6,7 @@
 // products run on the tensor cores (16x8x16, f16 in, f32 sums) with keys and values as the 16-row operand and 8 query
 // rows as the columns: nothing is padded, and no quant is rounded. What an operand's 16 bits hold:
 //   - keys: the quant's bits alone, i.e. the f16 subnormal q * 2^-24 (or q * 2^-20 for a nibble left in bits 4-7): one
-//     AND unpacks two values. The offset -off * sum(Q) of a block is the sum's start value, a constant of the row.
+//     AND unpacks two values. The offset -off * sum(Q) of a block is a constant of the row, added to the block's sum.
 //   - queries: scaled by a power of two to 2^13..2^14, so that 16-bit queries are exact; f32 queries take two parts.
 //     A block's scale dk (per key and block) multiplies the f32 sum of the block.
 //   - values: the quant minus its offset, again as an exact subnormal; no running sum can then cancel.
@@ -16,10 +16,9 @@
 // A weight matrix leaves the first product with keys along the lanes' rows and enters the second with keys along their
 // pairs: one 8x8 transpose in registers each.
 //
-// What bounds it: the cache's bytes. Every warp is on its own: it owns every W-th stage of 16 to 64 keys of its CTA's
-// share, copied by its own ring of bulk copies (contiguous pieces of a page), and joins the others
-// once at the end of a tile through shared memory. The CTAs fill the GPU once and take equal shares of all stages of
-// all sequences, heads and row tiles, whatever their lengths; tiles that cross shares are joined by a second kernel.
+// What bounds it: the cache's bytes. The CTAs fill the GPU once and take equal shares of all stages (16 to 128 keys) of all
+// sequences, heads and row tiles, whatever their lengths; a tile's stages go round the four warps, each with a ring of its
+// own, and the warps join at the tile's end. Tiles that cross shares are joined by a second kernel.
 #pragma once
 
 #include <climits>
@@ -28,6 +27,7 @@
 
 #include "kv_device.cuh"
 #include "kv_internal.h"
+#include "tc_device.cuh"
 
 namespace b2q {
 
@@ -206,24 +206,15 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   constexpr int D = NB * 32, W = C::kWarps, S = C::kStages, STG = C::kTokens, SUB = STG / 16, R = NT * 8;
   constexpr bool SIGNED = PARTS == 2;  // quants enter the products with their offset taken off
   constexpr float kOff = FMT == 0 ? 8.f : 128.f;
-  // the start values of a block's sum as a whole accumulator (4 registers a block and row tile) where registers allow,
-  // else added after the product
-  constexpr bool QUAD = NB * NT <= 4;
   constexpr int UN = SUB % 2 == 0 && NB * NT <= 4 && PARTS == 1 ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];  // [stage][warp] ring; the last stage holds the queries at first
-  __shared__ uint64_t bars[W * S];
   __shared__ int s_lo[R], s_hi[R], s_pos[R], s_out[R], s_top[R], s_entry, s_head, s_skip;
   __shared__ float s_slope[R], s_rowf[R];
   __shared__ int64_t s_scan[W];
   __shared__ uint32_t s_off[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  const uint32_t my_bars = smem_addr(&bars[warp * S]);
-  const uint32_t ring = smem_addr(smem) + warp * C::kStage;
-  if (lane == 0) {
-    for (int s = 0; s < S; ++s) mbar_init(my_bars + 8 * s, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
+  uint8_t* const ring = smem + warp * C::kStage;  // stage s of this warp: s * W stages on
   if (threadIdx.x < 8) s_off[threadIdx.x] = threadIdx.x < 4 ? 0x80088008u : 0x80808080u;
   pdl_wait_then_trigger();
 
@@ -280,17 +271,8 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   int entry = s_entry, h = s_head, skip = s_skip;
   AttnJoin join = {-1, 0, 0, 0, 0};
 
-  const uint64_t pol = evict_first_policy();
-  const int page = 1 << p.page_shift;
-  const int piece = min(page, STG), pieces = STG / piece;
-  const int my_piece = lane >> 2, plane = lane & 3;  // the ring: lane i copies plane i % 4 of piece i / 4
-  const int copy_row = plane < 2 ? C::kRow : NB * 2, copy_bytes = piece * copy_row;
-  const uint32_t copy_to = ring + (plane & 1) * (plane < 2 ? C::kQuants : C::kScales) + (plane < 2 ? 0 : 2 * C::kQuants) +
-                           my_piece * copy_bytes;
-  const uint8_t* copy_from = plane == 0   ? p.kq
-                             : plane == 1 ? p.vq
-                             : plane == 2 ? reinterpret_cast<const uint8_t*>(p.ks)
-                                          : reinterpret_cast<const uint8_t*>(p.vs);
+  const int page = 1 << p.page_shift, piece_shift = min(p.page_shift, __ffs(STG) - 1);
+  const int pieces = STG >> piece_shift;  // a stage's contiguous pieces, each of a page
   const bool special = p.softcap > 0.f || p.slopes != nullptr;
   const int tokA = tile_token(g);  // key rows g and g + 8 of a tile: tokA, tokA + 8
   const int vtok0 = tile_token(2 * t), vtok1 = tile_token(2 * t + 1);
@@ -302,9 +284,6 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     off1[i] = *const_cast<volatile uint32_t*>(&s_off[4 + i]);
     off0[i] = FMT == 0 ? *const_cast<volatile uint32_t*>(&s_off[i]) : off1[i];
   }
-  uint32_t phases = 0;  // the parity of each stage's next completion
-  bool ok = true;
-
   while (pos < end) {
     // -------------------------------------------------------------- the next tile of the share: (b, rt, h), its rows
     const int b = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - b * p.row_tiles;
@@ -327,10 +306,10 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     const int begin = span.first + from, stop = span.first + to;
 
     const int32_t* table = p.table + (int64_t)b * p.table_stride;
-    // the page of this lane's piece of a stage, or -1
+    // the page of piece `lane` of a stage, or -1
     auto page_of = [&](int stage) -> int {
-      const int tok = stage * STG + my_piece * piece;
-      if (stage >= stop || my_piece >= pieces || tok >= q.len) return -1;
+      const int tok = stage * STG + (lane << piece_shift);
+      if (stage >= stop || lane >= pieces || tok >= q.len) return -1;
       const int id = table[tok >> p.page_shift];
       if (id < 0 || id >= p.pages) {
         atomicCAS(&g_device_error, 0, kErrPage);
@@ -338,17 +317,46 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
       }
       return id;
     };
-    auto issue = [&](int stage, int s, int id, uint32_t vote) {
-      const uint32_t bar = my_bars + 8 * s;
-      if (lane == 0) mbar_expect_tx(bar, (uint32_t)(__popc(vote) >> 2) * (uint32_t)(2 * piece * (C::kRow + NB * 2)));
-      __syncwarp();
-      if (id >= 0) {
-        const int off = (stage * STG + my_piece * piece) & (page - 1);
-        const int64_t row = (((int64_t)id * p.heads + h) << p.page_shift) + off;
-        bulk_g2s(copy_to + s * (W * C::kStage), copy_from + row * copy_row, copy_bytes, bar, pol);
+    // copies a stage into ring slot s, 16 bytes a lane at a time; pieces without a page are filled with zeros
+    auto copy = [&](int stage, int s, int id) {
+      const uint32_t to = smem_addr(ring + s * (W * C::kStage)) + lane * 16;
+      if (stage < stop) {
+        if (pieces == 1) {
+          const int one = __shfl_sync(0xffffffffu, id, 0);
+          const bool is = one >= 0;
+          const int64_t row = is ? (((int64_t)one * p.heads + h) << p.page_shift) + ((stage * STG) & (page - 1)) : 0;
+          const uint8_t* k = p.kq + row * C::kRow + lane * 16;
+          const uint8_t* v = p.vq + row * C::kRow + lane * 16;
+#pragma unroll
+          for (int j = 0; j < C::kQuants; j += 512) cp_async16(to + j, k + j, is);
+#pragma unroll
+          for (int j = 0; j < C::kQuants; j += 512) cp_async16(to + C::kQuants + j, v + j, is);
+          if (lane * 16 < C::kScales) {
+            cp_async16(to + 2 * C::kQuants, reinterpret_cast<const uint8_t*>(p.ks + row * NB) + lane * 16, is);
+            cp_async16(to + 2 * C::kQuants + C::kScales, reinterpret_cast<const uint8_t*>(p.vs + row * NB) + lane * 16,
+                       is);
+          }
+        } else {
+          // chunk c of a plane: its token, that token's piece and page
+          auto chunk = [&](int c, int row_bytes, const uint8_t* a, const uint8_t* b, uint32_t to_a, uint32_t to_b) {
+            const int tok = c * 16 / row_bytes, pc = tok >> piece_shift;
+            const int one = __shfl_sync(0xffffffffu, id, pc & 31);
+            const bool is = one >= 0 && pc < pieces;
+            const int64_t row = is ? ((int64_t)one * p.heads + h) << p.page_shift : 0;
+            const int64_t src = row * row_bytes + (is ? c * 16 - (pc << piece_shift) * row_bytes : 0);
+            if (pc < pieces) cp_async16(to_a, a + src, is), cp_async16(to_b, b + src, is);
+          };
+#pragma unroll 1
+          for (int j = 0; j < C::kQuants; j += 512)
+            chunk(j / 16 + lane, C::kRow, p.kq, p.vq, to + j, to + C::kQuants + j);
+          chunk(lane, NB * 2, reinterpret_cast<const uint8_t*>(p.ks), reinterpret_cast<const uint8_t*>(p.vs),
+                to + 2 * C::kQuants, to + 2 * C::kQuants + C::kScales);
+        }
       }
+      cp_async_commit();  // a group a stage, empty past the last
     };
-    // a page that cannot be read masks its tokens: the bits of a stage's good pieces (its lanes vote)
+    // a page that cannot be read masks its tokens: bit i of a stage's word is whether piece i was
+    const uint32_t full = (1u << pieces) - 1;
     uint32_t good[S];
     int ids[S];
 #pragma unroll
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       good[i] = __ballot_sync(0xffffffffu, ids[i] >= 0);
-      if (i + 1 < S && begin + warp + i * W < stop) issue(begin + warp + i * W, i, ids[i], good[i]);
+      if (i + 1 < S) copy(begin + warp + i * W, i, ids[i]);
     }
 
     // -------------------------------------------------------------- queries: the tile's rows as B operands of f16
@@ -444,7 +452,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     }
     __syncthreads();
     uint4 qb[NT][NB][PARTS];
-    float start[NT][NB][QUAD ? 4 : 2], mul[NT][2];  // mul: scores to exponents of 2 (1 where they are that already)
+    float start[NT][NB][2], mul[NT][2];  // mul: scores to exponents of 2 (1 where they are that already)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -452,8 +460,8 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) qb[nt][k][part] = sq[(part * R + nt * 8 + g) * NB * 4 + k * 4 + t];
 #pragma unroll
-        for (int c = 0; c < (QUAD ? 4 : 2); ++c)
-          start[nt][k][c] = SIGNED ? 0.f : s_start[(nt * 8 + 2 * t + (c & 1)) * NB + k];
+        for (int c = 0; c < 2; ++c)
+          start[nt][k][c] = SIGNED ? 0.f : s_start[(nt * 8 + 2 * t + c) * NB + k];
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) mul[nt][c] = special ? 1.f : s_rowf[nt * 8 + 2 * t + c];
@@ -462,11 +470,9 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (r < rows) all_lo = max(all_lo, s_lo[r]), all_hi = min(all_hi, s_hi[r]);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the operands are read before the last stage fills
-    __syncthreads();
-    int st = begin + warp;
-    if (st + (S - 1) * W < stop) issue(st + (S - 1) * W, S - 1, ids[S - 1], good[S - 1]);
-    int id = page_of(st + S * W);
+    __syncthreads();  // the operands are read: the last stage may fill
+    copy(begin + warp + (S - 1) * W, S - 1, ids[S - 1]);
+    int id = page_of(begin + warp + S * W);
 
     float o[NT][NB][2][4], ref[NT][2], sum[NT][2];
 #pragma unroll
@@ -480,21 +486,20 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     }
 
     int slot = 0;
-    for (; st < stop; st += W) {
-      if (!__all_sync(0xffffffffu, mbar_wait(my_bars + 8 * slot, (phases >> slot) & 1, kWaitLimit))) {
-        ok = false;
-        break;
-      }
-      phases ^= 1u << slot;
-      const uint8_t* base = smem + (slot * W + warp) * C::kStage;
+    for (int st = begin + warp; st < stop; st += W) {
+      cp_async_wait<S - 1>();
+      __syncwarp();
+      const uint8_t* base = ring + slot * (W * C::kStage);
       const uint8_t* kscales = base + 2 * C::kQuants;
       const uint8_t* vscales = kscales + C::kScales;
       uint32_t here = 0;
 #pragma unroll
       for (int s = 0; s < S; ++s) here = s == slot ? good[s] : here;
-      const bool whole = st * STG >= all_lo && st * STG + STG <= all_hi && __popc(here) == 4 * pieces;
+      const bool whole = st * STG >= all_lo && st * STG + STG <= all_hi && here == full;
 
-      // UN sub-tiles of 16 keys at a time: their chains of dependent instructions overlap
+      // UN sub-tiles of 16 keys at a time: their chains of dependent instructions overlap. Twice: with (careful) and
+      // without what only some calls and a sequence's ends need, so that the common loop is short and runs straight on.
+      auto steps = [&](auto careful) {
 #pragma unroll 1
       for (int u0 = 0; u0 < SUB; u0 += UN) {
         // ---- scores
@@ -535,17 +540,13 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float c[4];
-              if constexpr (QUAD && !SIGNED)
-                mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0].x, qb[nt][k][0].y, start[nt][k][0],
-                          start[nt][k][1], start[nt][k][2], start[nt][k][3]);
-              else
-                mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0].x, qb[nt][k][0].y, 0.f, 0.f, 0.f, 0.f);
+              mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][0].x, qb[nt][k][0].y, 0.f, 0.f, 0.f, 0.f);
               mma_16816(c, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][k][0].z, qb[nt][k][0].w);
               if constexpr (PARTS == 2) {
                 mma_16816(c, a[0][0], a[0][1], a[0][2], a[0][3], qb[nt][k][1].x, qb[nt][k][1].y);
                 mma_16816(c, a[1][0], a[1][1], a[1][2], a[1][3], qb[nt][k][1].z, qb[nt][k][1].w);
               }
-              if constexpr (!QUAD && !SIGNED) {
+              if constexpr (!SIGNED) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[e] += start[nt][k][e & 1];
               }
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
           lds_scales<NB>(vscales + rowA * NB * 2, dA[i]);  // from here on the value scales of the lane's two tokens
           lds_scales<NB>(vscales + (rowA + 8) * NB * 2, dB[i]);
         }
-        if (special) {
+        if (careful.value && special) {
           const float inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
 #pragma unroll
           for (int i = 0; i < UN; ++i)
@@ -570,13 +571,13 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
                 x[i][nt][e] = y - s_slope[r] * (float)abs(s_pos[r] - j);
               }
         }
-        if (!whole) {
+        if (careful.value && !whole) {
 #pragma unroll
           for (int i = 0; i < UN; ++i)
 #pragma unroll
             for (int e2 = 0; e2 < 2; ++e2) {
               const int row = (u0 + i) * 16 + tokA + e2 * 8, j = st * STG + row;
-              const bool read = (here >> (4 * (row / piece))) & 1;  // its page was read
+              const bool read = (here >> (row >> piece_shift)) & 1;  // its page was read
               bool seen = false;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
             top[nt][c] = fmaf(m, mul[nt][c], dlog);
             raise |= top[nt][c] > ref[nt][c] + 15.f;
           }
-        if (__any_sync(0xffffffffu, raise)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -730,20 +731,24 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
           }
         }
       }
+      };
+      if (whole && !special)
+        steps(std::false_type{});
+      else
+        steps(std::true_type{});
 
       // ---- the stage is read: refill it
       __syncwarp();
-      const uint32_t vote = __ballot_sync(0xffffffffu, id >= 0);
 #pragma unroll
       for (int s = 0; s < S; ++s)
-        if (s == slot) good[s] = vote;
-      if (st + S * W < stop) issue(st + S * W, slot, id, vote);
+        if (s == slot) good[s] = __ballot_sync(0xffffffffu, id >= 0);
+      copy(st + S * W, slot, id);
       id = page_of(st + (S + 1) * W);
       if (++slot == S) slot = 0;
     }
 
     // -------------------------------------------------------------- join the warps (in the ring's memory: all is read)
-    if (__syncthreads_or(!ok)) break;
+    __syncthreads();
     float* so = reinterpret_cast<float*>(smem);              // [W][R][D]
     float2* sm = reinterpret_cast<float2*>(so + W * R * D);  // [W][R] reference, sum
 #pragma unroll
@@ -797,16 +802,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     }
     pos += take, skip += take;
     if (skip == units) skip = 0, ++h;
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // these reads and writes before the next copies
     __syncthreads();
-  }
-  if (pos < end) {  // a wait gave up: no copy may be in flight when the CTA leaves
-    if (!ok && lane == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
-    for (int s = 0; s < S; ++s) {
-      mbar_wait(my_bars + 8 * s, 0, kWaitLimit);
-      mbar_wait(my_bars + 8 * s, 1, kWaitLimit);
-    }
-    join.first = -1;
   }
   if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
 }
@@ -869,6 +865,7 @@ static int launch_attention_as(const AttnParams& p, int sms, int64_t max_len, cu
   constexpr int kJoin = C::kWarps * NT * 8 * (NB * 32 + 2) * 4;  // the warps' results, in the ring's place
   constexpr int kSmem = C::kRing > kJoin ? C::kRing : kJoin;
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(kv_ctas_per_sm<FMT, NB, NT, PARTS>() <= kMaxCtasPerSm, "the workspace's parts");
   auto kernel = attention_kernel<FMT, NB, NT, PARTS>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));

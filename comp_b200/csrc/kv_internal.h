@@ -45,6 +45,6 @@ int kv_attention_q8_error(int* code, int clear);
 // Streaming kernels by format: `rows` is 8 or 16 query rows a tile, max_len bounds the lengths from above.
 int launch_attention_q4(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream);
 int launch_attention_q8(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream);
-constexpr int kMaxCtasPerSm = 4;
+constexpr int kMaxCtasPerSm = 3;  // the workspace holds parts for so many
 
 }  // namespace b2q
