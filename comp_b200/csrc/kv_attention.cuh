@@ -5,7 +5,7 @@
 // in one pass, with a running reference exponent `ref` and sum L for each row. The quants are whole numbers, so both
 // products run on the tensor cores (16x8x16, f16 in, f32 sums) with keys and values as the 16-row operand and 8 query
 // rows as the columns: nothing is padded, and no quant is rounded. What an operand's 16 bits hold:
-//   - keys: the quant's bits alone, i.e. the f16 subnormal q * 2^-24 (or q * 2^-20 for a nibble left in bits 4-7): one
+//   - keys (16-bit calls): the quant's bits alone, i.e. the f16 subnormal q * 2^-24 (or q * 2^-20 for a nibble left in bits 4-7): one
 //     AND unpacks two values. The offset -off * sum(Q) of a block is a constant of the row, added to the block's sum.
 //   - queries: scaled by a power of two to 2^13..2^14, so that 16-bit queries are exact; f32 queries take two parts.
 //     A block's scale dk (per key and block) multiplies the f32 sum of the block.
@@ -102,6 +102,24 @@ __device__ __forceinline__ void lds_scales(const uint8_t* at, float (&d)[NB]) {
     const __half2 h = *reinterpret_cast<const __half2*>(&w[b / 2]);
     d[b] = (b & 1) ? __high2float(h) : __low2float(h);
   }
+}
+
+// Quants as pairs of f16, from 16 bits each of a register: the nibbles of bits 0-3 or of bits 4-7 (worth 16 each), or the
+// bytes 0, 1 or 2, 3 of a word. SIGNED: the quant less its offset, as a normal number. Else the quant's bits alone, the
+// subnormal of 2^-24 times it, in one instruction; but the tensor cores take the exponent of a subnormal as 2^-14 where
+// they align a sum's terms, which costs up to 10 of the sum's bits (measured, f32 calls: error 5e-6, and 5e-7 so).
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) {
+  return SIGNED ? add_half2((w & 0x000f000fu) | 0x64006400u, 0xe408e408u) : w & 0x000f000fu;  // 1024 + q - 1032
+}
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) {
+  return SIGNED ? add_half2((w & 0x00f000f0u) | 0x64006400u, 0xe480e480u) : w & 0x00f000f0u;  // 1024 + 16 q - 1152
+}
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t two_bytes(uint32_t w, int upper) {
+  return SIGNED ? add_half2(__byte_perm(w, 0x64646464u, upper ? 0x4342 : 0x4140), 0xe480e480u)  // 1024 + u - 1152
+                : __byte_perm(w, 0, upper ? 0x4342 : 0x4140);
 }
 
 // 4 values at p (of type dtype, p counted in elements), 4-element aligned.
@@ -444,7 +462,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
         }
         if (l == 0) s_start[r * NB + k] = sum * (-kOff * 0x1p-24f);
         if (c == 0) {
-          float f = __int_as_float((127 + e2 - 13) << 23) * p.scale * 0x1p24f;
+          float f = __int_as_float((127 + e2 - 13) << 23) * p.scale * (SIGNED ? 1.f : 0x1p24f);
           if (p.softcap <= 0.f) f *= kLog2e;
           s_rowf[r] = f;
         }
@@ -522,19 +540,11 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
               if constexpr (FMT == 0) {
-                a[s][0] = (wA[k] >> (8 * s)) & 0x000f000fu, a[s][1] = (wB[k] >> (8 * s)) & 0x000f000fu;
-                a[s][2] = (wA[k] >> (8 * s)) & 0x00f000f0u, a[s][3] = (wB[k] >> (8 * s)) & 0x00f000f0u;
-                if constexpr (SIGNED) {
-                  a[s][0] = add_half2(a[s][0], 0x80088008u), a[s][1] = add_half2(a[s][1], 0x80088008u);
-                  a[s][2] = add_half2(a[s][2], 0x80808080u), a[s][3] = add_half2(a[s][3], 0x80808080u);
-                }
+                a[s][0] = low_nibbles<SIGNED>(wA[k] >> (8 * s)), a[s][1] = low_nibbles<SIGNED>(wB[k] >> (8 * s));
+                a[s][2] = high_nibbles<SIGNED>(wA[k] >> (8 * s)), a[s][3] = high_nibbles<SIGNED>(wB[k] >> (8 * s));
               } else {
-                a[s][0] = __byte_perm(wA[2 * k + s], 0, 0x4140), a[s][1] = __byte_perm(wB[2 * k + s], 0, 0x4140);
-                a[s][2] = __byte_perm(wA[2 * k + s], 0, 0x4342), a[s][3] = __byte_perm(wB[2 * k + s], 0, 0x4342);
-                if constexpr (SIGNED) {
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) a[s][j] = add_half2(a[s][j], 0x80808080u);
-                }
+                a[s][0] = two_bytes<SIGNED>(wA[2 * k + s], 0), a[s][1] = two_bytes<SIGNED>(wB[2 * k + s], 0);
+                a[s][2] = two_bytes<SIGNED>(wA[2 * k + s], 1), a[s][3] = two_bytes<SIGNED>(wB[2 * k + s], 1);
               }
             }
 #pragma unroll
@@ -677,25 +687,18 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
               // the 16 bits of both tokens of a pair: values 2g, 16+2g, 2g+1, 17+2g in nibbles 0..3
               const uint32_t lo = __byte_perm(v[0][k / 2], v[1][k / 2], (k & 1) ? 0x7632 : 0x5410);
               const uint32_t hi = __byte_perm(v[2][k / 2], v[3][k / 2], (k & 1) ? 0x7632 : 0x5410);
-              a[0][0] = lo & 0x000f000fu, a[0][1] = (lo >> 8) & 0x000f000fu;
-              a[0][2] = hi & 0x000f000fu, a[0][3] = (hi >> 8) & 0x000f000fu;
-              a[1][0] = lo & 0x00f000f0u, a[1][1] = (lo >> 8) & 0x00f000f0u;
-              a[1][2] = hi & 0x00f000f0u, a[1][3] = (hi >> 8) & 0x00f000f0u;
+              a[0][0] = low_nibbles<SIGNED>(lo), a[0][1] = low_nibbles<SIGNED>(lo >> 8);
+              a[0][2] = low_nibbles<SIGNED>(hi), a[0][3] = low_nibbles<SIGNED>(hi >> 8);
+              a[1][0] = high_nibbles<SIGNED>(lo), a[1][1] = high_nibbles<SIGNED>(lo >> 8);
+              a[1][2] = high_nibbles<SIGNED>(hi), a[1][3] = high_nibbles<SIGNED>(hi >> 8);
             } else {
               // bytes i of both tokens of a pair: values 4g + i
 #pragma unroll
               for (int mt = 0; mt < 2; ++mt) {
                 const uint32_t lo = __byte_perm(v[0][k], v[1][k], mt ? 0x7362 : 0x5140);
                 const uint32_t hi = __byte_perm(v[2][k], v[3][k], mt ? 0x7362 : 0x5140);
-                a[mt][0] = __byte_perm(lo, 0, 0x4140), a[mt][1] = __byte_perm(lo, 0, 0x4342);
-                a[mt][2] = __byte_perm(hi, 0, 0x4140), a[mt][3] = __byte_perm(hi, 0, 0x4342);
-              }
-            }
-            if constexpr (SIGNED) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                a[0][j] = add_half2(a[0][j], FMT == 0 ? 0x80088008u : 0x80808080u);
-                a[1][j] = add_half2(a[1][j], 0x80808080u);
+                a[mt][0] = two_bytes<SIGNED>(lo, 0), a[mt][1] = two_bytes<SIGNED>(lo, 1);
+                a[mt][2] = two_bytes<SIGNED>(hi, 0), a[mt][3] = two_bytes<SIGNED>(hi, 1);
               }
             }
 #pragma unroll
@@ -766,7 +769,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
         for (int k = 0; k < NB; ++k)
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            const float f = FMT == 0 && mt ? 0x1p20f : 0x1p24f;  // the unit of the quants' bits
+            const float f = (FMT == 0 && mt ? 0.0625f : 1.f) * (SIGNED ? 1.f : 0x1p24f);  // the operands' unit
             *reinterpret_cast<float2*>(dst + 32 * k + (FMT == 0 ? 16 : 2) * mt) =
                 make_float2(o[nt][k][mt][c] * f, o[nt][k][mt][2 + c] * f);
           }
