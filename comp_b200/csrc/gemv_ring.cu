@@ -60,7 +60,8 @@ extern "C" int b2q_device_error(int* code, int clear) {
     if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_device_error: %s", cudaGetErrorString(e));
   }
   // the words of the KV cache's and the attention's translation units; the first that is set is reported
-  for (auto read : {kv_cache_error, kv_attention_q4_error, kv_attention_q8_error}) {
+  for (auto read : {kv_cache_error, kv_attention_q4_error, kv_attention_q8_error, kv_attention_tc_q4_error,
+                    kv_attention_tc_q8_error}) {
     int word = 0;
     const int rc = read(&word, clear);
     if (rc) return rc;

@@ -4,21 +4,29 @@
 namespace b2q {
 
 struct AttnPlan {
+  bool tc;  // the tensor-core kernels
   int rows, row_tiles, sms;
   size_t part_m, joins, bytes;  // workspace: partial outputs, then references and sums, then the joins
 };
 
-// Rows of a tile: 8, or 16 where more have to read the cache anyway (heads of 256 leave registers for 8).
+// 16-bit calls with at least kTcLeastRows query rows a sequence and KV head take the tensor-core kernels. Else the rows of
+// a tile are 8, or 16 where more have to read the cache anyway (heads of 256 leave registers for 8).
+constexpr int kTcLeastRows = 64;
+
 static AttnPlan plan_attention(const b2q_kv_cache& c, const b2q_attention_args& a) {
   AttnPlan pl;
   const int group = a.q_heads / c.heads;
   const int64_t max_q = !a.cu_q ? 1 : (a.max_q > 0 && a.max_q < a.T ? a.max_q : a.T);
   const int64_t rows = max_q * group;
-  pl.rows = rows > 8 && c.dim != 256 ? 16 : 8;
+  pl.tc = rows >= kTcLeastRows && a.dtype != B2Q_DTYPE_F32;
+  if (pl.tc)
+    pl.rows = c.dim == 256 ? kTcRows / 2 : kTcRows;
+  else
+    pl.rows = rows > 8 && c.dim != 256 ? 16 : 8;
   pl.row_tiles = (int)((rows + pl.rows - 1) / pl.rows);
   DeviceInfo di;
   pl.sms = device_info(&di) == B2Q_OK ? di.sms : 148;
-  const size_t ctas = (size_t)pl.sms * kMaxCtasPerSm;
+  const size_t ctas = (size_t)pl.sms * (pl.tc ? 1 : kMaxCtasPerSm);
   pl.part_m = 2 * ctas * pl.rows * c.dim * 4;
   pl.joins = pl.part_m + 2 * ctas * pl.rows * 8;
   pl.bytes = pl.joins + ctas * sizeof(AttnJoin);
@@ -93,6 +101,9 @@ int b2q_attention(const b2q_kv_cache* cache, const b2q_attention_args* args, voi
   while ((1 << p.page_shift) < c.page) ++p.page_shift;
   p.row_tiles = pl.row_tiles, p.window = a.window, p.dtype = a.dtype;
   p.scale = a.scale, p.softcap = a.softcap;
+  if (pl.tc)
+    return c.fmt == B2Q_FMT_Q4_0 ? launch_attention_tc_q4(p, c.dim, pl.sms, (cudaStream_t)stream)
+                                 : launch_attention_tc_q8(p, c.dim, pl.sms, (cudaStream_t)stream);
   const int64_t held = a.table_pages * c.page, max_len = a.max_len > 0 && a.max_len < held ? a.max_len : held;
   return c.fmt == B2Q_FMT_Q4_0 ? launch_attention_q4(p, c.dim, pl.rows, pl.sms, max_len, (cudaStream_t)stream)
                                : launch_attention_q8(p, c.dim, pl.rows, pl.sms, max_len, (cudaStream_t)stream);

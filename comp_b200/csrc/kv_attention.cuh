@@ -217,6 +217,67 @@ __device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
 
 __device__ __forceinline__ int tile_units(Span s) { return s.count ? s.count + kTileCost : 0; }
 
+// The plan: every CTA an equal share of all stages. Entries (sequence, row tile) have their stages, after kTileCost units
+// without any, once a KV head; a CTA's share is [pos, end) of their run, at least `least` units (unless none are left),
+// and begins `skip` units into the tile of (entry, head). All W warps call it; the scratch is read until the barrier
+// that ends it.
+struct Share {
+  int64_t per, pos, end;
+  int entry, head, skip;
+};
+template <int W>
+struct ShareScratch {
+  int64_t scan[W];
+  int entry, head, skip;
+};
+template <int STG, int R, int W>
+__device__ __forceinline__ Share plan_share(const AttnParams& p, int least, ShareScratch<W>& scratch) {
+  constexpr int kThreads = W * 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int entries = p.batch * p.row_tiles, chunk = (entries + kThreads - 1) / kThreads;
+  const int e0 = min(entries, (int)threadIdx.x * chunk), e1 = min(entries, e0 + chunk);
+  Share s;
+  int64_t mine = 0;
+  for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
+  mine *= p.heads;
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) scratch.scan[warp] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w < warp) upto += scratch.scan[w];
+    total += scratch.scan[w];
+  }
+  if (total < (int64_t)1 << 31)
+    s.per = max((int)((uint32_t)(total + gridDim.x - 1) / gridDim.x), least);
+  else
+    s.per = (total + gridDim.x - 1) / gridDim.x;
+  s.pos = s.per * blockIdx.x;
+  s.end = min(total, s.pos + s.per);
+  if (s.pos < s.end && s.pos >= upto - mine && s.pos < upto) {  // the thread whose entries hold the beginning
+    int64_t off = s.pos - (upto - mine);
+    for (int e = e0; e < e1; ++e) {
+      const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
+      if (off < (int64_t)count * p.heads) {
+        int h = 0;
+        while (off >= count) off -= count, ++h;
+        scratch.entry = e, scratch.head = h, scratch.skip = (int)off;
+        break;
+      }
+      off -= (int64_t)count * p.heads;
+    }
+  }
+  __syncthreads();
+  s.entry = scratch.entry, s.head = scratch.head, s.skip = scratch.skip;
+  return s;
+}
+
 // FMT 0 (q4_0) or 2 (q8_0), NB blocks a head, NT tiles of 8 query rows, PARTS f16 parts of queries and weights.
 template <int FMT, int NB, int NT, int PARTS>
 __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) attention_kernel(const AttnParams p) {
@@ -226,9 +287,8 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   constexpr float kOff = FMT == 0 ? 8.f : 128.f;
   constexpr int UN = SUB % 2 == 0 && NB * NT <= 4 && PARTS == 1 ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];  // [stage][warp] ring; the last stage holds the queries at first
-  __shared__ int s_lo[R], s_hi[R], s_pos[R], s_out[R], s_top[R], s_entry, s_head, s_skip;
+  __shared__ int s_lo[R], s_hi[R], s_pos[R], s_out[R], s_top[R];
   __shared__ float s_slope[R], s_rowf[R];
-  __shared__ int64_t s_scan[W];
   __shared__ uint32_t s_off[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
@@ -236,57 +296,15 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   if (threadIdx.x < 8) s_off[threadIdx.x] = threadIdx.x < 4 ? 0x80088008u : 0x80808080u;
   pdl_wait_then_trigger();
 
-  // ---------------------------------------------------------------- the plan: every CTA an equal share of all stages
-  // entries (sequence, row tile) have their stages, after kTileCost units without any, once a KV head; a CTA's share is
-  // [pos, end) of their run
-  const int entries = p.batch * p.row_tiles;
-  int64_t per, pos, end;
-  {
-    const int chunk = (entries + 127) / 128, e0 = min(entries, (int)threadIdx.x * chunk), e1 = min(entries, e0 + chunk);
-    int64_t mine = 0;
-    for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
-    mine *= p.heads;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    if (lane == 31) s_scan[warp] = upto;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      if (w < warp) upto += s_scan[w];
-      total += s_scan[w];
-    }
-    // a share is at least a stage for each warp
-    if (total < (int64_t)1 << 31)
-      per = max((int)((uint32_t)(total + gridDim.x - 1) / gridDim.x), W);
-    else
-      per = (total + gridDim.x - 1) / gridDim.x;
-    pos = per * blockIdx.x;
-    end = min(total, pos + per);
-    if (pos >= end) {
-      if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
-      return;
-    }
-    if (pos >= upto - mine && pos < upto) {
-      int64_t off = pos - (upto - mine);
-      for (int e = e0; e < e1; ++e) {
-        const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
-        if (off < (int64_t)count * p.heads) {
-          int h = 0;
-          while (off >= count) off -= count, ++h;
-          s_entry = e, s_head = h, s_skip = (int)off;
-          break;
-        }
-        off -= (int64_t)count * p.heads;
-      }
-    }
+  __shared__ ShareScratch<W> plan;
+  const Share share = plan_share<STG, R, W>(p, W, plan);
+  const int64_t per = share.per, end = share.end;
+  int64_t pos = share.pos;
+  if (pos >= end) {
+    if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
+    return;
   }
-  __syncthreads();
-  int entry = s_entry, h = s_head, skip = s_skip;
+  int entry = share.entry, h = share.head, skip = share.skip;
   AttnJoin join = {-1, 0, 0, 0, 0};
 
   const int page = 1 << p.page_shift, piece_shift = min(p.page_shift, __ffs(STG) - 1);

@@ -1,0 +1,591 @@
+// Attention over the quantized cache for many query rows (prompt chunks): the fifth-generation tensor cores.
+//
+// A CTA works on up to 256 rows (two tiles of 128) of one KV head against blocks of 128 keys. Four roles:
+//   - a warpgroup unpacks the block's keys and values to f16 once for all rows, into tiles of core matrices (8 rows of 16
+//     bytes, K-major, no swizzle): keys as [8 values of a key][key], values transposed, as [8 keys of a column][column];
+//   - one thread issues the products: S = Q K^T into tensor memory, and O += P V with P read from tensor memory;
+//   - two warpgroups, a row a thread, turn S into P (f16, in S's own columns) and keep the row's reference exponent and
+//     sum in f32; the other tile's products run meanwhile. The reference follows the row's maximum only when that has
+//     grown by more than 2^8: then the thread rescales its row of O, which no product is using at that time.
+// Queries are scaled by a power of two a row (exact for 16-bit queries) and take the order of the keys' packed words, so
+// that one word of a key becomes one 16-byte chunk of its operand. Keys and values are rounded to f16 (11 bits), weights
+// to f16; values past f16's range (65504) come out as NaN, for every row that sees the key.
+//
+// What bounds it: 128 x 128 keys and rows of 128 values take 2 x 512 cycles on the tensor cores and 1024 on the units
+// that compute 2^x (16 a cycle), and the two tiles overlap the one with the other.
+#pragma once
+
+#include "kv_attention.cuh"
+
+namespace b2q {
+
+template <int FMT, int NB>
+struct TcTile {
+  static constexpr int D = NB * 32;
+  static constexpr int kRow = NB * (FMT == 0 ? 16 : 32);  // quant bytes of a token's row
+  static constexpr int MT = NB == 8 ? 1 : 2;              // row tiles: tensor memory holds O (D) and S (128) of each
+  static constexpr int kBufs = NB == 8 ? 1 : 2;           // key and value tiles in shared memory
+  static constexpr int kRows = MT * 128, kKeys = 128;
+  static constexpr int kQ = 128 * D * 2, kTile = 128 * D * 2;
+  static constexpr int kSmem = MT * kQ + 2 * kBufs * kTile;
+  static constexpr int kSoftmaxWarps = MT * 4, kWarps = MT * 4 + 5;  // + 4 unpacking, 1 issuing
+  static constexpr uint32_t kS = 256;                     // column of S (and P) of tile 0; O is at 0
+};
+
+namespace tc {
+
+// K-major, no swizzle: the next 16 bytes of K are `lbo` bytes on, the next 8 rows 128
+__device__ __forceinline__ uint64_t smem_desc_kmajor(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) |
+         ((uint64_t)1 << 46);
+}
+// kind::f16: f32 accumulator, A and B f16, both K-major, M = 128, N = n
+__device__ __forceinline__ uint32_t instr_desc_f16(int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+#define B2Q_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), \
+                     "=r"(v[i + 6]), "=r"(v[i + 7])
+#define B2Q_I8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), \
+                     "r"(v[i + 6]), "r"(v[i + 7])
+#define B2Q_RW8(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]), \
+                      "+r"(v[i + 6]), "+r"(v[i + 7])
+// 32 consecutive columns of this thread's lane, without waiting
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : B2Q_R8(v, 0), B2Q_R8(v, 8), B2Q_R8(v, 16), B2Q_R8(v, 24)
+      : "r"(taddr));
+}
+// tcgen05.wait::ld that names the registers of a load, so that no use of them is scheduled above it
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : B2Q_RW8(v, 0), B2Q_RW8(v, 8), B2Q_RW8(v, 16), B2Q_RW8(v, 24)
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::B2Q_I8(v, 0),
+      B2Q_I8(v, 8), B2Q_I8(v, 16), B2Q_I8(v, 24), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::B2Q_I8(
+          v, 0),
+      B2Q_I8(v, 8), "r"(taddr)
+      : "memory");
+}
+#undef B2Q_R8
+#undef B2Q_I8
+#undef B2Q_RW8
+
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// generic writes to shared memory before the tensor cores' reads of it
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+}  // namespace tc
+
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// (1024 + 16 q) / 16 - 72 = q - 8
+__device__ __forceinline__ uint32_t high_nibbles_int(uint32_t w) {
+  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u, s = 0x2c002c00u, o = 0xd480d480u;
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&s),
+                            *reinterpret_cast<const __half2*>(&o));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// N bytes (a multiple of 2) of global memory into 32-bit words; 16, 8, 4 or 2 at a time as N allows (N aligned).
+template <int N>
+__device__ __forceinline__ void ldg_bytes(const uint8_t* at, uint32_t (&w)[(N + 3) / 4]) {
+  if constexpr (N % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(at + i));
+      w[i / 4] = v.x, w[i / 4 + 1] = v.y, w[i / 4 + 2] = v.z, w[i / 4 + 3] = v.w;
+    }
+  } else if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(at + i));
+      w[i / 4] = v.x, w[i / 4 + 1] = v.y;
+    }
+  } else if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) w[i / 4] = __ldg(reinterpret_cast<const uint32_t*>(at + i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint32_t v = __ldg(reinterpret_cast<const uint16_t*>(at + i));
+      w[i / 4] = (i & 2) ? (w[i / 4] | v << 16) : v;
+    }
+  }
+}
+
+template <int FMT, int NB>
+__global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_kernel(const AttnParams p) {
+  using C = TcTile<FMT, NB>;
+  constexpr int D = C::D, MT = C::MT, KB = C::kBufs, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
+  extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB], values [KB]
+  __shared__ uint64_t b_kfull[KB], b_kempty[KB], b_vfull[KB], b_vempty[KB], b_s[MT], b_p[MT], b_o[MT], b_q, b_end;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ ShareScratch<C::kWarps> plan;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // The next kernel may start only once this CTA has its tensor memory: one that took tensor memory first and then waited
+  // for this grid would leave both waiting.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Share share = plan_share<STG, R, C::kWarps>(p, 1, plan);
+  int64_t pos = share.pos;
+  if (pos >= share.end) {
+    if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
+    return;
+  }
+  int entry = share.entry, h = share.head, skip = share.skip;
+  AttnJoin join = {-1, 0, 0, 0, 0};
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KB; ++i) {
+      mbar_init(smem_addr(&b_kfull[i]), 128), mbar_init(smem_addr(&b_vfull[i]), 128);
+      mbar_init(smem_addr(&b_kempty[i]), 1), mbar_init(smem_addr(&b_vempty[i]), 1);
+    }
+    for (int i = 0; i < MT; ++i) {
+      mbar_init(smem_addr(&b_s[i]), 1), mbar_init(smem_addr(&b_p[i]), 128), mbar_init(smem_addr(&b_o[i]), 1);
+    }
+    mbar_init(smem_addr(&b_q), SW * 32), mbar_init(smem_addr(&b_end), 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = s_tmem;
+  const uint32_t q_smem = smem_addr(smem), k_smem = q_smem + MT * C::kQ, v_smem = k_smem + KB * C::kTile;
+  // a wait that ran out ends the role's work, and the kernel at the end of the tile: every later wait is skipped
+  bool ok = true;
+  auto wait_one = [&](uint64_t* bar, uint32_t phase) {  // by one thread
+    if (ok && !mbar_wait(smem_addr(bar), phase & 1, kWaitLimit)) ok = false, atomicExch(&s_abort, 1);
+    return ok;
+  };
+  auto wait = [&](uint64_t* bar, uint32_t phase) {  // by a whole warp, which goes on or stops as one
+    if (ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_addr(bar), phase & 1, kWaitLimit));
+      if (!ok) atomicExch(&s_abort, 1);
+    }
+    return ok;
+  };
+
+  uint32_t blocks = 0, done_tiles[2] = {0, 0}, done_blocks[2] = {0, 0}, segments = 0;  // so far: the barriers' phases
+  while (pos < share.end) {
+    // -------------------------------------------------------------- the next tile of the share, as in the other kernel
+    const int b = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - b * p.row_tiles;
+    const Span span = tile_span<STG, R>(p, b, rt);
+    if (h == p.heads || span.count == 0) {
+      ++entry, h = 0;
+      continue;
+    }
+    const int units = tile_units(span), take = (int)min((int64_t)(units - skip), share.end - pos);
+    const int from = max(0, skip - kTileCost), to = max(0, skip + take - kTileCost);
+    if (to == from) {
+      pos += take, skip += take;
+      if (skip == units) skip = 0, ++h;
+      continue;
+    }
+    const Sequence q = sequence(p, b);
+    const int rows = q.n * p.group - rt * R;  // rows from this tile on (at least 1)
+    if (p.lens[b] > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
+    const int begin = span.first + from, n = to - from, tiles = MT == 1 || rows <= 128 ? 1 : 2;
+
+    if (warp < SW) {
+      // ------------------------------------------------------------ softmax: a thread owns a row
+      const int tile = warp >> 2, r = tile * 128 + (warp & 3) * 32 + lane, rr = rt * R + r;
+      const bool there = r < rows;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t col_s = tmem + lanes + C::kS + tile * 128, col_o = tmem + lanes + tile * 128;
+      int lo = 0, hi = 0, where = 0;
+      float mul = 1.f, rowf = 0.f, slope = 0.f;
+      int64_t out_row = 0;
+      const bool special = p.softcap > 0.f || p.slopes != nullptr;
+      uint8_t* my_q = smem + tile * C::kQ + (r & 127) * 16;
+      if (there) {
+        const int i = p.cu_q ? rr / p.group : 0, head = h * p.group + (rr - i * p.group);
+        const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
+        lo = s.lo, hi = s.hi, where = s.pos;
+        out_row = (q.q0 + i) * p.q_heads + head;
+        slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;
+        const int64_t src = (q.q0 + i) * p.q_st + (int64_t)head * p.q_sh;
+        float top = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < D; c += 4) {
+          float v[4];
+          load4_as(p.q, src + c, p.dtype, v);
+          top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        }
+        // to 2^6 .. 2^7: products with keys of up to 2^16 stay far below f32's range, and 16-bit queries exact
+        const int e2 = max(-100, (__float_as_int(top) >> 23) - 127);
+        const float up = __int_as_float((127 + 6 - e2) << 23);
+        rowf = __int_as_float((127 + e2 - 6) << 23) * p.scale;
+        if (p.softcap <= 0.f) rowf *= kLog2e;
+        mul = rowf;
+#pragma unroll 2
+        for (int w = 0; w < NB * 4; ++w) {  // chunk w = word (t, block) of a packed key: its 8 values in its order
+          const int t = w / NB, k = w - t * NB;
+          float a[4], z[4];
+          load4_as(p.q, src + 32 * k + (FMT == 0 ? 4 : 8) * t, p.dtype, a);
+          load4_as(p.q, src + 32 * k + (FMT == 0 ? 16 + 4 * t : 8 * t + 4), p.dtype, z);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] *= up, z[e] *= up;
+          uint4 x;
+          if (FMT == 0)
+            x = make_uint4(pack_half2(a[0], a[2]), pack_half2(z[0], z[2]), pack_half2(a[1], a[3]), pack_half2(z[1], z[3]));
+          else
+            x = make_uint4(pack_half2(a[0], a[1]), pack_half2(a[2], a[3]), pack_half2(z[0], z[1]), pack_half2(z[2], z[3]));
+          *reinterpret_cast<uint4*>(my_q + w * 2048) = x;
+        }
+      } else if (tile < tiles) {
+#pragma unroll 2
+        for (int w = 0; w < NB * 4; ++w) *reinterpret_cast<uint4*>(my_q + w * 2048) = make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
+      tc::fence_async_smem();
+      tc::arrive(smem_addr(&b_q));
+      if (tile < tiles) {
+        float ref = kNoRef, sum = 0.f;
+        for (int j = 0; j < n; ++j) {
+          if (!wait(&b_s[tile], done_blocks[tile] + j)) break;
+          tc::fence_after();
+          const int kb = (begin + j) * STG;
+          const bool careful = special || __any_sync(0xffffffffu, kb < lo || kb + STG > hi);
+          const float scale = careful ? 1.f : mul;
+          // scores as exponents of 2, and -inf where masked
+          auto finish = [&](uint32_t (&v)[32], int c) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x = __uint_as_float(v[e]) * rowf;
+              const int key = kb + c + e;
+              if (special) {
+                if (p.softcap > 0.f) x = soft_cap(x, p.softcap, 1.f / p.softcap) * kLog2e;
+                x -= slope * (float)abs(where - key);
+              }
+              v[e] = __float_as_uint(key >= lo && key < hi ? x : -INFINITY);
+            }
+          };
+          uint32_t v[32];
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < STG; c += 32) {
+            tc::tmem_ld32_nowait(col_s + c, v);
+            tc::tmem_wait_ld32(v);
+            if (careful) finish(v, c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+          }
+          top *= scale;
+          if (__any_sync(0xffffffffu, top > ref + 8.f)) {
+            const float now = top > ref + 8.f ? top : ref, f = exp2_approx(ref - now);
+            ref = now, sum *= f;
+            if (j > 0) {  // the block before is in O already: its product ended before this block's scores
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                tc::tmem_ld32_nowait(col_o + c, v);
+                tc::tmem_wait_ld32(v);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                tc::tmem_st32(col_o + c, v);
+              }
+            }
+          }
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+          for (int c = 0; c < STG; c += 32) {
+            tc::tmem_ld32_nowait(col_s + c, v);
+            tc::tmem_wait_ld32(v);
+            if (careful) finish(v, c);
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float a = exp2_approx(fmaf(__uint_as_float(v[e]), scale, -ref));
+              const float z = exp2_approx(fmaf(__uint_as_float(v[e + 1]), scale, -ref));
+              s0 += a, s1 += z;
+              w[e / 2] = pack_half2(a, z);
+            }
+            tc::tmem_st16(col_s + c / 2, w);  // columns of S that have been read
+          }
+          sum += s0 + s1;
+          tc::tmem_wait_st();
+          tc::fence_before();
+          tc::arrive(smem_addr(&b_p[tile]));
+        }
+        // ---------------------------------------------------------- the row's result, or this share's part of it
+        if (wait(&b_o[tile], done_tiles[tile])) {
+          tc::fence_after();
+          const bool begun = from > 0, done = to == span.count;
+          const int part = 2 * (int)blockIdx.x + (begun ? 0 : 1);
+          const bool final = !begun && done;
+          const float inv = !final ? 1.f : (sum > 0.f || sum != sum ? __fdividef(1.f, sum) : 0.f);
+          float* dst = p.part_o + ((int64_t)part * R + r) * D;
+#pragma unroll 1
+          for (int k = 0; k < NB; ++k) {
+            uint32_t v[32];
+            tc::tmem_ld32_nowait(col_o + k * 32, v);
+            tc::tmem_wait_ld32(v);
+            if (there) {
+              // columns of a block: q4_0 [nibble][g] of values 2g, 16+2g, 2g+1, 17+2g; q8_0 [i][g] of values 4g + i
+              float y[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int g = e & 7, i = e >> 3;
+                y[FMT == 0 ? 2 * g + (i >> 1) + 16 * (i & 1) : 4 * g + i] = __uint_as_float(v[e]) * inv;
+              }
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                if (!final)
+                  store4(dst + k * 32 + e, y[e], y[e + 1], y[e + 2], y[e + 3]);
+                else if (p.dtype == B2Q_DTYPE_F16)
+                  store4(static_cast<__half*>(p.out) + out_row * D + k * 32 + e, y[e], y[e + 1], y[e + 2], y[e + 3]);
+                else
+                  store4(static_cast<__nv_bfloat16*>(p.out) + out_row * D + k * 32 + e, y[e], y[e + 1], y[e + 2],
+                         y[e + 3]);
+              }
+            }
+          }
+          if (there && !final) p.part_m[part * R + r] = make_float2(ref, sum);
+          if (there && final && p.lse) p.lse[out_row] = (ref + log2f(sum)) * kLn2;
+          tc::fence_before();
+        }
+      }
+    } else if (warp < SW + 4) {
+      // ------------------------------------------------------------ unpacking: a thread a key, then 8 keys' columns
+      const int th = threadIdx.x - SW * 32, kg = th >> 3, g = th & 7;
+      const int32_t* table = p.table + (int64_t)b * p.table_stride;
+      constexpr int UV = FMT == 0 ? NB * 2 : NB * 4;  // bytes of a value unit's slice of a row
+      // the row (of heads' tokens) of a token of this KV head, or -1
+      auto row_of = [&](int tok) -> int64_t {
+        if (tok >= q.len) return -1;
+        const int id = table[tok >> p.page_shift];
+        if (id < 0 || id >= p.pages) {
+          atomicCAS(&g_device_error, 0, kErrPage);
+          return -1;
+        }
+        return ((((int64_t)id * p.heads) + h) << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
+      };
+      uint32_t kw[C::kRow / 4], ksc[(NB + 1) / 2], kvs[(NB + 1) / 2];  // a key's row, its scales, its value's scales
+      uint32_t vw[8][(UV + 3) / 4], vsc[8][(NB + 1) / 2];
+      bool read_k = false;
+      int read_v = 0;  // of the 8 keys
+      auto load_k = [&](int j) {
+        const int64_t row = j < n ? row_of((begin + j) * STG + th) : -1;
+        read_k = row >= 0;
+        if (read_k) {
+          ldg_bytes<C::kRow>(p.kq + row * C::kRow, kw);
+          ldg_bytes<NB * 2>(reinterpret_cast<const uint8_t*>(p.ks + row * NB), ksc);
+          ldg_bytes<NB * 2>(reinterpret_cast<const uint8_t*>(p.vs + row * NB), kvs);
+        }
+      };
+      auto load_v = [&](int j) {
+        const int tok = (begin + j) * STG + kg * 8;
+        const int64_t row = j < n ? row_of(tok) : -1;
+        read_v = row >= 0 ? min(8, q.len - tok) : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < read_v) {
+            ldg_bytes<UV>(p.vq + (row + i) * C::kRow + g * UV, vw[i]);
+            ldg_bytes<NB * 2>(reinterpret_cast<const uint8_t*>(p.vs + (row + i) * NB), vsc[i]);
+          }
+      };
+      // the largest magnitude of a scale whose values all fit f16; others make their key NaN for the rows that see it
+      const uint32_t most = FMT == 0 ? 0x6ffeu : 0x5ffcu;  // 8 * 8184 < 65504, 128 * 511 < 65504
+      load_k(0);
+      load_v(0);
+      for (int j = 0; j < n && ok; ++j) {
+        const uint32_t at = blocks + j;
+        const int buf = at % KB;
+        if (at >= KB && !wait(&b_kempty[buf], at / KB - 1)) break;
+        uint8_t* kt = smem + MT * C::kQ + buf * C::kTile + th * 16;
+        bool fits = true;
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+          fits &= !read_k || ((kvs[k / 2] >> (16 * (k & 1))) & 0x7fffu) <= most;
+#pragma unroll
+        for (int w = 0; w < NB * 4; ++w) {  // word w = (t, block)
+          const int k = w % NB;
+          const uint32_t d = __byte_perm(ksc[k / 2], 0, (k & 1) ? 0x3232 : 0x1010);
+          uint4 x;
+          if constexpr (FMT == 0) {
+            x.x = mul_half2(low_nibbles<true>(kw[w]), d), x.y = mul_half2(high_nibbles_int(kw[w]), d);
+            x.z = mul_half2(low_nibbles<true>(kw[w] >> 8), d), x.w = mul_half2(high_nibbles_int(kw[w] >> 8), d);
+          } else {
+            x.x = mul_half2(two_bytes<true>(kw[2 * w], 0), d), x.y = mul_half2(two_bytes<true>(kw[2 * w], 1), d);
+            x.z = mul_half2(two_bytes<true>(kw[2 * w + 1], 0), d), x.w = mul_half2(two_bytes<true>(kw[2 * w + 1], 1), d);
+          }
+          if (!read_k) x = make_uint4(0, 0, 0, 0);
+          if (!fits) x = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+          *reinterpret_cast<uint4*>(kt + w * 2048) = x;
+        }
+        load_k(j + 1);
+        tc::fence_async_smem();
+        tc::arrive(smem_addr(&b_kfull[buf]));
+
+        if (at >= KB && !wait(&b_vempty[buf], at / KB - 1)) break;
+        uint8_t* vt = smem + MT * C::kQ + (KB + buf) * C::kTile + kg * (D * 16) + g * 16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // keys that are not there, or do not fit, are zeros
+          bool use = i < read_v;
+#pragma unroll
+          for (int k = 0; k < NB; ++k) use &= ((vsc[i][k / 2] >> (16 * (k & 1))) & 0x7fffu) <= most;
+          if (!use) {
+#pragma unroll
+            for (int k = 0; k < (NB + 1) / 2; ++k) vsc[i][k] = 0;
+#pragma unroll
+            for (int k = 0; k < (UV + 3) / 4; ++k) vw[i][k] = 0;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          uint32_t x[4][4];  // [column of the unit][pair of keys]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t d = __byte_perm(vsc[2 * i][k / 2], vsc[2 * i + 1][k / 2], (k & 1) ? 0x7632 : 0x5410);
+            if constexpr (FMT == 0) {
+              const uint32_t w = __byte_perm(vw[2 * i][k / 2], vw[2 * i + 1][k / 2], (k & 1) ? 0x7632 : 0x5410);
+              x[0][i] = mul_half2(low_nibbles<true>(w), d), x[1][i] = mul_half2(high_nibbles_int(w), d);
+              x[2][i] = mul_half2(low_nibbles<true>(w >> 8), d), x[3][i] = mul_half2(high_nibbles_int(w >> 8), d);
+            } else {
+              const uint32_t lo = __byte_perm(vw[2 * i][k], vw[2 * i + 1][k], 0x5140);
+              const uint32_t hi = __byte_perm(vw[2 * i][k], vw[2 * i + 1][k], 0x7362);
+              x[0][i] = mul_half2(two_bytes<true>(lo, 0), d), x[1][i] = mul_half2(two_bytes<true>(lo, 1), d);
+              x[2][i] = mul_half2(two_bytes<true>(hi, 0), d), x[3][i] = mul_half2(two_bytes<true>(hi, 1), d);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(vt + (k * 32 + c * 8) * 16) = make_uint4(x[c][0], x[c][1], x[c][2], x[c][3]);
+        }
+        load_v(j + 1);
+        tc::fence_async_smem();
+        tc::arrive(smem_addr(&b_vfull[buf]));
+      }
+    } else if (lane == 0) {
+      // ------------------------------------------------------------ the products, issued in the order in which they run
+      const uint32_t is = tc::instr_desc_f16(STG), io = tc::instr_desc_f16(D);
+      const uint64_t dq = tc::smem_desc_kmajor(q_smem, 2048), dk = tc::smem_desc_kmajor(k_smem, 2048);
+      const uint64_t dv = tc::smem_desc_kmajor(v_smem, D * 16);
+      auto scores = [&](int tile, uint32_t at) {
+        const uint64_t a = dq + (uint64_t)((tile * C::kQ) >> 4), z = dk + (uint64_t)(((at % KB) * C::kTile) >> 4);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          tc::mma_f16_ss(tmem + C::kS + tile * 128, a + s * (4096 >> 4), z + s * (4096 >> 4), is, s > 0);
+        tc::mma_commit(smem_addr(&b_s[tile]));
+      };
+      if (wait_one(&b_q, segments) && wait_one(&b_kfull[blocks % KB], blocks / KB)) {
+        tc::fence_after();
+        for (int i = 0; i < tiles; ++i) scores(i, blocks);
+        tc::mma_commit(smem_addr(&b_kempty[blocks % KB]));
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t at = blocks + j;
+          for (int i = 0; i < tiles; ++i) {
+            if (i == 0 && !wait_one(&b_vfull[at % KB], at / KB)) break;
+            if (!wait_one(&b_p[i], done_blocks[i] + j)) break;
+            tc::fence_after();
+            const uint64_t z = dv + (uint64_t)(((at % KB) * C::kTile) >> 4);
+#pragma unroll
+            for (int s = 0; s < STG / 16; ++s)
+              tc::mma_f16_ts(tmem + i * 128, tmem + C::kS + i * 128 + s * 8, z + (uint64_t)s * ((2 * D * 16) >> 4), io,
+                             j > 0 || s > 0);
+            if (j + 1 == n) {
+              tc::mma_commit(smem_addr(&b_o[i]));
+            } else {
+              if (i == 0 && !wait_one(&b_kfull[(at + 1) % KB], (at + 1) / KB)) break;
+              tc::fence_after();
+              scores(i, at + 1);
+            }
+          }
+          if (!ok) break;
+          tc::mma_commit(smem_addr(&b_vempty[at % KB]));
+          if (j + 1 < n) tc::mma_commit(smem_addr(&b_kempty[(at + 1) % KB]));
+        }
+      }
+    }
+
+    const bool begun = from > 0, done = to == span.count;
+    if (begun && done && threadIdx.x == 0) {  // this CTA ends a tile that others began: the joining kernel's work
+      join.first = (int)((pos - skip + kTileCost) / share.per);
+      join.rows = min(rows, R), join.row0 = rt * R, join.head0 = h * p.group, join.q0 = (int)q.q0;
+    }
+    blocks += n, ++segments;
+    for (int i = 0; i < tiles; ++i) done_blocks[i] += n, ++done_tiles[i];
+    pos += take, skip += take;
+    if (skip == units) skip = 0, ++h;
+    tc::fence_before();
+    __syncthreads();  // the queries' memory, O and S are free
+    tc::fence_after();
+    if (s_abort) break;
+  }
+  // nothing is in flight: a segment ends when its last products have been waited for. Where a wait ran out, they may not
+  // have: let the products issued so far end (they need nothing more) before their memory goes away.
+  if (s_abort) {
+    if (warp == SW + 4 && lane == 0) {
+      tc::mma_commit(smem_addr(&b_end));
+      mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
+    }
+    if (threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
+    join.first = -1;
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <int FMT, int NB>
+static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t stream) {
+  using C = TcTile<FMT, NB>;
+  static_assert(C::kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = attention_tc_kernel<FMT, NB>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
+  launch_maybe_pdl(kernel, dim3((unsigned)sms), dim3(C::kWarps * 32), C::kSmem, stream, p);
+  int rc = after_launch("attention_tc");
+  if (rc) return rc;
+  launch_maybe_pdl(attention_join_kernel<NB, C::kRows>, dim3((unsigned)(sms * C::kRows / 4)), dim3(128), 0, stream, p,
+                   sms);
+  return after_launch("attention_join");
+}
+
+template <int FMT>
+static int launch_attention_tc_fmt(const AttnParams& p, int dim, int sms, cudaStream_t stream) {
+  switch (dim) {
+    case 64: return launch_attention_tc_as<FMT, 2>(p, sms, stream);
+    case 96: return launch_attention_tc_as<FMT, 3>(p, sms, stream);
+    case 128: return launch_attention_tc_as<FMT, 4>(p, sms, stream);
+    default: return launch_attention_tc_as<FMT, 8>(p, sms, stream);
+  }
+}
+
+}  // namespace b2q

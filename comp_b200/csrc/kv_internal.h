@@ -41,10 +41,16 @@ struct AttnParams {
 int kv_cache_error(int* code, int clear);
 int kv_attention_q4_error(int* code, int clear);
 int kv_attention_q8_error(int* code, int clear);
+int kv_attention_tc_q4_error(int* code, int clear);
+int kv_attention_tc_q8_error(int* code, int clear);
 
 // Streaming kernels by format: `rows` is 8 or 16 query rows a tile, max_len bounds the lengths from above.
 int launch_attention_q4(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream);
 int launch_attention_q8(const AttnParams& p, int dim, int rows, int sms, int64_t max_len, cudaStream_t stream);
+// Tensor-core kernels by format, for tiles of kTcRows (heads of 256: half as many) query rows; 16-bit queries only.
+int launch_attention_tc_q4(const AttnParams& p, int dim, int sms, cudaStream_t stream);
+int launch_attention_tc_q8(const AttnParams& p, int dim, int sms, cudaStream_t stream);
+constexpr int kTcRows = 256;
 constexpr int kMaxCtasPerSm = 3;  // the workspace holds parts for so many
 
 }  // namespace b2q
