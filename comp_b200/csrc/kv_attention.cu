@@ -9,7 +9,8 @@ struct AttnPlan {
   size_t part_m, joins, bytes;  // workspace: partial outputs, then references and sums, then the joins
 };
 
-// 16-bit calls with at least kTcLeastRows query rows a sequence and KV head take the tensor-core kernels. Else the rows of
+// 16-bit calls with at least kTcLeastRows query rows a sequence and KV head take the tensor-core kernels (but not those with
+// heads of 256 and lse: shared memory has no room for keys in two parts). Else the rows of
 // a tile are 8, or 16 where more have to read the cache anyway (heads of 256 leave registers for 8).
 constexpr int kTcLeastRows = 64;
 
@@ -18,7 +19,7 @@ static AttnPlan plan_attention(const b2q_kv_cache& c, const b2q_attention_args& 
   const int group = a.q_heads / c.heads;
   const int64_t max_q = !a.cu_q ? 1 : (a.max_q > 0 && a.max_q < a.T ? a.max_q : a.T);
   const int64_t rows = max_q * group;
-  pl.tc = rows >= kTcLeastRows && a.dtype != B2Q_DTYPE_F32;
+  pl.tc = rows >= kTcLeastRows && a.dtype != B2Q_DTYPE_F32 && !(c.dim == 256 && a.lse);
   if (pl.tc)
     pl.rows = c.dim == 256 ? kTcRows / 2 : kTcRows;
   else

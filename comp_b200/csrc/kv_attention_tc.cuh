@@ -19,15 +19,18 @@
 
 namespace b2q {
 
-template <int FMT, int NB>
+// EXACT: the scores from keys in two f16 parts, what calls that return lse need: one part's rounding is 1e-4 of a score,
+// which a weight of 16 bits does not show, but an f32 lse does (1e-5 of it; with two parts 1e-7).
+template <int FMT, int NB, bool EXACT>
 struct TcTile {
   static constexpr int D = NB * 32;
   static constexpr int kRow = NB * (FMT == 0 ? 16 : 32);  // quant bytes of a token's row
   static constexpr int MT = NB == 8 ? 1 : 2;              // row tiles: tensor memory holds O (D) and S (128) of each
-  static constexpr int kBufs = NB == 8 ? 1 : 2;           // key and value tiles in shared memory
+  static constexpr int kBufs = NB == 8 ? 1 : 2;           // value tiles in shared memory
+  static constexpr int kKeyBufs = EXACT ? 1 : kBufs, kParts = EXACT ? 2 : 1;  // key tiles, and the parts of each
   static constexpr int kRows = MT * 128, kKeys = 128;
   static constexpr int kQ = 128 * D * 2, kTile = 128 * D * 2;
-  static constexpr int kSmem = MT * kQ + 2 * kBufs * kTile;
+  static constexpr int kSmem = MT * kQ + (kKeyBufs * kParts + kBufs) * kTile;
   static constexpr int kSoftmaxWarps = MT * 4, kWarps = MT * 4 + 5;  // + 4 unpacking, 1 issuing
   static constexpr uint32_t kS = 256;                     // column of S (and P) of tile 0; O is at 0
 };
@@ -106,12 +109,14 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 // (1024 + 16 q) / 16 - 72 = q - 8
 __device__ __forceinline__ uint32_t high_nibbles_int(uint32_t w) {
-  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u, s = 0x2c002c00u, o = 0xd480d480u;
-  const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&s),
-                            *reinterpret_cast<const __half2*>(&o));
-  return *reinterpret_cast<const uint32_t*>(&h);
+  return fma_half2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
 }
 
 // N bytes (a multiple of 2) of global memory into 32-bit words; 16, 8, 4 or 2 at a time as N allows (N aligned).
@@ -141,12 +146,12 @@ __device__ __forceinline__ void ldg_bytes(const uint8_t* at, uint32_t (&w)[(N + 
   }
 }
 
-template <int FMT, int NB>
-__global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_kernel(const AttnParams p) {
-  using C = TcTile<FMT, NB>;
-  constexpr int D = C::D, MT = C::MT, KB = C::kBufs, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
-  extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB], values [KB]
-  __shared__ uint64_t b_kfull[KB], b_kempty[KB], b_vfull[KB], b_vempty[KB], b_s[MT], b_p[MT], b_o[MT], b_q, b_end;
+template <int FMT, int NB, bool EXACT>
+__global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attention_tc_kernel(const AttnParams p) {
+  using C = TcTile<FMT, NB, EXACT>;
+  constexpr int D = C::D, MT = C::MT, KB = C::kKeyBufs, VB = C::kBufs, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
+  extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB][parts], values [VB]
+  __shared__ uint64_t b_kfull[KB], b_kempty[KB], b_vfull[VB], b_vempty[VB], b_s[MT], b_p[MT], b_o[MT], b_q, b_end;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ ShareScratch<C::kWarps> plan;
@@ -169,10 +174,8 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < KB; ++i) {
-      mbar_init(smem_addr(&b_kfull[i]), 128), mbar_init(smem_addr(&b_vfull[i]), 128);
-      mbar_init(smem_addr(&b_kempty[i]), 1), mbar_init(smem_addr(&b_vempty[i]), 1);
-    }
+    for (int i = 0; i < KB; ++i) mbar_init(smem_addr(&b_kfull[i]), 128), mbar_init(smem_addr(&b_kempty[i]), 1);
+    for (int i = 0; i < VB; ++i) mbar_init(smem_addr(&b_vfull[i]), 128), mbar_init(smem_addr(&b_vempty[i]), 1);
     for (int i = 0; i < MT; ++i) {
       mbar_init(smem_addr(&b_s[i]), 1), mbar_init(smem_addr(&b_p[i]), 128), mbar_init(smem_addr(&b_o[i]), 1);
     }
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
   tc::fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  const uint32_t q_smem = smem_addr(smem), k_smem = q_smem + MT * C::kQ, v_smem = k_smem + KB * C::kTile;
+  const uint32_t q_smem = smem_addr(smem), k_smem = q_smem + MT * C::kQ, v_smem = k_smem + KB * C::kParts * C::kTile;
   // a wait that ran out ends the role's work, and the kernel at the end of the tile: every later wait is skipped
   bool ok = true;
   auto wait_one = [&](uint64_t* bar, uint32_t phase) {  // by one thread
@@ -231,6 +234,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
       float mul = 1.f, rowf = 0.f, slope = 0.f;
       int64_t out_row = 0;
       const bool special = p.softcap > 0.f || p.slopes != nullptr;
+      const float cap = p.softcap * kLog2e;
       uint8_t* my_q = smem + tile * C::kQ + (r & 127) * 16;
       if (there) {
         const int i = p.cu_q ? rr / p.group : 0, head = h * p.group + (rr - i * p.group);
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
         const int e2 = max(-100, (__float_as_int(top) >> 23) - 127);
         const float up = __int_as_float((127 + 6 - e2) << 23);
         rowf = __int_as_float((127 + e2 - 6) << 23) * p.scale;
-        if (p.softcap <= 0.f) rowf *= kLog2e;
+        rowf *= p.softcap > 0.f ? 2.f * kLog2e / p.softcap : kLog2e;
         mul = rowf;
 #pragma unroll 2
         for (int w = 0; w < NB * 4; ++w) {  // chunk w = word (t, block) of a packed key: its 8 values in its order
@@ -280,31 +284,39 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
           if (!wait(&b_s[tile], done_blocks[tile] + j)) break;
           tc::fence_after();
           const int kb = (begin + j) * STG;
-          const bool careful = special || __any_sync(0xffffffffu, kb < lo || kb + STG > hi);
+          // masked or special scores are finished in the first pass and put back
+          const bool mask = __any_sync(0xffffffffu, kb < lo || kb + STG > hi), careful = special || mask;
           const float scale = careful ? 1.f : mul;
-          // scores as exponents of 2, and -inf where masked
-          auto finish = [&](uint32_t (&v)[32], int c) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              float x = __uint_as_float(v[e]) * rowf;
-              const int key = kb + c + e;
-              if (special) {
-                if (p.softcap > 0.f) x = soft_cap(x, p.softcap, 1.f / p.softcap) * kLog2e;
-                x -= slope * (float)abs(where - key);
-              }
-              v[e] = __float_as_uint(key >= lo && key < hi ? x : -INFINITY);
-            }
-          };
           uint32_t v[32];
           float top = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < STG; c += 32) {
             tc::tmem_ld32_nowait(col_s + c, v);
             tc::tmem_wait_ld32(v);
-            if (careful) finish(v, c);
+            if (careful) {
+              // softcap: cap - 2 cap / (2^(x rowf) + 1), rowf to twice the capped argument's exponent of 2
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float x = __uint_as_float(v[e]) * rowf;
+                if (p.softcap > 0.f) x = fmaf(__fdividef(1.f, exp2_approx(x) + 1.f), -2.f * cap, cap);
+                v[e] = __float_as_uint(x);
+              }
+              if (p.slopes) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  v[e] = __float_as_uint(fmaf(-slope, fabsf((float)(where - kb - c - e)), __uint_as_float(v[e])));
+              }
+              if (mask) {
+                const int from_e = lo - kb - c, to_e = hi - kb - c;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = e >= from_e && e < to_e ? v[e] : 0xff800000u;
+              }
+              tc::tmem_st32(col_s + c, v);
+            }
 #pragma unroll
             for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
           }
+          if (careful) tc::tmem_wait_st();
           top *= scale;
           if (__any_sync(0xffffffffu, top > ref + 8.f)) {
             const float now = top > ref + 8.f ? top : ref, f = exp2_approx(ref - now);
@@ -325,7 +337,6 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
           for (int c = 0; c < STG; c += 32) {
             tc::tmem_ld32_nowait(col_s + c, v);
             tc::tmem_wait_ld32(v);
-            if (careful) finish(v, c);
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
@@ -421,12 +432,13 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
       // the largest magnitude of a scale whose values all fit f16; others make their key NaN for the rows that see it
       const uint32_t most = FMT == 0 ? 0x6ffeu : 0x5ffcu;  // 8 * 8184 < 65504, 128 * 511 < 65504
       load_k(0);
-      load_v(0);
+      if (FMT == 0) load_v(0);  // q8_0: no registers to have them a block ahead
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t at = blocks + j;
-        const int buf = at % KB;
-        if (at >= KB && !wait(&b_kempty[buf], at / KB - 1)) break;
-        uint8_t* kt = smem + MT * C::kQ + buf * C::kTile + th * 16;
+        const int kbuf = at % KB, vbuf = at % VB;
+        if (FMT == 2) load_v(j);
+        if (at >= KB && !wait(&b_kempty[kbuf], at / KB - 1)) break;
+        uint8_t* kt = smem + MT * C::kQ + kbuf * C::kParts * C::kTile + th * 16;
         bool fits = true;
 #pragma unroll
         for (int k = 0; k < NB; ++k)
@@ -435,24 +447,32 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
         for (int w = 0; w < NB * 4; ++w) {  // word w = (t, block)
           const int k = w % NB;
           const uint32_t d = __byte_perm(ksc[k / 2], 0, (k & 1) ? 0x3232 : 0x1010);
-          uint4 x;
+          uint32_t i[4], x[4];  // the quants as f16, and times their scale
           if constexpr (FMT == 0) {
-            x.x = mul_half2(low_nibbles<true>(kw[w]), d), x.y = mul_half2(high_nibbles_int(kw[w]), d);
-            x.z = mul_half2(low_nibbles<true>(kw[w] >> 8), d), x.w = mul_half2(high_nibbles_int(kw[w] >> 8), d);
+            i[0] = low_nibbles<true>(kw[w]), i[1] = high_nibbles_int(kw[w]);
+            i[2] = low_nibbles<true>(kw[w] >> 8), i[3] = high_nibbles_int(kw[w] >> 8);
           } else {
-            x.x = mul_half2(two_bytes<true>(kw[2 * w], 0), d), x.y = mul_half2(two_bytes<true>(kw[2 * w], 1), d);
-            x.z = mul_half2(two_bytes<true>(kw[2 * w + 1], 0), d), x.w = mul_half2(two_bytes<true>(kw[2 * w + 1], 1), d);
+            i[0] = two_bytes<true>(kw[2 * w], 0), i[1] = two_bytes<true>(kw[2 * w], 1);
+            i[2] = two_bytes<true>(kw[2 * w + 1], 0), i[3] = two_bytes<true>(kw[2 * w + 1], 1);
           }
-          if (!read_k) x = make_uint4(0, 0, 0, 0);
-          if (!fits) x = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-          *reinterpret_cast<uint4*>(kt + w * 2048) = x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = read_k ? mul_half2(i[e], d) : 0u;
+            if (!fits) x[e] = 0x7fff7fffu;
+          }
+          *reinterpret_cast<uint4*>(kt + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
+          if constexpr (EXACT) {  // what the rounding left: one exact fused multiply-add
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = read_k && fits ? fma_half2(i[e], d, x[e] ^ 0x80008000u) : 0u;
+            *reinterpret_cast<uint4*>(kt + C::kTile + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
         }
         load_k(j + 1);
         tc::fence_async_smem();
-        tc::arrive(smem_addr(&b_kfull[buf]));
+        tc::arrive(smem_addr(&b_kfull[kbuf]));
 
-        if (at >= KB && !wait(&b_vempty[buf], at / KB - 1)) break;
-        uint8_t* vt = smem + MT * C::kQ + (KB + buf) * C::kTile + kg * (D * 16) + g * 16;
+        if (at >= VB && !wait(&b_vempty[vbuf], at / VB - 1)) break;
+        uint8_t* vt = smem + MT * C::kQ + (KB * C::kParts + vbuf) * C::kTile + kg * (D * 16) + g * 16;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // keys that are not there, or do not fit, are zeros
           bool use = i < read_v;
@@ -486,9 +506,9 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4*>(vt + (k * 32 + c * 8) * 16) = make_uint4(x[c][0], x[c][1], x[c][2], x[c][3]);
         }
-        load_v(j + 1);
+        if (FMT == 0) load_v(j + 1);
         tc::fence_async_smem();
-        tc::arrive(smem_addr(&b_vfull[buf]));
+        tc::arrive(smem_addr(&b_vfull[vbuf]));
       }
     } else if (lane == 0) {
       // ------------------------------------------------------------ the products, issued in the order in which they run
@@ -496,10 +516,14 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
       const uint64_t dq = tc::smem_desc_kmajor(q_smem, 2048), dk = tc::smem_desc_kmajor(k_smem, 2048);
       const uint64_t dv = tc::smem_desc_kmajor(v_smem, D * 16);
       auto scores = [&](int tile, uint32_t at) {
-        const uint64_t a = dq + (uint64_t)((tile * C::kQ) >> 4), z = dk + (uint64_t)(((at % KB) * C::kTile) >> 4);
+        const uint64_t a = dq + (uint64_t)((tile * C::kQ) >> 4);
+        const uint64_t z = dk + (uint64_t)(((at % KB) * C::kParts * C::kTile) >> 4);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          tc::mma_f16_ss(tmem + C::kS + tile * 128, a + s * (4096 >> 4), z + s * (4096 >> 4), is, s > 0);
+        for (int part = 0; part < C::kParts; ++part)
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s)
+            tc::mma_f16_ss(tmem + C::kS + tile * 128, a + s * (4096 >> 4), z + ((part * C::kTile + s * 4096) >> 4), is,
+                           part > 0 || s > 0);
         tc::mma_commit(smem_addr(&b_s[tile]));
       };
       if (wait_one(&b_q, segments) && wait_one(&b_kfull[blocks % KB], blocks / KB)) {
@@ -509,10 +533,10 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
         for (int j = 0; j < n && ok; ++j) {
           const uint32_t at = blocks + j;
           for (int i = 0; i < tiles; ++i) {
-            if (i == 0 && !wait_one(&b_vfull[at % KB], at / KB)) break;
+            if (i == 0 && !wait_one(&b_vfull[at % VB], at / VB)) break;
             if (!wait_one(&b_p[i], done_blocks[i] + j)) break;
             tc::fence_after();
-            const uint64_t z = dv + (uint64_t)(((at % KB) * C::kTile) >> 4);
+            const uint64_t z = dv + (uint64_t)(((at % VB) * C::kTile) >> 4);
 #pragma unroll
             for (int s = 0; s < STG / 16; ++s)
               tc::mma_f16_ts(tmem + i * 128, tmem + C::kS + i * 128 + s * 8, z + (uint64_t)s * ((2 * D * 16) >> 4), io,
@@ -526,7 +550,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
             }
           }
           if (!ok) break;
-          tc::mma_commit(smem_addr(&b_vempty[at % KB]));
+          tc::mma_commit(smem_addr(&b_vempty[at % VB]));
           if (j + 1 < n) tc::mma_commit(smem_addr(&b_kempty[(at + 1) % KB]));
         }
       }
@@ -563,11 +587,11 @@ __global__ void __launch_bounds__(TcTile<FMT, NB>::kWarps * 32, 1) attention_tc_
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-template <int FMT, int NB>
+template <int FMT, int NB, bool EXACT>
 static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t stream) {
-  using C = TcTile<FMT, NB>;
+  using C = TcTile<FMT, NB, EXACT>;
   static_assert(C::kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = attention_tc_kernel<FMT, NB>;
+  auto kernel = attention_tc_kernel<FMT, NB, EXACT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
   launch_maybe_pdl(kernel, dim3((unsigned)sms), dim3(C::kWarps * 32), C::kSmem, stream, p);
@@ -581,10 +605,16 @@ static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t str
 template <int FMT>
 static int launch_attention_tc_fmt(const AttnParams& p, int dim, int sms, cudaStream_t stream) {
   switch (dim) {
-    case 64: return launch_attention_tc_as<FMT, 2>(p, sms, stream);
-    case 96: return launch_attention_tc_as<FMT, 3>(p, sms, stream);
-    case 128: return launch_attention_tc_as<FMT, 4>(p, sms, stream);
-    default: return launch_attention_tc_as<FMT, 8>(p, sms, stream);
+    case 64:
+      return p.lse ? launch_attention_tc_as<FMT, 2, true>(p, sms, stream)
+                   : launch_attention_tc_as<FMT, 2, false>(p, sms, stream);
+    case 96:
+      return p.lse ? launch_attention_tc_as<FMT, 3, true>(p, sms, stream)
+                   : launch_attention_tc_as<FMT, 3, false>(p, sms, stream);
+    case 128:
+      return p.lse ? launch_attention_tc_as<FMT, 4, true>(p, sms, stream)
+                   : launch_attention_tc_as<FMT, 4, false>(p, sms, stream);
+    default: return launch_attention_tc_as<FMT, 8, false>(p, sms, stream);
   }
 }
 
