@@ -34,6 +34,16 @@ static AttnPlan plan_attention(const b2q_kv_cache& c, const b2q_attention_args& 
   return pl;
 }
 
+int allow_smem_once(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return B2Q_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return B2Q_OK;
+}
+
 static int check_attention(const char* who, const b2q_kv_cache* c, const b2q_attention_args* a) {
   int rc = check_kv_cache(who, c);
   if (rc) return rc;

@@ -888,15 +888,16 @@ static int launch_attention_as(const AttnParams& p, int sms, int64_t max_len, cu
   static_assert(kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
   static_assert(kv_ctas_per_sm<FMT, NB, NT, PARTS>() <= kMaxCtasPerSm, "the workspace's parts");
   auto kernel = attention_kernel<FMT, NB, NT, PARTS>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
+  static std::atomic<unsigned long long> allowed{0};
+  int rc = allow_smem_once(reinterpret_cast<const void*>(kernel), kSmem, allowed);
+  if (rc) return rc;
   static_assert(kv_ctas_per_sm<FMT, NB, NT, PARTS>() * (kSmem + 1024 + 1024) <= 228 * 1024, "shared memory of an SM");
   const int64_t slots = (int64_t)sms * kv_ctas_per_sm<FMT, NB, NT, PARTS>();
   // no more CTAs than there can be stages; max_len bounds the lengths from above
   const int64_t most = (int64_t)p.batch * p.row_tiles * p.heads * ((max_len + C::kTokens - 1) / C::kTokens + 1);
   const int64_t ctas = most < slots ? most : slots;
   launch_maybe_pdl(kernel, dim3((unsigned)ctas), dim3(128), kSmem, stream, p);
-  int rc = after_launch("attention");
+  rc = after_launch("attention");
   if (rc) return rc;
   const int64_t warps = ctas * NT * 8;
   launch_maybe_pdl(attention_join_kernel<NB, NT * 8>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p, (int)ctas);

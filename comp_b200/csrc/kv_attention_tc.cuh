@@ -592,10 +592,11 @@ static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t str
   using C = TcTile<FMT, NB, EXACT>;
   static_assert(C::kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
   auto kernel = attention_tc_kernel<FMT, NB, EXACT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-  if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
+  static std::atomic<unsigned long long> allowed{0};
+  int rc = allow_smem_once(reinterpret_cast<const void*>(kernel), C::kSmem, allowed);
+  if (rc) return rc;
   launch_maybe_pdl(kernel, dim3((unsigned)sms), dim3(C::kWarps * 32), C::kSmem, stream, p);
-  int rc = after_launch("attention_tc");
+  rc = after_launch("attention_tc");
   if (rc) return rc;
   launch_maybe_pdl(attention_join_kernel<NB, C::kRows>, dim3((unsigned)(sms * C::kRows / 4)), dim3(128), 0, stream, p,
                    sms);

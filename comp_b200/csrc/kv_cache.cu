@@ -1,9 +1,10 @@
 // Quantized KV cache: quantizing keys and values into their slots, and reading slots back.
 //
-// Both are one pass, bound by memory: a write reads the values once and stores 4.5 (q4_0) or 8.5 (q8_0) bits for each,
-// a read the reverse. A thread takes a quarter of a 32-value block (8 values): for q4_0 the values 4l..4l+3 and
-// 16+4l..16+4l+3, which are the two nibbles of the block's bytes 4l..4l+3 (one key unit, two value units), for q8_0 the
-// values 8l..8l+7. Every 32-byte sector of input, quants and output is then touched by one warp in whole.
+// Both are one pass, bound by memory: a write reads the values once and stores 4.5 (q4_0) or 8.5 (q8_0) bits for each, a
+// read the reverse. A thread takes quarter l of every 32-value block of a head's row: for q4_0 the values 4l..4l+3 and
+// 16+4l..16+4l+3 of a block (the two nibbles of the block's bytes 4l..4l+3), for q8_0 the values 8l..8l+7. In the cache's
+// order those are one run of the row, so that a thread's quants are one wide load or store, and four threads' values whole
+// 32-byte sectors.
 #include <type_traits>
 
 #include "kv_device.cuh"
@@ -27,21 +28,19 @@ __device__ __forceinline__ void load_quarter(const T* block, int l, float (&v)[8
 
 // ggml's q4_0 block of 32 values held by 4 consecutive lanes (values 4l.. and 16+4l..): the lane's 4 bytes, f16 d bits.
 __device__ __forceinline__ uint32_t quant_q4_0_quarter(const float (&v)[8], int l, uint16_t* d_bits) {
-  float best = 0.f, mag = -1.f;
-  int at = 0;
+  float mag = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(v[i]);
-    const int idx = (i < 4 ? 0 : 12) + 4 * l + i;
-    if (a > mag) mag = a, best = v[i], at = idx;  // ascending: the first of equals stays
-  }
+  for (int i = 0; i < 8; ++i) mag = fmaxf(mag, fabsf(v[i]));
+  mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
+  mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
+  // the first value of that magnitude decides d's sign: the lowest (index, sign) among the lanes
+  int first = 64;
 #pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, mag, o), b2 = __shfl_xor_sync(0xffffffffu, best, o);
-    const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-    if (m2 > mag || (m2 == mag && a2 < at)) mag = m2, best = b2, at = a2;
-  }
-  const float d = __fmul_rn(best, -0.125f);  // m / -8, exact but for underflow
+  for (int i = 7; i >= 0; --i)
+    if (fabsf(v[i]) == mag) first = 2 * ((i < 4 ? 0 : 12) + 4 * l + i) + (signbit(v[i]) ? 1 : 0);
+  first = min(first, __shfl_xor_sync(0xffffffffu, first, 1));
+  first = min(first, __shfl_xor_sync(0xffffffffu, first, 2));
+  const float d = __fmul_rn((first & 1) ? -mag : mag, -0.125f);  // m / -8, exact but for underflow
   const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
   uint32_t w = 0;
 #pragma unroll
@@ -72,118 +71,176 @@ __device__ __forceinline__ uint2 quant_q8_0_quarter(const float (&v)[8], uint16_
   return make_uint2(w[0], w[1]);
 }
 
-// One thread per (token, head, block, quarter); blockIdx.y 0 = keys, 1 = values. `tpb` tokens a CTA.
+// N 16-bit words (two to a register) to `dst`, and back, in the widest pieces that N's alignment allows.
+template <int N>
+__device__ __forceinline__ void store_halves(uint8_t* dst, const uint32_t (&w)[(N + 1) / 2]) {
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 4) *reinterpret_cast<uint4*>(dst + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  } else if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 2) *reinterpret_cast<uint2*>(dst + 4 * i) = make_uint2(w[i], w[i + 1]);
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) *reinterpret_cast<uint32_t*>(dst + 4 * i) = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *reinterpret_cast<uint16_t*>(dst + 2 * i) = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_halves(const uint8_t* src, uint32_t (&w)[(N + 1) / 2]) {
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(src + 4 * i);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  } else if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(src + 4 * i);
+      w[i] = v.x, w[i + 1] = v.y;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = *reinterpret_cast<const uint32_t*>(src + 4 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t v = *reinterpret_cast<const uint16_t*>(src + 2 * i);
+      w[i / 2] = (i & 1) ? (w[i / 2] | v << 16) : v;
+    }
+  }
+}
+
+// A quarter's share of a row, KW 32-bit words: keys as [block][word], values as [unit 2l, 2l + 1][block] of half of that.
+// One thread per (token, head, quarter); blockIdx.y 0 = keys, 1 = values.
 template <int FMT, int NB, typename T>
 __global__ void __launch_bounds__(256)
     kv_write_kernel(const T* __restrict__ k, int64_t k_st, int64_t k_sh, const T* __restrict__ v, int64_t v_st,
-                    int64_t v_sh, const int64_t* __restrict__ slots, b2q_kv_cache c, int page_shift, int64_t ntok,
-                    int tpb) {
+                    int64_t v_sh, const int64_t* __restrict__ slots, b2q_kv_cache c, int page_shift, int64_t ntok) {
   pdl_wait_then_trigger();
-  constexpr int kRow = NB * (FMT == 0 ? 16 : 32);
+  constexpr int kRow = NB * (FMT == 0 ? 16 : 32), KW = kRow / 16;
   const bool val = blockIdx.y != 0;
-  const T* x = val ? v : k;
-  const int64_t st = val ? v_st : k_st, sh = val ? v_sh : k_sh;
-  uint8_t* quants = val ? c.vq : c.kq;
-  int16_t* scales = val ? c.vs : c.ks;
-  const int per_token = c.heads * NB * 4;
-  const int items = tpb * per_token;
-  const int64_t t0 = (int64_t)blockIdx.x * tpb;
-  for (int base = 0; base < items; base += 256) {  // CTA-uniform: the shuffles need whole warps
-    const int i = base + threadIdx.x;
-    const int tt = i / per_token, r = i - tt * per_token;
-    const int64_t tok = t0 + tt;
-    const int l = r & 3, b = (r >> 2) % NB, h = (r >> 2) / NB;
-    int64_t slot = -1;
-    if (i < items && tok < ntok) slot = slots[tok];
-    if (slot >= (c.pages << page_shift)) {
-      atomicCAS(&g_kv_error, 0, kErrSlot);
-      slot = -1;
-    }
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0) load_quarter<FMT>(x + tok * st + h * sh + b * 32, l, f);
-    uint16_t d;
-    const int64_t row = ((slot >> page_shift) * c.heads + h << page_shift) + (slot & ((1 << page_shift) - 1));
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, r = item >> 2;
+  const int l = (int)item & 3;
+  const int64_t tok = r < (1u << 31) ? (int64_t)((uint32_t)r / (uint32_t)c.heads) : r / c.heads;
+  const int h = (int)(r - tok * c.heads);
+  int64_t slot = tok < ntok ? slots[tok] : -1;
+  if (slot >= (c.pages << page_shift)) {
+    atomicCAS(&g_kv_error, 0, kErrSlot);
+    slot = -1;
+  }
+  // no early return: the four lanes of a row stay together for the shuffles
+  float f[NB][8];
+  const T* x = (val ? v : k) + tok * (val ? v_st : k_st) + h * (val ? v_sh : k_sh);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[b][e] = 0.f;
+    if (slot >= 0) load_quarter<FMT>(x + b * 32, l, f[b]);
+  }
+  uint32_t w[KW];
+  uint16_t d[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
     if constexpr (FMT == 0) {
-      const uint32_t w = quant_q4_0_quarter(f, l, &d);
-      if (slot >= 0) {
-        uint8_t* dst = quants + row * kRow;
-        if (!val) {
-          *reinterpret_cast<uint32_t*>(dst + (l * NB + b) * 4) = w;
-        } else {
-          *reinterpret_cast<uint16_t*>(dst + ((2 * l) * NB + b) * 2) = (uint16_t)w;
-          *reinterpret_cast<uint16_t*>(dst + ((2 * l + 1) * NB + b) * 2) = (uint16_t)(w >> 16);
-        }
-      }
+      w[b] = quant_q4_0_quarter(f[b], l, &d[b]);
     } else {
-      const uint2 w = quant_q8_0_quarter(f, &d);
-      if (slot >= 0) {
-        uint8_t* dst = quants + row * kRow;
-        if (!val) {
-          *reinterpret_cast<uint2*>(dst + (l * NB + b) * 8) = w;
-        } else {
-          *reinterpret_cast<uint32_t*>(dst + ((2 * l) * NB + b) * 4) = w.x;
-          *reinterpret_cast<uint32_t*>(dst + ((2 * l + 1) * NB + b) * 4) = w.y;
-        }
-      }
+      const uint2 q = quant_q8_0_quarter(f[b], &d[b]);
+      w[2 * b] = q.x, w[2 * b + 1] = q.y;
     }
-    if (slot >= 0 && l == 0) scales[row * NB + b] = (int16_t)d;
+  }
+  if (slot < 0) return;
+  const int64_t row = (((slot >> page_shift) * c.heads + h) << page_shift) + (slot & ((1 << page_shift) - 1));
+  uint8_t* dst = (val ? c.vq : c.kq) + row * kRow + l * (KW * 4);
+  if (!val) {
+    store_halves<2 * KW>(dst, w);
+  } else if constexpr (FMT == 0) {  // the words' low halves are unit 2l, their high halves unit 2l + 1
+    uint32_t u[2 * NB + 1];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) u[b] = w[b] & 0xffffu, u[NB + b] = w[b] >> 16;
+    uint32_t y[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) y[b] = u[2 * b] | u[2 * b + 1] << 16;
+    store_halves<2 * NB>(dst, y);
+  } else {
+    uint32_t y[KW];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) y[b] = w[2 * b], y[NB + b] = w[2 * b + 1];
+    store_halves<2 * KW>(dst, y);
+  }
+  if (l == 0) {
+    uint32_t y[(NB + 1) / 2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) y[b / 2] = (b & 1) ? (y[b / 2] | (uint32_t)d[b] << 16) : d[b];
+    store_halves<NB>(reinterpret_cast<uint8_t*>((val ? c.vs : c.ks) + row * NB), y);
   }
 }
 
 template <int FMT, int NB, typename T>
 __global__ void __launch_bounds__(256)
     kv_read_kernel(T* __restrict__ k, T* __restrict__ v, const int64_t* __restrict__ slots, b2q_kv_cache c,
-                   int page_shift, int64_t ntok, int tpb) {
+                   int page_shift, int64_t ntok) {
   pdl_wait_then_trigger();
-  constexpr int kRow = NB * (FMT == 0 ? 16 : 32);
+  constexpr int kRow = NB * (FMT == 0 ? 16 : 32), KW = kRow / 16;
   const bool val = k == nullptr || blockIdx.y != 0;
-  T* x = val ? v : k;
-  const uint8_t* quants = val ? c.vq : c.kq;
-  const int16_t* scales = val ? c.vs : c.ks;
-  const int per_token = c.heads * NB * 4;
-  const int items = tpb * per_token;
-  const int64_t t0 = (int64_t)blockIdx.x * tpb;
-  for (int i = threadIdx.x; i < items; i += 256) {
-    const int tt = i / per_token, r = i - tt * per_token;
-    const int64_t tok = t0 + tt;
-    if (tok >= ntok) return;
-    const int l = r & 3, b = (r >> 2) % NB, h = (r >> 2) / NB;
-    int64_t slot = slots[tok];
-    if (slot >= (c.pages << page_shift)) {
-      atomicCAS(&g_kv_error, 0, kErrSlot);
-      slot = -1;
-    }
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0) {
-      const int64_t row = ((slot >> page_shift) * c.heads + h << page_shift) + (slot & ((1 << page_shift) - 1));
-      const float d = f16_bits_to_f32((uint16_t)scales[row * NB + b]);
-      const uint8_t* src = quants + row * kRow;
-      if constexpr (FMT == 0) {
-        uint32_t w;
-        if (!val)
-          w = *reinterpret_cast<const uint32_t*>(src + (l * NB + b) * 4);
-        else
-          w = *reinterpret_cast<const uint16_t*>(src + ((2 * l) * NB + b) * 2) |
-              (uint32_t) * reinterpret_cast<const uint16_t*>(src + ((2 * l + 1) * NB + b) * 2) << 16;
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, r = item >> 2;
+  const int l = (int)item & 3;
+  const int64_t tok = r < (1u << 31) ? (int64_t)((uint32_t)r / (uint32_t)c.heads) : r / c.heads;
+  const int h = (int)(r - tok * c.heads);
+  if (tok >= ntok) return;
+  int64_t slot = slots[tok];
+  if (slot >= (c.pages << page_shift)) {
+    atomicCAS(&g_kv_error, 0, kErrSlot);
+    slot = -1;
+  }
+  uint32_t w[KW], s[(NB + 1) / 2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = d * (float)((int)((w >> ((e & 3) * 8 + (e >> 2) * 4)) & 15) - 8);
-      } else {
-        uint2 w;
-        if (!val) {
-          w = *reinterpret_cast<const uint2*>(src + (l * NB + b) * 8);
-        } else {
-          w.x = *reinterpret_cast<const uint32_t*>(src + ((2 * l) * NB + b) * 4);
-          w.y = *reinterpret_cast<const uint32_t*>(src + ((2 * l + 1) * NB + b) * 4);
-        }
+  for (int i = 0; i < KW; ++i) w[i] = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          f[e] = d * (float)((int)(((e < 4 ? w.x : w.y) >> ((e & 3) * 8)) & 255) - 128);
+  for (int i = 0; i < (NB + 1) / 2; ++i) s[i] = 0;
+  if (slot >= 0) {
+    const int64_t row = (((slot >> page_shift) * c.heads + h) << page_shift) + (slot & ((1 << page_shift) - 1));
+    load_halves<2 * KW>((val ? c.vq : c.kq) + row * kRow + l * (KW * 4), w);
+    load_halves<NB>(reinterpret_cast<const uint8_t*>((val ? c.vs : c.ks) + row * NB), s);
+  }
+  if (val) {  // back to [block][word]
+    uint32_t y[KW];
+#pragma unroll
+    for (int i = 0; i < KW; ++i) y[i] = w[i];
+    if constexpr (FMT == 0) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const uint32_t lo = (y[b / 2] >> (16 * (b & 1))) & 0xffffu;
+        const uint32_t hi = (y[(NB + b) / 2] >> (16 * ((NB + b) & 1))) & 0xffffu;
+        w[b] = lo | hi << 16;
       }
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) w[2 * b] = y[b], w[2 * b + 1] = y[NB + b];
     }
-    T* dst = x + (tok * c.heads + h) * (NB * 32) + b * 32;
-    constexpr int kSecond = FMT == 0 ? 16 : 4, kStep = FMT == 0 ? 4 : 8;
-    store4(dst + kStep * l, f[0], f[1], f[2], f[3]);
-    store4(dst + kStep * l + kSecond, f[4], f[5], f[6], f[7]);
+  }
+  T* dst = (val ? v : k) + r * (NB * 32);
+  constexpr int kSecond = FMT == 0 ? 16 : 4, kStep = FMT == 0 ? 4 : 8;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const float d = slot >= 0 ? f16_bits_to_f32((uint16_t)(s[b / 2] >> (16 * (b & 1)))) : 0.f;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (FMT == 0)
+        f[e] = d * (float)((int)((w[b] >> ((e & 3) * 8 + (e >> 2) * 4)) & 15) - 8);
+      else
+        f[e] = d * (float)((int)((w[2 * b + (e >> 2)] >> ((e & 3) * 8)) & 255) - 128);
+    }
+    if (slot < 0) {  // zeros, not minus zeros
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    }
+    store4(dst + 32 * b + kStep * l, f[0], f[1], f[2], f[3]);
+    store4(dst + 32 * b + kStep * l + kSecond, f[4], f[5], f[6], f[7]);
   }
 }
 
@@ -210,31 +267,20 @@ static int log2_of(int x) {
   return s;
 }
 
-// Tokens a CTA: about 1024 threads' items, fewer when the tokens alone do not fill the GPU.
-static int tokens_per_cta(int64_t T, int per_token) {
-  DeviceInfo di;
-  const int sms = device_info(&di) == B2Q_OK ? di.sms : 148;
-  int tpb = 1024 / per_token;
-  if (tpb > T / (2 * sms)) tpb = (int)(T / (2 * sms));
-  return tpb < 1 ? 1 : tpb;
-}
-
 template <int FMT, int NB, typename T>
 static int write_as(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                     const int64_t* slots, const b2q_kv_cache& c, int64_t ntok, cudaStream_t stream) {
-  const int tpb = tokens_per_cta(ntok, c.heads * NB * 4);
-  const dim3 grid((unsigned)((ntok + tpb - 1) / tpb), 2);
+  const dim3 grid((unsigned)((ntok * c.heads * 4 + 255) / 256), 2);
   launch_maybe_pdl(kv_write_kernel<FMT, NB, T>, grid, dim3(256), 0, stream, static_cast<const T*>(k), k_st, k_sh,
-                   static_cast<const T*>(v), v_st, v_sh, slots, c, log2_of(c.page), ntok, tpb);
+                   static_cast<const T*>(v), v_st, v_sh, slots, c, log2_of(c.page), ntok);
   return after_launch("kv_write");
 }
 
 template <int FMT, int NB, typename T>
 static int read_as(void* k, void* v, const int64_t* slots, const b2q_kv_cache& c, int64_t ntok, cudaStream_t stream) {
-  const int tpb = tokens_per_cta(ntok, c.heads * NB * 4);
-  const dim3 grid((unsigned)((ntok + tpb - 1) / tpb), k && v ? 2 : 1);
+  const dim3 grid((unsigned)((ntok * c.heads * 4 + 255) / 256), k && v ? 2 : 1);
   launch_maybe_pdl(kv_read_kernel<FMT, NB, T>, grid, dim3(256), 0, stream, static_cast<T*>(k), static_cast<T*>(v),
-                   slots, c, log2_of(c.page), ntok, tpb);
+                   slots, c, log2_of(c.page), ntok);
   return after_launch("kv_read");
 }
 
@@ -285,7 +331,7 @@ int b2q_kv_write(const b2q_kv_cache* cache, int dtype, const void* k, int64_t k_
   if (!aligned(k, 16) || !aligned(v, 16) || k_st % mult || k_sh % mult || v_st % mult || v_sh % mult)
     return fail(B2Q_EALIGN, "%s: k and v must be 16-byte aligned, in their strides too", who);
   if (!aligned(slots, 8)) return fail(B2Q_EALIGN, "%s: slots must be 8-byte aligned", who);
-  if (T > (int64_t)1 << 31) return fail(B2Q_ERANGE, "%s: T=%lld", who, (long long)T);
+  if (T > ((int64_t)1 << 36) / cache->heads) return fail(B2Q_ERANGE, "%s: T=%lld", who, (long long)T);
   return by_type(*cache, dtype, [&](auto fmt, auto nb, auto elt) {
     return write_as<decltype(fmt)::value, decltype(nb)::value, decltype(elt)>(
         k, k_st, k_sh, v, v_st, v_sh, slots, *cache, T, (cudaStream_t)stream);
@@ -303,7 +349,7 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
   if (!slots) return fail(B2Q_EINVAL, "%s: null pointer", who);
   if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 8))
     return fail(B2Q_EALIGN, "%s: k and v must be 16-byte aligned, slots 8-byte aligned", who);
-  if (T > (int64_t)1 << 31) return fail(B2Q_ERANGE, "%s: T=%lld", who, (long long)T);
+  if (T > ((int64_t)1 << 36) / cache->heads) return fail(B2Q_ERANGE, "%s: T=%lld", who, (long long)T);
   return by_type(*cache, dtype, [&](auto fmt, auto nb, auto elt) {
     return read_as<decltype(fmt)::value, decltype(nb)::value, decltype(elt)>(k, v, slots, *cache, T, (cudaStream_t)stream);
   });

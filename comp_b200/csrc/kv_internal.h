@@ -2,6 +2,8 @@
 // the attention kernels and the launchers that the dispatcher picks from.
 #pragma once
 
+#include <atomic>
+
 #include "b2q_internal.h"
 
 namespace b2q {
@@ -14,6 +16,9 @@ inline int dtype_size(int dtype) { return dtype == B2Q_DTYPE_F32 ? 4 : 2; }
 
 // The checks of a cache descriptor that every entry point makes (kv_cache.cu).
 int check_kv_cache(const char* who, const b2q_kv_cache* c);
+
+// Lets `kernel` (told apart by the caller's own `done` word) take `bytes` of shared memory, once a device.
+int allow_smem_once(const void* kernel, int bytes, std::atomic<unsigned long long>& done);
 
 // A tile that several CTAs worked on, told by the CTA that ended it: the CTA that began it (-1: no such tile), the tile's
 // rows, its first row and head, and its sequence's first query token.

@@ -13,11 +13,17 @@ their device, and raise TypeError / ValueError / RuntimeError on what they do no
 """
 
 import ctypes
+import struct
 
 import torch
 
 from . import _lib
-from .host import FMT_ID, _need_cuda, _on, _stream
+from .host import FMT_ID, _need_cuda
+
+# A decode step's attention runs a few microseconds on the GPU, so that what these functions cost on the host is what a
+# caller waits for: they check in few steps, take the stream's handle without making a Stream object, and pack the
+# arguments in one call (measured on one sequence of 4097 tokens: 26 us a call before that, 18 since).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 FORMATS = ("q4_0", "q8_0")
 HEAD_DIMS = (64, 96, 128, 256)
@@ -77,6 +83,7 @@ class KVCache:
         self._desc = _lib.KVCacheDesc(kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr(), pages, heads, page,
                                       nb * 32, FMT_ID[fmt])
         self._ref = ctypes.addressof(self._desc)
+        self._sizes = {}  # attention workspaces by shape
 
     @property
     def nbytes(self):
@@ -84,12 +91,29 @@ class KVCache:
 
 
 def _dtype_id(name, t):
-    if t.dtype not in DTYPE_ID:
+    did = DTYPE_ID.get(t.dtype)
+    if did is None:
         raise TypeError(f"{name}: dtype {t.dtype}, expected float32, float16 or bfloat16")
-    return DTYPE_ID[t.dtype]
+    return did
 
 
-def _slots(name, cache, slots):
+def _on_device(name, dev, *tensors):
+    """Raises unless all are tensors on dev."""
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.device != dev:
+            _need_cuda(name, t)
+            raise RuntimeError(f"comp_b200.{name}: tensors on different devices ({dev} and {t.device})")
+
+
+def _call(dev, name, *args):
+    """_lib.call with dev the current device."""
+    if torch.cuda.current_device() == dev.index:
+        return _lib.call(name, *args)
+    with torch.cuda.device(dev):
+        return _lib.call(name, *args)
+
+
+def _slots(name, slots):
     if slots.dtype != torch.int64 or slots.dim() != 1:
         raise TypeError(f"{name}: slots must be a 1-D int64 tensor, got {slots.dtype} {tuple(slots.shape)}")
     return slots if slots.is_contiguous() else slots.contiguous()
@@ -97,8 +121,9 @@ def _slots(name, cache, slots):
 
 def _heads_aligned(t):
     """t with a contiguous last axis, a 16-byte aligned base and strides of whole 16 bytes (a copy only when needed)."""
-    size = t.element_size()
-    if t.stride(2) != 1 or t.data_ptr() % 16 or t.stride(0) * size % 16 or t.stride(1) * size % 16:
+    a, b, c = t.stride()
+    mult = 16 // t.element_size()
+    if c != 1 or a % mult or b % mult or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -107,51 +132,69 @@ def kv_write(cache, k, v, slots):
     """Quantizes k and v [T][heads][head_dim] (f32, f16 or bf16; any token and head strides) into the slots int64 [T] of
     the cache (page * page_size + offset). Negative slots are skipped (padding tokens). The blocks are ggml's, bit for
     bit (quantize_row_q4_0 / q8_0 of the value widened to f32); a 16-bit caller needs no cast."""
-    dev = _need_cuda("kv_write", cache.kq, k, v, slots)
+    dev = cache.device
+    _on_device("kv_write", dev, k, v, slots)
+    slots = _slots("kv_write", slots)
     shape = (slots.shape[0], cache.heads, cache.head_dim)
     did = _dtype_id("kv_write: k", k)
     if v.dtype != k.dtype:
         raise TypeError(f"kv_write: k is {k.dtype}, v is {v.dtype}")
     if k.shape != shape or v.shape != shape:
         raise ValueError(f"kv_write: k {tuple(k.shape)} and v {tuple(v.shape)}, expected {shape}")
-    slots = _slots("kv_write", cache, slots)
     k, v = _heads_aligned(k), _heads_aligned(v)
     ks, vs = k.stride(), v.stride()
-    with _on(dev):
-        _lib.call("b2q_kv_write", cache._ref, did, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                  slots.data_ptr(), shape[0], _stream(dev))
+    _call(dev, "b2q_kv_write", cache._ref, did, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+          slots.data_ptr(), shape[0], _raw_stream(dev.index))
 
 
 def kv_read(cache, slots, dtype=torch.float32):
     """-> (k, v) [T][heads][head_dim] of `dtype`: the values that the slots int64 [T] hold (f16 scale times quant, rounded
     once). Negative slots give zeros."""
-    dev = _need_cuda("kv_read", cache.kq, slots)
-    if dtype not in DTYPE_ID:
+    dev = cache.device
+    _on_device("kv_read", dev, slots)
+    did = DTYPE_ID.get(dtype)
+    if did is None:
         raise TypeError(f"kv_read: dtype {dtype}, expected float32, float16 or bfloat16")
-    slots = _slots("kv_read", cache, slots)
-    shape = (slots.shape[0], cache.heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=dev)
-    v = torch.empty(shape, dtype=dtype, device=dev)
-    with _on(dev):
-        _lib.call("b2q_kv_read", cache._ref, DTYPE_ID[dtype], k.data_ptr(), v.data_ptr(), slots.data_ptr(), shape[0],
-                  _stream(dev))
+    slots = _slots("kv_read", slots)
+    n = slots.shape[0]
+    k = slots.new_empty((n, cache.heads, cache.head_dim), dtype=dtype)
+    v = torch.empty_like(k)
+    _call(dev, "b2q_kv_read", cache._ref, did, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n,
+          _raw_stream(dev.index))
     return k, v
 
 
 def _index(t, name, shape, dev, dtype=torch.int32):
+    """The address of an index tensor (0: None), and the tensor that holds it."""
     if t is None:
-        return None
+        return 0, None
+    _on_device("attention", dev, t)
     if t.dtype != dtype:
         raise TypeError(f"attention: {name}: dtype {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"attention: {name}: shape {tuple(t.shape)}, expected {shape}")
-    if t.device != dev:
-        raise RuntimeError(f"comp_b200.attention: {name} must be on {dev}")
-    return t if t.is_contiguous() else t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.data_ptr(), t
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+_pack_args = struct.Struct("@9P8q3i2f").pack  # b2q_attention_args, field by field
+assert struct.calcsize("@9P8q3i2f") <= ctypes.sizeof(_lib.AttentionArgs)
+
+
+def attention_workspace_size(cache, T, batch, q_heads, dtype, max_q=1, return_lse=False):
+    """Bytes of device workspace that attention needs for such a call (max_q as there: 1 without cu_q)."""
+    key = (T > 0 and batch > 0, q_heads, dtype, max_q if max_q and max_q < T else T, return_lse)
+    size = cache._sizes.get(key)
+    if size is None:
+        one = 256  # any address: the plan looks at sizes and at whether lse and cu_q are given
+        args = _lib.AttentionArgs(one, one, one if return_lse else None, one, one, one, None, None, None,
+                                  cache.head_dim * q_heads, cache.head_dim, T, batch, 1, 1, max_q or 0, 0, q_heads,
+                                  DTYPE_ID[dtype], 0, 1.0, 0.0)
+        with torch.cuda.device(cache.device):
+            size = _lib.load().b2q_attention_workspace_size(cache._ref, ctypes.addressof(args))
+        cache._sizes[key] = size
+    return size
 
 
 def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_len=None, softcap=0.0, window=0,
@@ -172,7 +215,8 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     T, or 1 without cu_q, and what the table can hold): max_q must not be less than what cu_q has, max_len only plans
     the work. workspace: a CUDA byte tensor of attention_workspace_size(...) bytes (allocated here when None). out: a
     contiguous tensor for the result."""
-    dev = _need_cuda("attention", q, cache.kq, table, lens)
+    dev = cache.device
+    _on_device("attention", dev, q, table, lens)
     did = _dtype_id("attention: q", q)
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         raise ValueError(f"attention: q {tuple(q.shape)}, expected [T][q_heads][{cache.head_dim}]")
@@ -184,32 +228,30 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     B, P = table.shape
     if P and table.stride(1) != 1:
         table = table.contiguous()
-    lens = _index(lens, "lens", (B,), dev)
+    lens_at, lens = _index(lens, "lens", (B,), dev)
     if cu_q is None:
         if T != B:
             raise ValueError(f"attention: {T} query tokens for {B} sequences need cu_q")
         max_q = 1
-    else:
-        cu_q = _index(cu_q, "cu_q", (B + 1,), dev)
-        max_q = T if max_q is None else max_q
-    prefix = _index(prefix, "prefix", (B,), dev)
-    starts = _index(starts, "starts", (T,), dev)
-    slopes = _index(slopes, "slopes", (heads,), dev, torch.float32)
+    elif max_q is None:
+        max_q = T
+    cu_at, cu_q = _index(cu_q, "cu_q", (B + 1,), dev)
+    prefix_at, prefix = _index(prefix, "prefix", (B,), dev)
+    starts_at, starts = _index(starts, "starts", (T,), dev)
+    slopes_at, slopes = _index(slopes, "slopes", (heads,), dev, torch.float32)
     q = _heads_aligned(q)
     if out is None:
-        out = torch.empty((T, heads, dim), dtype=q.dtype, device=dev)
+        out = q.new_empty((T, heads, dim))
     elif out.dtype != q.dtype or out.shape != q.shape or out.device != dev or not out.is_contiguous():
         raise ValueError(f"attention: out must be a contiguous {q.dtype} {tuple(q.shape)} tensor on {dev}")
-    lse = torch.empty((T, heads), dtype=torch.float32, device=dev) if return_lse else None
-    args = _lib.AttentionArgs(q.data_ptr(), out.data_ptr(), _ptr(lse), table.data_ptr(), lens.data_ptr(), _ptr(cu_q),
-                              _ptr(prefix), _ptr(starts), _ptr(slopes), q.stride(0), q.stride(1), T, B,
-                              table.stride(0) if P else 0, P, max_q, P * cache.page_size if max_len is None else max_len,
-                              heads, did, window, dim**-0.5 if scale is None else scale, softcap)
-    ref = ctypes.addressof(args)
-    with _on(dev):
-        need = _lib.load().b2q_attention_workspace_size(cache._ref, ref)
-        if need and workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("b2q_attention", cache._ref, ref, workspace.data_ptr() if need else None,
-                  workspace.numel() * workspace.element_size() if need else 0, _stream(dev))
+    lse = q.new_empty((T, heads), dtype=torch.float32) if return_lse else None
+    if workspace is None:
+        workspace = lens.new_empty(attention_workspace_size(cache, T, B, heads, q.dtype, max_q, return_lse) + 3 >> 2)
+    q_st, q_sh, _ = q.stride()
+    args = _pack_args(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, table.data_ptr(), lens_at,
+                      cu_at, prefix_at, starts_at, slopes_at, q_st, q_sh, T, B, table.stride(0) if P else 0, P, max_q,
+                      P * cache.page_size if max_len is None else max_len, heads, did, window,
+                      dim**-0.5 if scale is None else scale, softcap)
+    _call(dev, "b2q_attention", cache._ref, args, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+          _raw_stream(dev.index))
     return (out, lse) if return_lse else out
