@@ -9,7 +9,8 @@
 //     AND unpacks two values. The offset -off * sum(Q) of a block is a constant of the row, added to the block's sum.
 //   - queries: scaled by a power of two to 2^13..2^14, so that 16-bit queries are exact; f32 queries take two parts.
 //     A block's scale dk (per key and block) multiplies the f32 sum of the block.
-//   - values: the quant minus its offset, again as an exact subnormal; no running sum can then cancel.
+//   - values: the quant minus its offset, again as an exact subnormal (an addition more for two values): offsets taken
+//     off the sums instead would cancel there, and leave their cut-off bits.
 //   - weights: 2^(x - ref) * dv in f32 for each block, rounded once to f16 (f32 calls: two parts, 22 bits). `ref` follows
 //     the row's scores and the value scales, so that the products stay at most 2^15 and a row's largest near 2^8: they
 //     cannot overflow whatever the scales, and lose no bits to f16's small exponents until 2^-22 of the largest.
@@ -289,11 +290,9 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   extern __shared__ __align__(128) uint8_t smem[];  // [stage][warp] ring; the last stage holds the queries at first
   __shared__ int s_lo[R], s_hi[R], s_pos[R], s_out[R], s_top[R];
   __shared__ float s_slope[R], s_rowf[R];
-  __shared__ uint32_t s_off[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   uint8_t* const ring = smem + warp * C::kStage;  // stage s of this warp: s * W stages on
-  if (threadIdx.x < 8) s_off[threadIdx.x] = threadIdx.x < 4 ? 0x80088008u : 0x80808080u;
   pdl_wait_then_trigger();
 
   __shared__ ShareScratch<W> plan;
@@ -312,14 +311,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   const bool special = p.softcap > 0.f || p.slopes != nullptr;
   const int tokA = tile_token(g);  // key rows g and g + 8 of a tile: tokA, tokA + 8
   const int vtok0 = tile_token(2 * t), vtok1 = tile_token(2 * t + 1);
-  // The offsets as operands. Read from shared memory, and as volatile: from constants the compiler would make their eight
-  // registers anew for every product (measured: 32 moves of the 350 instructions of a 16-key step).
-  uint32_t off0[4], off1[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    off1[i] = *const_cast<volatile uint32_t*>(&s_off[4 + i]);
-    off0[i] = FMT == 0 ? *const_cast<volatile uint32_t*>(&s_off[i]) : off1[i];
-  }
+
   while (pos < end) {
     // -------------------------------------------------------------- the next tile of the share: (b, rt, h), its rows
     const int b = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - b * p.row_tiles;
@@ -719,6 +711,13 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
                 a[mt][2] = two_bytes<SIGNED>(hi, 0), a[mt][3] = two_bytes<SIGNED>(hi, 1);
               }
             }
+            if constexpr (!SIGNED) {  // less the offset, still as subnormals: values cancel in no sum
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                a[0][j] = add_half2(a[0][j], FMT == 0 ? 0x80088008u : 0x80808080u);
+                a[1][j] = add_half2(a[1][j], 0x80808080u);
+              }
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               float y[4];
@@ -727,9 +726,6 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
               const uint32_t p0 = pack_half2(y[0], y[1]), p1 = pack_half2(y[2], y[3]);
               const uint32_t b0 = transpose_8x8(p0), b1 = transpose_8x8(p1);
               if constexpr (PARTS == 1) {
-                // the offsets of these 16 keys, at once: the sum does not drift and cancel
-                mma_16816(o[nt][k][0], off0[0], off0[1], off0[2], off0[3], b0, b1);
-                mma_16816(o[nt][k][1], off1[0], off1[1], off1[2], off1[3], b0, b1);
                 mma_16816(o[nt][k][0], a[0][0], a[0][1], a[0][2], a[0][3], b0, b1);
                 mma_16816(o[nt][k][1], a[1][0], a[1][1], a[1][2], a[1][3], b0, b1);
               } else {
