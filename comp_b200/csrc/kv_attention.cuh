@@ -197,7 +197,8 @@ constexpr int kTileCost = 8;
 struct Span {
   int first, count;
 };
-template <int STG, int R>
+// One thread's answer, or (WARP) a warp's for the same tile, its lanes sharing the queries.
+template <int STG, int R, bool WARP = false>
 __device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
   const Sequence q = sequence(p, b);
   if (rt * R >= q.n * p.group) return {0, 0};
@@ -207,10 +208,12 @@ __device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
   if (!p.starts) {  // both ends grow with the position
     lo = query_span(p, b, i0, q.q0, q.n, q.len).lo, hi = query_span(p, b, i1, q.q0, q.n, q.len).hi;
   } else {
-    for (int i = i0; i <= i1; ++i) {
+#pragma unroll 4
+    for (int i = i0 + (WARP ? (int)(threadIdx.x & 31) : 0); i <= i1; i += WARP ? 32 : 1) {
       const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
       if (s.lo < s.hi) lo = min(lo, s.lo), hi = max(hi, s.hi);
     }
+    if (WARP) lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
   }
   if (lo >= hi) return {0, 1};
   return {lo / STG, (hi + STG - 1) / STG - lo / STG};
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   while (pos < end) {
     // -------------------------------------------------------------- the next tile of the share: (b, rt, h), its rows
     const int b = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - b * p.row_tiles;
-    const Span span = tile_span<STG, R>(p, b, rt);
+    const Span span = tile_span<STG, R, true>(p, b, rt);
     if (h == p.heads || span.count == 0) {
       ++entry, h = 0;
       continue;

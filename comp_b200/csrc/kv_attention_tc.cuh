@@ -31,7 +31,11 @@ struct TcTile {
   static constexpr int kRows = MT * 128, kKeys = 128;
   static constexpr int kQ = 128 * D * 2, kTile = 128 * D * 2;
   static constexpr int kSmem = MT * kQ + (kKeyBufs * kParts + kBufs) * kTile;
-  static constexpr int kSoftmaxWarps = MT * 4, kWarps = MT * 4 + 5;  // + 4 unpacking, 1 issuing
+  // 4 unpacking, then 1 issuing; with two row tiles three more, which only hand their registers on
+  static constexpr int kSoftmaxWarps = MT * 4, kWarps = MT == 2 ? 16 : MT * 4 + 5;
+  // registers of a thread at launch and after the split: 2 x 128 x 160 + 128 x 128 + 128 x 64 = 512 x 128
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kIssueRegs = 80;
+  static_assert(MT == 1 || 256 * kSoftmaxRegs + 128 * kLaunchRegs + 128 * kIssueRegs <= 512 * kLaunchRegs, "registers");
   static constexpr uint32_t kS = 256;                     // column of S (and P) of tile 0; O is at 0
 };
 
@@ -161,14 +165,10 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   // for this grid would leave both waiting.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Share share = plan_share<STG, R, C::kWarps>(p, 1, plan);
-  int64_t pos = share.pos;
-  if (pos >= share.end) {
+  if (share.pos >= share.end) {
     if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
     return;
   }
-  int entry = share.entry, h = share.head, skip = share.skip;
-  AttnJoin join = {-1, 0, 0, 0, 0};
-
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -203,11 +203,17 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
     return ok;
   };
 
+  // Each role runs through the share's tiles in code of its own, so that the registers it is given are its own too.
+  auto work = [&](auto role) {
+    constexpr int ROLE = decltype(role)::value;  // 0 softmax, 1 unpacking, 2 issuing
+  int64_t pos = share.pos;
+  int entry = share.entry, h = share.head, skip = share.skip;
+  AttnJoin join = {-1, 0, 0, 0, 0};
   uint32_t blocks = 0, done_tiles[2] = {0, 0}, done_blocks[2] = {0, 0}, segments = 0;  // so far: the barriers' phases
   while (pos < share.end) {
     // -------------------------------------------------------------- the next tile of the share, as in the other kernel
     const int b = p.row_tiles == 1 ? entry : entry / p.row_tiles, rt = entry - b * p.row_tiles;
-    const Span span = tile_span<STG, R>(p, b, rt);
+    const Span span = tile_span<STG, R, true>(p, b, rt);
     if (h == p.heads || span.count == 0) {
       ++entry, h = 0;
       continue;
@@ -224,7 +230,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
     if (p.lens[b] > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
     const int begin = span.first + from, n = to - from, tiles = MT == 1 || rows <= 128 ? 1 : 2;
 
-    if (warp < SW) {
+    if constexpr (ROLE == 0) {
       // ------------------------------------------------------------ softmax: a thread owns a row
       const int tile = warp >> 2, r = tile * 128 + (warp & 3) * 32 + lane, rr = rt * R + r;
       const bool there = r < rows;
@@ -243,12 +249,30 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         out_row = (q.q0 + i) * p.q_heads + head;
         slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;
         const int64_t src = (q.q0 + i) * p.q_st + (int64_t)head * p.q_sh;
+        // the row's 16-byte pieces, all in flight at once (heads of 256: in two halves, the second time from cache)
+        constexpr int kPieces = D / 8, kOnce = kPieces > 16 ? 16 : kPieces;
+        uint4 raw[kOnce];
+        auto load = [&](int c0) {
+          const uint4* at = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + src) + c0;
+#pragma unroll
+          for (int c = 0; c < kOnce; ++c) raw[c] = __ldg(at + c);
+        };
+        // values 2i, 2i + 1 of the pieces held
+        auto pair = [&](int i) -> float2 {
+          const uint4 x = raw[i / 4];
+          const uint32_t w = (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
+          if (p.dtype == B2Q_DTYPE_F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+          return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        };
         float top = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < D; c += 4) {
-          float v[4];
-          load4_as(p.q, src + c, p.dtype, v);
-          top = fmaxf(fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+        for (int c0 = kPieces - kOnce; c0 >= 0; c0 -= kOnce) {
+          load(c0);
+#pragma unroll
+          for (int i = 0; i < kOnce * 4; ++i) {
+            const float2 v = pair(i);
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
         }
         // to 2^6 .. 2^7: products with keys of up to 2^16 stay far below f32's range, and 16-bit queries exact
         const int e2 = max(-100, (__float_as_int(top) >> 23) - 127);
@@ -256,20 +280,23 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         rowf = __int_as_float((127 + e2 - 6) << 23) * p.scale;
         rowf *= p.softcap > 0.f ? 2.f * kLog2e / p.softcap : kLog2e;
         mul = rowf;
-#pragma unroll 2
-        for (int w = 0; w < NB * 4; ++w) {  // chunk w = word (t, block) of a packed key: its 8 values in its order
-          const int t = w / NB, k = w - t * NB;
-          float a[4], z[4];
-          load4_as(p.q, src + 32 * k + (FMT == 0 ? 4 : 8) * t, p.dtype, a);
-          load4_as(p.q, src + 32 * k + (FMT == 0 ? 16 + 4 * t : 8 * t + 4), p.dtype, z);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] *= up, z[e] *= up;
-          uint4 x;
-          if (FMT == 0)
-            x = make_uint4(pack_half2(a[0], a[2]), pack_half2(z[0], z[2]), pack_half2(a[1], a[3]), pack_half2(z[1], z[3]));
-          else
-            x = make_uint4(pack_half2(a[0], a[1]), pack_half2(a[2], a[3]), pack_half2(z[0], z[1]), pack_half2(z[2], z[3]));
-          *reinterpret_cast<uint4*>(my_q + w * 2048) = x;
+        for (int c0 = 0; c0 < kPieces; c0 += kOnce) {
+          if (c0 > 0) load(c0);
+#pragma unroll
+          for (int w = 0; w < kOnce; ++w) {  // chunk (t, block) = a word of a packed key: its 8 values in its order
+            const int k = w / 4, t = w & 3;
+            // first and second run of 4 values
+            float2 a0 = pair(16 * k + (FMT == 0 ? 2 : 4) * t), a1 = pair(16 * k + (FMT == 0 ? 2 : 4) * t + 1);
+            float2 z0 = pair(16 * k + (FMT == 0 ? 8 + 2 * t : 4 * t + 2)), z1 = pair(16 * k + (FMT == 0 ? 9 + 2 * t : 4 * t + 3));
+            a0.x *= up, a0.y *= up, a1.x *= up, a1.y *= up, z0.x *= up, z0.y *= up, z1.x *= up, z1.y *= up;
+            uint4 x;
+            if (FMT == 0)
+              x = make_uint4(pack_half2(a0.x, a1.x), pack_half2(z0.x, z1.x), pack_half2(a0.y, a1.y), pack_half2(z0.y, z1.y));
+            else
+              x = make_uint4(pack_half2(a0.x, a0.y), pack_half2(a1.x, a1.y), pack_half2(z0.x, z0.y), pack_half2(z1.x, z1.y));
+            *reinterpret_cast<uint4*>(my_q + (t * NB + c0 / 4 + k) * 2048) = x;
+          }
         }
       } else if (tile < tiles) {
 #pragma unroll 2
@@ -287,43 +314,16 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           // masked or special scores are finished in the first pass and put back
           const bool mask = __any_sync(0xffffffffu, kb < lo || kb + STG > hi), careful = special || mask;
           const float scale = careful ? 1.f : mul;
-          uint32_t v[32];
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < STG; c += 32) {
-            tc::tmem_ld32_nowait(col_s + c, v);
-            tc::tmem_wait_ld32(v);
-            if (careful) {
-              // softcap: cap - 2 cap / (2^(x rowf) + 1), rowf to twice the capped argument's exponent of 2
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                float x = __uint_as_float(v[e]) * rowf;
-                if (p.softcap > 0.f) x = fmaf(__fdividef(1.f, exp2_approx(x) + 1.f), -2.f * cap, cap);
-                v[e] = __float_as_uint(x);
-              }
-              if (p.slopes) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  v[e] = __float_as_uint(fmaf(-slope, fabsf((float)(where - kb - c - e)), __uint_as_float(v[e])));
-              }
-              if (mask) {
-                const int from_e = lo - kb - c, to_e = hi - kb - c;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = e >= from_e && e < to_e ? v[e] : 0xff800000u;
-              }
-              tc::tmem_st32(col_s + c, v);
-            }
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-          }
-          if (careful) tc::tmem_wait_st();
-          top *= scale;
-          if (__any_sync(0xffffffffu, top > ref + 8.f)) {
-            const float now = top > ref + 8.f ? top : ref, f = exp2_approx(ref - now);
+          // takes the reference to the row's maximum where that has grown by more than 2^8, and O with it
+          auto follow = [&](float top) {
+            const bool grown = top > ref + 8.f;
+            if (!__any_sync(0xffffffffu, grown)) return;
+            const float now = grown ? top : ref, f = exp2_approx(ref - now);
             ref = now, sum *= f;
             if (j > 0) {  // the block before is in O already: its product ended before this block's scores
 #pragma unroll 1
               for (int c = 0; c < D; c += 32) {
+                uint32_t v[32];
                 tc::tmem_ld32_nowait(col_o + c, v);
                 tc::tmem_wait_ld32(v);
 #pragma unroll
@@ -331,23 +331,60 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
                 tc::tmem_st32(col_o + c, v);
               }
             }
-          }
-          float s0 = 0.f, s1 = 0.f;
+          };
+          // Two passes over S, 32 columns at a time: for the maximum (masked and special scores are finished then, and put
+          // back), and for the weights.
+          float top = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < STG; c += 32) {
-            tc::tmem_ld32_nowait(col_s + c, v);
-            tc::tmem_wait_ld32(v);
-            uint32_t w[16];
+            uint32_t x[32];
+            tc::tmem_ld32_nowait(col_s + c, x);
+            tc::tmem_wait_ld32(x);
+            if (careful) {
+              if (p.softcap > 0.f) {  // cap - 2 cap / (2^(x rowf) + 1), rowf to twice the capped argument's exponent of 2
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[e] = __float_as_uint(
+                      fmaf(__fdividef(1.f, exp2_approx(__uint_as_float(x[e]) * rowf) + 1.f), -2.f * cap, cap));
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * rowf);
+              }
+              if (p.slopes) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[e] = __float_as_uint(fmaf(-slope, fabsf((float)(where - kb - c - e)), __uint_as_float(x[e])));
+              }
+              if (mask) {
+                const int from_e = lo - kb - c, to_e = hi - kb - c;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = e >= from_e && e < to_e ? x[e] : 0xff800000u;
+              }
+              tc::tmem_st32(col_s + c, x);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+          }
+          if (careful) tc::tmem_wait_st();
+          follow(top * scale);
+          float2 s01 = make_float2(0.f, 0.f);
+          const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
+#pragma unroll 1
+          for (int c = 0; c < STG; c += 32) {
+            uint32_t x[32], w[16];
+            tc::tmem_ld32_nowait(col_s + c, x);
+            tc::tmem_wait_ld32(x);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float a = exp2_approx(fmaf(__uint_as_float(v[e]), scale, -ref));
-              const float z = exp2_approx(fmaf(__uint_as_float(v[e + 1]), scale, -ref));
-              s0 += a, s1 += z;
-              w[e / 2] = pack_half2(a, z);
+              float2 y = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+              y = __ffma2_rn(y, scale2, ref2);
+              y.x = exp2_approx(y.x), y.y = exp2_approx(y.y);
+              s01 = __fadd2_rn(s01, y);
+              w[e / 2] = pack_half2(y.x, y.y);
             }
             tc::tmem_st16(col_s + c / 2, w);  // columns of S that have been read
           }
-          sum += s0 + s1;
+          sum += s01.x + s01.y;
           tc::tmem_wait_st();
           tc::fence_before();
           tc::arrive(smem_addr(&b_p[tile]));
@@ -390,7 +427,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           tc::fence_before();
         }
       }
-    } else if (warp < SW + 4) {
+    } else if constexpr (ROLE == 1) {
       // ------------------------------------------------------------ unpacking: a thread a key, then 8 keys' columns
       const int th = threadIdx.x - SW * 32, kg = th >> 3, g = th & 7;
       const int32_t* table = p.table + (int64_t)b * p.table_stride;
@@ -510,7 +547,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         tc::fence_async_smem();
         tc::arrive(smem_addr(&b_vfull[vbuf]));
       }
-    } else if (lane == 0) {
+    } else if (warp == SW + 4 && lane == 0) {
       // ------------------------------------------------------------ the products, issued in the order in which they run
       const uint32_t is = tc::instr_desc_f16(STG), io = tc::instr_desc_f16(D);
       const uint64_t dq = tc::smem_desc_kmajor(q_smem, 2048), dk = tc::smem_desc_kmajor(k_smem, 2048);
@@ -566,9 +603,24 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
     pos += take, skip += take;
     if (skip == units) skip = 0, ++h;
     tc::fence_before();
-    __syncthreads();  // the queries' memory, O and S are free
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(C::kWarps * 32) : "memory");  // the queries' memory, O and S are free
     tc::fence_after();
     if (s_abort) break;
+  }
+  if (ROLE == 0 && threadIdx.x == 0) {
+    if (s_abort) join.first = -1;
+    p.joins[blockIdx.x] = join;
+  }
+  };
+  if (warp < SW) {
+    if constexpr (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+    work(std::integral_constant<int, 0>{});
+  } else if (warp < SW + 4) {
+    work(std::integral_constant<int, 1>{});
+  } else {
+    if constexpr (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kIssueRegs));
+    work(std::integral_constant<int, 2>{});
   }
   // nothing is in flight: a segment ends when its last products have been waited for. Where a wait ran out, they may not
   // have: let the products issued so far end (they need nothing more) before their memory goes away.
@@ -578,12 +630,10 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
     }
     if (threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
-    join.first = -1;
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
@@ -595,6 +645,18 @@ static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t str
   static std::atomic<unsigned long long> allowed{0};
   int rc = allow_smem_once(reinterpret_cast<const void*>(kernel), C::kSmem, allowed);
   if (rc) return rc;
+  if (C::MT == 2) {  // the split waits for registers that the block was not launched with: never launch it short of them
+    static std::atomic<int> regs{0};
+    if (!regs.load(std::memory_order_relaxed)) {
+      cudaFuncAttributes attr;
+      const cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+      if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_attention: %s", cudaGetErrorString(e));
+      regs.store(attr.numRegs, std::memory_order_relaxed);
+    }
+    if (regs.load(std::memory_order_relaxed) != C::kLaunchRegs)
+      return fail(B2Q_ECUDA, "b2q_attention: built with %d registers a thread, not %d",
+                  regs.load(std::memory_order_relaxed), C::kLaunchRegs);
+  }
   launch_maybe_pdl(kernel, dim3((unsigned)sms), dim3(C::kWarps * 32), C::kSmem, stream, p);
   rc = after_launch("attention_tc");
   if (rc) return rc;
