@@ -39,19 +39,20 @@ constexpr float kNoRef = -1e30f;  // reference exponent of a row that has seen n
 template <int FMT, int NB>
 struct KvTile {
   static constexpr int kRow = NB * (FMT == 0 ? 16 : 32);  // quant bytes of a token's row
-  // tokens a stage: at most 9216 bytes, so that 12 warps with two stages each fill an SM
-  static constexpr int kTokens = kRow <= 32 ? 128 : (kRow <= 64 ? 64 : (kRow <= 128 ? 32 : 16));
+  // tokens a stage: at most 9216 bytes, so that 12 warps with two stages (four of the
+  // smallest rows) each fill an SM
+  static constexpr int kTokens = kRow <= 64 ? 64 : (kRow <= 128 ? 32 : 16);
   static constexpr int kQuants = kTokens * kRow, kScales = kTokens * NB * 2;
   static constexpr int kStage = 2 * (kQuants + kScales);
   static constexpr int kWarps = 4;
-  static constexpr int kStages = 2;
+  static constexpr int kStages = kRow <= 32 ? 4 : 2;
   static constexpr int kRing = kStage * kStages * kWarps;
 };
 
 // CTAs an SM: as many as their registers and rings leave room for.
 template <int FMT, int NB, int NT, int PARTS>
 constexpr int kv_ctas_per_sm() {
-  return NB == 8 || NT == 2 || PARTS == 2 ? 2 : 3;
+  return NB == 8 || NT == 2 || (PARTS == 2 && NB > 2) ? 2 : 3;
 }
 
 // Row r of a 16-token tile is this token: chosen so that both the key loads (lanes of two rows side by side) and the
@@ -531,6 +532,17 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
       // UN sub-tiles of 16 keys at a time: their chains of dependent instructions overlap. Twice: with (careful) and
       // without what only some calls and a sequence's ends need, so that the common loop is short and runs straight on.
       auto steps = [&](auto careful) {
+        float rowf[NT][2], slope[NT][2];
+        int where[NT][2];
+        if (careful.value && special) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int r = nt * 8 + 2 * t + c;
+              rowf[nt][c] = s_rowf[r], slope[nt][c] = s_slope[r], where[nt][c] = s_pos[r] - st * STG - tokA;
+            }
+        }
 #pragma unroll 1
       for (int u0 = 0; u0 < SUB; u0 += UN) {
         // ---- scores
@@ -588,10 +600,10 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const int r = nt * 8 + 2 * t + (e & 1), j = st * STG + (u0 + i) * 16 + tokA + (e >> 1) * 8;
-                float y = x[i][nt][e] * s_rowf[r];
+                float y = x[i][nt][e] * rowf[nt][e & 1];
                 if (p.softcap > 0.f) y = soft_cap(y, p.softcap, inv_cap) * kLog2e;
-                x[i][nt][e] = y - s_slope[r] * (float)abs(s_pos[r] - j);
+                const int far = where[nt][e & 1] - (u0 + i) * 16 - (e >> 1) * 8;
+                x[i][nt][e] = fmaf(-slope[nt][e & 1], fabsf((float)far), y);
               }
         }
         if (careful.value && !whole) {

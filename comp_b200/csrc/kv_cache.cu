@@ -26,33 +26,41 @@ __device__ __forceinline__ void load_quarter(const T* block, int l, float (&v)[8
   }
 }
 
+// floor of 0 <= x < 2^23 in the low bits of the result: one addition rounded down, where a conversion would take the unit
+// of the special functions (measured: 16384 tokens' write 25 -> WRITE us with the conversions and index search gone).
+__device__ __forceinline__ uint32_t floor_bits(float x) { return __float_as_uint(__fadd_rd(x, 8388608.f)); }
+
 // ggml's q4_0 block of 32 values held by 4 consecutive lanes (values 4l.. and 16+4l..): the lane's 4 bytes, f16 d bits.
 __device__ __forceinline__ uint32_t quant_q4_0_quarter(const float (&v)[8], int l, uint16_t* d_bits) {
-  float mag = 0.f;
+  float hi = v[0], lo = v[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) mag = fmaxf(mag, fabsf(v[i]));
-  mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
-  mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
-  // the first value of that magnitude decides d's sign: the lowest (index, sign) among the lanes
-  int first = 64;
+  for (int i = 1; i < 8; ++i) hi = fmaxf(hi, v[i]), lo = fminf(lo, v[i]);
 #pragma unroll
-  for (int i = 7; i >= 0; --i)
-    if (fabsf(v[i]) == mag) first = 2 * ((i < 4 ? 0 : 12) + 4 * l + i) + (signbit(v[i]) ? 1 : 0);
-  first = min(first, __shfl_xor_sync(0xffffffffu, first, 1));
-  first = min(first, __shfl_xor_sync(0xffffffffu, first, 2));
-  const float d = __fmul_rn((first & 1) ? -mag : mag, -0.125f);  // m / -8, exact but for underflow
-  const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int q = max(0, min(15, (int)__fadd_rn(__fmul_rn(v[i], id), 8.5f)));
-    w |= (uint32_t)q << ((i & 3) * 8 + (i >> 2) * 4);
+  for (int o = 1; o < 4; o <<= 1) {
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
+  float m = hi >= -lo ? hi : lo;  // the value of largest magnitude
+  if (__any_sync(0xffffffffu, hi == -lo)) {  // both signs have it somewhere in the warp: there the first one counts
+    int first = 64;
+#pragma unroll
+    for (int i = 7; i >= 0; --i)
+      if (fabsf(v[i]) == hi) first = 2 * ((i < 4 ? 0 : 12) + 4 * l + i) + (signbit(v[i]) ? 1 : 0);
+    first = min(first, __shfl_xor_sync(0xffffffffu, first, 1));
+    first = min(first, __shfl_xor_sync(0xffffffffu, first, 2));
+    if (hi == -lo) m = (first & 1) ? lo : hi;
+  }
+  const float d = __fmul_rn(m, -0.125f);  // m / -8, exact but for underflow
+  const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
+  uint32_t q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = floor_bits(fminf(__fadd_rn(__fmul_rn(v[i], id), 8.5f), 15.5f));  // 0.5 .. 15.5
   *d_bits = __half_as_ushort(__float2half_rn(d));
-  return w;
+  return pack_low_bytes(q[0], q[1], q[2], q[3]) | pack_low_bytes(q[4], q[5], q[6], q[7]) << 4;
 }
 
-// ggml's q8_0 block, the quants plus 128: the lane's 8 bytes (values 8l..8l+7).
+// ggml's q8_0 block, the quants plus 128: the lane's 8 bytes (values 8l..8l+7). roundf(y) is the floor of |y| + 1/2 cut off
+// (no sum that is cut off reaches a whole number that it does not hold), with y's sign.
 __device__ __forceinline__ uint2 quant_q8_0_quarter(const float (&v)[8], uint16_t* d_bits) {
   float amax = 0.f;
 #pragma unroll
@@ -61,14 +69,15 @@ __device__ __forceinline__ uint2 quant_q8_0_quarter(const float (&v)[8], uint16_
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   const float d = __fdiv_rn(amax, 127.0f);
   const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
-  uint32_t w[2] = {0, 0};
+  uint32_t q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int q = (int)roundf(__fmul_rn(v[i], id)) + 128;
-    w[i >> 2] |= (uint32_t)(q & 0xff) << ((i & 3) * 8);
+    const float y = __fmul_rn(v[i], id);
+    const uint32_t r = floor_bits(__fadd_rz(fabsf(y), 0.5f));
+    q[i] = signbit(y) ? 128u - r : 128u + r;  // the low byte
   }
   *d_bits = __half_as_ushort(__float2half_rn(d));
-  return make_uint2(w[0], w[1]);
+  return make_uint2(pack_low_bytes(q[0], q[1], q[2], q[3]), pack_low_bytes(q[4], q[5], q[6], q[7]));
 }
 
 // N 16-bit words (two to a register) to `dst`, and back, in the widest pieces that N's alignment allows.
