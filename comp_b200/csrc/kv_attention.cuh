@@ -151,12 +151,16 @@ __device__ __forceinline__ void store_elt(void* p, int64_t i, int dtype, float v
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// cap * tanh(x / cap): an odd polynomial below 1/4 (next term under 3e-9 of it), 1 - 2 / (e^2z + 1) above.
-__device__ __forceinline__ float soft_cap(float x, float cap, float inv_cap) {
-  const float z = fabsf(x * inv_cap), z2 = z * z;
-  const float poly = z * fmaf(z2, fmaf(z2, fmaf(z2, fmaf(z2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-  const float far = 1.f - __fdividef(2.f, exp2_approx(z * (2.f * kLog2e)) + 1.f);
-  return copysignf(cap * (z < 0.25f ? poly : far), x);
+// tanh(z) / z of u = z^2 for |z| <= 0.6: fitted to the smallest largest relative error (7.3e-8). Beyond, tanh(|z|) =
+// 1 - 2 / (e^2z + 1); scores near the cap are rare, and where a warp has none it skips that (two of the slow units' steps).
+constexpr float kTanhLimit = 0.6f;
+constexpr float kTanh0 = 0.99999994f, kTanh1 = -0.3333231f, kTanh2 = 0.13310172f, kTanh3 = -0.05210143f, kTanh4 = 0.015475366f;
+__device__ __forceinline__ float tanh_near(float z) {
+  const float u = z * z;
+  return z * fmaf(u, fmaf(u, fmaf(u, fmaf(u, kTanh4, kTanh3), kTanh2), kTanh1), kTanh0);
+}
+__device__ __forceinline__ float tanh_far(float z) {
+  return copysignf(1.f - __fdividef(2.f, exp2_approx(fabsf(z) * (2.f * kLog2e)) + 1.f), z);
 }
 
 // Position and visible keys [lo, hi) of query i of sequence b.
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
         if (l == 0) s_start[r * NB + k] = sum * (-kOff * 0x1p-24f);
         if (c == 0) {
           float f = __int_as_float((127 + e2 - 13) << 23) * p.scale * (SIGNED ? 1.f : 0x1p24f);
-          if (p.softcap <= 0.f) f *= kLog2e;
+          f *= p.softcap > 0.f ? 1.f / p.softcap : kLog2e;
           s_rowf[r] = f;
         }
       }
@@ -593,18 +597,49 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
           lds_scales<NB>(vscales + (rowA + 8) * NB * 2, dB[i]);
         }
         if (careful.value && special) {
-          const float inv_cap = p.softcap > 0.f ? 1.f / p.softcap : 0.f;
+          if (p.softcap > 0.f) {  // rowf makes these the cap's arguments
+            float far = 0.f;
 #pragma unroll
-          for (int i = 0; i < UN; ++i)
+            for (int i = 0; i < UN; ++i)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float y = x[i][nt][e] * rowf[nt][e & 1];
-                if (p.softcap > 0.f) y = soft_cap(y, p.softcap, inv_cap) * kLog2e;
-                const int far = where[nt][e & 1] - (u0 + i) * 16 - (e >> 1) * 8;
-                x[i][nt][e] = fmaf(-slope[nt][e & 1], fabsf((float)far), y);
-              }
+                for (int e = 0; e < 4; ++e) {
+                  x[i][nt][e] *= rowf[nt][e & 1];
+                  far = fmaxf(far, fabsf(x[i][nt][e]));
+                }
+            const float cap = p.softcap * kLog2e;
+            const bool any_far = __any_sync(0xffffffffu, far > kTanhLimit);
+#pragma unroll
+            for (int i = 0; i < UN; ++i)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float z = x[i][nt][e];
+                  float y = tanh_near(z);
+                  if (any_far) y = fabsf(z) <= kTanhLimit ? y : tanh_far(z);
+                  x[i][nt][e] = cap * y;
+                }
+          } else {
+#pragma unroll
+            for (int i = 0; i < UN; ++i)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][nt][e] *= rowf[nt][e & 1];
+          }
+          if (p.slopes) {
+#pragma unroll
+            for (int i = 0; i < UN; ++i)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int far = where[nt][e & 1] - (u0 + i) * 16 - (e >> 1) * 8;
+                  x[i][nt][e] = fmaf(-slope[nt][e & 1], fabsf((float)far), x[i][nt][e]);
+                }
+          }
         }
         if (careful.value && !whole) {
 #pragma unroll

@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         const int e2 = max(-100, (__float_as_int(top) >> 23) - 127);
         const float up = __int_as_float((127 + 6 - e2) << 23);
         rowf = __int_as_float((127 + e2 - 6) << 23) * p.scale;
-        rowf *= p.softcap > 0.f ? 2.f * kLog2e / p.softcap : kLog2e;
+        rowf *= p.softcap > 0.f ? 1.f / p.softcap : kLog2e;
         mul = rowf;
 #pragma unroll
         for (int c0 = 0; c0 < kPieces; c0 += kOnce) {
@@ -341,14 +341,35 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
             tc::tmem_ld32_nowait(col_s + c, x);
             tc::tmem_wait_ld32(x);
             if (careful) {
-              if (p.softcap > 0.f) {  // cap - 2 cap / (2^(x rowf) + 1), rowf to twice the capped argument's exponent of 2
+              const float2 rowf2 = make_float2(rowf, rowf);
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[e] = __float_as_uint(
-                      fmaf(__fdividef(1.f, exp2_approx(__uint_as_float(x[e]) * rowf) + 1.f), -2.f * cap, cap));
-              } else {
+              for (int e = 0; e < 32; e += 2) {
+                const float2 y = __fmul2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), rowf2);
+                x[e] = __float_as_uint(y.x), x[e + 1] = __float_as_uint(y.y);
+              }
+              if (p.softcap > 0.f) {  // rowf made these the cap's arguments
+                float far = 0.f;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * rowf);
+                for (int e = 0; e < 32; ++e) far = fmaxf(far, fabsf(__uint_as_float(x[e])));
+                if (!__any_sync(0xffffffffu, far > kTanhLimit)) {
+#pragma unroll
+                  for (int e = 0; e < 32; e += 2) {  // cap * tanh_near, two at a time
+                    const float2 z = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), u = __fmul2_rn(z, z);
+                    float2 y = make_float2(kTanh4, kTanh4);
+                    y = __ffma2_rn(y, u, make_float2(kTanh3, kTanh3));
+                    y = __ffma2_rn(y, u, make_float2(kTanh2, kTanh2));
+                    y = __ffma2_rn(y, u, make_float2(kTanh1, kTanh1));
+                    y = __ffma2_rn(y, u, make_float2(kTanh0, kTanh0));
+                    y = __fmul2_rn(y, __fmul2_rn(z, make_float2(cap, cap)));
+                    x[e] = __float_as_uint(y.x), x[e + 1] = __float_as_uint(y.y);
+                  }
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) {
+                    const float z = __uint_as_float(x[e]);
+                    x[e] = __float_as_uint(cap * (fabsf(z) <= kTanhLimit ? tanh_near(z) : tanh_far(z)));
+                  }
+                }
               }
               if (p.slopes) {
 #pragma unroll
