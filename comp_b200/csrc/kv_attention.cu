@@ -10,9 +10,12 @@ struct AttnPlan {
 };
 
 // 16-bit calls with at least kTcLeastRows query rows a sequence and KV head take the tensor-core kernels (but not those with
-// heads of 256 and lse: shared memory has no room for keys in two parts). Else the rows of
-// a tile are 8, or 16 where more have to read the cache anyway (heads of 256 leave registers for 8).
-constexpr int kTcLeastRows = 64;
+// heads of 256 and lse: shared memory has no room for keys in two parts). Measured, us, streaming / tensor cores: 16
+// sequences of 4096 keys, 8 KV heads of 128: 32 rows 69 / 91, 48 rows 94 / 92, 64 rows 118 / 95, 256 rows 415 / 123; one of
+// 8192: 24 / 25 at 48, 64 / 37 at 256; 16 of 4096, heads of 256: 156 / 174 at 32, 226 / 181 at 48. (One of 500 keys: 16 / 16
+// at 48, 21 / 27 at 256: that little work is launches and tile ends.) Else the rows of a tile are 8, or 16 where more have
+// to read the cache anyway (heads of 256 leave registers for 8).
+constexpr int kTcLeastRows = 48;
 
 static AttnPlan plan_attention(const b2q_kv_cache& c, const b2q_attention_args& a) {
   AttnPlan pl;

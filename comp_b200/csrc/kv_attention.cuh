@@ -874,56 +874,56 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   if (threadIdx.x == 0) p.joins[blockIdx.x] = join;
 }
 
-// Joins the parts of tiles that several CTAs worked on: one warp for each CTA that ended such a tile and each of its
-// rows, its lanes over the dimension. The CTA that began the tile left its second part, the others their first.
+// Joins the parts of tiles that several CTAs worked on: CTAs (c, y) for each CTA c that ended such a tile, a warp a row at
+// a time, its lanes over the dimension. The CTA that began the tile left its second part, the others their first.
 template <int NB, int R>
-__global__ void __launch_bounds__(128) attention_join_kernel(const AttnParams p, int ctas) {
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttnParams p) {
   constexpr int D = NB * 32;
   pdl_wait_then_trigger();
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int cta = item / R, r = item - cta * R;
-  if (cta >= ctas) return;
+  const int cta = blockIdx.x, lane = threadIdx.x & 31;
   const AttnJoin join = p.joins[cta];
-  if (join.first < 0 || r >= join.rows) return;
-  const int rr = join.row0 + r, qi = p.cu_q ? rr / p.group : 0;
-  const int64_t out_row = (int64_t)(join.q0 + qi) * p.q_heads + join.head0 + (rr - qi * p.group);
-  const int n = cta - join.first + 1;
-  auto part_of = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? 1 : 0)) * R + r; };
-  float top = kNoRef, l = 0.f, y[NB];
+  if (join.first < 0) return;
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < join.rows; r += gridDim.y * 4) {
+    const int rr = join.row0 + r, qi = p.cu_q ? rr / p.group : 0;
+    const int64_t out_row = (int64_t)(join.q0 + qi) * p.q_heads + join.head0 + (rr - qi * p.group);
+    const int n = cta - join.first + 1;
+    auto part_of = [&](int i) { return (int64_t)(2 * (join.first + i) + (i == 0 ? 1 : 0)) * R + r; };
+    float top = kNoRef, l = 0.f, y[NB];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) y[i] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {  // 32 parts at a time: a lane holds the reference and sum of one
-    const int m = min(32, n - i0);
-    const float2 v = lane < m ? p.part_m[part_of(i0 + lane)] : make_float2(kNoRef, 0.f);
-    float now = fmaxf(top, v.x);
+    for (int i = 0; i < NB; ++i) y[i] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {  // 32 parts at a time: a lane holds the reference and sum of one
+      const int m = min(32, n - i0);
+      const float2 v = lane < m ? p.part_m[part_of(i0 + lane)] : make_float2(kNoRef, 0.f);
+      float now = fmaxf(top, v.x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
-    const float old = exp2_approx(top - now), f = lane < m ? exp2_approx(v.x - now) : 0.f;
-    float s = v.y * f;
+      for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+      const float old = exp2_approx(top - now), f = lane < m ? exp2_approx(v.x - now) : 0.f;
+      float s = v.y * f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    l = fmaf(l, old, s), top = now;
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      l = fmaf(l, old, s), top = now;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) y[i] *= old;
-    constexpr int kOnce = NB <= 4 ? 16 : 8;  // loads of so many parts in flight
-    for (int j0 = 0; j0 < m; j0 += kOnce) {
-      float z[kOnce][NB];
+      for (int i = 0; i < NB; ++i) y[i] *= old;
+      constexpr int kOnce = NB <= 4 ? 16 : 8;  // loads of so many parts in flight
+      for (int j0 = 0; j0 < m; j0 += kOnce) {
+        float z[kOnce][NB];
 #pragma unroll
-      for (int j = 0; j < kOnce; ++j)
+        for (int j = 0; j < kOnce; ++j)
 #pragma unroll
-        for (int c = 0; c < NB; ++c) z[j][c] = j0 + j < m ? p.part_o[part_of(i0 + j0 + j) * D + c * 32 + lane] : 0.f;
+          for (int c = 0; c < NB; ++c) z[j][c] = j0 + j < m ? p.part_o[part_of(i0 + j0 + j) * D + c * 32 + lane] : 0.f;
 #pragma unroll
-      for (int j = 0; j < kOnce; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, j0 + j);  // 0 past the last part
+        for (int j = 0; j < kOnce; ++j) {
+          const float fj = __shfl_sync(0xffffffffu, f, j0 + j);  // 0 past the last part
 #pragma unroll
-        for (int c = 0; c < NB; ++c) y[c] = fmaf(z[j][c], fj, y[c]);
+          for (int c = 0; c < NB; ++c) y[c] = fmaf(z[j][c], fj, y[c]);
+        }
       }
     }
-  }
-  const float inv = l > 0.f || l != l ? __fdividef(1.f, l) : 0.f;
+    const float inv = l > 0.f || l != l ? __fdividef(1.f, l) : 0.f;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) store_elt(p.out, out_row * D + i * 32 + lane, p.dtype, y[i] * inv);
-  if (p.lse && lane == 0) p.lse[out_row] = (top + log2f(l)) * kLn2;
+    for (int i = 0; i < NB; ++i) store_elt(p.out, out_row * D + i * 32 + lane, p.dtype, y[i] * inv);
+    if (p.lse && lane == 0) p.lse[out_row] = (top + log2f(l)) * kLn2;
+  }
 }
 
 template <int FMT, int NB, int NT, int PARTS>
@@ -945,8 +945,7 @@ static int launch_attention_as(const AttnParams& p, int sms, int64_t max_len, cu
   launch_maybe_pdl(kernel, dim3((unsigned)ctas), dim3(128), kSmem, stream, p);
   rc = after_launch("attention");
   if (rc) return rc;
-  const int64_t warps = ctas * NT * 8;
-  launch_maybe_pdl(attention_join_kernel<NB, NT * 8>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p, (int)ctas);
+  launch_maybe_pdl(attention_join_kernel<NB, NT * 8>, dim3((unsigned)ctas, NT * 2), dim3(128), 0, stream, p);
   return after_launch("attention_join");
 }
 

@@ -236,10 +236,10 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       const bool there = r < rows;
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t col_s = tmem + lanes + C::kS + tile * 128, col_o = tmem + lanes + tile * 128;
-      int lo = 0, hi = 0, where = 0;
+      int lo = 0, hi = INT_MAX, where = 0;  // rows that are not there need no mask: nothing of theirs is kept
       float mul = 1.f, rowf = 0.f, slope = 0.f;
       int64_t out_row = 0;
-      const bool special = p.softcap > 0.f || p.slopes != nullptr;
+      const bool special = (p.softcap > 0.f || p.slopes != nullptr) && __any_sync(0xffffffffu, there);
       const float cap = p.softcap * kLog2e;
       uint8_t* my_q = smem + tile * C::kQ + (r & 127) * 16;
       if (there) {
@@ -681,8 +681,7 @@ static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t str
   launch_maybe_pdl(kernel, dim3((unsigned)sms), dim3(C::kWarps * 32), C::kSmem, stream, p);
   rc = after_launch("attention_tc");
   if (rc) return rc;
-  launch_maybe_pdl(attention_join_kernel<NB, C::kRows>, dim3((unsigned)(sms * C::kRows / 4)), dim3(128), 0, stream, p,
-                   sms);
+  launch_maybe_pdl(attention_join_kernel<NB, C::kRows>, dim3((unsigned)sms, 16), dim3(128), 0, stream, p);
   return after_launch("attention_join");
 }
 
