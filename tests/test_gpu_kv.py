@@ -284,7 +284,7 @@ def test_default_bounds_and_fused_queries(cuda):
     ws = torch.full((size,), 255, dtype=torch.uint8, device=cuda)  # whatever it held
     got = kv.attention(wide[:, :8], cache, t[0], t[1], cu_q=t[2], max_q=9, out=out, workspace=ws)
     assert got is out and torch.equal(out, want)
-    # max_q left out: T bounds it (here over 64 rows, so that the other kernels run)
+    # max_q left out: T bounds it
     keys, values = _gather("q4_0", planes, table, lens)
     o, _, reach, mass = ref.attention(q.float().numpy(), keys, values, lens, cu, 128**-0.5)
     bound, _ = _bounds("f16", True, False, 128, 0.0, o, reach, mass)
