@@ -198,8 +198,9 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int b) {
   return s;
 }
 
-// What beginning a tile costs a CTA, in stages of its share (measured: 6 us against 0.8 us a stage): without it, a share
-// of many short tiles takes far longer than one long run (decode of 64 sequences of 100 to 8192 tokens).
+// What beginning a tile costs a CTA, in stages of its share (measured: 6 us against 0.8 us a stage of 64 keys): without it,
+// a share of many short tiles takes far longer than one long run (64 sequences of 100 to 8192 tokens: 115 us, so 80; with
+// 4 stages 89, with 14 82).
 constexpr int kTileCost = 8;
 
 // The stages that hold the visible keys of row tile rt of sequence b: `count` is 0 for a tile without rows and at least 1
@@ -229,10 +230,11 @@ __device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
   return {lo / STG, (hi + STG - 1) / STG - lo / STG};
 }
 
-__device__ __forceinline__ int tile_units(Span s) { return s.count ? s.count + kTileCost : 0; }
+// A tile's units of a share: `cost` without stages, then its stages.
+__device__ __forceinline__ int tile_units(Span s, int cost) { return s.count ? s.count + cost : 0; }
 
-// The plan: every CTA an equal share of all stages. Entries (sequence, row tile) have their stages, after kTileCost units
-// without any, once a KV head; a CTA's share is [pos, end) of their run, at least `least` units (unless none are left),
+// The plan: every CTA an equal share of all stages. Entries (sequence, row tile) have their stages, after COST units without
+// any, once a KV head; a CTA's share is [pos, end) of their run, at least `least` units (unless none are left),
 // and begins `skip` units into the tile of (entry, head). All W warps call it; the scratch is read until the barrier
 // that ends it.
 struct Share {
@@ -244,7 +246,7 @@ struct ShareScratch {
   int64_t scan[W];
   int entry, head, skip;
 };
-template <int STG, int R, int W>
+template <int STG, int R, int W, int COST>
 __device__ __forceinline__ Share plan_share(const AttnParams& p, int least, ShareScratch<W>& scratch) {
   constexpr int kThreads = W * 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -252,7 +254,7 @@ __device__ __forceinline__ Share plan_share(const AttnParams& p, int least, Shar
   const int e0 = min(entries, (int)threadIdx.x * chunk), e1 = min(entries, e0 + chunk);
   Share s;
   int64_t mine = 0;
-  for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
+  for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles), COST);
   mine *= p.heads;
   int64_t upto = mine;
 #pragma unroll
@@ -277,7 +279,7 @@ __device__ __forceinline__ Share plan_share(const AttnParams& p, int least, Shar
   if (s.pos < s.end && s.pos >= upto - mine && s.pos < upto) {  // the thread whose entries hold the beginning
     int64_t off = s.pos - (upto - mine);
     for (int e = e0; e < e1; ++e) {
-      const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles));
+      const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles), COST);
       if (off < (int64_t)count * p.heads) {
         int h = 0;
         while (off >= count) off -= count, ++h;
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   pdl_wait_then_trigger();
 
   __shared__ ShareScratch<W> plan;
-  const Share share = plan_share<STG, R, W>(p, W, plan);
+  const Share share = plan_share<STG, R, W, kTileCost>(p, W, plan);
   const int64_t per = share.per, end = share.end;
   int64_t pos = share.pos;
   if (pos >= end) {
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
       ++entry, h = 0;
       continue;
     }
-    const int units = tile_units(span), take = (int)min((int64_t)(units - skip), end - pos);
+    const int units = tile_units(span, kTileCost), take = (int)min((int64_t)(units - skip), end - pos);
     // this share's stages of the tile: [from, to) of span.count
     const int from = max(0, skip - kTileCost), to = max(0, skip + take - kTileCost);
     if (to == from) {

@@ -154,6 +154,10 @@ __device__ __forceinline__ void ldg_bytes(const uint8_t* at, uint32_t (&w)[(N + 
   }
 }
 
+// What beginning a tile costs a CTA, in blocks of 128 keys (as kTileCost; packed documents, tiles of 4 blocks: 148 us with 8,
+// 138 with 3, 133 with 2, 141 with 1).
+constexpr int kTcTileCost = 2;
+
 template <int FMT, int NB, bool EXACT>
 __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attention_tc_kernel(const AttnParams p) {
   using C = TcTile<FMT, NB, EXACT>;
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   // The next kernel may start only once this CTA has its tensor memory: one that took tensor memory first and then waited
   // for this grid would leave both waiting.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Share share = plan_share<STG, R, C::kWarps>(p, 1, plan);
+  const Share share = plan_share<STG, R, C::kWarps, kTcTileCost>(p, 1, plan);
   if (share.pos >= share.end) {
     if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
     return;
@@ -222,8 +226,8 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       ++entry, h = 0;
       continue;
     }
-    const int units = tile_units(span), take = (int)min((int64_t)(units - skip), share.end - pos);
-    const int from = max(0, skip - kTileCost), to = max(0, skip + take - kTileCost);
+    const int units = tile_units(span, kTcTileCost), take = (int)min((int64_t)(units - skip), share.end - pos);
+    const int from = max(0, skip - kTcTileCost), to = max(0, skip + take - kTcTileCost);
     if (to == from) {
       pos += take, skip += take;
       if (skip == units) skip = 0, ++h;
@@ -620,7 +624,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
 
     const bool begun = from > 0, done = to == span.count;
     if (begun && done && threadIdx.x == 0) {  // this CTA ends a tile that others began: the joining kernel's work
-      join.first = (int)((pos - skip + kTileCost) / share.per);
+      join.first = (int)((pos - skip + kTcTileCost) / share.per);
       join.rows = min(rows, R), join.row0 = rt * R, join.head0 = h * p.group, join.q0 = (int)q.q0;
     }
     blocks += n, ++segments;
