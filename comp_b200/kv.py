@@ -248,10 +248,13 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     if workspace is None:
         workspace = lens.new_empty(attention_workspace_size(cache, T, B, heads, q.dtype, max_q, return_lse) + 3 >> 2)
     q_st, q_sh, _ = q.stride()
-    args = _pack_args(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, table.data_ptr(), lens_at,
-                      cu_at, prefix_at, starts_at, slopes_at, q_st, q_sh, T, B, table.stride(0) if P else 0, P, max_q,
-                      P * cache.page_size if max_len is None else max_len, heads, did, window,
-                      dim**-0.5 if scale is None else scale, softcap)
+    try:
+        args = _pack_args(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, table.data_ptr(), lens_at,
+                          cu_at, prefix_at, starts_at, slopes_at, q_st, q_sh, T, B, table.stride(0) if P else 0, P, max_q,
+                          P * cache.page_size if max_len is None else max_len, heads, did, window,
+                          dim**-0.5 if scale is None else scale, softcap)
+    except struct.error as e:
+        raise TypeError(f"attention: max_q, max_len and window are whole numbers, scale and softcap numbers: {e}") from None
     _call(dev, "b2q_attention", cache._ref, args, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
           _raw_stream(dev.index))
     return (out, lse) if return_lse else out

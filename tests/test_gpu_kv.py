@@ -485,7 +485,8 @@ def test_refusals(cuda):
                     (dict(softcap=float("nan")), ValueError), (dict(window=-1), ValueError), (dict(scale=0.0), ValueError),
                     (dict(scale=-1.0), ValueError), (dict(out=z(2, 4, 64, dtype=torch.float16)), ValueError),
                     (dict(workspace=z(4, dtype=torch.uint8)), ValueError), (dict(q=q.cpu()), RuntimeError),
-                    (dict(prefix=i32(2).cpu()), RuntimeError), (dict(q=None), RuntimeError)):
+                    (dict(prefix=i32(2).cpu()), RuntimeError), (dict(q=None), RuntimeError),
+                    (dict(window=4.5), TypeError), (dict(scale="1"), TypeError), (dict(max_len=2.0), TypeError)):
         a = dict(q=q, table=table, lens=lens)
         a.update({k: v for k, v in kw.items() if k in a})
         rest = {k: v for k, v in kw.items() if k not in a}
