@@ -57,7 +57,8 @@ static int check_attention(const char* who, const b2q_kv_cache* c, const b2q_att
     return fail(B2Q_EINVAL, "%s: %d query heads over %d KV heads", who, a->q_heads, c->heads);
   if (a->dtype < 0 || a->dtype > 2) return fail(B2Q_EINVAL, "%s: dtype %d", who, a->dtype);
   if (!(a->scale > 0.f) || a->scale > 1e30f) return fail(B2Q_EINVAL, "%s: scale must be positive", who);
-  if (!(a->softcap >= 0.f)) return fail(B2Q_EINVAL, "%s: softcap must not be negative", who);
+  if (!(a->softcap == 0.f || (a->softcap >= 1e-20f && a->softcap <= 1e20f)))
+    return fail(B2Q_EINVAL, "%s: softcap must be 0 (none) or from 1e-20 to 1e20", who);
   if (a->window < 0) return fail(B2Q_EINVAL, "%s: window must not be negative", who);
   if (!a->cu_q && a->T != a->batch)
     return fail(B2Q_EINVAL, "%s: without cu_q there is one query token a sequence (T=%lld, batch=%lld)", who,
@@ -113,7 +114,8 @@ int b2q_attention(const b2q_kv_cache* cache, const b2q_attention_args* args, voi
   p.table_pages = (int)a.table_pages, p.batch = (int)a.batch, p.q_heads = a.q_heads, p.heads = c.heads;
   p.group = a.q_heads / c.heads;
   while ((1 << p.page_shift) < c.page) ++p.page_shift;
-  p.row_tiles = pl.row_tiles, p.window = a.window, p.dtype = a.dtype;
+  p.row_tiles = pl.row_tiles, p.dtype = a.dtype;
+  p.window = a.window < a.table_pages * c.page ? a.window : 0;  // (a window of all keys: positions less it stay in 32 bits)
   p.scale = a.scale, p.softcap = a.softcap;
   if (pl.tc)
     return c.fmt == B2Q_FMT_Q4_0 ? launch_attention_tc_q4(p, c.dim, pl.sms, (cudaStream_t)stream)

@@ -130,7 +130,7 @@ def _heads_aligned(t):
 
 def kv_write(cache, k, v, slots):
     """Quantizes k and v [T][heads][head_dim] (f32, f16 or bf16; any token and head strides) into the slots int64 [T] of
-    the cache (page * page_size + offset). Negative slots are skipped (padding tokens). The blocks are ggml's, bit for
+    the cache (page * page_size + offset; no slot twice). Negative slots are skipped (padding tokens). The blocks are ggml's, bit for
     bit (quantize_row_q4_0 / q8_0 of the value widened to f32); a 16-bit caller needs no cast."""
     dev = cache.device
     _on_device("kv_write", dev, k, v, slots)
@@ -193,6 +193,8 @@ def attention_workspace_size(cache, T, batch, q_heads, dtype, max_q=1, return_ls
                                   DTYPE_ID[dtype], 0, 1.0, 0.0)
         with torch.cuda.device(cache.device):
             size = _lib.load().b2q_attention_workspace_size(cache._ref, ctypes.addressof(args))
+        if len(cache._sizes) >= 4096:  # every T of a long-lived server would stay
+            cache._sizes.clear()
         cache._sizes[key] = size
     return size
 
@@ -214,7 +216,7 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     max_q / max_len: the most query tokens of a sequence and the longest length, where the caller knows them (default:
     T, or 1 without cu_q, and what the table can hold): max_q must not be less than what cu_q has, max_len only plans
     the work. workspace: a CUDA byte tensor of attention_workspace_size(...) bytes (allocated here when None). out: a
-    contiguous tensor for the result."""
+    contiguous tensor for the result that shares no memory with q. Rows outside cu_q's range (padding) stay unwritten."""
     dev = cache.device
     _on_device("attention", dev, q, table, lens)
     did = _dtype_id("attention: q", q)
@@ -226,8 +228,8 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     if table.dtype != torch.int32 or table.dim() != 2:
         raise TypeError(f"attention: table must be a 2-D int32 tensor, got {table.dtype} {tuple(table.shape)}")
     B, P = table.shape
-    if P and table.stride(1) != 1:
-        table = table.contiguous()
+    if B > 1 and (table.stride(1) != 1 or table.stride(0) < P) or P > 1 and table.stride(1) != 1:
+        table = table.clone(memory_format=torch.contiguous_format)  # one row for all sequences, rows that overlap
     lens_at, lens = _index(lens, "lens", (B,), dev)
     if cu_q is None:
         if T != B:
@@ -247,10 +249,14 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     lse = q.new_empty((T, heads), dtype=torch.float32) if return_lse else None
     if workspace is None:
         workspace = lens.new_empty(attention_workspace_size(cache, T, B, heads, q.dtype, max_q, return_lse) + 3 >> 2)
+    else:
+        _on_device("attention", dev, workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("attention: workspace must be contiguous")
     q_st, q_sh, _ = q.stride()
     try:
         args = _pack_args(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, table.data_ptr(), lens_at,
-                          cu_at, prefix_at, starts_at, slopes_at, q_st, q_sh, T, B, table.stride(0) if P else 0, P, max_q,
+                          cu_at, prefix_at, starts_at, slopes_at, q_st, q_sh, T, B, table.stride(0) if B > 1 else P, P, max_q,
                           P * cache.page_size if max_len is None else max_len, heads, did, window,
                           dim**-0.5 if scale is None else scale, softcap)
     except struct.error as e:

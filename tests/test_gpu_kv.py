@@ -486,6 +486,9 @@ def test_refusals(cuda):
                     (dict(scale=-1.0), ValueError), (dict(out=z(2, 4, 64, dtype=torch.float16)), ValueError),
                     (dict(workspace=z(4, dtype=torch.uint8)), ValueError), (dict(q=q.cpu()), RuntimeError),
                     (dict(prefix=i32(2).cpu()), RuntimeError), (dict(q=None), RuntimeError),
+                    (dict(workspace=torch.zeros(64 << 20, dtype=torch.uint8)), RuntimeError),
+                    (dict(workspace=z(128 << 20, dtype=torch.uint8)[::2]), ValueError),
+                    (dict(softcap=float("inf")), ValueError), (dict(softcap=1e-30), ValueError),
                     (dict(window=4.5), TypeError), (dict(scale="1"), TypeError), (dict(max_len=2.0), TypeError)):
         a = dict(q=q, table=table, lens=lens)
         a.update({k: v for k, v in kw.items() if k in a})
@@ -500,6 +503,40 @@ def test_refusals(cuda):
         kv.KVCache.from_planes("q8_0", c.kq, c.ks, c.vq, c.vs)
     with pytest.raises(TypeError):
         kv.KVCache.from_planes("q4_0", c.kq, c.ks.float(), c.vq, c.vs)
+
+
+@pytest.mark.parametrize("queries", [1, 70])
+def test_tables_with_other_strides(cuda, queries):
+    """One table row for every sequence, rows that overlap, columns of a wider table, one column: as their copies."""
+    planes, _, _, _, q = _problem(91, "q4_0", "f16", [200, 150, 37], [queries] * 3, 8, 2, 64, 16)
+    cache = _cache("q4_0", planes, cuda)
+    q = q.to(cuda)
+    lens = torch.tensor([180, 150, 72], dtype=torch.int32, device=cuda)
+    cu = torch.tensor([0, queries, 2 * queries, 3 * queries], dtype=torch.int32, device=cuda)
+    row = torch.randperm(24, device=cuda).int()
+    for table in (row[:12].expand(3, 12), row.as_strided((3, 12), (4, 1)), torch.stack([row, row + 1, row], 1)[:12].t(),
+                  row[:3].view(1, 3).t(), row[:3].view(3, 1)):
+        want = kv.attention(q, cache, table.clone(memory_format=torch.contiguous_format), lens, cu_q=cu, max_q=queries)
+        _device_error()
+        assert torch.equal(kv.attention(q, cache, table, lens, cu_q=cu, max_q=queries), want)
+    for table in (row.view(1, 24), row.view(24, 1)[:12].t(), row.as_strided((1, 12), (0, 1)), row.as_strided((1, 12), (1, 2))):
+        want = kv.attention(q[:queries], cache, table.clone(memory_format=torch.contiguous_format), lens[:1], cu_q=cu[:2])
+        assert torch.equal(kv.attention(q[:queries], cache, table, lens[:1], cu_q=cu[:2]), want)
+    _device_error()
+
+
+@pytest.mark.parametrize("dtype,queries", [("f32", 9), ("bf16", 9), ("f16", 90)])
+def test_a_window_of_all_keys_is_none(cuda, dtype, queries):
+    """The largest window, with queries before the first key (more of them than keys) that see a prefix."""
+    planes, table, lens, cu, q = _problem(92, "q8_0", dtype, [5, 40], [queries] * 2, 4, 2, 64, 16)
+    cache = _cache("q8_0", planes, cuda)
+    t = [torch.from_numpy(x).to(cuda) for x in (table, lens, cu)]
+    prefix = torch.tensor([3, 3], dtype=torch.int32, device=cuda)
+    a = dict(cu_q=t[2], max_q=queries, prefix=prefix)
+    want = kv.attention(q.to(cuda), cache, t[0], t[1], **a)
+    assert (want[0] != 0).any()
+    for window in (2**31 - 1, 64):
+        assert torch.equal(kv.attention(q.to(cuda), cache, t[0], t[1], window=window, **a), want)
 
 
 def test_the_example_runs(cuda, capsys):
