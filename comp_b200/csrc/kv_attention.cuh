@@ -233,7 +233,7 @@ __device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
 // A tile's units of a share: `cost` without stages, then its stages.
 __device__ __forceinline__ int tile_units(Span s, int cost) { return s.count ? s.count + cost : 0; }
 
-// The plan: every CTA an equal share of all stages. Entries (sequence, row tile) have their stages, after COST units without
+// The plan: every CTA an equal share of all stages. Entries (sequence, row tile) have their stages, after cost units without
 // any, once a KV head; a CTA's share is [pos, end) of their run, at least `least` units (unless none are left),
 // and begins `skip` units into the tile of (entry, head). All W warps call it; the scratch is read until the barrier
 // that ends it.
@@ -246,15 +246,15 @@ struct ShareScratch {
   int64_t scan[W];
   int entry, head, skip;
 };
-template <int STG, int R, int W, int COST>
-__device__ __forceinline__ Share plan_share(const AttnParams& p, int least, ShareScratch<W>& scratch) {
+template <int STG, int R, int W>
+__device__ __forceinline__ Share plan_share(const AttnParams& p, int cost, int least, ShareScratch<W>& scratch) {
   constexpr int kThreads = W * 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int entries = p.batch * p.row_tiles, chunk = (entries + kThreads - 1) / kThreads;
   const int e0 = min(entries, (int)threadIdx.x * chunk), e1 = min(entries, e0 + chunk);
   Share s;
   int64_t mine = 0;
-  for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles), COST);
+  for (int e = e0; e < e1; ++e) mine += tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles), cost);
   mine *= p.heads;
   int64_t upto = mine;
 #pragma unroll
@@ -279,7 +279,7 @@ __device__ __forceinline__ Share plan_share(const AttnParams& p, int least, Shar
   if (s.pos < s.end && s.pos >= upto - mine && s.pos < upto) {  // the thread whose entries hold the beginning
     int64_t off = s.pos - (upto - mine);
     for (int e = e0; e < e1; ++e) {
-      const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles), COST);
+      const int count = tile_units(tile_span<STG, R>(p, e / p.row_tiles, e % p.row_tiles), cost);
       if (off < (int64_t)count * p.heads) {
         int h = 0;
         while (off >= count) off -= count, ++h;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   pdl_wait_then_trigger();
 
   __shared__ ShareScratch<W> plan;
-  const Share share = plan_share<STG, R, W, kTileCost>(p, W, plan);
+  const Share share = plan_share<STG, R, W>(p, kTileCost, W, plan);
   const int64_t per = share.per, end = share.end;
   int64_t pos = share.pos;
   if (pos >= end) {

@@ -154,9 +154,12 @@ __device__ __forceinline__ void ldg_bytes(const uint8_t* at, uint32_t (&w)[(N + 
   }
 }
 
-// What beginning a tile costs a CTA, in blocks of 128 keys (as kTileCost; packed documents, tiles of 4 blocks: 148 us with 8,
-// 138 with 3, 133 with 2, 141 with 1).
-constexpr int kTcTileCost = 2;
+// What beginning a tile costs a CTA, in blocks of 128 keys (as kTileCost), which take longer with a cap or a bias by
+// distance. Measured with costs of 2 / 3 / 4 / 5 / 6 / 8, us, 32 heads on 8 of 128: four fresh prompts of 2048 tokens 378 /
+// 320 / 298 / 278 / 276 / 282, with a cap 414 / 363 / 370 / 378 / 384 / 394; 16 ragged chunks of 32 to 300 tokens on 300 to
+// 6000 keys 316 / 302 / 280 / 254 / 253 / 261, with a cap 391 / 367 / 365 / 365 / 370 / 386; documents of 500 tokens with lse
+// 236 / 233 / 229 / 234 / 233 / 240, with a cap too 259 / 264 / 265 / 272 / 273 / 282.
+static inline int tc_tile_cost(const AttnParams& p) { return p.softcap > 0.f || p.slopes ? 3 : 5; }
 
 template <int FMT, int NB, bool EXACT>
 __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attention_tc_kernel(const AttnParams p) {
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   // The next kernel may start only once this CTA has its tensor memory: one that took tensor memory first and then waited
   // for this grid would leave both waiting.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Share share = plan_share<STG, R, C::kWarps, kTcTileCost>(p, 1, plan);
+  const Share share = plan_share<STG, R, C::kWarps>(p, p.tile_cost, 1, plan);
   if (share.pos >= share.end) {
     if (threadIdx.x == 0) p.joins[blockIdx.x].first = -1;
     return;
@@ -226,8 +229,8 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       ++entry, h = 0;
       continue;
     }
-    const int units = tile_units(span, kTcTileCost), take = (int)min((int64_t)(units - skip), share.end - pos);
-    const int from = max(0, skip - kTcTileCost), to = max(0, skip + take - kTcTileCost);
+    const int units = tile_units(span, p.tile_cost), take = (int)min((int64_t)(units - skip), share.end - pos);
+    const int from = max(0, skip - p.tile_cost), to = max(0, skip + take - p.tile_cost);
     if (to == from) {
       pos += take, skip += take;
       if (skip == units) skip = 0, ++h;
@@ -624,7 +627,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
 
     const bool begun = from > 0, done = to == span.count;
     if (begun && done && threadIdx.x == 0) {  // this CTA ends a tile that others began: the joining kernel's work
-      join.first = (int)((pos - skip + kTcTileCost) / share.per);
+      join.first = (int)((pos - skip + p.tile_cost) / share.per);
       join.rows = min(rows, R), join.row0 = rt * R, join.head0 = h * p.group, join.q0 = (int)q.q0;
     }
     blocks += n, ++segments;
@@ -694,7 +697,8 @@ static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t str
 }
 
 template <int FMT>
-static int launch_attention_tc_fmt(const AttnParams& p, int dim, int sms, cudaStream_t stream) {
+static int launch_attention_tc_fmt(AttnParams p, int dim, int sms, cudaStream_t stream) {
+  p.tile_cost = tc_tile_cost(p);
   switch (dim) {
     case 64:
       return p.lse ? launch_attention_tc_as<FMT, 2, true>(p, sms, stream)

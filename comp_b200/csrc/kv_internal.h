@@ -39,6 +39,7 @@ struct AttnParams {
   AttnJoin* joins;  // [CTAs]
   int64_t q_st, q_sh, T, table_stride, pages;
   int table_pages, batch, q_heads, heads, group, page_shift, row_tiles, window, dtype;
+  int tile_cost;  // tensor-core kernels: what beginning a tile costs, in blocks of keys
   float scale, softcap;
 };
 
