@@ -198,10 +198,14 @@ __device__ __forceinline__ Sequence sequence(const AttnParams& p, int b) {
   return s;
 }
 
-// What beginning a tile costs a CTA, in stages of its share (measured: 6 us against 0.8 us a stage of 64 keys): without it,
-// a share of many short tiles takes far longer than one long run (64 sequences of 100 to 8192 tokens: 115 us, so 80; with
-// 4 stages 89, with 14 82).
-constexpr int kTileCost = 8;
+// What beginning a tile costs a CTA, in stages of its share: without it, a share of many short tiles takes far longer than
+// one long run. Measured with costs of 4 / 8 / 12 / 24, us, bf16, 32 heads on 8: 64 sequences of 100 to 8192 tokens, q4_0
+// heads of 128 88 / 80 / 81 / 86, of 256 173 / 160 / 154 / 158, four tokens each of 48 such 131 / 117 / 99 / 105, 300 of 20
+// to 2048 133 / 123 / 118 / 126 and in q8_0 154 / 138 / 131 / 139; f32 (whose
+// stages take longer), heads of 128 128 / 122 / 124 / 131, five tokens each of 16 of 7 to 6001, heads of 64: 37 with 8, 40
+// with 12.
+template <int PARTS>
+constexpr int kTileCost = PARTS == 2 ? 8 : 12;
 
 // The stages that hold the visible keys of row tile rt of sequence b: `count` is 0 for a tile without rows and at least 1
 // for any other, so that a tile that sees nothing is somebody's work too.
@@ -299,6 +303,7 @@ template <int FMT, int NB, int NT, int PARTS>
 __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) attention_kernel(const AttnParams p) {
   using C = KvTile<FMT, NB>;
   constexpr int D = NB * 32, W = C::kWarps, S = C::kStages, STG = C::kTokens, SUB = STG / 16, R = NT * 8;
+  constexpr int kCost = kTileCost<PARTS>;
   constexpr bool SIGNED = PARTS == 2;  // quants enter the products with their offset taken off
   constexpr float kOff = FMT == 0 ? 8.f : 128.f;
   constexpr int UN = SUB % 2 == 0 && NB * NT <= 4 && PARTS == 1 ? 2 : 1;
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
   pdl_wait_then_trigger();
 
   __shared__ ShareScratch<W> plan;
-  const Share share = plan_share<STG, R, W>(p, kTileCost, W, plan);
+  const Share share = plan_share<STG, R, W>(p, kCost, W, plan);
   const int64_t per = share.per, end = share.end;
   int64_t pos = share.pos;
   if (pos >= end) {
@@ -335,9 +340,9 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
       ++entry, h = 0;
       continue;
     }
-    const int units = tile_units(span, kTileCost), take = (int)min((int64_t)(units - skip), end - pos);
+    const int units = tile_units(span, kCost), take = (int)min((int64_t)(units - skip), end - pos);
     // this share's stages of the tile: [from, to) of span.count
-    const int from = max(0, skip - kTileCost), to = max(0, skip + take - kTileCost);
+    const int from = max(0, skip - kCost), to = max(0, skip + take - kCost);
     if (to == from) {
       pos += take, skip += take;
       if (skip == units) skip = 0, ++h;
@@ -871,7 +876,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
       }
     }
     if (begun && done && threadIdx.x == 0) {  // this CTA ends a tile that others began: the joining kernel's work
-      join.first = (int)((pos - skip + kTileCost) / per);
+      join.first = (int)((pos - skip + kCost) / per);
       join.rows = min(rows, R), join.row0 = rt * R, join.head0 = h * p.group, join.q0 = (int)q.q0;
     }
     pos += take, skip += take;
