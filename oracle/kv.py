@@ -1,4 +1,4 @@
-"""Plain restatement of the quantized KV cache and its attention (numpy, 64 bits), the checker of comp_b200.kv.
+"""Plain restatement of the quantized KV cache and its attention (numpy, 64 bits), the oracle of comp_b200.kv.
 
 The cache's layout is stated here element by element, apart from the kernels: element e of a head's row lies in block
 b = e // 32 at i = e % 32; its ggml quant byte (q4_0: byte i % 16, low nibble for i < 16; q8_0: byte i, the quant plus
