@@ -167,6 +167,11 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   constexpr int D = C::D, MT = C::MT, KB = C::kKeyBufs, VB = C::kBufs, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
   extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB][parts], values [VB]
   __shared__ uint64_t b_kfull[KB], b_kempty[KB], b_vfull[VB], b_vempty[VB], b_s[MT], b_p[MT], b_o[MT], b_q, b_end;
+  // A block's keys without a page, a bit each. The unpacking warps write a block's words before they hand its keys on; the
+  // issuing thread, which waits for the keys, passes that on to the softmax with its own arrival at b_s. Four in turn: the
+  // words of block b are written when the scores of block b - KB have ended, so when the softmax is done with b - KB - 1.
+  __shared__ __align__(16) uint32_t s_unread[4][STG / 32];
+  static_assert(KB < 4, "words in turn");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ ShareScratch<C::kWarps> plan;
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
     for (int i = 0; i < KB; ++i) mbar_init(smem_addr(&b_kfull[i]), 128), mbar_init(smem_addr(&b_kempty[i]), 1);
     for (int i = 0; i < VB; ++i) mbar_init(smem_addr(&b_vfull[i]), 128), mbar_init(smem_addr(&b_vempty[i]), 1);
     for (int i = 0; i < MT; ++i) {
-      mbar_init(smem_addr(&b_s[i]), 1), mbar_init(smem_addr(&b_p[i]), 128), mbar_init(smem_addr(&b_o[i]), 1);
+      mbar_init(smem_addr(&b_s[i]), 2), mbar_init(smem_addr(&b_p[i]), 128), mbar_init(smem_addr(&b_o[i]), 1);
     }
     mbar_init(smem_addr(&b_q), SW * 32), mbar_init(smem_addr(&b_end), 1);
     s_abort = 0;
@@ -322,9 +327,12 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           if (!wait(&b_s[tile], done_blocks[tile] + j)) break;
           tc::fence_after();
           const int kb = (begin + j) * STG;
+          const uint4 unread = *reinterpret_cast<const uint4*>(s_unread[(blocks + j) & 3]);
+          const bool holes = (unread.x | unread.y | unread.z | unread.w) != 0;
           // masked or special scores are finished in the first pass and put back
-          const bool mask = __any_sync(0xffffffffu, kb < lo || kb + STG > hi), careful = special || mask;
-          const float scale = careful ? 1.f : mul;
+          const bool mask = __any_sync(0xffffffffu, kb < lo || kb + STG > hi);
+          const bool careful = special || mask;
+          float scale = careful ? 1.f : mul;
           // takes the reference to the row's maximum where that has grown by more than 2^8, and O with it
           auto follow = [&](float top) {
             const bool grown = top > ref + 8.f;
@@ -398,6 +406,24 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
             for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
           }
           if (careful) tc::tmem_wait_st();
+          if (__builtin_expect(holes, 0)) {  // another pass: keys without a page are masked
+            top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < STG; c += 32) {
+              const uint32_t unread = s_unread[(blocks + j) & 3][c >> 5];
+              uint32_t x[32];
+              tc::tmem_ld32_nowait(col_s + c, x);
+              tc::tmem_wait_ld32(x);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                x[e] = (unread >> e) & 1 ? 0xff800000u : __float_as_uint(__uint_as_float(x[e]) * scale);
+                top = fmaxf(top, __uint_as_float(x[e]));
+              }
+              tc::tmem_st32(col_s + c, x);
+            }
+            tc::tmem_wait_st();
+            scale = 1.f;
+          }
           follow(top * scale);
           float2 s01 = make_float2(0.f, 0.f);
           const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
@@ -507,6 +533,8 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         const int kbuf = at % KB, vbuf = at % VB;
         if (FMT == 2) load_v(j);
         if (at >= KB && !wait(&b_kempty[kbuf], at / KB - 1)) break;
+        const uint32_t unread = __ballot_sync(0xffffffffu, !read_k && (begin + j) * STG + th < q.len);
+        if (lane == 0) s_unread[at & 3][warp - SW] = unread;
         uint8_t* kt = smem + MT * C::kQ + kbuf * C::kParts * C::kTile + th * 16;
         bool fits = true;
 #pragma unroll
@@ -594,6 +622,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
             tc::mma_f16_ss(tmem + C::kS + tile * 128, a + s * (4096 >> 4), z + ((part * C::kTile + s * 4096) >> 4), is,
                            part > 0 || s > 0);
         tc::mma_commit(smem_addr(&b_s[tile]));
+        tc::arrive(smem_addr(&b_s[tile]));
       };
       if (wait_one(&b_q, segments) && wait_one(&b_kfull[blocks % KB], blocks / KB)) {
         tc::fence_after();

@@ -77,10 +77,12 @@ def visible(lens, cu, prefix=None, starts=None, window=0):
     return out
 
 
-def attention(q, keys, values, lens, cu, scale, softcap=0.0, slopes=None, prefix=None, starts=None, window=0):
+def attention(q, keys, values, lens, cu, scale, softcap=0.0, slopes=None, prefix=None, starts=None, window=0,
+              unread=None):
     """-> (out [T][q_heads][dim], lse [T][q_heads], reach [T][q_heads], mass [T][q_heads][dim]), all f64. keys / values:
-    per sequence [len][heads][dim]. reach is the largest scale * sum |q_i k_i| of a visible key and mass the attention of
-    |v|: what a rounding of a score or a weight can move an output by is measured in them."""
+    per sequence [len][heads][dim]; unread: per sequence bool [len], tokens that are masked for every query. reach is the
+    largest scale * sum |q_i k_i| of a visible key and mass the attention of |v|: what a rounding of a score or a weight can
+    move an output by is measured in them."""
     T, qh, dim = q.shape
     out, lse = np.zeros((T, qh, dim)), np.full((T, qh), -np.inf)
     reach, mass = np.zeros((T, qh)), np.zeros((T, qh, dim))
@@ -90,7 +92,12 @@ def attention(q, keys, values, lens, cu, scale, softcap=0.0, slopes=None, prefix
             p, lo, hi = see[t]
             if lo >= hi:
                 continue
-            k, v = keys[b][lo:hi], values[b][lo:hi]
+            j = np.arange(lo, hi)
+            if unread is not None:
+                j = j[~unread[b][lo:hi]]
+            if not len(j):
+                continue
+            k, v = keys[b][j], values[b][j]
             group = qh // k.shape[1]
             for h in range(qh):
                 kh, vh, qt = k[:, h // group], v[:, h // group], q[t, h].astype(np.float64)
@@ -98,7 +105,7 @@ def attention(q, keys, values, lens, cu, scale, softcap=0.0, slopes=None, prefix
                 if softcap:
                     s = softcap * np.tanh(s / softcap)
                 if slopes is not None:
-                    s = s - float(slopes[h]) * np.abs(p - np.arange(lo, hi))
+                    s = s - float(slopes[h]) * np.abs(p - j)
                 top = s.max()
                 w = np.exp(s - top)
                 total = w.sum()
