@@ -115,7 +115,7 @@ int b2q_attention(const b2q_kv_cache* cache, const b2q_attention_args* args, voi
   p.group = a.q_heads / c.heads;
   while ((1 << p.page_shift) < c.page) ++p.page_shift;
   p.row_tiles = pl.row_tiles, p.dtype = a.dtype;
-  p.window = a.window < a.table_pages * c.page ? a.window : 0;  // (a window of all keys: positions less it stay in 32 bits)
+  p.window = a.window;
   p.scale = a.scale, p.softcap = a.softcap;
   if (pl.tc)
     return c.fmt == B2Q_FMT_Q4_0 ? launch_attention_tc_q4(p, c.dim, pl.sms, (cudaStream_t)stream)

@@ -168,33 +168,35 @@ __device__ __forceinline__ float tanh_far(float z) {
   return copysignf(1.f - __fdividef(2.f, exp2_approx(fabsf(z) * (2.f * kLog2e)) + 1.f), z);
 }
 
-// Position and visible keys [lo, hi) of query i of sequence b.
-struct QuerySpan {
-  int pos, lo, hi;
-};
-__device__ __forceinline__ QuerySpan query_span(const AttnParams& p, int b, int i, int64_t q0, int n, int len) {
-  QuerySpan s;
-  s.pos = len - n + i;
-  s.hi = s.pos + 1;
-  if (p.prefix) s.hi = max(s.hi, p.prefix[b]);
-  s.hi = max(0, min(s.hi, len));
-  s.lo = p.starts ? max(0, p.starts[q0 + i]) : 0;
-  if (p.window > 0) s.lo = max(s.lo, s.pos - p.window + 1);
-  return s;
-}
-
-// Sequence b's query tokens (held within q whatever cu_q says) and length (within its table).
+// Sequence b's query tokens (held within q whatever cu_q says), its length, which the queries' positions go by, and what of
+// it the table holds, past which no key is visible.
 struct Sequence {
   int64_t q0;
-  int n, len;
+  int n, end, len;
 };
 __device__ __forceinline__ Sequence sequence(const AttnParams& p, int b) {
-  Sequence s = {b, 1, 0};
+  Sequence s = {b, 1, 0, 0};
   if (p.cu_q) {
     s.q0 = max((int64_t)0, min((int64_t)p.cu_q[b], p.T));
     s.n = (int)(min((int64_t)p.cu_q[b + 1], p.T) - s.q0);
   }
-  s.len = max(0, min(p.lens[b], p.table_pages << p.page_shift));
+  s.end = max(0, p.lens[b]);
+  s.len = min(s.end, p.table_pages << p.page_shift);
+  return s;
+}
+
+// Position and visible keys [lo, hi) of query i of sequence b.
+struct QuerySpan {
+  int pos, lo, hi;
+};
+__device__ __forceinline__ QuerySpan query_span(const AttnParams& p, int b, int i, const Sequence& q) {
+  QuerySpan s;
+  s.pos = q.end - q.n + i;
+  s.hi = s.pos + 1;
+  if (p.prefix) s.hi = max(s.hi, p.prefix[b]);
+  s.hi = max(0, min(s.hi, q.len));
+  s.lo = p.starts ? max(0, p.starts[q.q0 + i]) : 0;
+  if (p.window > 0 && s.pos >= p.window) s.lo = max(s.lo, s.pos - p.window + 1);
   return s;
 }
 
@@ -221,11 +223,11 @@ __device__ __forceinline__ Span tile_span(const AttnParams& p, int b, int rt) {
   if (p.cu_q) i0 = rt * R / p.group, i1 = min(q.n - 1, (rt * R + R - 1) / p.group);
   int lo = INT_MAX, hi = 0;
   if (!p.starts) {  // both ends grow with the position
-    lo = query_span(p, b, i0, q.q0, q.n, q.len).lo, hi = query_span(p, b, i1, q.q0, q.n, q.len).hi;
+    lo = query_span(p, b, i0, q).lo, hi = query_span(p, b, i1, q).hi;
   } else {
 #pragma unroll 4
     for (int i = i0 + (WARP ? (int)(threadIdx.x & 31) : 0); i <= i1; i += WARP ? 32 : 1) {
-      const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
+      const QuerySpan s = query_span(p, b, i, q);
       if (s.lo < s.hi) lo = min(lo, s.lo), hi = max(hi, s.hi);
     }
     if (WARP) lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     }
     const Sequence q = sequence(p, b);
     const int rows = q.n * p.group - rt * R;  // rows from this tile on (at least 1)
-    if (p.lens[b] > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
+    if (q.end > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
     const int begin = span.first + from, stop = span.first + to;
 
     const int32_t* table = p.table + (int64_t)b * p.table_stride;
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     if (threadIdx.x < R) {
       const int r = threadIdx.x, rr = rt * R + (r < rows ? r : 0);
       const int i = p.cu_q ? rr / p.group : 0, head = h * p.group + (rr - i * p.group);
-      const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
+      const QuerySpan s = query_span(p, b, i, q);
       s_lo[r] = s.lo, s_hi[r] = r < rows ? s.hi : 0, s_pos[r] = s.pos;
       s_out[r] = (int)(q.q0 + i) * p.q_heads + head;
       s_slope[r] = p.slopes ? p.slopes[head] * kLog2e : 0.f;

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
     }
     const Sequence q = sequence(p, b);
     const int rows = q.n * p.group - rt * R;  // rows from this tile on (at least 1)
-    if (p.lens[b] > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
+    if (q.end > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
     const int begin = span.first + from, n = to - from, tiles = MT == 1 || rows <= 128 ? 1 : 2;
 
     if constexpr (ROLE == 0) {
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       uint8_t* my_q = smem + tile * C::kQ + (r & 127) * 16;
       if (there) {
         const int i = p.cu_q ? rr / p.group : 0, head = h * p.group + (rr - i * p.group);
-        const QuerySpan s = query_span(p, b, i, q.q0, q.n, q.len);
+        const QuerySpan s = query_span(p, b, i, q);
         lo = s.lo, hi = s.hi, where = s.pos;
         out_row = (q.q0 + i) * p.q_heads + head;
         slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;

@@ -334,8 +334,8 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
  * prefix (per sequence: keys that every query sees) are int32, slopes f32 [q_heads]; each may be NULL. scale > 0.
  * Scores, softmax sums and outputs are held in f32.
  * max_q: at least the most queries of a sequence (0: max_q = T); max_len: at least the longest lens, used to plan the
- * split of the keys only. Tokens beyond the table or in pages outside the cache read as masked, and set the device
- * error word to 3. out [T][q_heads][dim] contiguous, of q's dtype; lse f32 [T][q_heads] or NULL. Rows outside
+ * split of the keys only. Tokens beyond the table or in pages outside the cache read as masked (the queries' positions
+ * stay those of the whole sequence), and set the device error word to 3. out [T][q_heads][dim] contiguous, of q's dtype; lse f32 [T][q_heads] or NULL. Rows outside
  * cu_q[0] .. cu_q[batch] - 1 are left unwritten; out shares no memory with q. q: element strides per token and head, last
  * axis contiguous, 16-byte aligned in base and strides. scale in (0, 1e30], softcap 0 or in [1e-20, 1e20].
  */

@@ -93,3 +93,16 @@ def test_rows_that_see_unread_pages_alone_are_empty(cuda, fmt, dtype, with_lse):
     assert empty[:32].all() and not empty[32:500].any() and empty[500:516].all()
     _check_unread(204, fmt, dtype, [700, 33], [60, 33], 4, 2, 64, 16, cuda,
                   lambda t: _put(t, *((0, i) for i in range(7, 27))), with_lse)
+
+
+@pytest.mark.parametrize("fmt,dtype,queries,with_lse", [
+    ("q4_0", "f32", [1, 1], True), ("q8_0", "bf16", [5, 9], True), ("q4_0", "bf16", [70, 130], False),
+    ("q8_0", "f16", [70, 130], True)])
+@pytest.mark.parametrize("window", [0, 40, 90, 1000])
+def test_a_table_shorter_than_its_sequence(cuda, fmt, dtype, queries, with_lse, window):
+    """Tokens past the table are masked; the queries stay where they are, at the end of the whole sequence."""
+    for keep in (4, 9):
+        _check_unread(205, fmt, dtype, [150, 170], queries, 4, 2, 64, 16, cuda, lambda t: t[:, :keep].copy(), with_lse,
+                      window=window)
+        _check_unread(206, fmt, dtype, [150, 170], queries, 4, 2, 64, 16, cuda, lambda t: t[:, :keep].copy(), with_lse,
+                      window=window, slopes=2.0 ** -np.arange(1, 5), prefix=[70, 10])
