@@ -9,7 +9,8 @@
 //     grown by more than 2^8: then the thread rescales its row of O, which no product is using at that time.
 // Queries are scaled by a power of two a row (exact for 16-bit queries) and take the order of the keys' packed words, so
 // that one word of a key becomes one 16-byte chunk of its operand. Keys and values are rounded to f16 (11 bits), weights
-// to f16; values past f16's range (65504) come out as NaN, for every row that sees the key.
+// to f16. A key with values past f16's range (65504) enters its operand a power of two smaller, and its scores, or its
+// weights, are made as much larger: passes of their own over such a block, as for keys without a page, which are masked.
 //
 // What bounds it: 128 keys for 256 rows of 128 values take 2048 cycles on the tensor cores, 2048 on the units that compute
 // 2^x (16 a cycle), and about 2048 of shared memory's (operands of S from there twice, unpacked tiles into it); a tile's
@@ -41,6 +42,10 @@ struct TcTile {
   static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kIssueRegs = 80;
   static_assert(MT == 1 || 256 * kSoftmaxRegs + 128 * kLaunchRegs + 128 * kIssueRegs <= 512 * kLaunchRegs, "registers");
   static constexpr uint32_t kS = 256;                     // column of S (and P) of tile 0; O is at 0
+  // the largest scale (f16 bits) whose values all fit f16: 8 * 8188 and 128 * 511.75 are 65504; and by what power of two a
+  // key or value row with a larger one is less in its operand
+  static constexpr uint32_t kMost = FMT == 0 ? 0x6fffu : 0x5fffu;
+  static constexpr int kLess = FMT == 0 ? 4 : 8;
 };
 
 namespace tc {
@@ -127,6 +132,15 @@ __device__ __forceinline__ uint32_t high_nibbles_int(uint32_t w) {
   return fma_half2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
 }
 
+// The largest magnitude of N f16 numbers, two to a register (an odd N's last half is 0), as f16 bits.
+template <int N>
+__device__ __forceinline__ uint32_t largest_half(const uint32_t (&w)[(N + 1) / 2]) {
+  uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < (N + 1) / 2; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
+}
+
 // N bytes (a multiple of 2) of global memory into 32-bit words; 16, 8, 4 or 2 at a time as N allows (N aligned).
 template <int N>
 __device__ __forceinline__ void ldg_bytes(const uint8_t* at, uint32_t (&w)[(N + 3) / 4]) {
@@ -167,10 +181,13 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   constexpr int D = C::D, MT = C::MT, KB = C::kKeyBufs, VB = C::kBufs, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
   extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB][parts], values [VB]
   __shared__ uint64_t b_kfull[KB], b_kempty[KB], b_vfull[VB], b_vempty[VB], b_s[MT], b_p[MT], b_o[MT], b_q, b_end;
-  // A block's keys without a page, a bit each. The unpacking warps write a block's words before they hand its keys on; the
-  // issuing thread, which waits for the keys, passes that on to the softmax with its own arrival at b_s. Four in turn: the
-  // words of block b are written when the scores of block b - KB have ended, so when the softmax is done with b - KB - 1.
-  __shared__ __align__(16) uint32_t s_unread[4][STG / 32];
+  // A block's odd keys, a bit each: those without a page, and those whose keys or whose values (s_less, written where a word
+  // of s_odd is not 0) are 2^kLess less in their operands. The unpacking warps write a block's words before they hand its
+  // keys on; the issuing thread, which waits for the keys, passes that on to the softmax with its own arrival at b_s. Four in
+  // turn: the words of block b are written when the scores of block b - KB have ended, so when the softmax is done with
+  // b - KB - 1.
+  __shared__ __align__(16) uint32_t s_odd[4][STG / 32];
+  __shared__ uint32_t s_less[4][2][STG / 32];
   static_assert(KB < 4, "words in turn");
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -327,12 +344,13 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           if (!wait(&b_s[tile], done_blocks[tile] + j)) break;
           tc::fence_after();
           const int kb = (begin + j) * STG;
-          const uint4 unread = *reinterpret_cast<const uint4*>(s_unread[(blocks + j) & 3]);
-          const bool holes = (unread.x | unread.y | unread.z | unread.w) != 0;
+          const int turn = (blocks + j) & 3;
+          const uint4 odds = *reinterpret_cast<const uint4*>(s_odd[turn]);
+          const bool odd = (odds.x | odds.y | odds.z | odds.w) != 0;
           // masked or special scores are finished in the first pass and put back
           const bool mask = __any_sync(0xffffffffu, kb < lo || kb + STG > hi);
           const bool careful = special || mask;
-          float scale = careful ? 1.f : mul;
+          const float scale = careful ? 1.f : mul;
           // takes the reference to the row's maximum where that has grown by more than 2^8, and O with it
           auto follow = [&](float top) {
             const bool grown = top > ref + 8.f;
@@ -351,6 +369,48 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
               }
             }
           };
+          if (__builtin_expect(odd, 0)) {  // the two passes below, an element at a time
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < STG; c += 32) {
+              const uint32_t odds = s_odd[turn][c >> 5], large_k = odds ? s_less[turn][0][c >> 5] : 0,
+                             large_v = odds ? s_less[turn][1][c >> 5] : 0, unread = odds & ~(large_k | large_v);
+              uint32_t x[32];
+              tc::tmem_ld32_nowait(col_s + c, x);
+              tc::tmem_wait_ld32(x);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float y = __uint_as_float(x[e]) * (large_k >> e & 1 ? rowf * (float)(1 << C::kLess) : rowf);
+                if (p.softcap > 0.f) y = cap * (fabsf(y) <= kTanhLimit ? tanh_near(y) : tanh_far(y));
+                if (p.slopes) y = fmaf(-slope, fabsf((float)(where - kb - c - e)), y);
+                if (kb + c + e < lo || kb + c + e >= hi || (unread >> e & 1)) y = -INFINITY;
+                top = fmaxf(top, large_v >> e & 1 ? y + C::kLess : y);
+                x[e] = __float_as_uint(y);
+              }
+              tc::tmem_st32(col_s + c, x);
+            }
+            tc::tmem_wait_st();
+            follow(top);
+#pragma unroll 1
+            for (int c = 0; c < STG; c += 32) {
+              const uint32_t large_v = s_odd[turn][c >> 5] ? s_less[turn][1][c >> 5] : 0;
+              uint32_t x[32], w[16];
+              tc::tmem_ld32_nowait(col_s + c, x);
+              tc::tmem_wait_ld32(x);
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float y0 = exp2_approx(__uint_as_float(x[e]) - ref), y1 = exp2_approx(__uint_as_float(x[e + 1]) - ref);
+                sum += y0 + y1;
+                w[e / 2] = pack_half2(large_v >> e & 1 ? y0 * (float)(1 << C::kLess) : y0,
+                                      large_v >> (e + 1) & 1 ? y1 * (float)(1 << C::kLess) : y1);
+              }
+              tc::tmem_st16(col_s + c / 2, w);
+            }
+            tc::tmem_wait_st();
+            tc::fence_before();
+            tc::arrive(smem_addr(&b_p[tile]));
+            continue;
+          }
           // Two passes over S, 32 columns at a time: for the maximum (masked and special scores are finished then, and put
           // back), and for the weights.
           float top = -INFINITY;
@@ -406,24 +466,6 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
             for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
           }
           if (careful) tc::tmem_wait_st();
-          if (__builtin_expect(holes, 0)) {  // another pass: keys without a page are masked
-            top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < STG; c += 32) {
-              const uint32_t unread = s_unread[(blocks + j) & 3][c >> 5];
-              uint32_t x[32];
-              tc::tmem_ld32_nowait(col_s + c, x);
-              tc::tmem_wait_ld32(x);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                x[e] = (unread >> e) & 1 ? 0xff800000u : __float_as_uint(__uint_as_float(x[e]) * scale);
-                top = fmaxf(top, __uint_as_float(x[e]));
-              }
-              tc::tmem_st32(col_s + c, x);
-            }
-            tc::tmem_wait_st();
-            scale = 1.f;
-          }
           follow(top * scale);
           float2 s01 = make_float2(0.f, 0.f);
           const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
@@ -511,6 +553,9 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           ldg_bytes<C::kRow>(p.kq + row * C::kRow, kw);
           ldg_bytes<NB * 2>(reinterpret_cast<const uint8_t*>(p.ks + row * NB), ksc);
           ldg_bytes<NB * 2>(reinterpret_cast<const uint8_t*>(p.vs + row * NB), kvs);
+        } else {  // zeros, whatever the quants held are
+#pragma unroll
+          for (int k = 0; k < (NB + 1) / 2; ++k) ksc[k] = kvs[k] = 0;
         }
       };
       auto load_v = [&](int j) {
@@ -522,10 +567,12 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           if (i < read_v) {
             ldg_bytes<UV>(p.vq + (row + i) * C::kRow + g * UV, vw[i]);
             ldg_bytes<NB * 2>(reinterpret_cast<const uint8_t*>(p.vs + (row + i) * NB), vsc[i]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < (NB + 1) / 2; ++k) vsc[i][k] = 0;
           }
       };
-      // the largest magnitude of a scale whose values all fit f16; others make their key NaN for the rows that see it
-      const uint32_t most = FMT == 0 ? 0x6ffeu : 0x5ffcu;  // 8 * 8184 < 65504, 128 * 511 < 65504
+      constexpr uint32_t kOne = 0x3c003c00u, kLessHalf = (15 - C::kLess) << 10;  // f16: 1 and 1, 2^-kLess
       load_k(0);
       if (FMT == 0) load_v(0);  // q8_0: no registers to have them a block ahead
       for (int j = 0; j < n && ok; ++j) {
@@ -533,35 +580,53 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         const int kbuf = at % KB, vbuf = at % VB;
         if (FMT == 2) load_v(j);
         if (at >= KB && !wait(&b_kempty[kbuf], at / KB - 1)) break;
-        const uint32_t unread = __ballot_sync(0xffffffffu, !read_k && (begin + j) * STG + th < q.len);
-        if (lane == 0) s_unread[at & 3][warp - SW] = unread;
+        const uint32_t largest_k = largest_half<NB>(ksc), largest_v = largest_half<NB>(kvs);
+        const bool large = max(largest_k, largest_v) > C::kMost;  // or not finite
+        const uint32_t odd = __ballot_sync(0xffffffffu, large || (!read_k && (begin + j) * STG + th < q.len));
+        if (lane == 0) s_odd[at & 3][warp - SW] = odd;
         uint8_t* kt = smem + MT * C::kQ + kbuf * C::kParts * C::kTile + th * 16;
-        bool fits = true;
-#pragma unroll
-        for (int k = 0; k < NB; ++k)
-          fits &= !read_k || ((kvs[k / 2] >> (16 * (k & 1))) & 0x7fffu) <= most;
-#pragma unroll
-        for (int w = 0; w < NB * 4; ++w) {  // word w = (t, block)
-          const int k = w % NB;
-          const uint32_t d = __byte_perm(ksc[k / 2], 0, (k & 1) ? 0x3232 : 0x1010);
+        // word w = (t, block) of the key, its packed quants and its scale -> the operand's 16 bytes
+        auto unpack_key = [&](int w, uint32_t q0, uint32_t q1, uint32_t d, uint32_t less) {
           uint32_t i[4], x[4];  // the quants as f16, and times their scale
           if constexpr (FMT == 0) {
-            i[0] = low_nibbles<true>(kw[w]), i[1] = high_nibbles_int(kw[w]);
-            i[2] = low_nibbles<true>(kw[w] >> 8), i[3] = high_nibbles_int(kw[w] >> 8);
+            i[0] = low_nibbles<true>(q0), i[1] = high_nibbles_int(q0);
+            i[2] = low_nibbles<true>(q0 >> 8), i[3] = high_nibbles_int(q0 >> 8);
           } else {
-            i[0] = two_bytes<true>(kw[2 * w], 0), i[1] = two_bytes<true>(kw[2 * w], 1);
-            i[2] = two_bytes<true>(kw[2 * w + 1], 0), i[3] = two_bytes<true>(kw[2 * w + 1], 1);
+            i[0] = two_bytes<true>(q0, 0), i[1] = two_bytes<true>(q0, 1);
+            i[2] = two_bytes<true>(q1, 0), i[3] = two_bytes<true>(q1, 1);
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] = read_k ? mul_half2(i[e], d) : 0u;
-            if (!fits) x[e] = 0x7fff7fffu;
+            if (less != kOne) i[e] = mul_half2(i[e], less);
+            x[e] = mul_half2(i[e], d);
           }
           *reinterpret_cast<uint4*>(kt + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
           if constexpr (EXACT) {  // what the rounding left: one exact fused multiply-add
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = read_k && fits ? fma_half2(i[e], d, x[e] ^ 0x80008000u) : 0u;
+            for (int e = 0; e < 4; ++e) x[e] = fma_half2(i[e], d, x[e] ^ 0x80008000u);
             *reinterpret_cast<uint4*>(kt + C::kTile + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        };
+#pragma unroll
+        for (int w = 0; w < NB * 4; ++w) {
+          const int k = w % NB;
+          unpack_key(w, kw[FMT == 0 ? w : 2 * w], FMT == 0 ? 0 : kw[2 * w + 1],
+                     __byte_perm(ksc[k / 2], 0, (k & 1) ? 0x3232 : 0x1010), kOne);
+        }
+        if (__builtin_expect(odd != 0, 0)) {
+          const uint32_t k = __ballot_sync(0xffffffffu, largest_k > C::kMost), v = __ballot_sync(0xffffffffu, largest_v > C::kMost);
+          if (lane == 0) s_less[at & 3][0][warp - SW] = k, s_less[at & 3][1][warp - SW] = v;
+          if (large) {  // once more: 2^kLess less, or NaN where a scale is not finite, and so the rows that see this key
+            const int64_t row = row_of((begin + j) * STG + th);
+            const bool finite = max(largest_k, largest_v) < 0x7c00u;
+            const uint32_t less = largest_k > C::kMost ? kLessHalf * 0x10001u : kOne;
+#pragma unroll 1
+            for (int w = 0; w < NB * 4; ++w) {
+              const uint8_t* at = p.kq + row * C::kRow + w * (C::kRow / (NB * 4));
+              const uint32_t q0 = __ldg(reinterpret_cast<const uint32_t*>(at));
+              const uint32_t q1 = FMT == 0 ? 0 : __ldg(reinterpret_cast<const uint32_t*>(at) + 1);
+              unpack_key(w, q0, q1, finite ? p.ks[row * NB + w % NB] * 0x10001u : 0x7fff7fffu, less);
+            }
           }
         }
         load_k(j + 1);
@@ -570,38 +635,71 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
 
         if (at >= VB && !wait(&b_vempty[vbuf], at / VB - 1)) break;
         uint8_t* vt = smem + MT * C::kQ + (KB * C::kParts + vbuf) * C::kTile + kg * (D * 16) + g * 16;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // keys that are not there, or do not fit, are zeros
-          bool use = i < read_v;
-#pragma unroll
-          for (int k = 0; k < NB; ++k) use &= ((vsc[i][k / 2] >> (16 * (k & 1))) & 0x7fffu) <= most;
-          if (!use) {
-#pragma unroll
-            for (int k = 0; k < (NB + 1) / 2; ++k) vsc[i][k] = 0;
-#pragma unroll
-            for (int k = 0; k < (UV + 3) / 4; ++k) vw[i][k] = 0;
+        // column 4k + c of the unit: 8 keys' values, from two keys' packed quants and scales at a time
+        auto unpack_values = [&](uint32_t w0, uint32_t w1, int odd_block, uint32_t d, uint32_t less, uint32_t (&x)[4]) {
+          if constexpr (FMT == 0) {
+            const uint32_t w = __byte_perm(w0, w1, odd_block ? 0x7632 : 0x5410);
+            x[0] = low_nibbles<true>(w), x[1] = high_nibbles_int(w);
+            x[2] = low_nibbles<true>(w >> 8), x[3] = high_nibbles_int(w >> 8);
+          } else {
+            const uint32_t lo = __byte_perm(w0, w1, 0x5140), hi = __byte_perm(w0, w1, 0x7362);
+            x[0] = two_bytes<true>(lo, 0), x[1] = two_bytes<true>(lo, 1);
+            x[2] = two_bytes<true>(hi, 0), x[3] = two_bytes<true>(hi, 1);
           }
-        }
 #pragma unroll
-        for (int k = 0; k < NB; ++k) {
-          uint32_t x[4][4];  // [column of the unit][pair of keys]
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t d = __byte_perm(vsc[2 * i][k / 2], vsc[2 * i + 1][k / 2], (k & 1) ? 0x7632 : 0x5410);
-            if constexpr (FMT == 0) {
-              const uint32_t w = __byte_perm(vw[2 * i][k / 2], vw[2 * i + 1][k / 2], (k & 1) ? 0x7632 : 0x5410);
-              x[0][i] = mul_half2(low_nibbles<true>(w), d), x[1][i] = mul_half2(high_nibbles_int(w), d);
-              x[2][i] = mul_half2(low_nibbles<true>(w >> 8), d), x[3][i] = mul_half2(high_nibbles_int(w >> 8), d);
-            } else {
-              const uint32_t lo = __byte_perm(vw[2 * i][k], vw[2 * i + 1][k], 0x5140);
-              const uint32_t hi = __byte_perm(vw[2 * i][k], vw[2 * i + 1][k], 0x7362);
-              x[0][i] = mul_half2(two_bytes<true>(lo, 0), d), x[1][i] = mul_half2(two_bytes<true>(lo, 1), d);
-              x[2][i] = mul_half2(two_bytes<true>(hi, 0), d), x[3][i] = mul_half2(two_bytes<true>(hi, 1), d);
-            }
-          }
+          for (int c = 0; c < 4; ++c) x[c] = mul_half2(less != kOne ? mul_half2(x[c], less) : x[c], d);
+        };
+        auto store_values = [&](int k, const uint32_t (&x)[4][4]) {  // [pair of keys][column]
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(vt + (k * 32 + c * 8) * 16) = make_uint4(x[c][0], x[c][1], x[c][2], x[c][3]);
+            *reinterpret_cast<uint4*>(vt + (k * 32 + c * 8) * 16) = make_uint4(x[0][c], x[1][c], x[2][c], x[3][c]);
+        };
+        uint32_t top = vsc[0][0] & 0x7fff7fffu;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int k = 0; k < (NB + 1) / 2; ++k) top = __vmaxu2(top, vsc[i][k] & 0x7fff7fffu);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          uint32_t x[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int word = FMT == 0 ? k / 2 : k;
+            unpack_values(vw[2 * i][word], vw[2 * i + 1][word], k & 1,
+                          __byte_perm(vsc[2 * i][k / 2], vsc[2 * i + 1][k / 2], (k & 1) ? 0x7632 : 0x5410), kOne, x[i]);
+          }
+          store_values(k, x);
+        }
+        if (__builtin_expect(max(top & 0xffffu, top >> 16) > C::kMost, 0)) {
+          // once more: rows with a large scale 2^kLess less, those with one that is not finite zeros (their keys are NaN)
+          const int64_t row = row_of((begin + j) * STG + kg * 8);
+          uint32_t use = 0, large = 0;
+#pragma unroll 1
+          for (int i = 0; i < read_v; ++i) {
+            uint32_t m = 0;
+#pragma unroll 1
+            for (int k = 0; k < NB; ++k) m = max(m, p.vs[(row + i) * NB + k] & 0x7fffu);
+            use |= (m < 0x7c00u) << i, large |= (m > C::kMost) << i;
+          }
+#pragma unroll 1
+          for (int k = 0; k < NB; ++k) {
+            uint32_t x[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[2], d[2], less[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = 2 * i + e;
+                const bool is = use >> key & 1;
+                const uint8_t* at = p.vq + (row + (is ? key : 0)) * C::kRow + g * UV + k * (UV / NB);
+                w[e] = FMT == 0 ? *reinterpret_cast<const uint16_t*>(at) : *reinterpret_cast<const uint32_t*>(at);
+                d[e] = is ? p.vs[(row + key) * NB + k] : 0;
+                less[e] = large >> key & 1 ? kLessHalf : 0x3c00u;
+              }
+              unpack_values(w[0], w[1], 0, d[0] | d[1] << 16, less[0] | less[1] << 16, x[i]);
+            }
+            store_values(k, x);
+          }
         }
         if (FMT == 0) load_v(j + 1);
         tc::fence_async_smem();

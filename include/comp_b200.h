@@ -330,6 +330,8 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
  *   s_j = scale * q.k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);  slopes: s_j -= slopes[h] * |p - j|
  *   over the visible keys  max(starts[t], window ? p - window + 1 : 0) <= j < min(lens[b], max(p + 1, prefix[b])),
  *   out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j).
+ * Values of any finite scale are attended to; a scale that is not finite makes the rows that see its token NaN, or, as a
+ * key's, leaves them undefined, and no other row.
  * A row that sees no key gives out = 0 and lse = -inf. starts (per query token: the first key of its document) and
  * prefix (per sequence: keys that every query sees) are int32, slopes f32 [q_heads]; each may be NULL. scale > 0.
  * Scores, softmax sums and outputs are held in f32.

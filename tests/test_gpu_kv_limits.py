@@ -106,3 +106,107 @@ def test_a_table_shorter_than_its_sequence(cuda, fmt, dtype, queries, with_lse, 
                       window=window)
         _check_unread(206, fmt, dtype, [150, 170], queries, 4, 2, 64, 16, cuda, lambda t: t[:, :keep].copy(), with_lse,
                       window=window, slopes=2.0 ** -np.arange(1, 5), prefix=[70, 10])
+
+
+# ------------------------------------------------------------------------------------------- values past f16's range
+
+
+def _large(planes, table, lens, page, fmt, which, rng, every):
+    """Raises the scales of every `every`-th token of each sequence: one block past the largest whose values all fit f16,
+    up to f16's largest; the token's other blocks as they were."""
+    scales = planes[1 if which == "k" else 3]
+    past = 8192.0 if fmt == "q4_0" else 512.0
+    for b, n in enumerate(lens):
+        for j in range(every // 2, n, every):
+            h, blk = rng.integers(scales.shape[1]), rng.integers(scales.shape[3])
+            d = np.float16(np.exp(rng.uniform(np.log(past), np.log(65504.0))))
+            scales[table[b, j // page], h, j % page, blk] = d.view(np.uint16)
+
+
+def _resolution(fmt, planes, table, lens, cu, keys, values, q, page, scale, softcap, tensor):
+    """What an f16 weight's smallest step can move an output by, where a row's weights or its values' scales lie far apart.
+    Streaming: products of weight and value scale are held to 2^-25, their largest (the largest weight times the largest
+    scale, rounded up to a power of two) at 2^8 or more: 2^-32 of it for each whole quant. Tensor cores: weights to 2^-25,
+    the largest at 2^7 or more, times 2^4 (q8_0: 2^8) for keys whose values need it: 2^-32 of it for each value."""
+    out = np.zeros(q.shape)
+    group = q.shape[1] // keys[0].shape[1]
+    for b, n in enumerate(lens):
+        at = table[b, np.arange(n) // page], np.arange(n) % page
+        d = np.abs(planes[3][at[0], :, at[1]].view(np.float16).astype(np.float64))  # [len][heads][dim / 32]
+        for t in range(cu[b], cu[b + 1]):
+            hi = n - (cu[b + 1] - cu[b]) + t - cu[b] + 1
+            for h in range(q.shape[1]):
+                g = h // group
+                s = scale * (keys[b][:hi, g] @ q[t, h])
+                s = softcap * np.tanh(s / softcap) if softcap else s
+                w = np.exp(s - s.max())
+                top = 1 / w.sum()
+                if tensor:
+                    past = d[:hi, g].max() >= (8192.0 if fmt == "q4_0" else 512.0)
+                    step = top * (1 if not past else 16 if fmt == "q4_0" else 256)
+                    out[t, h] = 2.0**-32 * step * np.abs(values[b][:hi, g]).sum(0)
+                else:
+                    quants = np.abs(values[b][:hi, g]) / np.repeat(d[:hi, g], 32, axis=-1)
+                    out[t, h] = 2.0**-32 * top * d[:, g].max() * quants.sum(0)
+    return out
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+@pytest.mark.parametrize("dtype,queries,q_heads,heads,dim,with_lse", [
+    ("f32", [1, 3], 4, 2, 64, True), ("bf16", [1, 1], 8, 2, 128, True), ("bf16", [80, 30], 4, 2, 128, False),
+    ("bf16", [80, 30], 4, 2, 64, True), ("bf16", [130, 30], 6, 2, 96, True), ("bf16", [50, 50], 4, 2, 256, False)])
+@pytest.mark.parametrize("softcap", [0.0, 10.0])
+def test_values_past_the_range_of_f16(cuda, fmt, which, dtype, queries, q_heads, heads, dim, with_lse, softcap):
+    """Finite values of up to 128 * 65504 are attended to like any others. Scores are scaled so that the large keys
+    do not decide alone. A token that holds a value past 65504 keeps its values to 2^-17 (q4_0: 2^-21) at least."""
+    rng = np.random.default_rng(301)
+    planes, table, lens, cu, q = _problem(302, fmt, dtype, [170, 90], queries, q_heads, heads, dim, 16)
+    scale = dim**-0.5
+    for w in which:
+        _large(planes, table, lens, 16, fmt, w, rng, 11)
+    if "k" in which:
+        scale *= 2.0 / 65504.0 / (2.0 if fmt == "q4_0" else 32.0)
+    keys, values = _gather(fmt, planes, table, lens)
+    assert max(np.abs(x).max() for x in (keys if "k" in which else values)) > 65504
+    o, l, reach, mass = ref.attention(q.float().numpy(), keys, values, lens, cu, scale, softcap)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    one = list(queries) == [1] * len(lens)
+    _device_error()
+    got = kv.attention(q.to(cuda), _cache(fmt, planes, cuda), tt, tl, scale=scale, cu_q=None if one else tc,
+                       max_q=max(queries), softcap=softcap, return_lse=with_lse)
+    assert _device_error() == 0
+    got, lse = got if with_lse else (got, None)
+    tensor = _tensor_cores(dtype, max(queries) * (q_heads // heads), dim, with_lse)
+    bound, e = _bounds(dtype, tensor, with_lse, dim, softcap, o, reach, mass)
+    if "v" in which:
+        bound = bound + _resolution(fmt, planes, table, lens, cu, keys, values, q.double().numpy(), 16, scale, softcap, tensor)
+        if tensor:
+            bound = bound + (2.0**-21 if fmt == "q4_0" else 2.0**-17)
+    g = got.double().cpu().numpy()
+    assert np.isfinite(g).all()
+    assert (np.abs(g - o) <= bound).all(), float((np.abs(g - o) / bound).max())
+    if with_lse:
+        d = np.abs(lse.double().cpu().numpy() - l)
+        assert (d <= e + 2.0**-21 * (1 + np.abs(l))).all()
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("with_lse", [True, False])
+def test_one_large_key_alone(cuda, fmt, sign, with_lse):
+    """Rows that see a single key, whose values lie past f16's range: its value, whatever the score's sign."""
+    planes, table, lens, cu, _ = _problem(303, fmt, "bf16", [60], [60], 2, 1, 64, 16)
+    planes[1][...] = np.float16(65504.0).view(np.uint16)
+    planes[3][...] = np.float16(60000.0).view(np.uint16)
+    keys, values = _gather(fmt, planes, table, lens)
+    q = torch.from_numpy(np.sign(keys[0]).repeat(2, 1).astype(np.float32) * sign).to(torch.bfloat16)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    got = kv.attention(q.to(cuda), _cache(fmt, planes, cuda), tt, tl, cu_q=tc, max_q=60, window=1, scale=1e-6,
+                       return_lse=with_lse)
+    got, lse = got if with_lse else (got, None)
+    want = values[0].repeat(2, 1)
+    assert (np.abs(got.double().cpu().numpy() - want) <= 2.0**-8 * np.abs(want)).all()
+    if with_lse:
+        s = 1e-6 * (keys[0].repeat(2, 1) * q.double().numpy()).sum(-1)
+        assert (np.abs(lse.double().cpu().numpy() - s) <= 2.0**-15 * np.abs(s)).all()
