@@ -5,10 +5,11 @@
 //     bytes, K-major, no swizzle): keys as [8 values of a key][key], values transposed, as [8 keys of a column][column];
 //   - one thread issues the products: S = Q K^T into tensor memory, and O += P V with P read from tensor memory;
 //   - two warpgroups, a row a thread, turn S into P (f16, in S's own columns) and keep the row's reference exponent and
-//     sum in f32; the other tile's products run meanwhile. The reference follows the row's maximum only when that has
-//     grown by more than 2^8: then the thread rescales its row of O, which no product is using at that time.
-// Queries are scaled by a power of two a row (exact for 16-bit queries) and take the order of the keys' packed words, so
-// that one word of a key becomes one 16-byte chunk of its operand. Keys and values are rounded to f16 (11 bits), weights
+//     sum in f32; the other tile's products run meanwhile. The reference lies 2^7 below the row's maximum
+//     (so that f16 holds small weights) and follows it only when that has grown by more than 2^8: then the thread rescales
+//     its row of O, which no product is using at that time.
+// Queries are scaled by a power of two a row, its largest to 2^6 (exact for f16 values down to 2^-20 of that and bf16 values
+// down to 2^-23, the others within 2^-31 of it), and take the order of the keys' packed words, so that one word of a key becomes one 16-byte chunk of its operand. Keys and values are rounded to f16 (11 bits), weights
 // to f16. A key with values past f16's range (65504) enters its operand a power of two smaller, and its scores, or its
 // weights, are made as much larger: passes of their own over such a block, as for keys without a page, which are masked.
 //
@@ -351,11 +352,12 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           const bool mask = __any_sync(0xffffffffu, kb < lo || kb + STG > hi);
           const bool careful = special || mask;
           const float scale = careful ? 1.f : mul;
-          // takes the reference to the row's maximum where that has grown by more than 2^8, and O with it
+          // takes the reference to 2^-7 of the row's maximum where that has grown by more than 2^8, and O with it: a row's
+          // largest weight lies from 2^7 to 2^15, and weights down to 2^-21 of it keep all of f16's bits
           auto follow = [&](float top) {
-            const bool grown = top > ref + 8.f;
+            const bool grown = top > ref + 15.f;
             if (!__any_sync(0xffffffffu, grown)) return;
-            const float now = grown ? top : ref, f = exp2_approx(ref - now);
+            const float now = grown ? top - 7.f : ref, f = exp2_approx(ref - now);
             ref = now, sum *= f;
             if (j > 0) {  // the block before is in O already: its product ended before this block's scores
 #pragma unroll 1

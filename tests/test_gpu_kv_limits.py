@@ -210,3 +210,41 @@ def test_one_large_key_alone(cuda, fmt, sign, with_lse):
     if with_lse:
         s = 1e-6 * (keys[0].repeat(2, 1) * q.double().numpy()).sum(-1)
         assert (np.abs(lse.double().cpu().numpy() - s) <= 2.0**-15 * np.abs(s)).all()
+
+
+# ------------------------------------------------------------------------------------------------ scales, caps, tails
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dtype,queries", [("f32", 1), ("bf16", 1), ("f16", 16), ("bf16", 16)])
+@pytest.mark.parametrize("nats", [8.0, 12.0, 17.0, 19.0])
+def test_a_long_tail_of_small_weights(cuda, fmt, dtype, queries, nats):
+    """One key of weight 1 and value 0 before many equal small weights, whose values are the answer; enough sequences that
+    a thread block takes each of them whole. A weight is at least 2^7 for the row's largest and rounded at 2^-25 at worst:
+    2^-32 of the largest for each key, beside its own 2^-11."""
+    n, batch, page = 1088, 160, 64
+    planes, table, lens, cu, q = _problem(403, fmt, dtype, [n] * batch, [queries] * batch, 4, 1, 64, page)
+    off = 8 if fmt == "q4_0" else 128
+    # keys of zeros but for the first one's first value, 7; values of 1 but for the first key's, 0
+    kx, vx = np.zeros((n, 64)), np.ones((n, 64))
+    kx[0, 0], vx[0] = 7.0, 0.0
+    for x, (rows, scales), which in ((kx, planes[:2], "k"), (vx, planes[2:], "v")):
+        place, shift = ref._places(fmt, 64, which)
+        r = np.zeros((n, rows.shape[-1]), np.uint8)
+        for e in range(64):
+            r[:, place[e]] |= (x[:, e] + off).astype(np.uint8) << np.uint8(shift[e])
+        rows[table, 0] = r.reshape(n // page, page, -1)
+        scales[...] = np.float16(1.0).view(np.uint16)
+    q = torch.zeros_like(q)
+    q[:, :, 0] = 1.0
+    keys, values = _gather(fmt, planes, table[:1], [n])
+    assert np.array_equal(keys[0][:, 0], kx) and np.array_equal(values[0][:, 0], vx)
+    scale = nats / 7.0
+    # every sequence is the same one
+    o, _, reach, mass = ref.attention(q[:queries].float().numpy(), keys, values, [n], cu[:2], scale)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    got = kv.attention(q.to(cuda), _cache(fmt, planes, cuda), tt, tl, cu_q=tc, max_q=queries, scale=scale)
+    bound, _ = _bounds(dtype, _tensor_cores(dtype, 4 * queries, 64, False), False, 64, 0.0, o, reach, mass)
+    bound = bound + n * 2.0**-32
+    d = np.abs(got.double().cpu().numpy().reshape(batch, *o.shape) - o)
+    assert (d <= bound).all(), float((d / bound).max())
