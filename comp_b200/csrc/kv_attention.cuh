@@ -27,6 +27,7 @@
 // bulk copies instead of cp.async (the same), the next keys' scores beside these keys' products (229 us).
 #pragma once
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -496,7 +497,9 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
         if (c == 0) {
           float f = __int_as_float((127 + e2 - 13) << 23) * p.scale * (SIGNED ? 1.f : 0x1p24f);
           f *= p.softcap > 0.f ? 1.f / p.softcap : kLog2e;
-          s_rowf[r] = f;
+          // a positive number always: masked scores are -inf times it, and a row of zeros has scores of 0 (what passes f32
+          // here are scales for which scores are 0, or equal to the largest alone, either way)
+          s_rowf[r] = fminf(fmaxf(f, FLT_MIN), FLT_MAX);
         }
       }
     }

@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
         const float up = __int_as_float((127 + 6 - e2) << 23);
         rowf = __int_as_float((127 + e2 - 6) << 23) * p.scale;
         rowf *= p.softcap > 0.f ? 1.f / p.softcap : kLog2e;
+        rowf = fminf(rowf, FLT_MAX);  // (times a score of 0)
         mul = rowf;
 #pragma unroll
         for (int c0 = 0; c0 < kPieces; c0 += kOnce) {

@@ -9,7 +9,7 @@ import torch
 from comp_b200 import kv
 from oracle import kv as ref
 
-from .test_gpu_kv import _bounds, _cache, _device_error, _gather, _problem
+from .test_gpu_kv import DT, _bounds, _cache, _device_error, _gather, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -213,6 +213,36 @@ def test_one_large_key_alone(cuda, fmt, sign, with_lse):
 
 
 # ------------------------------------------------------------------------------------------------ scales, caps, tails
+
+
+@pytest.mark.parametrize("dtype,n", [("f32", 1), ("bf16", 1), ("f16", 3), ("f32", 20), ("f16", 64), ("bf16", 64)])
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 1e-30, 1e-12, 1.0, 1e12, 1e30])
+@pytest.mark.parametrize("softcap", [0.0, 1e-20, 20.0, 1e20])
+def test_rows_of_zeros_at_every_scale(cuda, dtype, n, fmt, scale, softcap):
+    """Equal scores whatever the scale and the cap: the mean of the values, with keys that are masked beside them."""
+    planes, table, lens, cu, q = _problem(401, fmt, dtype, [77, 130], [n, n], 4, 2, 64, 16)
+    keys, values = _gather(fmt, planes, table, lens)
+    o, l, reach, mass = ref.attention(q.float().numpy() * 0, keys, values, lens, cu, 1.0, window=70)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    got, lse = kv.attention(q.to(cuda) * 0, _cache(fmt, planes, cuda), tt, tl, cu_q=tc, max_q=n, scale=scale,
+                            softcap=softcap, window=70, return_lse=True)
+    bound, _ = _bounds(dtype, _tensor_cores(dtype, 2 * n, 64, True), True, 64, 0.0, o, reach, mass)
+    assert (np.abs(got.double().cpu().numpy() - o) <= bound).all()
+    assert (np.abs(lse.double().cpu().numpy() - l) <= 2.0**-19 * (1 + np.abs(l))).all()
+
+
+@pytest.mark.parametrize("dtype,n", [("f32", 1), ("bf16", 1), ("f32", 20), ("bf16", 64)])
+def test_tiny_queries_and_scales(cuda, dtype, n):
+    """Scores far below 1 in products that pass f32's range on the way."""
+    planes, table, lens, cu, q = _problem(402, "q4_0", dtype, [77, 130], [n, n], 4, 2, 64, 16)
+    keys, values = _gather("q4_0", planes, table, lens)
+    q = q * torch.tensor(1e-33, dtype=DT[dtype])
+    o, l, reach, mass = ref.attention(q.float().numpy(), keys, values, lens, cu, 1e-20, window=70)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    got = kv.attention(q.to(cuda), _cache("q4_0", planes, cuda), tt, tl, cu_q=tc, max_q=n, scale=1e-20, window=70)
+    bound, _ = _bounds(dtype, _tensor_cores(dtype, 2 * n, 64, False), False, 64, 0.0, o, reach, mass)
+    assert (np.abs(got.double().cpu().numpy() - o) <= bound).all()
 
 
 @pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
