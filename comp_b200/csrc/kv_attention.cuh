@@ -353,7 +353,8 @@ __global__ void __launch_bounds__(128, (kv_ctas_per_sm<FMT, NB, NT, PARTS>())) a
     }
     const Sequence q = sequence(p, b);
     const int rows = q.n * p.group - rt * R;  // rows from this tile on (at least 1)
-    if (q.end > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
+    if (threadIdx.x == 0 && (q.end > q.len || (rt + 1 == p.row_tiles && rows > R)))
+      atomicCAS(&g_device_error, 0, q.end > q.len ? kErrPage : kErrQueries);
     const int begin = span.first + from, stop = span.first + to;
 
     const int32_t* table = p.table + (int64_t)b * p.table_stride;

@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
     }
     const Sequence q = sequence(p, b);
     const int rows = q.n * p.group - rt * R;  // rows from this tile on (at least 1)
-    if (q.end > q.len && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrPage);
+    if (threadIdx.x == 0 && (q.end > q.len || (rt + 1 == p.row_tiles && rows > R)))
+      atomicCAS(&g_device_error, 0, q.end > q.len ? kErrPage : kErrQueries);
     const int begin = span.first + from, n = to - from, tiles = MT == 1 || rows <= 128 ? 1 : 2;
 
     if constexpr (ROLE == 0) {

@@ -214,9 +214,10 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
     document. A query that sees no key gives zeros (lse -inf).
 
     max_q / max_len: the most query tokens of a sequence and the longest length, where the caller knows them (default:
-    T, or 1 without cu_q, and what the table can hold): max_q must not be less than what cu_q has, max_len only plans
-    the work. workspace: a CUDA byte tensor of attention_workspace_size(...) bytes (allocated here when None). out: a
-    contiguous tensor for the result that shares no memory with q. Rows outside cu_q's range (padding) stay unwritten."""
+    T, or 1 without cu_q, and what the table can hold): max_q must not be less than what cu_q has (rows past it
+    stay unwritten and set the device error word to 4), max_len only plans the work. workspace: a CUDA byte tensor of
+    attention_workspace_size(...) bytes (allocated here when None). out: a contiguous tensor for the result that shares no
+    memory with q. Rows outside cu_q's range (padding) stay unwritten."""
     dev = cache.device
     _on_device("attention", dev, q, table, lens)
     did = _dtype_id("attention: q", q)

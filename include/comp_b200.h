@@ -335,7 +335,8 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
  * A row that sees no key gives out = 0 and lse = -inf. starts (per query token: the first key of its document) and
  * prefix (per sequence: keys that every query sees) are int32, slopes f32 [q_heads]; each may be NULL. scale > 0.
  * Scores, softmax sums and outputs are held in f32.
- * max_q: at least the most queries of a sequence (0: max_q = T); max_len: at least the longest lens, used to plan the
+ * max_q: at least the most queries of a sequence (0: max_q = T; rows that a smaller one leaves out stay unwritten, and the
+ * device error word is set to 4); max_len: at least the longest lens, used to plan the
  * split of the keys only. Tokens beyond the table or in pages outside the cache read as masked (the queries' positions
  * stay those of the whole sequence), and set the device error word to 3. out [T][q_heads][dim] contiguous, of q's dtype; lse f32 [T][q_heads] or NULL. Rows outside
  * cu_q[0] .. cu_q[batch] - 1 are left unwritten; out shares no memory with q. q: element strides per token and head, last
@@ -404,7 +405,7 @@ int b2q_set_cluster(int ctas);
 
 /* Reads (and with clear != 0 resets) the library's device error word: 1 if a kernel's bounded wait on an mbarrier gave
  * up (the kernel then returned early; its outputs are invalid), 2 if a KV cache slot was beyond its cache, 3 if an
- * attention call met a token without a valid page. Synchronizes with the device. */
+ * attention call met a token without a valid page, 4 if a sequence of one had more query tokens than its max_q. Synchronizes with the device. */
 int b2q_device_error(int* code, int clear);
 
 /* CUDA IPC helpers for the multi-GPU path. b2q_ipc_get_handle exports the allocation containing dev_ptr as a 64-byte

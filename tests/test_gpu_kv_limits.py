@@ -278,3 +278,19 @@ def test_a_long_tail_of_small_weights(cuda, fmt, dtype, queries, nats):
     bound = bound + n * 2.0**-32
     d = np.abs(got.double().cpu().numpy().reshape(batch, *o.shape) - o)
     assert (d <= bound).all(), float((d / bound).max())
+
+
+# ----------------------------------------------------------------------------------------------------------- refusals
+
+
+def test_more_queries_than_max_q_are_reported(cuda):
+    _device_error()
+    for dtype, n, most in ((torch.float32, 40, 2), (torch.bfloat16, 300, 48)):
+        cache = kv.KVCache("q4_0", 30, 16, 1, 64, device=cuda)
+        q = torch.randn(n, 1, 64, device=cuda, dtype=dtype)
+        table = torch.arange(30, dtype=torch.int32, device=cuda)[None]
+        lens, cu = torch.tensor([400], dtype=torch.int32, device=cuda), torch.tensor([0, n], dtype=torch.int32, device=cuda)
+        kv.attention(q, cache, table, lens, cu_q=cu, max_q=n)
+        assert _device_error() == 0
+        kv.attention(q, cache, table, lens, cu_q=cu, max_q=most)
+        assert _device_error() == 4
