@@ -52,6 +52,7 @@ __device__ __forceinline__ uint32_t quant_q4_0_quarter(const float (&v)[8], int 
     first = min(first, __shfl_xor_sync(0xffffffffu, first, 2));
     if (hi == -lo) m = (first & 1) ? lo : hi;
   }
+  m = __fadd_rn(m, 0.f);  // ggml's maximum begins at +0: a block of zeros, of either sign, has the scale -0
   const float d = __fmul_rn(m, -0.125f);  // m / -8, exact but for underflow
   const float id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
   uint32_t q[8];

@@ -29,7 +29,7 @@ def quantize(fmt, x):
     with np.errstate(over="ignore", invalid="ignore", divide="ignore"):
         if fmt == "q4_0":
             first = np.abs(b).argmax(-1)[..., None]
-            d = np.take_along_axis(b, first, -1) / f(-8)
+            d = (np.take_along_axis(b, first, -1) + f(0)) / f(-8)  # the maximum begins at +0: zeros have the scale -0
         else:
             d = np.abs(b).max(-1, keepdims=True) / f(127)
         inv = np.divide(f(1), d, out=np.zeros_like(d), where=d != 0)

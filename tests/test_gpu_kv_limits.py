@@ -294,3 +294,22 @@ def test_more_queries_than_max_q_are_reported(cuda):
         assert _device_error() == 0
         kv.attention(q, cache, table, lens, cu_q=cu, max_q=most)
         assert _device_error() == 4
+
+
+# -------------------------------------------------------------------------------------------------------------- write
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_blocks_of_zeros_have_ggmls_scale(cuda, dtype):
+    """ggml's maximum begins at +0 and takes larger magnitudes only: a block of zeros of either sign has the scale
+    +0 / -8 = -0 in q4_0, and +0 in q8_0."""
+    x = torch.zeros(4, 1, 64, dtype=DT[dtype])
+    x[1], x[2, :, ::2], x[3, :, 1:] = -0.0, -0.0, -0.0
+    slots = torch.arange(4, device=cuda)
+    for fmt, bits in (("q4_0", 0x8000), ("q8_0", 0)):
+        cache = kv.KVCache(fmt, 1, 16, 1, 64, device=cuda)
+        kv.kv_write(cache, x.to(cuda), x.to(cuda), slots)
+        for scales in (cache.ks, cache.vs):
+            assert (scales.cpu().numpy().view(np.uint16)[0, 0, :4] == bits).all()
+        for got in kv.kv_read(cache, slots):
+            assert (got == 0).all()

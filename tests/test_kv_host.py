@@ -125,3 +125,22 @@ def test_oracle_attention_masks():
     v = [np.arange(3.0)[:, None, None] * np.ones((3, 1, 32))]
     o, l, _, _ = ref.attention(np.zeros((1, 1, 32)), k, v, [3], np.array([0, 1]), 1.0)
     assert np.allclose(o, 1.0) and np.allclose(l, np.log(3))
+
+
+def test_quantize_is_ggmls_loop():
+    """ggml's q4_0 block as its steps are: the maximum begins at +0 and takes a value of larger magnitude only."""
+    f = np.float32
+    x = np.random.default_rng(4).standard_normal((9, 32)).astype(f)
+    x[0], x[1] = 0.0, -0.0
+    x[2, ::3], x[3] = -0.0, np.where(np.arange(32) % 2, f(-0.0), f(0.0))
+    x[4, 7], x[4, 9], x[5, 7], x[5, 9] = 9.0, -9.0, -9.0, 9.0
+    q, s = ref.quantize("q4_0", x)
+    for row, quants, bits in zip(x, q, s[:, 0]):
+        top, at = f(0), f(0)
+        for v in row:
+            if top < abs(v):
+                top, at = abs(v), v
+        d = at / f(-8)
+        inv = f(1) / d if d else f(0)
+        assert bits == np.float16(d).view(np.uint16)
+        assert np.array_equal(quants, [min(15, int(v * inv + f(8.5))) for v in row])
