@@ -13,6 +13,7 @@ their device, and raise TypeError / ValueError / RuntimeError on what they do no
 """
 
 import ctypes
+import numbers
 import struct
 
 import torch
@@ -184,6 +185,8 @@ assert struct.calcsize("@9P8q3i2f") <= ctypes.sizeof(_lib.AttentionArgs)
 
 def attention_workspace_size(cache, T, batch, q_heads, dtype, max_q=1, return_lse=False):
     """Bytes of device workspace that attention needs for such a call (max_q as there: 1 without cu_q)."""
+    if dtype not in DTYPE_ID:
+        raise TypeError(f"attention_workspace_size: dtype {dtype}, expected float32, float16 or bfloat16")
     key = (T > 0 and batch > 0, q_heads, dtype, max_q if max_q and max_q < T else T, return_lse)
     size = cache._sizes.get(key)
     if size is None:
@@ -260,7 +263,11 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
                           cu_at, prefix_at, starts_at, slopes_at, q_st, q_sh, T, B, table.stride(0) if B > 1 else P, P, max_q,
                           P * cache.page_size if max_len is None else max_len, heads, did, window,
                           dim**-0.5 if scale is None else scale, softcap)
-    except struct.error as e:
+    except (struct.error, OverflowError) as e:
+        kinds = ((numbers.Integral, (max_q, window, 0 if max_len is None else max_len)),
+                 (numbers.Real, (softcap, 1.0 if scale is None else scale)))
+        if all(isinstance(x, kind) for kind, given in kinds for x in given):
+            raise ValueError(f"attention: max_q, max_len, window, scale or softcap out of range: {e}") from None
         raise TypeError(f"attention: max_q, max_len and window are whole numbers, scale and softcap numbers: {e}") from None
     _call(dev, "b2q_attention", cache._ref, args, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
           _raw_stream(dev.index))

@@ -296,6 +296,18 @@ def test_more_queries_than_max_q_are_reported(cuda):
         assert _device_error() == 4
 
 
+def test_numbers_out_of_range_are_value_errors(cuda):
+    c = kv.KVCache("q4_0", 4, 16, 2, 64, device=cuda)
+    q = torch.zeros(2, 4, 64, device=cuda)
+    table, lens = torch.zeros(2, 3, dtype=torch.int32, device=cuda), torch.zeros(2, dtype=torch.int32, device=cuda)
+    for bad in (dict(scale=1e39), dict(scale=float("inf")), dict(scale=1e-60), dict(softcap=1e39), dict(window=2**31),
+                dict(window=-(2**40)), dict(max_len=2**63), dict(max_len=-1)):
+        with pytest.raises(ValueError):
+            kv.attention(q, c, table, lens, **bad)
+    with pytest.raises(TypeError):
+        kv.attention_workspace_size(c, 2, 2, 4, torch.int8)
+
+
 # -------------------------------------------------------------------------------------------------------------- write
 
 
