@@ -280,6 +280,95 @@ def test_a_long_tail_of_small_weights(cuda, fmt, dtype, queries, nats):
     assert (d <= bound).all(), float((d / bound).max())
 
 
+@pytest.mark.parametrize("cap", [0.3, 1.0, 50.0])
+@pytest.mark.parametrize("dtype,n", [("f32", 1), ("bf16", 50)])
+def test_the_cap_against_tanh(cuda, cap, dtype, n):
+    """lse of a row that sees one key is its capped score: scores from 1e-4 to 30 times the cap, both signs. The cap's own
+    steps cost 2^-21 of its result at most (tanh within 2^-22, two roundings), the score 2^-19 of it (16-bit calls: 2^-15),
+    which tanh, of slope at most 1, passes on; 2^x costs 2^-20, and lse is a product and a sum of logarithms, 2^-21 of 1 + |lse|."""
+    rng = np.random.default_rng(404)
+    batch = 400
+    planes, table, lens, cu, q = _problem(405, "q8_0", dtype, [n] * batch, [n] * batch, 1, 1, 64, 64)
+    keys, values = _gather("q8_0", planes, table, lens)
+    k = np.concatenate([x[:, 0] for x in keys])
+    x = np.exp(rng.uniform(np.log(1e-4), np.log(30.0), len(k))) * rng.choice([-1.0, 1.0], len(k)) * cap
+    q = torch.from_numpy((k * (x / (k * k).sum(-1))[:, None]).astype(np.float32)[:, None]).to(DT[dtype])
+    s = (q.double().numpy()[:, 0] * k).sum(-1)
+    reach = np.abs(q.double().numpy()[:, 0] * k).sum(-1)
+    want = cap * np.tanh(s / cap)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    _, lse = kv.attention(q.to(cuda), _cache("q8_0", planes, cuda), tt, tl, cu_q=tc, max_q=n, scale=1.0, softcap=cap,
+                          window=1, return_lse=True)
+    d = np.abs(lse.double().cpu().numpy()[:, 0] - want)
+    slope = 1 - np.tanh(np.maximum(np.abs(s) - 2.0**-10 * reach, 0) / cap) ** 2
+    bound = (2.0**-19 if dtype == "f32" else 2.0**-15) * reach * slope
+    bound = bound + 2.0**-21 * np.abs(want) + 2.0**-20 + 2.0**-21 * (1 + np.abs(want))
+    assert (d <= bound).all(), float((d / bound).max())
+
+
+# ------------------------------------------------------------------------------------ the kernels' boundary, streams
+
+
+@pytest.mark.parametrize("rows", [47, 48, 49, 63, 64])
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("with_lse", [True, False])
+def test_rows_around_the_kernels_boundary(cuda, rows, fmt, dim, with_lse):
+    """One query head a KV head, so that the rows are the query tokens; and the same rows with a group of heads."""
+    for dtype in ("f16", "bf16"):
+        shapes = [(rows, 1)] + [(rows // g, g) for g in (3, 7) if rows % g == 0]
+        for n, group in shapes:
+            planes, table, lens, cu, q = _problem(501, fmt, dtype, [200, 61], [n, n // 2], 2 * group, 2, dim, 32)
+            keys, values = _gather(fmt, planes, table, lens)
+            o, l, reach, mass = ref.attention(q.float().numpy(), keys, values, lens, cu, dim**-0.5)
+            tt, tl, tc = _to(cuda, table, lens, cu)
+            got = kv.attention(q.to(cuda), _cache(fmt, planes, cuda), tt, tl, cu_q=tc, max_q=n, return_lse=with_lse)
+            got, lse = got if with_lse else (got, None)
+            bound, e = _bounds(dtype, _tensor_cores(dtype, rows, dim, with_lse), with_lse, dim, 0.0, o, reach, mass)
+            assert (np.abs(got.double().cpu().numpy() - o) <= bound).all()
+            if with_lse:
+                assert (np.abs(lse.double().cpu().numpy() - l) <= e + 2.0**-21 * (1 + np.abs(l))).all()
+
+
+@pytest.mark.parametrize("dtype,queries", [("bf16", [30, 12]), ("f16", [100, 7]), ("f32", [9, 11])])
+def test_without_max_q(cuda, dtype, queries):
+    """T bounds the queries of a sequence: on the tensor cores with 42 * 4 and 107 * 4 rows."""
+    planes, table, lens, cu, q = _problem(502, "q4_0", dtype, [177, 130], queries, 8, 2, 128, 16)
+    keys, values = _gather("q4_0", planes, table, lens)
+    o, l, reach, mass = ref.attention(q.float().numpy(), keys, values, lens, cu, 128**-0.5)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    for with_lse in (False, True):
+        got = kv.attention(q.to(cuda), _cache("q4_0", planes, cuda), tt, tl, cu_q=tc, return_lse=with_lse)
+        g = (got[0] if with_lse else got).double().cpu().numpy()
+        bound, _ = _bounds(dtype, dtype != "f32", with_lse, 128, 0.0, o, reach, mass)
+        assert (np.abs(g - o) <= bound).all()
+
+
+def test_calls_on_streams_that_overlap(cuda):
+    """Calls of both kernels on three streams at once, each with a workspace: the same bits as one after the other."""
+    jobs = []
+    for seed, dtype, lens, queries in ((601, "bf16", [3000, 900], [1, 1]), (602, "f16", [4000, 150], [300, 100]),
+                                       (603, "f32", [2500, 1200], [4, 3])):
+        planes, table, ln, cu, q = _problem(seed, "q4_0", dtype, lens, queries, 8, 2, 128, 64)
+        tt, tl, tc = _to(cuda, table, ln, cu)
+        cache, q = _cache("q4_0", planes, cuda), q.to(cuda)
+        a = dict(cu_q=tc, max_q=max(queries))
+        ws = torch.empty(kv.attention_workspace_size(cache, q.shape[0], 2, 8, q.dtype, max(queries)), dtype=torch.uint8,
+                         device=cuda)
+        jobs.append((q, cache, tt, tl, a, ws, kv.attention(q, cache, tt, tl, **a), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[] for _ in jobs]
+    for _ in range(20):
+        for (q, cache, tt, tl, a, ws, want, stream), got in zip(jobs, outs):
+            with torch.cuda.stream(stream):
+                got.append(kv.attention(q, cache, tt, tl, workspace=ws, **a))
+    torch.cuda.synchronize()
+    for job, got in zip(jobs, outs):
+        for x in got:
+            assert torch.equal(x, job[6])
+    assert _device_error() == 0
+
+
 # ----------------------------------------------------------------------------------------------------------- refusals
 
 
