@@ -18,7 +18,6 @@ I64 = ctypes.c_int64
 INT = ctypes.c_int
 
 
-
 class KVCacheDesc(ctypes.Structure):
     """b2q_kv_cache (include/comp_b200.h)."""
 

@@ -7,7 +7,9 @@
 // rows as the columns: nothing is padded, and no quant is rounded. What an operand's 16 bits hold:
 //   - keys (16-bit calls): the quant's bits alone, i.e. the f16 subnormal q * 2^-24 (or q * 2^-20 for a nibble left in bits 4-7): one
 //     AND unpacks two values. The offset -off * sum(Q) of a block is a constant of the row, added to the block's sum.
-//   - queries: scaled by a power of two to 2^13..2^14, so that 16-bit queries are exact; f32 queries take two parts.
+//   - queries: scaled by a power of two to 2^13..2^14; f32 queries take two parts. 16-bit queries are exact where a row's
+//     values lie within 2^27 (f16; bf16 2^30; q4_0 keys' high nibbles take a 16th: 2^23 and 2^26), smaller ones are within
+//     2^-38 (2^-34) of its largest.
 //     A block's scale dk (per key and block) multiplies the f32 sum of the block.
 //   - values: the quant minus its offset, again as an exact subnormal (an addition more for two values): offsets taken
 //     off the sums instead would cancel there, and leave their cut-off bits.
@@ -157,8 +159,8 @@ __device__ __forceinline__ void store_elt(void* p, int64_t i, int dtype, float v
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// tanh(z) / z of u = z^2 for |z| <= 0.6: fitted to the smallest largest relative error (7.3e-8). Beyond, tanh(|z|) =
-// 1 - 2 / (e^2z + 1); scores near the cap are rare, and where a warp has none it skips that (two of the slow units' steps).
+// tanh(z) / z of u = z^2 for |z| <= 0.6: fitted to the smallest largest relative error (9.0e-8 with the constants as they
+// stand in f32, 1.8e-7 with the steps' roundings). Beyond, tanh(|z|) = 1 - 2 / (e^2z + 1); scores near the cap are rare, and where a warp has none it skips that (two of the slow units' steps).
 constexpr float kTanhLimit = 0.6f;
 constexpr float kTanh0 = 0.99999994f, kTanh1 = -0.3333231f, kTanh2 = 0.13310172f, kTanh3 = -0.05210143f, kTanh4 = 0.015475366f;
 __device__ __forceinline__ float tanh_near(float z) {

@@ -39,7 +39,7 @@ struct TcTile {
   static constexpr int kSmem = MT * kQ + (kKeyBufs * kParts + kBufs) * kTile;
   // 4 unpacking, then 1 issuing; with two row tiles three more, which only hand their registers on
   static constexpr int kSoftmaxWarps = MT * 4, kWarps = MT == 2 ? 16 : MT * 4 + 5;
-  // registers of a thread at launch and after the split: 2 x 128 x 160 + 128 x 128 + 128 x 64 = 512 x 128
+  // registers of a thread at launch and after the split: 2 x 128 x 152 + 128 x 128 + 128 x 80 = 512 x 128
   static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kIssueRegs = 80;
   static_assert(MT == 1 || 256 * kSoftmaxRegs + 128 * kLaunchRegs + 128 * kIssueRegs <= 512 * kLaunchRegs, "registers");
   static constexpr uint32_t kS = 256;                     // column of S (and P) of tile 0; O is at 0
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
         }
-        // to 2^6 .. 2^7: products with keys of up to 2^16 stay far below f32's range, and 16-bit queries exact
+        // to 2^6 .. 2^7: products with keys of up to 2^16 stay far below f32's range
         const int e2 = max(-100, (__float_as_int(top) >> 23) - 127);
         const float up = __int_as_float((127 + 6 - e2) << 23);
         rowf = __int_as_float((127 + e2 - 6) << 23) * p.scale;

@@ -12,7 +12,6 @@ constexpr int kErrSlot = 2;  // device error word: a slot beyond the cache
 constexpr int kErrPage = 3;  // device error word: a token whose page is outside the table or the cache
 constexpr int kErrQueries = 4;  // device error word: query tokens past the tiles that max_q gave a sequence
 
-inline int kv_row_bytes(const b2q_kv_cache& c) { return c.fmt == B2Q_FMT_Q4_0 ? c.dim / 2 : c.dim; }
 inline int dtype_size(int dtype) { return dtype == B2Q_DTYPE_F32 ? 4 : 2; }
 
 // The checks of a cache descriptor that every entry point makes (kv_cache.cu).

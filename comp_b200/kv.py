@@ -132,7 +132,7 @@ def _heads_aligned(t):
 def kv_write(cache, k, v, slots):
     """Quantizes k and v [T][heads][head_dim] (f32, f16 or bf16; any token and head strides) into the slots int64 [T] of
     the cache (page * page_size + offset; no slot twice). Negative slots are skipped (padding tokens). The blocks are ggml's, bit for
-    bit (quantize_row_q4_0 / q8_0 of the value widened to f32); a 16-bit caller needs no cast."""
+    bit, of the value widened to f32; a 16-bit caller needs no cast."""
     dev = cache.device
     _on_device("kv_write", dev, k, v, slots)
     slots = _slots("kv_write", slots)
@@ -213,8 +213,8 @@ def attention(q, cache, table, lens, scale=None, *, cu_q=None, max_q=None, max_l
 
     softcap > 0: scores s -> softcap * tanh(s / softcap); slopes f32 [q_heads]: minus slopes[h] times the distance of
     query and key. A query at p sees the keys max(starts, p - window + 1) <= j < min(lens, max(p + 1, prefix)): window
-    (0: none) slides, prefix int32 [B] keys are seen by every query, starts int32 [T] is the first key of a query's
-    document. A query that sees no key gives zeros (lse -inf).
+    (0: none) slides, prefix int32 [B] keys are seen by the queries before them too (where their window and document reach
+    back so far), starts int32 [T] is the first key of a query's document. A query that sees no key gives zeros (lse -inf).
 
     max_q / max_len: the most query tokens of a sequence and the longest length, where the caller knows them (default:
     T, or 1 without cu_q, and what the table can hold): max_q must not be less than what cu_q has (rows past it

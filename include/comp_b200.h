@@ -330,17 +330,22 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
  *   s_j = scale * q.k_j;  softcap > 0: s_j = softcap * tanh(s_j / softcap);  slopes: s_j -= slopes[h] * |p - j|
  *   over the visible keys  max(starts[t], window ? p - window + 1 : 0) <= j < min(lens[b], max(p + 1, prefix[b])),
  *   out = sum_j softmax(s)_j v_j,  lse = log sum_j exp(s_j).
- * Values of any finite scale are attended to; a scale that is not finite makes the rows that see its token NaN, or, as a
- * key's, leaves them undefined, and no other row.
  * A row that sees no key gives out = 0 and lse = -inf. starts (per query token: the first key of its document) and
- * prefix (per sequence: keys that every query sees) are int32, slopes f32 [q_heads]; each may be NULL. scale > 0.
- * Scores, softmax sums and outputs are held in f32.
+ * prefix (per sequence: keys that the queries before them see too) are int32, slopes f32 [q_heads]; each may be NULL.
+ * scale in (0, 1e30], softcap 0 or in [1e-20, 1e20]. Cache values of any finite scale are attended to; a scale that is not
+ * finite makes the rows that see its token NaN, or, as a key's, leaves them undefined, and no other row.
+ * Scores, softmax sums and outputs are held in f32. f32 queries and weights enter the products in two parts of f16 (22
+ * bits), the cache's whole quants as they are. 16-bit calls round a weight to f16 (11 bits), and from 48 rows (queries times
+ * q_heads / heads) a sequence on keys and values too, but keys only where lse is NULL: max_q and lse so choose among
+ * results that differ by such roundings.
  * max_q: at least the most queries of a sequence (0: max_q = T; rows that a smaller one leaves out stay unwritten, and the
- * device error word is set to 4); max_len: at least the longest lens, used to plan the
- * split of the keys only. Tokens beyond the table or in pages outside the cache read as masked (the queries' positions
- * stay those of the whole sequence), and set the device error word to 3. out [T][q_heads][dim] contiguous, of q's dtype; lse f32 [T][q_heads] or NULL. Rows outside
- * cu_q[0] .. cu_q[batch] - 1 are left unwritten; out shares no memory with q. q: element strides per token and head, last
- * axis contiguous, 16-byte aligned in base and strides. scale in (0, 1e30], softcap 0 or in [1e-20, 1e20].
+ * device error word is set to 4). Kernel, tile height and plan go by it: pass it where it is known. max_len: at least the
+ * longest lens, used to plan the split of the keys only.
+ * Tokens beyond the table or in pages outside the cache read as masked (the queries' positions stay those of the whole
+ * sequence), and set the device error word to 3.
+ * q: element strides per token and head, last axis contiguous, 16-byte aligned in base and strides. out [T][q_heads][dim]
+ * contiguous, of q's dtype, shares no memory with q; lse f32 [T][q_heads] or NULL. Rows outside cu_q[0] .. cu_q[batch] - 1
+ * are left unwritten.
  */
 typedef struct {
   const void* q;
