@@ -9,9 +9,12 @@
 //     (so that f16 holds small weights) and follows it only when that has grown by more than 2^8: then the thread rescales
 //     its row of O, which no product is using at that time.
 // Queries are scaled by a power of two a row, its largest to 2^6 (exact for f16 values down to 2^-20 of that and bf16 values
-// down to 2^-23, the others within 2^-31 of it), and take the order of the keys' packed words, so that one word of a key becomes one 16-byte chunk of its operand. Keys and values are rounded to f16 (11 bits), weights
-// to f16. A key with values past f16's range (65504) enters its operand a power of two smaller, and its scores, or its
-// weights, are made as much larger: passes of their own over such a block, as for keys without a page, which are masked.
+// down to 2^-23, the others within 2^-31 of it), and take the order of the keys' packed words, so that one word of a key
+// becomes one 16-byte chunk of its operand. Values are rounded to f16 (11 bits), and so are keys and weights for bf16 calls,
+// whose outputs' own rounding (8 bits) is far larger; for f16 calls, where it is not, both enter in two parts (22 bits; error
+// against 64 bits 1.3 to 1.4 times one rounding's, in one part 1.6 to 2.6). A key with values past f16's range (65504) enters
+// its operand a power of two smaller, and its scores, or its weights, are made as much larger: passes of their own over such
+// a block, as for keys without a page, which are masked.
 //
 // What bounds it: 128 keys for 256 rows of 128 values take 2048 cycles on the tensor cores, 2048 on the units that compute
 // 2^x (16 a cycle), and about 2048 of shared memory's (operands of S from there twice, unpacked tiles into it); a tile's
@@ -25,18 +28,23 @@
 
 namespace b2q {
 
-// EXACT: the scores from keys in two f16 parts, what calls that return lse need: one part's rounding is 1e-4 of a score,
-// which a weight of 16 bits does not show, but an f32 lse does (1e-5 of it; with two parts 1e-7).
+// EXACT: the scores from keys in two f16 parts, what f16 calls and calls that return lse need: one part's rounding is 1e-4
+// of a score, which a bf16 output does not show, but an f16 one does, and an f32 lse (1e-5 of it; with two parts 1e-7).
+// WIDE (f16 calls): the weights in two parts too, the second beside the first in S's columns. Measured in one part / in two,
+// us, 32 heads on 8 of 128: four f16 prompts of 2048 281 / 346 (with lse 315 / 347), 1024 x 16384 over q8_0 355 / 440, packed
+// documents 138 / 146; heads of 256, whose key parts take turns in one tile, 1024 x 8192 264 / 438.
 template <int FMT, int NB, bool EXACT>
 struct TcTile {
   static constexpr int D = NB * 32;
   static constexpr int kRow = NB * (FMT == 0 ? 16 : 32);  // quant bytes of a token's row
   static constexpr int MT = NB == 8 ? 1 : 2;              // row tiles: tensor memory holds O (D) and S (128) of each
   static constexpr int kBufs = NB == 8 ? 1 : 2;           // value tiles in shared memory
-  static constexpr int kKeyBufs = EXACT ? 1 : kBufs, kParts = EXACT ? 2 : 1;  // key tiles, and the parts of each
+  // key tiles, the parts of a key, and how many of them take turns in one tile (heads of 256: no room for both)
+  static constexpr int kKeyBufs = EXACT ? 1 : kBufs, kParts = EXACT ? 2 : 1, kTurns = EXACT && NB == 8 ? 2 : 1;
   static constexpr int kRows = MT * 128, kKeys = 128;
   static constexpr int kQ = 128 * D * 2, kTile = 128 * D * 2;
-  static constexpr int kSmem = MT * kQ + (kKeyBufs * kParts + kBufs) * kTile;
+  static constexpr int kHeld = kKeyBufs * kParts / kTurns;  // key tiles in shared memory
+  static constexpr int kSmem = MT * kQ + (kHeld + kBufs) * kTile;
   // 4 unpacking, then 1 issuing; with two row tiles three more, which only hand their registers on
   static constexpr int kSoftmaxWarps = MT * 4, kWarps = MT == 2 ? 16 : MT * 4 + 5;
   // registers of a thread at launch and after the split: 2 x 128 x 152 + 128 x 128 + 128 x 80 = 512 x 128
@@ -176,11 +184,11 @@ __device__ __forceinline__ void ldg_bytes(const uint8_t* at, uint32_t (&w)[(N + 
 // 236 / 233 / 229 / 234 / 233 / 240, with a cap too 259 / 264 / 265 / 272 / 273 / 282.
 static inline int tc_tile_cost(const AttnParams& p) { return p.softcap > 0.f || p.slopes ? 3 : 5; }
 
-template <int FMT, int NB, bool EXACT>
+template <int FMT, int NB, bool EXACT, bool WIDE>
 __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attention_tc_kernel(const AttnParams p) {
   using C = TcTile<FMT, NB, EXACT>;
-  constexpr int D = C::D, MT = C::MT, KB = C::kKeyBufs, VB = C::kBufs, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
-  extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB][parts], values [VB]
+  constexpr int D = C::D, MT = C::MT, KB = C::kKeyBufs, VB = C::kBufs, TURNS = C::kTurns, R = C::kRows, STG = C::kKeys, SW = C::kSoftmaxWarps;
+  extern __shared__ __align__(128) uint8_t smem[];  // queries [MT], keys [KB][parts side by side], values [VB]
   __shared__ uint64_t b_kfull[KB], b_kempty[KB], b_vfull[VB], b_vempty[VB], b_s[MT], b_p[MT], b_o[MT], b_q, b_end;
   // A block's odd keys, a bit each: those without a page, and those whose keys or whose values (s_less, written where a word
   // of s_odd is not 0) are 2^kLess less in their operands. The unpacking warps write a block's words before they hand its
@@ -222,7 +230,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   tc::fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  const uint32_t q_smem = smem_addr(smem), k_smem = q_smem + MT * C::kQ, v_smem = k_smem + KB * C::kParts * C::kTile;
+  const uint32_t q_smem = smem_addr(smem), k_smem = q_smem + MT * C::kQ, v_smem = k_smem + C::kHeld * C::kTile;
   // a wait that ran out ends the role's work, and the kernel at the end of the tile: every later wait is skipped
   bool ok = true;
   auto wait_one = [&](uint64_t* bar, uint32_t phase) {  // by one thread
@@ -342,6 +350,21 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       tc::fence_async_smem();
       tc::arrive(smem_addr(&b_q));
       if (tile < tiles) {
+        // the weights of 32 keys: 16 registers of pairs, and (WIDE) 16 more of what their rounding left
+        constexpr int kWords = WIDE ? 32 : 16;
+        auto put = [](uint32_t (&w)[kWords], int i, float y0, float y1) {
+          w[i] = pack_half2(y0, y1);
+          if constexpr (WIDE) {
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            w[16 + i] = pack_half2(y0 - back.x, y1 - back.y);
+          }
+        };
+        auto store = [&](int c, const uint32_t (&w)[kWords]) {
+          if constexpr (WIDE)
+            tc::tmem_st32(col_s + c, w);
+          else
+            tc::tmem_st16(col_s + c / 2, w);
+        };
         float ref = kNoRef, sum = 0.f;
         for (int j = 0; j < n; ++j) {
           if (!wait(&b_s[tile], done_blocks[tile] + j)) break;
@@ -398,17 +421,17 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
 #pragma unroll 1
             for (int c = 0; c < STG; c += 32) {
               const uint32_t large_v = s_odd[turn][c >> 5] ? s_less[turn][1][c >> 5] : 0;
-              uint32_t x[32], w[16];
+              uint32_t x[32], w[kWords];
               tc::tmem_ld32_nowait(col_s + c, x);
               tc::tmem_wait_ld32(x);
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
                 const float y0 = exp2_approx(__uint_as_float(x[e]) - ref), y1 = exp2_approx(__uint_as_float(x[e + 1]) - ref);
                 sum += y0 + y1;
-                w[e / 2] = pack_half2(large_v >> e & 1 ? y0 * (float)(1 << C::kLess) : y0,
-                                      large_v >> (e + 1) & 1 ? y1 * (float)(1 << C::kLess) : y1);
+                put(w, e / 2, large_v >> e & 1 ? y0 * (float)(1 << C::kLess) : y0,
+                    large_v >> (e + 1) & 1 ? y1 * (float)(1 << C::kLess) : y1);
               }
-              tc::tmem_st16(col_s + c / 2, w);
+              store(c, w);
             }
             tc::tmem_wait_st();
             tc::fence_before();
@@ -475,7 +498,7 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
           const float2 scale2 = make_float2(scale, scale), ref2 = make_float2(-ref, -ref);
 #pragma unroll 1
           for (int c = 0; c < STG; c += 32) {
-            uint32_t x[32], w[16];
+            uint32_t x[32], w[kWords];
             tc::tmem_ld32_nowait(col_s + c, x);
             tc::tmem_wait_ld32(x);
 #pragma unroll
@@ -484,9 +507,9 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
               y = __ffma2_rn(y, scale2, ref2);
               y.x = exp2_approx(y.x), y.y = exp2_approx(y.y);
               s01 = __fadd2_rn(s01, y);
-              w[e / 2] = pack_half2(y.x, y.y);
+              put(w, e / 2, y.x, y.y);
             }
-            tc::tmem_st16(col_s + c / 2, w);  // columns of S that have been read
+            store(c, w);  // to columns of S that have been read
           }
           sum += s01.x + s01.y;
           tc::tmem_wait_st();
@@ -581,64 +604,74 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       if (FMT == 0) load_v(0);  // q8_0: no registers to have them a block ahead
       for (int j = 0; j < n && ok; ++j) {
         const uint32_t at = blocks + j;
-        const int kbuf = at % KB, vbuf = at % VB;
+        const int vbuf = at % VB;
         if (FMT == 2) load_v(j);
-        if (at >= KB && !wait(&b_kempty[kbuf], at / KB - 1)) break;
         const uint32_t largest_k = largest_half<NB>(ksc), largest_v = largest_half<NB>(kvs);
         const bool large = max(largest_k, largest_v) > C::kMost;  // or not finite
         const uint32_t odd = __ballot_sync(0xffffffffu, large || (!read_k && (begin + j) * STG + th < q.len));
-        if (lane == 0) s_odd[at & 3][warp - SW] = odd;
-        uint8_t* kt = smem + MT * C::kQ + kbuf * C::kParts * C::kTile + th * 16;
-        // word w = (t, block) of the key, its packed quants and its scale -> the operand's 16 bytes
-        auto unpack_key = [&](int w, uint32_t q0, uint32_t q1, uint32_t d, uint32_t less) {
-          uint32_t i[4], x[4];  // the quants as f16, and times their scale
-          if constexpr (FMT == 0) {
-            i[0] = low_nibbles<true>(q0), i[1] = high_nibbles_int(q0);
-            i[2] = low_nibbles<true>(q0 >> 8), i[3] = high_nibbles_int(q0 >> 8);
-          } else {
-            i[0] = two_bytes<true>(q0, 0), i[1] = two_bytes<true>(q0, 1);
-            i[2] = two_bytes<true>(q1, 0), i[3] = two_bytes<true>(q1, 1);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (less != kOne) i[e] = mul_half2(i[e], less);
-            x[e] = mul_half2(i[e], d);
-          }
-          *reinterpret_cast<uint4*>(kt + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
-          if constexpr (EXACT) {  // what the rounding left: one exact fused multiply-add
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = fma_half2(i[e], d, x[e] ^ 0x80008000u);
-            *reinterpret_cast<uint4*>(kt + C::kTile + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-        };
-#pragma unroll
-        for (int w = 0; w < NB * 4; ++w) {
-          const int k = w % NB;
-          unpack_key(w, kw[FMT == 0 ? w : 2 * w], FMT == 0 ? 0 : kw[2 * w + 1],
-                     __byte_perm(ksc[k / 2], 0, (k & 1) ? 0x3232 : 0x1010), kOne);
-        }
-        if (__builtin_expect(odd != 0, 0)) {
-          const uint32_t k = __ballot_sync(0xffffffffu, largest_k > C::kMost), v = __ballot_sync(0xffffffffu, largest_v > C::kMost);
-          if (lane == 0) s_less[at & 3][0][warp - SW] = k, s_less[at & 3][1][warp - SW] = v;
-          if (large) {  // once more: 2^kLess less, or NaN where a scale is not finite, and so the rows that see this key
-            const int64_t row = row_of((begin + j) * STG + th);
-            const bool finite = max(largest_k, largest_v) < 0x7c00u;
-            const uint32_t less = largest_k > C::kMost ? kLessHalf * 0x10001u : kOne;
+        bool gone = false;
 #pragma unroll 1
-            for (int w = 0; w < NB * 4; ++w) {
-              const uint8_t* at = p.kq + row * C::kRow + w * (C::kRow / (NB * 4));
-              const uint32_t q0 = __ldg(reinterpret_cast<const uint32_t*>(at));
-              const uint32_t q1 = FMT == 0 ? 0 : __ldg(reinterpret_cast<const uint32_t*>(at) + 1);
-              unpack_key(w, q0, q1, finite ? p.ks[row * NB + w % NB] * 0x10001u : 0x7fff7fffu, less);
+        for (int turn = 0; turn < TURNS; ++turn) {
+          const uint32_t use = at * TURNS + turn;  // of the key tiles
+          const int kbuf = use % KB;
+          if (use >= KB && !wait(&b_kempty[kbuf], use / KB - 1)) {
+            gone = true;
+            break;
+          }
+          if (lane == 0) s_odd[at & 3][warp - SW] = odd;
+          uint8_t* kt = smem + MT * C::kQ + kbuf * (C::kParts / TURNS) * C::kTile + th * 16;
+          // word w = (t, block) of the key, its packed quants and its scale -> the operand's 16 bytes
+          auto unpack_key = [&](int w, uint32_t q0, uint32_t q1, uint32_t d, uint32_t less) {
+            uint32_t i[4], x[4];  // the quants as f16, and times their scale
+            if constexpr (FMT == 0) {
+              i[0] = low_nibbles<true>(q0), i[1] = high_nibbles_int(q0);
+              i[2] = low_nibbles<true>(q0 >> 8), i[3] = high_nibbles_int(q0 >> 8);
+            } else {
+              i[0] = two_bytes<true>(q0, 0), i[1] = two_bytes<true>(q0, 1);
+              i[2] = two_bytes<true>(q1, 0), i[3] = two_bytes<true>(q1, 1);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (less != kOne) i[e] = mul_half2(i[e], less);
+              x[e] = mul_half2(i[e], d);
+            }
+            if (TURNS == 1 || turn == 0) *reinterpret_cast<uint4*>(kt + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
+            if (EXACT && (TURNS == 1 || turn == 1)) {  // what the rounding left: one exact fused multiply-add
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = fma_half2(i[e], d, x[e] ^ 0x80008000u);
+              *reinterpret_cast<uint4*>(kt + (TURNS == 1 ? C::kTile : 0) + w * 2048) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+          };
+#pragma unroll
+          for (int w = 0; w < NB * 4; ++w) {
+            const int k = w % NB;
+            unpack_key(w, kw[FMT == 0 ? w : 2 * w], FMT == 0 ? 0 : kw[2 * w + 1],
+                       __byte_perm(ksc[k / 2], 0, (k & 1) ? 0x3232 : 0x1010), kOne);
+          }
+          if (__builtin_expect(odd != 0, 0)) {
+            const uint32_t k = __ballot_sync(0xffffffffu, largest_k > C::kMost), v = __ballot_sync(0xffffffffu, largest_v > C::kMost);
+            if (lane == 0) s_less[at & 3][0][warp - SW] = k, s_less[at & 3][1][warp - SW] = v;
+            if (large) {  // once more: 2^kLess less, or NaN where a scale is not finite, and so the rows that see this key
+              const int64_t row = row_of((begin + j) * STG + th);
+              const bool finite = max(largest_k, largest_v) < 0x7c00u;
+              const uint32_t less = largest_k > C::kMost ? kLessHalf * 0x10001u : kOne;
+#pragma unroll 1
+              for (int w = 0; w < NB * 4; ++w) {
+                const uint8_t* at = p.kq + row * C::kRow + w * (C::kRow / (NB * 4));
+                const uint32_t q0 = __ldg(reinterpret_cast<const uint32_t*>(at));
+                const uint32_t q1 = FMT == 0 ? 0 : __ldg(reinterpret_cast<const uint32_t*>(at) + 1);
+                unpack_key(w, q0, q1, finite ? p.ks[row * NB + w % NB] * 0x10001u : 0x7fff7fffu, less);
+              }
             }
           }
+          if (turn + 1 == TURNS) load_k(j + 1);
+          tc::fence_async_smem();
+          tc::arrive(smem_addr(&b_kfull[kbuf]));
         }
-        load_k(j + 1);
-        tc::fence_async_smem();
-        tc::arrive(smem_addr(&b_kfull[kbuf]));
+        if (gone) break;
 
         if (at >= VB && !wait(&b_vempty[vbuf], at / VB - 1)) break;
-        uint8_t* vt = smem + MT * C::kQ + (KB * C::kParts + vbuf) * C::kTile + kg * (D * 16) + g * 16;
+        uint8_t* vt = smem + MT * C::kQ + (C::kHeld + vbuf) * C::kTile + kg * (D * 16) + g * 16;
         // column 4k + c of the unit: 8 keys' values, from two keys' packed quants and scales at a time
         auto unpack_values = [&](uint32_t w0, uint32_t w1, int odd_block, uint32_t d, uint32_t less, uint32_t (&x)[4]) {
           if constexpr (FMT == 0) {
@@ -716,20 +749,26 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
       const uint64_t dv = tc::smem_desc_kmajor(v_smem, D * 16);
       auto scores = [&](int tile, uint32_t at) {
         const uint64_t a = dq + (uint64_t)((tile * C::kQ) >> 4);
-        const uint64_t z = dk + (uint64_t)(((at % KB) * C::kParts * C::kTile) >> 4);
+        const uint64_t z = dk + (uint64_t)((at * TURNS % KB * (C::kParts / TURNS) * C::kTile) >> 4);
 #pragma unroll
-        for (int part = 0; part < C::kParts; ++part)
+        for (int part = 0; part < C::kParts; ++part) {
+          if (TURNS == 2 && part == 1) {  // its turn comes when the first part has been read
+            tc::mma_commit(smem_addr(&b_kempty[0]));
+            if (!wait_one(&b_kfull[0], at * TURNS + 1)) return;
+            tc::fence_after();
+          }
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
-            tc::mma_f16_ss(tmem + C::kS + tile * 128, a + s * (4096 >> 4), z + ((part * C::kTile + s * 4096) >> 4), is,
-                           part > 0 || s > 0);
+            tc::mma_f16_ss(tmem + C::kS + tile * 128, a + s * (4096 >> 4),
+                           z + (((TURNS == 1 ? part * C::kTile : 0) + s * 4096) >> 4), is, part > 0 || s > 0);
+        }
         tc::mma_commit(smem_addr(&b_s[tile]));
         tc::arrive(smem_addr(&b_s[tile]));
       };
-      if (wait_one(&b_q, segments) && wait_one(&b_kfull[blocks % KB], blocks / KB)) {
+      if (wait_one(&b_q, segments) && wait_one(&b_kfull[blocks * TURNS % KB], blocks * TURNS / KB)) {
         tc::fence_after();
         for (int i = 0; i < tiles; ++i) scores(i, blocks);
-        tc::mma_commit(smem_addr(&b_kempty[blocks % KB]));
+        tc::mma_commit(smem_addr(&b_kempty[blocks * TURNS % KB]));
         for (int j = 0; j < n && ok; ++j) {
           const uint32_t at = blocks + j;
           for (int i = 0; i < tiles; ++i) {
@@ -739,19 +778,26 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
             const uint64_t z = dv + (uint64_t)(((at % VB) * C::kTile) >> 4);
 #pragma unroll
             for (int s = 0; s < STG / 16; ++s)
-              tc::mma_f16_ts(tmem + i * 128, tmem + C::kS + i * 128 + s * 8, z + (uint64_t)s * ((2 * D * 16) >> 4), io,
-                             j > 0 || s > 0);
+              if constexpr (WIDE) {
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+                  tc::mma_f16_ts(tmem + i * 128, tmem + C::kS + i * 128 + s / 2 * 32 + part * 16 + s % 2 * 8,
+                                 z + (uint64_t)s * ((2 * D * 16) >> 4), io, j > 0 || s > 0 || part > 0);
+              } else {
+                tc::mma_f16_ts(tmem + i * 128, tmem + C::kS + i * 128 + s * 8, z + (uint64_t)s * ((2 * D * 16) >> 4), io,
+                               j > 0 || s > 0);
+              }
             if (j + 1 == n) {
               tc::mma_commit(smem_addr(&b_o[i]));
             } else {
-              if (i == 0 && !wait_one(&b_kfull[(at + 1) % KB], (at + 1) / KB)) break;
+              if (i == 0 && !wait_one(&b_kfull[(at + 1) * TURNS % KB], (at + 1) * TURNS / KB)) break;
               tc::fence_after();
               scores(i, at + 1);
             }
           }
           if (!ok) break;
           tc::mma_commit(smem_addr(&b_vempty[at % VB]));
-          if (j + 1 < n) tc::mma_commit(smem_addr(&b_kempty[(at + 1) % KB]));
+          if (j + 1 < n) tc::mma_commit(smem_addr(&b_kempty[(at + 1) * TURNS % KB]));
         }
       }
     }
@@ -800,11 +846,11 @@ __global__ void __launch_bounds__(TcTile<FMT, NB, EXACT>::kWarps * 32, 1) attent
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-template <int FMT, int NB, bool EXACT>
+template <int FMT, int NB, bool EXACT, bool WIDE>
 static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t stream) {
   using C = TcTile<FMT, NB, EXACT>;
   static_assert(C::kSmem + 2048 <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = attention_tc_kernel<FMT, NB, EXACT>;
+  auto kernel = attention_tc_kernel<FMT, NB, EXACT, WIDE>;
   static std::atomic<unsigned long long> allowed{0};
   int rc = allow_smem_once(reinterpret_cast<const void*>(kernel), C::kSmem, allowed);
   if (rc) return rc;
@@ -830,17 +876,21 @@ static int launch_attention_tc_as(const AttnParams& p, int sms, cudaStream_t str
 template <int FMT>
 static int launch_attention_tc_fmt(AttnParams p, int dim, int sms, cudaStream_t stream) {
   p.tile_cost = tc_tile_cost(p);
+  const bool wide = p.dtype == B2Q_DTYPE_F16, exact = wide || p.lse;
+  auto by_parts = [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    if constexpr (NB == 8)
+      return wide ? launch_attention_tc_as<FMT, NB, true, true>(p, sms, stream) : launch_attention_tc_as<FMT, NB, false, false>(p, sms, stream);
+    else
+      return wide    ? launch_attention_tc_as<FMT, NB, true, true>(p, sms, stream)
+             : exact ? launch_attention_tc_as<FMT, NB, true, false>(p, sms, stream)
+                     : launch_attention_tc_as<FMT, NB, false, false>(p, sms, stream);
+  };
   switch (dim) {
-    case 64:
-      return p.lse ? launch_attention_tc_as<FMT, 2, true>(p, sms, stream)
-                   : launch_attention_tc_as<FMT, 2, false>(p, sms, stream);
-    case 96:
-      return p.lse ? launch_attention_tc_as<FMT, 3, true>(p, sms, stream)
-                   : launch_attention_tc_as<FMT, 3, false>(p, sms, stream);
-    case 128:
-      return p.lse ? launch_attention_tc_as<FMT, 4, true>(p, sms, stream)
-                   : launch_attention_tc_as<FMT, 4, false>(p, sms, stream);
-    default: return launch_attention_tc_as<FMT, 8, false>(p, sms, stream);
+    case 64: return by_parts(std::integral_constant<int, 2>{});
+    case 96: return by_parts(std::integral_constant<int, 3>{});
+    case 128: return by_parts(std::integral_constant<int, 4>{});
+    default: return by_parts(std::integral_constant<int, 8>{});
   }
 }
 

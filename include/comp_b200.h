@@ -335,9 +335,10 @@ int b2q_kv_read(const b2q_kv_cache* cache, int dtype, void* k, void* v, const in
  * scale in (0, 1e30], softcap 0 or in [1e-20, 1e20]. Cache values of any finite scale are attended to; a scale that is not
  * finite makes the rows that see its token NaN, or, as a key's, leaves them undefined, and no other row.
  * Scores, softmax sums and outputs are held in f32. f32 queries and weights enter the products in two parts of f16 (22
- * bits), the cache's whole quants as they are. 16-bit calls round a weight to f16 (11 bits), and from 48 rows (queries times
- * q_heads / heads) a sequence on keys and values too, but keys only where lse is NULL: max_q and lse so choose among
- * results that differ by such roundings.
+ * bits), the cache's whole quants as they are. 16-bit calls with few rows (queries times q_heads / heads) a sequence round
+ * a weight times a value's scale to f16 (11 bits); from 48 rows on bf16 calls round weights, values and, where lse is NULL,
+ * keys to f16, and from 64 on f16 calls round values: max_q, and lse for bf16, so choose among results that differ by
+ * roundings that are not larger than the output's own.
  * max_q: at least the most queries of a sequence (0: max_q = T; rows that a smaller one leaves out stay unwritten, and the
  * device error word is set to 4). Kernel, tile height and plan go by it: pass it where it is known. max_len: at least the
  * longest lens, used to plan the split of the keys only.

@@ -9,7 +9,7 @@ import torch
 from comp_b200 import kv
 from oracle import kv as ref
 
-from .test_gpu_kv import DT, _bounds, _cache, _device_error, _gather, _problem
+from .test_gpu_kv import DT, U, _bounds, _cache, _device_error, _gather, _problem
 
 pytestmark = pytest.mark.gpu
 
@@ -19,7 +19,7 @@ def _to(dev, *arrays):
 
 
 def _tensor_cores(dtype, rows, dim, with_lse):
-    return dtype != "f32" and rows >= 48 and not (dim == 256 and with_lse)
+    return dtype != "f32" and rows >= (64 if dtype == "f16" else 48) and not (dim == 256 and with_lse)
 
 
 # ------------------------------------------------------------------------------------------------------- unread tokens
@@ -280,6 +280,63 @@ def test_a_long_tail_of_small_weights(cuda, fmt, dtype, queries, nats):
     assert (d <= bound).all(), float((d / bound).max())
 
 
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dim,heads,group", [(64, 2, 4), (96, 2, 3), (128, 2, 4), (256, 2, 2)])
+@pytest.mark.parametrize("queries", [[1] * 24, [4] * 12, [200, 90]])
+@pytest.mark.parametrize("with_lse", [True, False])
+def test_f16_results_are_as_good_as_their_rounding(cuda, fmt, dim, heads, group, queries, with_lse):
+    """Of what an f16 call rounds, the output and the values (tensor cores) or the weights (streaming) have 11 bits, all else
+    20 or more: two roundings of a size, independent, so sqrt(2) of the output's own in the 2-norm."""
+    lens = [300 + 37 * i for i in range(len(queries))]
+    planes, table, lens, cu, q = _problem(406, fmt, "f16", lens, queries, heads * group, heads, dim, 32)
+    keys, values = _gather(fmt, planes, table, lens)
+    o, _, _, _ = ref.attention(q.float().numpy(), keys, values, lens, cu, dim**-0.5)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    got = kv.attention(q.to(cuda), _cache(fmt, planes, cuda), tt, tl, cu_q=tc, max_q=max(queries), return_lse=with_lse)
+    g = (got[0] if with_lse else got).double().cpu().numpy()
+    own = np.linalg.norm(o.astype(np.float16).astype(np.float64) - o)
+    assert np.linalg.norm(g - o) <= 1.5 * own, np.linalg.norm(g - o) / own
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("with_lse", [True, False])
+def test_f16_weights_of_values_that_cancel(cuda, fmt, dim, with_lse):
+    """Rows that see two keys of opposite values, whole numbers: the difference of nearly equal weights, which carry 20 bits."""
+    planes, table, lens, cu, q = _problem(407, fmt, "f16", [300], [200], 4, 2, dim, 32)
+    rows, scales = planes[2:]
+    one = np.random.default_rng(408).integers(-7, 8, dim)
+    place, shift = ref._places(fmt, dim, "v")
+    for sign in (1, -1):
+        r = np.zeros(rows.shape[-1], np.uint8)
+        for e in range(dim):
+            r[place[e]] |= np.uint8(sign * one[e] + (8 if fmt == "q4_0" else 128)) << np.uint8(shift[e])
+        rows[:, :, (0 if sign > 0 else 1) :: 2] = r
+    scales[...] = np.float16(1.0).view(np.uint16)
+    keys, values = _gather(fmt, planes, table, lens)
+    scale = 0.02 * dim**-0.5
+    o, _, reach, mass = ref.attention(q.float().numpy(), keys, values, lens, cu, scale, window=2)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    got = kv.attention(q.to(cuda), _cache(fmt, planes, cuda), tt, tl, cu_q=tc, max_q=200, scale=scale, window=2,
+                       return_lse=with_lse)
+    g = (got[0] if with_lse else got).double().cpu().numpy()
+    if dim == 256 and with_lse:  # the streaming kernel: weights of 11 bits
+        bound = U["f16"] * np.abs(o) + 2 * (2.0**-11 + 2.0**-15 * reach + 2.0**-20)[..., None] * mass
+    else:
+        bound = U["f16"] * np.abs(o) + 2 * (2.0**-20 + 2.0**-15 * reach + 2.0**-20)[..., None] * mass
+    assert (np.abs(g - o) <= bound).all(), float((np.abs(g - o)[mass > 0] / bound[mass > 0]).max())
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_f16_results_do_not_depend_on_lse(cuda, fmt, dim):
+    planes, table, lens, cu, q = _problem(409, fmt, "f16", [300, 150], [200, 60], 8, 2, dim, 32)
+    tt, tl, tc = _to(cuda, table, lens, cu)
+    cache, q = _cache(fmt, planes, cuda), q.to(cuda)
+    out, _ = kv.attention(q, cache, tt, tl, cu_q=tc, max_q=200, return_lse=True)
+    assert torch.equal(kv.attention(q, cache, tt, tl, cu_q=tc, max_q=200), out)
+
+
 @pytest.mark.parametrize("cap", [0.3, 1.0, 50.0])
 @pytest.mark.parametrize("dtype,n", [("f32", 1), ("bf16", 50)])
 def test_the_cap_against_tanh(cuda, cap, dtype, n):
@@ -309,7 +366,7 @@ def test_the_cap_against_tanh(cuda, cap, dtype, n):
 # ------------------------------------------------------------------------------------ the kernels' boundary, streams
 
 
-@pytest.mark.parametrize("rows", [47, 48, 49, 63, 64])
+@pytest.mark.parametrize("rows", [47, 48, 49, 63, 64, 65])
 @pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
 @pytest.mark.parametrize("dim", [64, 96, 128, 256])
 @pytest.mark.parametrize("with_lse", [True, False])
