@@ -19,14 +19,15 @@
 // A weight matrix leaves the first product with keys along the lanes' rows and enters the second with keys along their
 // pairs: one 8x8 transpose in registers each.
 //
-// What bounds it: the cache's bytes, and close behind the unpacking. The CTAs fill the GPU once and take equal shares of all
-// stages (16 to 64 keys) of all sequences, heads and row tiles, whatever their lengths; a tile's stages go round the four
+// What bounds it: latency, with the cache's bytes and the unpacking close behind each other: no unit is above 60% (issue
+// 59%, ALU 48%, DRAM 50%) at the 12 warps an SM that 168 registers leave. The CTAs fill the GPU once and take equal shares of
+// all stages (16 to 64 keys) of all sequences, heads and row tiles, whatever their lengths; a tile's stages go round the four
 // warps, each with a ring of its own, and the warps join at the tile's end. Tiles that cross shares are joined by a second
-// kernel. Measured: 8 sequences of 90001 to 131072 keys, 64 query heads on 8 of 128, f16: 204 us (5.0 TB/s; 228 us with
-// three such caches in turn); 64 sequences of 100 to 8192 keys: 80 us (3.8 TB/s), of which about 15 us are beginnings and
-// ends. Without its arithmetic the first takes 158 us, without its copies 193 us. What did not help: 16 warps of 128
-// registers (a stage of 32 keys then: 262 us), every warp on its own (225 us; its instructions come from farther away),
-// bulk copies instead of cp.async (the same), the next keys' scores beside these keys' products (229 us).
+// kernel. Measured: 8 sequences of 90001 to 131072 keys, 64 query heads on 8 of 128, f16: 231 us in a long run with three such
+// caches in turn (4.4 TB/s), 200 at best; 64 sequences of 100 to 8192 keys: 80 us (3.8 TB/s), of which about 15 us are
+// beginnings and ends. Without its arithmetic the first takes 158 us, without its copies 193 us. What did not help: 16 warps
+// of 128 registers (a stage of 32 keys then: 262 us), every warp on its own (225 us; its instructions come from farther
+// away), bulk copies instead of cp.async (the same), the next keys' scores beside these keys' products (229 us).
 #pragma once
 
 #include <cfloat>

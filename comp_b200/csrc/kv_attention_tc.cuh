@@ -19,9 +19,9 @@
 // What bounds it: 128 keys for 256 rows of 128 values take 2048 cycles on the tensor cores, 2048 on the units that compute
 // 2^x (16 a cycle), and about 2048 of shared memory's (operands of S from there twice, unpacked tiles into it); a tile's
 // chain - S, softmax, P V - is longer than the other tile's products that run beside it. Measured: a chunk of 2048 queries
-// at the end of 32768 keys, 32 heads on 8 of 128: 1.09 ms, 975 TFLOP/s (1.2 ms in a long run); the softmax of a tile takes
-// 1.5 us a block and waits 0.8 us. What did not help: a part of the 2^x as polynomials (1.12 to 1.28 ms for an eighth to a
-// half), loads of S ahead of their use (1.10 ms), one pass with the weights kept in registers (1.8 ms: they spill).
+// at the end of 32768 keys, 32 heads on 8 of 128, bf16: 1.22 ms in a long run, 874 TFLOP/s (1.11 ms at best); the softmax of
+// a tile takes 1.5 us a block and waits 0.8 us. What did not help: a part of the 2^x as polynomials (3 to 17% slower for an
+// eighth to a half), loads of S ahead of their use (1%), one pass with the weights kept in registers (65%: they spill).
 #pragma once
 
 #include "kv_attention.cuh"

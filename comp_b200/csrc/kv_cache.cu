@@ -5,8 +5,9 @@
 // 16+4l..16+4l+3 of a block (the two nibbles of the block's bytes 4l..4l+3), for q8_0 the values 8l..8l+7. In the cache's
 // order those are one run of the row, so that a thread's quants are one wide load or store, and four threads' values whole
 // 32-byte sectors. (A thread a block's quarter took 195 us for reading 131072 tokens of 8 heads of 128 as bf16: its index
-// arithmetic. So 117 us, 5.9 TB/s.) A write of 16384 tokens takes 24 us (3.6 TB/s): 16 instructions a value, of which the
-// rounding takes three, hold it there; written and read back 65 us at first, 39 us now.
+// arithmetic. So 117 us, 5.9 TB/s.) A write of 16384 tokens takes 24 us (3.6 TB/s): its bytes
+// are 13 us, and 16 instructions a value (the rounding takes three of them) 15 us of issue, which overlaps with them in part;
+// written and read back 65 us at first, 39 us now.
 #include <type_traits>
 
 #include "kv_device.cuh"
