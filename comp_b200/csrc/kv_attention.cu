@@ -9,13 +9,12 @@ struct AttnPlan {
   size_t part_m, joins, bytes;  // workspace: partial outputs, then references and sums, then the joins
 };
 
-// 16-bit calls with at least so many query rows a sequence and KV head take the tensor-core kernels (those with heads
-// of 256 and lse stay with the streaming one). Measured, us, streaming / tensor cores: 16 sequences of 4096 keys, 8 KV heads of 128, bf16: 32 rows
-// 69 / 91, 48 rows 94 / 92, 64 rows 118 / 93, 256 rows 415 / 123; f16: 48 rows 94 / 119, 64 rows 118 / 121, 80 rows 142 /
-// 123; one of 8192, bf16: 24 / 25 at 48, 64 / 37 at 256; 16 of 4096, heads of 256, bf16: 156 / 174 at 32, 226 / 162 at 48;
-// f16: 226 / 266 at 48, 300 / 270 at 64. (One of 500 keys, bf16: 16 / 16 at 48, 21 / 27 at 256: that little work is launches
-// and tile ends.) Else the rows of a tile are 8, or 16 where more have to read the cache anyway (heads of 256 leave
-// registers for 8).
+// 16-bit calls with at least so many query rows a sequence and KV head take the tensor-core kernels (those with heads of 256
+// and lse stay with the streaming one). Measured, us, streaming / tensor cores: 16 sequences of 4096 keys, 8 KV heads of 128,
+// bf16: 48 rows 95 / 91, 64 rows 120 / 93, 256 rows 417 / 126; f16: 48 rows 95 / 119, 64 rows 120 / 121, 80 rows 145 / 123;
+// one of 8192, bf16: 23 / 25 at 48, 63 / 39 at 256; 16 of 4096, heads of 256, bf16: 154 / 174 at 32, 223 / 163 at 48; f16: 222
+// / 266 at 48, 291 / 270 at 64. (One of 500 keys, bf16: 16 / 15 at 48, 21 / 27 at 256: that little work is launches and tile
+// ends.) Else the rows of a tile are 8, or 16 where more have to read the cache anyway (heads of 256 leave registers for 8).
 static int least_tc_rows(const b2q_attention_args& a) { return a.dtype == B2Q_DTYPE_F16 ? 64 : 48; }
 
 static AttnPlan plan_attention(const b2q_kv_cache& c, const b2q_attention_args& a) {
