@@ -1,6 +1,7 @@
 // Instantiations of the TMA-ring GEMV kernels (see gemv_kernels.cuh), and the device error word they write.
 #include "gemv_kernels.cuh"
 #include "kv_internal.h"
+#include "mx_internal.h"
 
 namespace b2q {
 
@@ -59,9 +60,10 @@ extern "C" int b2q_device_error(int* code, int clear) {
     e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     if (e != cudaSuccess) return fail(B2Q_ECUDA, "b2q_device_error: %s", cudaGetErrorString(e));
   }
-  // the words of the KV cache's and the attention's translation units; the first that is set is reported
+  // the words of the KV cache's, the attention's, the MXFP4 products' and the experts' translation units; the first that is
+  // set is reported
   for (auto read : {kv_cache_error, kv_attention_q4_error, kv_attention_q8_error, kv_attention_tc_q4_error,
-                    kv_attention_tc_q8_error}) {
+                    kv_attention_tc_q8_error, mx_gemm_error, experts_error}) {
     int word = 0;
     const int rc = read(&word, clear);
     if (rc) return rc;

@@ -1,0 +1,62 @@
+// Device helpers of the MXFP4 kernels: where a block lies in an operand image, and the 4-bit conversions.
+//
+// The image is laid out for the tensor cores, so that a kernel brings a stage of a tile (128 rows by 256 values) into shared
+// memory with one bulk copy and multiplies it as it lies there:
+//   codes   row r is 128 bytes: 8 blocks of 16, block b at place b ^ (r & 7) (the 128-byte swizzle, repeated every 8 rows);
+//           in a block byte i holds value i (low nibble) and value i + 16 (high). Both operands have this order, so that
+//           their products pair up as they should.
+//   scales  after the codes, two runs of 512 bytes (blocks 0..3 and 4..7): byte (r % 32) * 16 + (r / 32) * 4 + b % 4, the
+//           order in which tensor memory holds them: lane r % 32, column r / 32.
+// Codes and scales of values beyond K are zeros.
+#pragma once
+
+#include "kv_device.cuh"
+#include "mx_internal.h"
+
+namespace b2q {
+
+// Byte offsets of block b (0..7) of row r (0..127) in a stage: its 16 bytes of codes, its scale.
+__device__ __forceinline__ int mx_code_at(int r, int b) { return r * 128 + ((b ^ (r & 7)) << 4); }
+__device__ __forceinline__ int mx_scale_at(int r, int b) {
+  return kMxCodes + (b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3);
+}
+
+// 4 bytes of codes, byte i = lo[i] in the low nibble and hi[i] in the high one: round to nearest even, cut off at 6.
+__device__ __forceinline__ uint32_t to_e2m1x8(const float (&lo)[8], const float (&hi)[8], int i) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %5, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %6, %2;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %7, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %4;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(lo[i]), "f"(lo[i + 1]), "f"(lo[i + 2]), "f"(lo[i + 3]), "f"(hi[i]), "f"(hi[i + 1]), "f"(hi[i + 2]),
+        "f"(hi[i + 3]));
+  return w;
+}
+
+// The values of 4 bytes of codes: lo[i] from the low nibble of byte i, hi[i] from the high one.
+__device__ __forceinline__ void from_e2m1x8(uint32_t w, float (&lo)[8], float (&hi)[8], int i) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+    lo[i + j] = f.x, hi[i + j] = f.y;
+  }
+}
+
+// 2^(s - 127): s = 0 is below the normal numbers, 255 is NaN.
+__device__ __forceinline__ float mx_scale(uint32_t s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fffffffu : s << 23);
+}
+
+}  // namespace b2q

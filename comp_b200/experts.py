@@ -1,0 +1,170 @@
+"""Layers of experts on MXFP4 weights (an extension beyond the reference): routing, the experts' products, and back.
+
+    w_up, w_down = mx.pack(codes, scales), ...             # MXTensors [E][N][K]
+    plan = experts.route(logits, 8)                        # logits [T][E] -> 8 experts for each token, sorted by expert
+    h = act(experts.linear(x, w_up, plan))                 # x [T][K] -> sorted rows [T * 8][N]
+    y = experts.linear(h, w_down, plan, gather=False)      # sorted rows in, sorted rows out
+    out = experts.combine(y, plan, plan.weights)           # [T][K]: each token's rows, weighted and added
+
+Nothing synchronizes: how many rows an expert has stays on the device, and all of it can be captured in a CUDA graph. The
+kernels are this package's own, through the C-ABI (include/comp_b200.h, where layouts and formulas stand).
+"""
+
+import torch
+
+from .kv import _call, _dtype_id, _on_device, _raw_stream
+from .mx import MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _out_dtype, _rows, _stride
+
+MAX_TOP = 32
+
+
+class Plan:
+    """Choices (token * top + j) sorted by expert. int32 tensors: offsets [experts + 1] (the sorted rows where each expert's
+    begin), pos [tokens][top] (each choice's sorted row, -1: it goes nowhere), order [tokens * top] (each sorted row's choice, -1
+    past the last). From route also ids int32 and weights f32 [tokens][top]."""
+
+    def __init__(self, tokens, top, experts, dev):
+        choices = tokens * top
+        self.tokens, self.top, self.experts, self.device = tokens, top, experts, dev
+        self.ids = self.weights = None
+        self._words = torch.empty(2 * (experts + 1) + 4 * choices, dtype=torch.int32, device=dev)
+
+    @property
+    def offsets(self):
+        return self._words[: self.experts + 1]
+
+    @property
+    def pos(self):
+        at = 2 * (self.experts + 1)
+        return self._words[at : at + self.tokens * self.top].view(self.tokens, self.top)
+
+    @property
+    def order(self):
+        at, n = 2 * (self.experts + 1), self.tokens * self.top
+        return self._words[at + n : at + 2 * n]
+
+
+def _check_sizes(name, tokens, top, experts):
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"{name}: {experts} experts (1..{MAX_EXPERTS})")
+    if not 1 <= top <= MAX_TOP:
+        raise ValueError(f"{name}: {top} choices a token (1..{MAX_TOP})")
+    if tokens * top > 1 << 30:
+        raise ValueError(f"{name}: {tokens} tokens of {top} choices")
+
+
+def route(logits, top, normalize=True):
+    """logits [T][E] (f32, f16 or bf16) -> Plan of the `top` largest of each token: plan.ids (falling; the lowest index first
+    among equals) and plan.weights, their softmax over the chosen, or (normalize=False) over all E. -inf and NaN are never
+    chosen: a token with fewer others has ids -1, of weight 0, that go nowhere."""
+    dev = _cuda("route", logits)
+    did = _dtype_id("route: logits", logits)
+    if logits.dim() != 2:
+        raise ValueError(f"route: logits {tuple(logits.shape)}, expected [T][E]")
+    if not isinstance(top, int):
+        raise TypeError(f"route: top must be a whole number, got {type(top).__name__}")
+    tokens, experts = logits.shape
+    _check_sizes("route", tokens, top, experts)
+    if top > experts:
+        raise ValueError(f"route: {top} choices of {experts} experts")
+    s0, s1 = logits.stride()
+    if (s1 != 1 and experts > 1) or (tokens > 1 and s0 < experts):
+        logits = logits.clone(memory_format=torch.contiguous_format)
+    plan = Plan(tokens, top, experts, dev)
+    plan.ids = torch.empty((tokens, top), dtype=torch.int32, device=dev)
+    plan.weights = torch.empty((tokens, top), dtype=torch.float32, device=dev)
+    _call(dev, "b2q_experts_route", did, logits.data_ptr(), _stride(logits), tokens, experts, top, 1 if normalize else 0,
+          plan.ids.data_ptr(), plan.weights.data_ptr(), plan._words.data_ptr(), _raw_stream(dev.index))
+    return plan
+
+
+def sort(ids, experts):
+    """ids int32 [T][top], the experts of each token -> Plan. Negative ids go nowhere (experts held elsewhere, padding); so do
+    ids beyond the experts, which set the device error word to 5."""
+    dev = _cuda("sort", ids)
+    if ids.dtype != torch.int32:
+        raise TypeError(f"sort: ids dtype {ids.dtype}, expected torch.int32")
+    if ids.dim() != 2:
+        raise ValueError(f"sort: ids {tuple(ids.shape)}, expected [T][top]")
+    if not isinstance(experts, int):
+        raise TypeError(f"sort: experts must be a whole number, got {type(experts).__name__}")
+    tokens, top = ids.shape
+    _check_sizes("sort", tokens, top, experts)
+    ids = ids.contiguous()
+    plan = Plan(tokens, top, experts, dev)
+    plan.ids = ids
+    _call(dev, "b2q_experts_sort", ids.data_ptr(), tokens, top, experts, plan._words.data_ptr(), _raw_stream(dev.index))
+    return plan
+
+
+def _check_plan(name, plan):
+    if not isinstance(plan, Plan):
+        raise TypeError(f"{name}: plan must be a Plan (route, sort), got {type(plan).__name__}")
+
+
+def workspace_size(plan, k):
+    """Bytes of device workspace that linear needs for rows of k values."""
+    choices = plan.tokens * plan.top
+    return (choices // TILE_ROWS + min(plan.experts, choices)) * -(-k // STAGE) * STAGE_BYTES
+
+
+def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
+    """Each sorted row, quantized to MXFP4, times its expert's weights w (MXTensor [E][N][K]) -> [T * top][N] of `dtype`
+    (default: x's) in sorted order; rows past plan.offsets[E] stay unwritten. x: [T][K], a token's row for each of its choices,
+    or with gather=False the sorted rows [T * top][K]. workspace: a CUDA uint8 tensor of workspace_size(plan, K) bytes, 128-byte
+    aligned (allocated here when None)."""
+    if not isinstance(w, MXTensor):
+        raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
+    _check_plan("linear", plan)
+    if w.experts != plan.experts:
+        raise ValueError(f"linear: w {w.shape}, expected [{plan.experts}][N][K]")
+    dev, n, k = w.device, w.rows, w.k
+    if plan.device != dev:
+        raise RuntimeError(f"comp_b200.linear: tensors on different devices ({dev} and {plan.device})")
+    _on_device("linear", dev, x)
+    xid = _dtype_id("linear: x", x)
+    choices = plan.tokens * plan.top
+    if x.dim() != 2 or x.shape != (plan.tokens if gather else choices, k):
+        raise ValueError(f"linear: x {tuple(x.shape)}, expected [{plan.tokens if gather else choices}][{k}]")
+    dtype = x.dtype if dtype is None else dtype
+    did = _out_dtype("linear", dtype)
+    x = _rows(x)
+    y = _check_out("linear", out, dtype, (choices, n), dev)
+    need = workspace_size(plan, k)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        _on_device("linear", dev, workspace)
+        if not workspace.is_contiguous():
+            raise ValueError("linear: workspace must be contiguous")
+    _call(dev, "b2q_experts_linear", xid, x.data_ptr(), _stride(x), 1 if gather else 0, w.image.data_ptr(),
+          plan._words.data_ptr(), plan.tokens, plan.top, plan.experts, n, k, did, y.data_ptr(), _stride(y),
+          workspace.data_ptr(), workspace.numel() * workspace.element_size(), _raw_stream(dev.index))
+    return y
+
+
+def combine(y, plan, weights=None, out=None):
+    """Sorted rows y [T * top][N] back to their tokens -> [T][N] of y's type: the sum of weights[t][j] (f32 [T][top]; None: 1) times
+    y[pos[t][j]], in f32 and in order of j. A choice that goes nowhere adds nothing."""
+    _check_plan("combine", plan)
+    dev = plan.device
+    _on_device("combine", dev, y)
+    did = _dtype_id("combine: y", y)
+    choices = plan.tokens * plan.top
+    if y.dim() != 2 or y.shape[0] != choices:
+        raise ValueError(f"combine: y {tuple(y.shape)}, expected [{choices}][N]")
+    n = y.shape[1]
+    if weights is not None:
+        _on_device("combine", dev, weights)
+        if weights.dtype != torch.float32:
+            raise TypeError(f"combine: weights dtype {weights.dtype}, expected torch.float32")
+        if weights.shape != (plan.tokens, plan.top):
+            raise ValueError(f"combine: weights {tuple(weights.shape)}, expected ({plan.tokens}, {plan.top})")
+        weights = weights.contiguous()
+    if (n > 1 and y.stride(1) != 1) or (choices > 1 and y.stride(0) < n):
+        y = y.clone(memory_format=torch.contiguous_format)
+    o = _check_out("combine", out, y.dtype, (plan.tokens, n), dev)
+    _call(dev, "b2q_experts_combine", did, y.data_ptr(), _stride(y), plan._words.data_ptr(),
+          0 if weights is None else weights.data_ptr(), plan.tokens, plan.top, plan.experts, n, o.data_ptr(), _stride(o),
+          _raw_stream(dev.index))
+    return o

@@ -1,0 +1,206 @@
+"""MXFP4 operands and their products (an extension beyond the reference, whose formats are integer quants).
+
+MXFP4 holds 4-bit floating-point values (a sign over 0, 0.5, 1, 1.5, 2, 3, 4, 6) in blocks of 32 along K that share a power of
+two: 4.25 bits a value, for weights and activations alike, multiplied as they are by the tensor cores. An `MXTensor` is an
+operand in the order that they read; `quantize` makes one from values, `pack` from planes of codes and scales, `from_ggml` from
+ggml's block_mxfp4, and `dequantize` gives back the values that one stands for. `linear` is a layer's call: rows of f32, f16 or
+bf16, quantized and multiplied. The kernels are this package's own, through the C-ABI (include/comp_b200.h, where the formulas
+stand); like comp_b200.host the functions take CUDA tensors only, run on the current stream of their device, and raise
+TypeError / ValueError / RuntimeError on what they do not take.
+
+    w = mx.from_ggml(blocks, n, k)             # or mx.quantize(weights)
+    y = mx.linear(x, w)                        # x [M][k] -> y [M][n] of x's type
+"""
+
+import torch
+
+from .kv import DTYPE_ID, _call, _dtype_id, _on_device, _raw_stream
+
+TILE_ROWS, STAGE, STAGE_BYTES = 128, 256, 17408  # an image: 128 rows by 256 values a run of bytes
+MAX_EXPERTS = 1024
+
+
+def image_bytes(rows, k, experts=1):
+    """Bytes of the image of `experts` operands of [rows][k]."""
+    return experts * -(-rows // TILE_ROWS) * -(-k // STAGE) * STAGE_BYTES
+
+
+def _check_k(name, k):
+    if k < 32 or k % 32:
+        raise ValueError(f"{name}: K={k} is not a positive multiple of the MXFP4 block (32)")
+
+
+class MXTensor:
+    """An MXFP4 operand [rows][k], or [experts][rows][k], as its image: uint8, 128-byte aligned (include/comp_b200.h)."""
+
+    def __init__(self, image, rows, k, experts=None):
+        _check_k("MXTensor", k)
+        if rows < 0:
+            raise ValueError(f"MXTensor: {rows} rows")
+        if experts is not None and not 1 <= experts <= MAX_EXPERTS:
+            raise ValueError(f"MXTensor: {experts} experts (1..{MAX_EXPERTS})")
+        if not isinstance(image, torch.Tensor) or image.device.type != "cuda":
+            raise RuntimeError("comp_b200.MXTensor: the image must be a CUDA tensor (this backend has no CPU path)")
+        if image.dtype != torch.uint8:
+            raise TypeError(f"MXTensor: image dtype {image.dtype}, expected torch.uint8")
+        need = image_bytes(rows, k, experts or 1)
+        if image.dim() != 1 or image.numel() < need or not image.is_contiguous() or (need and image.data_ptr() % 128):
+            raise ValueError(f"MXTensor: the image must be {need} contiguous bytes, 128-byte aligned, got {tuple(image.shape)}")
+        self.image, self.rows, self.k, self.experts, self.device = image, rows, k, experts, image.device
+
+    @property
+    def shape(self):
+        return (self.rows, self.k) if self.experts is None else (self.experts, self.rows, self.k)
+
+    @property
+    def nbytes(self):
+        return image_bytes(self.rows, self.k, self.experts or 1)
+
+    def __repr__(self):
+        return f"MXTensor({list(self.shape)}, device={self.device})"
+
+
+def _cuda(name, t):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise RuntimeError(f"comp_b200.{name}: tensors must be CUDA tensors (this backend has no CPU path)")
+    return t.device
+
+
+def _rows(t):
+    """t with unit column stride and 16-byte aligned base and rows that do not overlap (a copy only when needed)."""
+    s0, s1 = t.stride()
+    if (s1 != 1 and t.shape[1] > 1) or t.data_ptr() % 16 or (t.shape[0] > 1 and (s0 * t.element_size() % 16 or s0 < t.shape[1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def quantize(x):
+    """x [M][K] (f32, f16 or bf16; any strides) -> MXTensor. Each block of 32 values along K takes the power of two that brings
+    its largest magnitude to 4 .. 8; values are rounded to nearest even and cut off at 6. Blocks with an infinity or a NaN
+    are NaN."""
+    dev = _cuda("quantize", x)
+    did = _dtype_id("quantize: x", x)
+    if x.dim() != 2:
+        raise ValueError(f"quantize: x {tuple(x.shape)}, expected [M][K]")
+    m, k = x.shape
+    _check_k("quantize", k)
+    x = _rows(x)
+    t = MXTensor(torch.empty(image_bytes(m, k), dtype=torch.uint8, device=dev), m, k)
+    _call(dev, "b2q_mx_quantize", did, x.data_ptr(), _stride(x), m, k, t.image.data_ptr(), _raw_stream(dev.index))
+    return t
+
+
+def dequantize(t, dtype=torch.float32):
+    """The values of an MXTensor, each rounded once to `dtype`: [rows][k], or [experts][rows][k]."""
+    if not isinstance(t, MXTensor):
+        raise TypeError(f"dequantize: expected an MXTensor, got {type(t).__name__}")
+    did = DTYPE_ID.get(dtype)
+    if did is None:
+        raise TypeError(f"dequantize: dtype {dtype}, expected float32, float16 or bfloat16")
+    dev = t.device
+    y = torch.empty(t.shape, dtype=dtype, device=dev)
+    for e in range(t.experts or 1):
+        out = y if t.experts is None else y[e]
+        at = t.image.data_ptr() + e * image_bytes(t.rows, t.k)
+        _call(dev, "b2q_mx_dequantize", at, t.rows, t.k, did, out.data_ptr(), t.k, _raw_stream(dev.index))
+    return y
+
+
+def pack(codes, scales):
+    """Planes codes uint8 [N][K/2] (in a block of 16 bytes byte i = value i in the low nibble, value i + 16 in the high one) and
+    scales uint8 [N][K/32], or with a leading axis of experts -> MXTensor."""
+    dev = _cuda("pack", codes)
+    _on_device("pack", dev, scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError(f"pack: codes {codes.dtype} and scales {scales.dtype}, expected torch.uint8")
+    if codes.dim() not in (2, 3) or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * scales.shape[-1]:
+        raise ValueError(f"pack: codes {tuple(codes.shape)} and scales {tuple(scales.shape)}, expected [..][N][K/2] and [..][N][K/32]")
+    n, k = codes.shape[-2], codes.shape[-1] * 2
+    _check_k("pack", k)
+    experts = codes.shape[0] if codes.dim() == 3 else None
+    if experts is not None and not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"pack: {experts} experts (1..{MAX_EXPERTS})")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    t = MXTensor(torch.empty(image_bytes(n, k, experts or 1), dtype=torch.uint8, device=dev), n, k, experts)
+    _call(dev, "b2q_mx_pack", codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, t.image.data_ptr(),
+          _raw_stream(dev.index))
+    return t
+
+
+def from_ggml(blocks, n, k, experts=None):
+    """ggml's block_mxfp4 (17 bytes: the scale, 16 bytes of codes) as a CUDA uint8 tensor, the bytes as stored in a GGUF file:
+    n rows of k values, or `experts` times as many -> MXTensor."""
+    _cuda("from_ggml", blocks)
+    _check_k("from_ggml", k)
+    count = (1 if experts is None else experts) * n * (k // 32)
+    if blocks.dtype != torch.uint8:
+        raise TypeError(f"from_ggml: blocks dtype {blocks.dtype}, expected torch.uint8")
+    if n < 0 or (experts is not None and experts < 1) or blocks.numel() != count * 17:
+        raise ValueError(f"from_ggml: {blocks.numel()} bytes do not hold {count} MXFP4 blocks of 17")
+    b = blocks.reshape((n, k // 32, 17) if experts is None else (experts, n, k // 32, 17))
+    return pack(b[..., 1:].flatten(-2), b[..., 0])
+
+
+def _check_out(name, out, dtype, shape, dev):
+    """An output tensor given or made: unit column stride, rows that do not overlap."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    _on_device(name, dev, out)
+    if out.dtype != dtype or out.shape != shape or (shape[1] > 1 and out.stride(1) != 1) or \
+            (shape[0] > 1 and out.stride(0) < shape[1]):
+        raise ValueError(f"{name}: out must be a {dtype} {shape} tensor with unit column stride on {dev}")
+    return out
+
+
+def _out_dtype(name, dtype):
+    did = DTYPE_ID.get(dtype)
+    if did is None:
+        raise TypeError(f"{name}: dtype {dtype}, expected float32, float16 or bfloat16")
+    return did
+
+
+def matmul(a, w, dtype=torch.bfloat16, out=None):
+    """MXTensors a [M][K] and w [N][K] -> a w^T [M][N]: exact products, f32 sums, rounded once to `dtype`. out: the tensor for
+    the result (any row stride)."""
+    for t, name in ((a, "a"), (w, "w")):
+        if not isinstance(t, MXTensor):
+            raise TypeError(f"matmul: {name} must be an MXTensor, got {type(t).__name__}")
+        if t.experts is not None:
+            raise ValueError(f"matmul: {name} {t.shape} has experts (comp_b200.experts.linear)")
+    if a.k != w.k or a.device != w.device:
+        raise ValueError(f"matmul: a {a.shape} on {a.device} and w {w.shape} on {w.device}")
+    did = _out_dtype("matmul", dtype)
+    dev = a.device
+    y = _check_out("matmul", out, dtype, (a.rows, w.rows), dev)
+    _call(dev, "b2q_mx_matmul", a.image.data_ptr(), w.image.data_ptr(), a.rows, w.rows, a.k, did, y.data_ptr(), _stride(y),
+          _raw_stream(dev.index))
+    return y
+
+
+def linear(x, w, dtype=None, out=None):
+    """x [M][K] (f32, f16 or bf16; any strides), quantized to MXFP4, times w [N][K] -> [M][N] of `dtype` (default: x's)."""
+    if not isinstance(w, MXTensor):
+        raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
+    if w.experts is not None:
+        raise ValueError(f"linear: w {w.shape} has experts (comp_b200.experts.linear)")
+    dev, k, n = w.device, w.k, w.rows
+    _on_device("linear", dev, x)
+    xid = _dtype_id("linear: x", x)
+    if x.dim() != 2 or x.shape[1] != k:
+        raise ValueError(f"linear: x {tuple(x.shape)}, expected [M][{k}]")
+    m = x.shape[0]
+    dtype = x.dtype if dtype is None else dtype
+    did = _out_dtype("linear", dtype)
+    x = _rows(x)
+    y = _check_out("linear", out, dtype, (m, n), dev)
+    need = image_bytes(m, k)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(dev, "b2q_mx_linear", xid, x.data_ptr(), _stride(x), w.image.data_ptr(), m, n, k, did, y.data_ptr(), _stride(y),
+          workspace.data_ptr(), need, _raw_stream(dev.index))
+    return y

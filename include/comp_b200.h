@@ -372,6 +372,82 @@ size_t b2q_attention_workspace_size(const b2q_kv_cache* cache, const b2q_attenti
 int b2q_attention(const b2q_kv_cache* cache, const b2q_attention_args* args, void* workspace, size_t workspace_bytes,
                   b2q_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * MXFP4 (extension: COMP has no counterpart): 4-bit floating-point values whose blocks of 32 share a power of two, their
+ * products on the tensor cores, and layers of experts on them.
+ *
+ * A block has a scale byte s, for 2^(s - 127) (255: NaN), and 32 codes: a sign bit over 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+ * Planes: codes u8 [rows][K/2], in a block byte i = value i (low nibble) and value i + 16 (high nibble), as in ggml's
+ * block_mxfp4; scales u8 [rows][K/32]. An operand image, which the products read, holds the same bytes in another order:
+ * [ceil(rows/128) tiles][ceil(K/256) stages] of 17408 bytes (comp_b200/csrc/mx_device.cuh), padded with zeros along K; the
+ * experts of a layer follow one another, each from a whole tile on. Images are 128-byte aligned; K is a multiple of 32.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* Bytes of the image of `experts` operands of [rows][K] (0 and an error message: refused). */
+size_t b2q_mx_bytes(int64_t experts, int64_t rows, int64_t K);
+
+/*
+ * Quantizes x [rows][K] (dtype B2Q_DTYPE_*, row stride ldx elements, 16-byte aligned in base and row stride) into an image:
+ * per block s = max(0, floor(log2 max|x|) + 125), values x / 2^(s - 127) rounded to nearest even, those above 6 cut off to 6.
+ * A block with an infinity or a NaN is NaN (s = 255, codes 0); one of zeros has s = 0. Asynchronous on `stream`.
+ */
+int b2q_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, uint8_t* image, b2q_stream_t stream);
+
+/* The values of an image, each rounded once to dtype, into y [rows][K] (16-byte aligned in base and row stride). */
+int b2q_mx_dequantize(const uint8_t* image, int64_t rows, int64_t K, int dtype, void* y, int64_t ldy, b2q_stream_t stream);
+
+/* Planes codes [experts][rows][K/2] (16-byte aligned) and scales [experts][rows][K/32], contiguous, into an image. */
+int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, int64_t rows, int64_t K, uint8_t* image,
+                b2q_stream_t stream);
+
+/*
+ * y[m][n] = sum over blocks of 2^(sa - 127) 2^(sw - 127) * sum over the block of a w: images a of [M][K] and w of [N][K], y
+ * [M][N] of dtype with row stride ldy. Products are exact, sums are f32 (the tensor cores', in an order that depends on M, N
+ * and K alone), rounded once to dtype. A NaN block makes its row (of a) or column (of w) NaN.
+ */
+int b2q_mx_matmul(const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y, int64_t ldy,
+                  b2q_stream_t stream);
+
+/* b2q_mx_quantize of x [M][K] and b2q_mx_matmul with it. workspace: b2q_mx_bytes(1, M, K) bytes of device memory, 128-byte
+ * aligned; calls that may overlap on the GPU need one each. */
+int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y,
+                  int64_t ldy, void* workspace, size_t workspace_bytes, b2q_stream_t stream);
+
+/*
+ * The plan of a layer of experts: which of `experts` (1..1024) the `top` (1..32) choices of each token go to, sorted by
+ * expert, and within one by token * top + choice. int32, one allocation of 2 (experts + 1) + 4 tokens * top words:
+ *   offsets [experts + 1]    the sorted rows where each expert's begin
+ *   tiles   [experts + 1]    the same in tiles of 128 rows, every expert from a whole tile on
+ *   pos     [tokens * top]   the sorted row of each choice (-1: it goes nowhere)
+ *   order   [tokens * top]   the choice of each sorted row (-1 from offsets[experts] on)
+ *   dest, dest_row           rows of the operand image, by choice and by sorted row
+ *
+ * b2q_experts_route: ids i32 [tokens][top] are the experts with the largest logits [tokens][experts] (dtype, row stride ld),
+ * in falling order, the lowest index first among equals. -inf and NaN are never chosen: where fewer are left, id -1 and weight 0.
+ * weights f32 [tokens][top]: softmax over the chosen (normalize != 0) or over all of the token's logits.
+ * b2q_experts_sort: the plan of given ids i32 [tokens][top]; negative ids go nowhere, and so do ids beyond the experts, which
+ * set the device error word to 5. A token may choose an expert twice.
+ */
+int b2q_experts_route(int dtype, const void* logits, int64_t ld, int64_t tokens, int64_t experts, int64_t top, int normalize,
+                      int32_t* ids, float* weights, int32_t* plan, b2q_stream_t stream);
+int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t experts, int32_t* plan, b2q_stream_t stream);
+
+/*
+ * Each sorted row times its expert's weights (image w of [experts][N][K]) -> y [tokens * top][N], in sorted order; rows from
+ * offsets[experts] on are left unwritten. x is [tokens][K] (gather != 0: a token's row for each of its choices) or the sorted
+ * rows [tokens * top][K]; it is quantized to MXFP4 on the way, into the workspace (128-byte aligned; calls that may overlap on
+ * the GPU need one each). The plan is one that b2q_experts_route or b2q_experts_sort wrote for the same sizes.
+ */
+size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int64_t K);
+int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, const uint8_t* w, const int32_t* plan, int64_t tokens,
+                       int64_t top, int64_t experts, int64_t N, int64_t K, int dtype, void* y, int64_t ldy, void* workspace,
+                       size_t workspace_bytes, b2q_stream_t stream);
+
+/* out[t] = sum over j of weights[t][j] * y[pos[t][j]] (f32, in order of j, rounded once; weights NULL: 1): sorted rows y
+ * [tokens * top][N] back to their tokens, out [tokens][N]; both of dtype. A choice that goes nowhere adds nothing. */
+int b2q_experts_combine(int dtype, const void* y, int64_t ldy, const int32_t* plan, const float* weights, int64_t tokens,
+                        int64_t top, int64_t experts, int64_t N, void* out, int64_t ldo, b2q_stream_t stream);
+
 /* Benchmark/tuning hook (process-wide): force rows per group (1, 2, 4), chunks per thread and grid size of the
  * GEMV schedule; 0 restores the planner's choice. Results do not depend on it (except the f32 summation order). */
 int b2q_set_tuning(int rows_per_group, int chunks_per_thread, int grid);
@@ -411,7 +487,8 @@ int b2q_set_cluster(int ctas);
 
 /* Reads (and with clear != 0 resets) the library's device error word: 1 if a kernel's bounded wait on an mbarrier gave
  * up (the kernel then returned early; its outputs are invalid), 2 if a KV cache slot was beyond its cache, 3 if an
- * attention call met a token without a valid page, 4 if a sequence of one had more query tokens than its max_q. Synchronizes with the device. */
+ * attention call met a token without a valid page, 4 if a sequence of one had more query tokens than its max_q, 5 if a choice
+ * named an expert beyond the experts. Synchronizes with the device. */
 int b2q_device_error(int* code, int clear);
 
 /* CUDA IPC helpers for the multi-GPU path. b2q_ipc_get_handle exports the allocation containing dev_ptr as a 64-byte
