@@ -450,11 +450,11 @@ int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t ex
                         (int)experts, plan_parts(plan, tokens * top, experts), stream);
 }
 
-size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int64_t K) {
+size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int gather, int64_t N, int64_t K) {
+  const char* who = "b2q_experts_linear_workspace_size";
   int32_t any = 0;
-  if (check_plan("b2q_experts_linear_workspace_size", &any, tokens, top, experts) ||
-      check_mx_shape("b2q_experts_linear_workspace_size", tokens, K))
-    return 0;
+  if (check_plan(who, &any, tokens, top, experts) || check_mx_shape(who, N, K)) return 0;
+  if (mx_gemv_takes(gather ? tokens : tokens * top, tokens * top, experts, N, K)) return 0;
   // each expert that has rows may leave all but one of its last tile's unused
   const int64_t choices = tokens * top, tiles = choices / kMxRows + std::min(experts, choices);
   return (size_t)tiles * mx_stages(K) * kMxBytes;
@@ -477,11 +477,14 @@ int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, cons
   if (!aligned(w, 128) || !aligned(y, mx_dtype_size(dtype)) || !aligned(x, 16) ||
       (rows > 1 && ldx * mx_dtype_size(x_dtype) % 16))
     return fail(B2Q_EALIGN, "%s: x and its row stride must be 16-byte aligned, w 128-byte, y to its type", who);
-  const size_t need = b2q_experts_linear_workspace_size(tokens, top, experts, K);
+  const PlanOut p = plan_parts(const_cast<int32_t*>(plan), choices, experts);
+  if (mx_gemv_takes(rows, choices, experts, N, K))
+    return launch_mx_gemv({w, x, y, p.offsets, p.order, ldx, ldy, rows, choices, experts, N, K, x_dtype, dtype,
+                           gather ? (int)top : 0}, stream);
+  const size_t need = b2q_experts_linear_workspace_size(tokens, top, experts, gather, N, K);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 128))
     return fail(B2Q_EINVAL, "%s: workspace of %zu bytes, 128-byte aligned, needed (%zu given)", who, need, workspace_bytes);
   uint8_t* image = static_cast<uint8_t*>(workspace);
-  const PlanOut p = plan_parts(const_cast<int32_t*>(plan), choices, experts);
   rc = launch_mx_quantize(x_dtype, x, ldx, rows, K, image, gather ? p.dest : p.dest_row, gather ? (int)top : 1, stream);
   if (rc) return rc;
   const MxGemm g = {w, image, y, p.offsets, p.tiles, ldy, choices, (int)N, (int)mx_tiles(N), (int)mx_stages(K), (int)experts,

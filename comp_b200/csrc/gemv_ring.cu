@@ -63,7 +63,7 @@ extern "C" int b2q_device_error(int* code, int clear) {
   // the words of the KV cache's, the attention's, the MXFP4 products' and the experts' translation units; the first that is
   // set is reported
   for (auto read : {kv_cache_error, kv_attention_q4_error, kv_attention_q8_error, kv_attention_tc_q4_error,
-                    kv_attention_tc_q8_error, mx_gemm_error, experts_error}) {
+                    kv_attention_tc_q8_error, mx_gemm_error, mx_gemv_error, experts_error}) {
     int word = 0;
     const int rc = read(&word, clear);
     if (rc) return rc;

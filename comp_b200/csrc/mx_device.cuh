@@ -54,6 +54,72 @@ __device__ __forceinline__ void from_e2m1x8(uint32_t w, float (&lo)[8], float (&
   }
 }
 
+// the 8 values from `p` on as f32, and the largest magnitude's bits (a NaN's are above infinity's)
+__device__ __forceinline__ uint32_t load8(const float* p, float (&v)[8]) {
+  load4(p, *reinterpret_cast<float(*)[4]>(&v[0]));
+  load4(p + 4, *reinterpret_cast<float(*)[4]>(&v[4]));
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ uint32_t load8(const __half* p, float (&v)[8]) {
+  const uint4 x = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  }
+  m = max(m & 0xffffu, m >> 16);
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+}
+__device__ __forceinline__ uint32_t load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 x = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  }
+  return max(m << 16, m & 0xffff0000u);
+}
+
+// Half a block, values 8h .. 8h + 7 and 16 + 8h .. 16 + 8h + 7 from `p` on (the two nibbles of bytes 8h .. 8h + 7), by one of two
+// neighbouring lanes; finish() gives the block's scale and leaves the codes. All 32 lanes call it.
+struct MxHalf {
+  float lo[8], hi[8];
+  uint32_t largest = 0;
+  uint2 codes;
+
+  template <typename T>
+  __device__ __forceinline__ void load(const T* p, bool there) {
+    if (there) {
+      largest = load8(p, lo);
+      largest = max(largest, load8(p + 16, hi));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
+    }
+  }
+  __device__ __forceinline__ uint32_t finish() {
+    const uint32_t m = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    if (m >= 0x7f800000u) {
+      codes = make_uint2(0, 0);
+      return 255;
+    }
+    const uint32_t s = max((int)(m >> 23) - 2, 0);
+    const float up = __uint_as_float((254 - s) << 23);  // 2^(127 - s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo[i] *= up, hi[i] *= up;
+    codes = make_uint2(to_e2m1x8(lo, hi, 0), to_e2m1x8(lo, hi, 4));
+    return s;
+  }
+};
+
 // 2^(s - 127): s = 0 is below the normal numbers, 255 is NaN.
 __device__ __forceinline__ float mx_scale(uint32_t s) {
   return __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fffffffu : s << 23);

@@ -19,8 +19,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "mx_device.cuh"
-#include "tc_device.cuh"
+#include "mx_tc.cuh"
 
 namespace b2q {
 
@@ -45,31 +44,6 @@ struct MxTile {
 
 constexpr int kThreads = 192;
 
-// K-major operand with the 128-byte swizzle: 8 rows every 1024 bytes
-__device__ __forceinline__ uint64_t desc_swizzled(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// 32 rows of 16 bytes without swizzle: 8 rows every 128 bytes
-__device__ __forceinline__ uint64_t desc_scales(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
-}
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc_scales(smem)) : "memory");
-}
-// kind::mxf4: f32 accumulator, A and B e2m1, both K-major, M = 128, N = n, ue8m0 scales; `half`: which two of a column's four
-// scale bytes count
-__device__ __forceinline__ uint32_t instr_desc_mxf4(int n, int half) {
-  const uint32_t id = half ? 2u : 0u;
-  return (id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (8u << 24) | (id << 29);
-}
-__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
-                                         uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
-      : "memory");
-}
 __device__ __forceinline__ void arrive_bar(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -89,15 +63,6 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&a)[16], 
   tc::tmem_ld16_nowait(taddr + 16, b);
   tc::tmem_wait_ld_regs(a);
   tc::regs_ready(b);
-}
-
-__device__ __forceinline__ void store_as(void* y, int64_t at, int dtype, float v) {
-  if (dtype == B2Q_DTYPE_BF16)
-    static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
-  else if (dtype == B2Q_DTYPE_F16)
-    static_cast<__half*>(y)[at] = __float2half_rn(v);
-  else
-    static_cast<float*>(y)[at] = v;
 }
 
 // A tile: its weight rows, its rows of y, and where its rows of x lie in the image.
@@ -454,6 +419,11 @@ int b2q_mx_matmul(const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int6
   return launch_mx_gemm(g, stream);
 }
 
+size_t b2q_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (check_mx_shape("b2q_mx_linear_workspace_size", M, K) || check_mx_shape("b2q_mx_linear_workspace_size", N, K)) return 0;
+  return mx_gemv_takes(M, 1, 1, N, K) ? 0 : b2q_mx_bytes(1, M, K);
+}
+
 int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y,
                   int64_t ldy, void* workspace, size_t workspace_bytes, b2q_stream_t stream) {
   const char* who = "b2q_mx_linear";
@@ -466,6 +436,8 @@ int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int
   if (rc) return rc;
   if (!aligned(x, 16) || (M > 1 && ldx * mx_dtype_size(x_dtype) % 16))
     return fail(B2Q_EALIGN, "%s: x and its row stride must be 16-byte aligned", who);
+  if (mx_gemv_takes(M, 1, 1, N, K))
+    return launch_mx_gemv({w, x, y, nullptr, nullptr, ldx, ldy, M, 1, 1, N, K, x_dtype, dtype, 0}, stream);
   const size_t need = b2q_mx_bytes(1, M, K);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 128))
     return fail(B2Q_EINVAL, "%s: workspace of %zu bytes, 128-byte aligned, needed (%zu given)", who, need, workspace_bytes);

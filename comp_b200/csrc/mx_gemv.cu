@@ -1,0 +1,341 @@
+// MXFP4 products of up to 16 rows (the next tokens of a few sequences), quantizing the rows on the way: one launch.
+//
+// What counts here is the stream of weights, 17/32 byte a value, and what a launch costs before and after it. As in mx_gemm.cu
+// a CTA's tile is 128 weight rows, whose stages of 256 values of K one thread copies into a ring and another one multiplies;
+// but all rows of x stay in shared memory, and their scales in tensor memory, for as long as the CTA lives: eight warps quantize
+// them there while the first weights are on their way. Before it waits for the preceding kernel a CTA asks for its first
+// weights to be brought into L2; that is only a hint, so that it does no harm where the preceding kernel writes them.
+//
+// A layer of experts needs no gathering: every expert that has rows is multiplied with all rows of x (the unit's other side
+// is 16 rows at the least), and of the results only those that its choices ask for are stored.
+//
+// Where there are fewer tiles than SMs the CTAs of a cluster split K: each sends the columns of its part to the CTAs that own
+// them (distributed shared memory, counted in bytes by the owner's barrier), which add them in order of rank.
+#include <algorithm>
+#include <atomic>
+
+#include "mx_tc.cuh"
+
+namespace b2q {
+
+namespace {
+
+constexpr int kThreads = 320;                   // copying, multiplying, then 8 warps that quantize, 4 of which store
+constexpr int kMaxRing = 8;
+constexpr int kMaxChoices = 128;                // rows of y that a layer of experts makes of the up to 16 of x
+constexpr uint32_t kScaleW = 32, kScaleX = 48;  // columns: accumulators 2 x 16, weight scales 2 x 8, then 4 a stage of x
+
+struct Gemv {
+  const uint8_t* w;
+  const void* x;
+  void* y;
+  const int32_t *offsets, *order;  // of a plan; null: one expert, whose row of y is the row of x
+  int64_t ldx, ldy;
+  int rows, K, N, row_tiles, stages, experts, dtype;
+  int top;      // choices a token where x has a row a token, else 0
+  int ring;     // stages of weights in shared memory
+  int rows8;    // rows of x there, in whole groups of 8
+  int columns;  // of tensor memory
+};
+
+// A tile: its weights, its first column of y, and which rows of y it makes.
+struct GemvTile {
+  int64_t w_tile;
+  int n0, row0, count;
+};
+__device__ __forceinline__ GemvTile gemv_tile(const Gemv& g, const int* used, const int* offsets, int t) {
+  if (!g.offsets) return {t, t * kMxRows, 0, g.rows};
+  const int nth = t / g.row_tiles, rt = t - nth * g.row_tiles, e = used[nth], r0 = offsets[nth];
+  return {(int64_t)e * g.row_tiles + rt, rt * kMxRows, r0, offsets[nth + 1] - r0};
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
+  extern __shared__ uint8_t smem_raw[];  // ring [ring][kMxBytes], x codes [stages][rows8 * 128], x scales [stages][512]
+  __shared__ uint64_t b_full[kMaxRing], b_empty[kMaxRing], b_acc[2], b_free[2], b_x, b_part, b_end;
+  __shared__ float s_part[16][kMxRows];  // the parts of the rows of x whose sums this CTA makes: [row / ranks * ranks + rank]
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_count, s_used[kMaxChoices], s_offsets[kMaxChoices + 1];
+  __shared__ uint8_t s_token[kMaxChoices];  // the row of x of each row of y
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t rank, ranks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const int step = gridDim.x / ranks, start = blockIdx.x / ranks;
+  const int k0 = (int)((int64_t)g.stages * rank / ranks), k1 = (int)((int64_t)g.stages * (rank + 1) / ranks), nk = k1 - k0;
+  const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
+  uint8_t* x_mem = smem_raw + (ring - smem_addr(smem_raw)) + g.ring * kMxBytes;
+  // (the products read 16 rows: with rows8 = 8 the next stage's for the second half, after the last stage a gap of 8)
+  const int x_bytes = (nk * g.rows8 + 16 - g.rows8) * 128;
+  const uint32_t x_codes = ring + g.ring * kMxBytes, x_scales = x_codes + x_bytes;
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < g.ring; ++i) mbar_init(smem_addr(&b_full[i]), 1), mbar_init(smem_addr(&b_empty[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&b_acc[i]), 1), mbar_init(smem_addr(&b_free[i]), 128);
+    mbar_init(smem_addr(&b_x), 256), mbar_init(smem_addr(&b_part), 1), mbar_init(smem_addr(&b_end), 1);
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (!g.offsets && start < g.row_tiles) {
+      const uint8_t* w = g.w + ((int64_t)start * g.stages + k0) * kMxBytes;
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(w), "r"(min(nk, 16) * kMxBytes) : "memory");
+    }
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
+                 "r"(g.columns));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (g.offsets && warp == 2) {  // the experts that have rows, and where those begin
+    int n = 0;
+    for (int e0 = 0; e0 < g.experts; e0 += 32) {
+      const int e = e0 + lane;
+      const int a = e < g.experts ? g.offsets[e] : 0, b = e < g.experts ? g.offsets[e + 1] : 0;
+      const uint32_t some = __ballot_sync(0xffffffffu, b > a);
+      const int at = n + __popc(some & ((1u << lane) - 1));
+      if (b > a && at < kMaxChoices) s_used[at] = e, s_offsets[at] = a, s_offsets[at + 1] = b;
+      n += __popc(some);
+    }
+    if (lane == 0) s_count = min(n, kMaxChoices);
+  } else if (g.offsets && warp == 3) {
+    const int n = g.offsets[g.experts];
+    for (int r = lane; r < kMaxChoices; r += 32) s_token[r] = r >= n ? 0 : g.top ? g.order[r] / g.top : r;
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // barriers are ready: waited for before the first parts
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = s_tmem;
+  const int tiles = g.offsets ? s_count * g.row_tiles : g.row_tiles;
+  bool ok = true;
+  auto wait_one = [&](uint64_t* bar, uint32_t phase) {
+    if (ok && !mbar_wait(smem_addr(bar), phase & 1, kWaitLimit)) ok = false, atomicExch(&s_abort, 1);
+    return ok;
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t phase) {
+    if (ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_addr(bar), phase & 1, kWaitLimit));
+      if (!ok) atomicExch(&s_abort, 1);
+    }
+    return ok;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t once = evict_first_policy();
+      uint32_t s = 0, round = 0;
+      for (int t = start; t < tiles && ok; t += step) {
+        const GemvTile at = gemv_tile(g, s_used, s_offsets, t);
+        const uint8_t* w = g.w + (at.w_tile * g.stages + k0) * kMxBytes;
+        for (int k = 0; k < nk; ++k, w += kMxBytes) {
+          if (round && !wait_one(&b_empty[s], round - 1)) break;
+          const uint32_t bar = smem_addr(&b_full[s]);
+          mbar_expect_tx(bar, kMxBytes);
+          bulk_g2s(ring + s * kMxBytes, w, kMxBytes, bar, once);
+          if (++s == (uint32_t)g.ring) s = 0, ++round;
+        }
+      }
+      // (after a wait that ran out: what is still under way lands before the CTA ends)
+      if (!ok)
+        for (uint32_t i = 0; i < (uint32_t)g.ring; ++i)
+          if (round || i < s) mbar_wait(smem_addr(&b_full[i]), (i < s ? round : round - 1) & 1, kWaitLimit);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && start < tiles) {
+      const uint32_t desc[2] = {instr_desc_mxf4(16, 0), instr_desc_mxf4(16, 1)};
+      wait_one(&b_x, 0);
+      for (int k = 0; k < nk && ok; ++k) copy_scales(tmem + kScaleX + 4 * k, x_scales + k * 512);
+      uint32_t s = 0, round = 0, it = 0, count = 0;
+      for (int t = start; t < tiles && ok; t += step, ++count) {
+        const uint32_t buf = count & 1, acc = tmem + buf * 16;
+        if (count >= 2) wait_one(&b_free[buf], (count >> 1) - 1);
+        tc::fence_after();
+        for (int k = 0; k < nk && ok; ++k, ++it) {
+          if (!wait_one(&b_full[s], round)) break;
+          tc::fence_after();
+          const uint32_t stage = ring + s * kMxBytes, sw = tmem + kScaleW + (it & 1) * 8, sx = tmem + kScaleX + 4 * k;
+          copy_scales(sw, stage + kMxCodes);
+          copy_scales(sw + 4, stage + kMxCodes + 512);
+          const uint64_t da = desc_swizzled(stage), db = desc_swizzled(x_codes + k * g.rows8 * 128);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_mxf4(acc, da + j * 2, db + j * 2, desc[j & 1], sw + (j >> 1) * 4, sx + (j >> 1) * 2, k > 0 || j > 0);
+          tc::mma_commit(smem_addr(&b_empty[s]));
+          if (++s == (uint32_t)g.ring) s = 0, ++round;
+        }
+        tc::mma_commit(smem_addr(&b_acc[buf]));
+      }
+    }
+    __syncwarp();
+  } else {
+    // quantize: two threads a block, as in mx_quant.cu
+    const int t0 = threadIdx.x - 64, items = g.rows * nk * 16;
+    for (int i = t0; i - lane < items; i += 256) {
+      const int row = i / (nk * 16), in = i - row * nk * 16, k = in >> 4, b = (in >> 1) & 7, half = in & 1;
+      const int at = (k0 + k) * kMxStage + b * 32 + 8 * half;
+      MxHalf q;
+      q.load(static_cast<const T*>(g.x) + row * g.ldx + at, i < items && at < g.K);
+      uint32_t scales = q.finish() << (8 * (b & 3));
+      scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
+      scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+      if (i < items) {
+        *reinterpret_cast<uint2*>(x_mem + k * g.rows8 * 128 + mx_code_at(row, b) + 8 * half) = q.codes;
+        // a stage's scales: row r is lane r, blocks 0..3 in column 0, blocks 4..7 in column 2
+        if ((threadIdx.x & 7) == 0)
+          *reinterpret_cast<uint32_t*>(x_mem + x_bytes + k * 512 + row * 16 + (b >> 2) * 8) = scales;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor cores read them
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&b_x)) : "memory");
+  }
+
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  uint32_t count = 0;
+  for (int t = start; t < tiles; t += step, ++count) {  // (once where CTAs share a tile: there are clusters enough)
+    const GemvTile at = gemv_tile(g, s_used, s_offsets, t);
+    const int in = (warp & 3) * 32 + lane, n = at.n0 + in;
+    const bool stores = warp >= 2 && warp < 6;
+    uint32_t v[16];
+    if (stores) {
+      const uint32_t buf = count & 1;
+      wait_warp(&b_acc[buf], count >> 1);
+      tc::fence_after();
+      if (ok) {
+        tc::tmem_ld16_nowait(tmem + ((uint32_t)((warp & 3) * 32) << 16) + buf * 16, v);
+        tc::tmem_wait_ld_regs(v);
+      }
+      tc::fence_before();
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&b_free[buf])) : "memory");
+    }
+    if (ranks == 1) {
+      if (stores && ok && n < g.N)
+        for (int i = 0; i < at.count; ++i) {
+          const int row = at.row0 + i, x_row = g.offsets ? s_token[row] : row;
+          uint32_t mine = v[0];
+#pragma unroll
+          for (int c = 1; c < 16; ++c) mine = c == x_row ? v[c] : mine;
+          store_as(g.y, (int64_t)row * g.ldy + n, g.dtype, __uint_as_float(mine));
+        }
+      continue;
+    }
+    // row r of x is summed by CTA r % ranks
+    const int owned = (g.rows - (int)rank + (int)ranks - 1) / (int)ranks;
+    if (threadIdx.x == 64) mbar_expect_tx(smem_addr(&b_part), (uint32_t)owned * ranks * kMxRows * 4);
+    if (stores && ok) {
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        if (c < g.rows) {
+          const uint32_t owner = (uint32_t)c % ranks, slot = (uint32_t)c / ranks * ranks + rank;
+          uint32_t to, bar;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_addr(&s_part[slot][in])), "r"(owner));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_addr(&b_part)), "r"(owner));
+          asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(to), "r"(v[c]), "r"(bar)
+                       : "memory");
+        }
+    }
+    __syncwarp();
+    // no CTA ends before all have sent their parts
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (stores && owned > 0 && wait_warp(&b_part, 0) && n < g.N)
+      for (int i = 0; i < owned; ++i) {
+        const int x_row = (int)rank + i * (int)ranks;
+        float sum = 0.f;
+        for (uint32_t r = 0; r < ranks; ++r) sum += s_part[i * ranks + r][in];
+        for (int row = at.row0; row < at.row0 + at.count; ++row)
+          if ((g.offsets ? s_token[row] : row) == x_row) store_as(g.y, (int64_t)row * g.ldy + n, g.dtype, sum);
+      }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (s_abort) {  // products may be under way still: they end before their tensor memory is given back
+    if (threadIdx.x == 32) {
+      atomicCAS(&g_device_error, 0, kErrTimeout);
+      tc::mma_commit(smem_addr(&b_end));
+      mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns));
+}
+
+struct GemvPlan {
+  int ranks, nk, ring, rows8;
+  size_t smem;
+};
+
+// Whether and how the kernel takes `rows` rows of x: CTAs in a cluster, the most stages one has, stages of its ring.
+bool plan_gemv(int64_t rows, int64_t used, int64_t row_tiles, int64_t stages, int sms, GemvPlan* p) {
+  if (rows < 1 || rows > 16) return false;
+  int ranks = 1;
+  while (ranks < 8 && used * row_tiles * ranks * 2 <= sms && stages >= ranks * 4) ranks *= 2;
+  const int64_t nk = (stages + ranks - 1) / ranks;
+  const int rows8 = rows <= 8 ? 8 : 16;
+  if (nk > (512 - (int)kScaleX) / 4) return false;
+  const size_t x = (size_t)nk * (rows8 * 128 + 512) + (16 - rows8) * 128 + 1024;  // 1024: the ring is aligned to that
+  // a ring that leaves room for the next kernel's CTA beside this one, or else for all that an SM has
+  const size_t half = 104 * 1024, all = 214 * 1024;
+  size_t ring = x + 4 * kMxBytes <= half ? (half - x) / kMxBytes : x + 3 * kMxBytes <= all ? (all - x) / kMxBytes : 0;
+  if (ring == 0) return false;
+  ring = std::min<size_t>(std::min<size_t>(ring, kMaxRing), std::max<int64_t>(nk, 2));
+  *p = {ranks, (int)nk, (int)ring, rows8, x + ring * kMxBytes};
+  return true;
+}
+
+template <typename T>
+int launch_gemv(const Gemv& g, const GemvPlan& p, int ctas, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};  // devices on which the kernel may take all of the shared memory
+  const auto kernel = mx_gemv_kernel<T>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1))) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 214 * 1024);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return fail(B2Q_ECUDA, "mx_gemv: %s", cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctas * p.ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, g);
+  return after_launch("mx_gemv");
+}
+
+}  // namespace
+
+bool mx_gemv_takes(int64_t rows, int64_t choices, int64_t experts, int64_t N, int64_t K) {
+  DeviceInfo dev;
+  GemvPlan p;
+  if (choices > kMaxChoices || device_info(&dev)) return false;
+  return plan_gemv(rows, std::min(choices, experts), mx_tiles(N), mx_stages(K), dev.sms, &p);
+}
+
+int launch_mx_gemv(const MxGemv& a, cudaStream_t stream) {
+  DeviceInfo dev;
+  int rc = device_info(&dev);
+  if (rc) return rc;
+  GemvPlan p;
+  const int64_t used = std::min<int64_t>(a.offsets ? a.choices : 1, a.experts), row_tiles = mx_tiles(a.N), stages = mx_stages(a.K);
+  if (!plan_gemv(a.rows, used, row_tiles, stages, dev.sms, &p)) return fail(B2Q_ERANGE, "mx_gemv: more rows than the kernel takes");
+  const Gemv g = {a.w, a.x, a.y, a.offsets, a.order, a.ldx, a.ldy, (int)a.rows, (int)a.K, (int)a.N, (int)row_tiles, (int)stages,
+                  (int)a.experts, a.dtype, a.top, p.ring, p.rows8, kScaleX + 4 * p.nk <= 256 ? 256 : 512};
+  // with several CTAs a tile every tile has a cluster of its own
+  const int64_t ctas = std::min<int64_t>(used * row_tiles, dev.sms / p.ranks);
+  if (a.x_dtype == B2Q_DTYPE_F32) return launch_gemv<float>(g, p, (int)ctas, stream);
+  if (a.x_dtype == B2Q_DTYPE_F16) return launch_gemv<__half>(g, p, (int)ctas, stream);
+  return launch_gemv<__nv_bfloat16>(g, p, (int)ctas, stream);
+}
+
+int mx_gemv_error(int* code, int clear) { return read_error_word(g_device_error, code, clear); }
+
+}  // namespace b2q

@@ -38,8 +38,21 @@ struct MxGemm {
 };
 int launch_mx_gemm(const MxGemm& g, cudaStream_t stream);
 
+// Up to 16 rows of x, quantized by the kernel itself.
+struct MxGemv {
+  const uint8_t* w;
+  const void* x;
+  void* y;
+  const int32_t *offsets, *order;  // of a plan (null: one expert)
+  int64_t ldx, ldy, rows, choices, experts, N, K;
+  int x_dtype, dtype, top;         // top: choices a token where x has a row a token (0: x has the sorted rows)
+};
+bool mx_gemv_takes(int64_t rows, int64_t choices, int64_t experts, int64_t N, int64_t K);
+int launch_mx_gemv(const MxGemv& a, cudaStream_t stream);
+
 // A translation unit's device error word (b2q_device_error reads them all).
 int mx_gemm_error(int* code, int clear);
+int mx_gemv_error(int* code, int clear);
 int experts_error(int* code, int clear);
 
 }  // namespace b2q

@@ -29,40 +29,6 @@ int check_mx_rows(const char* who, const char* name, int dtype, const void* x, i
 
 namespace {
 
-// the 8 values from `p` on as f32, and the largest magnitude's bits (a NaN's are above infinity's)
-__device__ __forceinline__ uint32_t load8(const float* p, float (&v)[8]) {
-  load4(p, *reinterpret_cast<float(*)[4]>(&v[0]));
-  load4(p + 4, *reinterpret_cast<float(*)[4]>(&v[4]));
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
-}
-__device__ __forceinline__ uint32_t load8(const __half* p, float (&v)[8]) {
-  const uint4 x = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-  }
-  m = max(m & 0xffffu, m >> 16);
-  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
-}
-__device__ __forceinline__ uint32_t load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 x = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-  }
-  return max(m << 16, m & 0xffff0000u);
-}
-
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   store4(p, v[0], v[1], v[2], v[3]);
   store4(p + 4, v[4], v[5], v[6], v[7]);
@@ -100,24 +66,9 @@ __global__ void __launch_bounds__(256)
   const Place p = place_of((int64_t)blockIdx.x * 256 + threadIdx.x, stages);
   const int at = p.stage * kMxStage + p.b * 32 + 8 * p.half;
   const bool there = p.row < rows && at < K;  // K is a multiple of 32: a whole block is there, or none of it
-  float lo[8] = {}, hi[8] = {};
-  uint32_t m = 0;
-  if (there) {
-    const T* src = x + p.row * ldx + at;
-    m = load8(src, lo);
-    m = max(m, load8(src + 16, hi));
-  }
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  uint32_t s = max((int)(m >> 23) - 2, 0);
-  const float up = __uint_as_float((254 - s) << 23);
-  uint2 q = {0, 0};
-  if (m < 0x7f800000u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] *= up, hi[i] *= up;
-    q = make_uint2(to_e2m1x8(lo, hi, 0), to_e2m1x8(lo, hi, 4));
-  } else {
-    s = 255;
-  }
+  MxHalf h;
+  h.load(x + p.row * ldx + at, there);
+  const uint32_t s = h.finish();
   uint32_t scales = s << (8 * (p.b & 3));  // the 4 blocks of a word: 8 lanes of the same row
   scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
@@ -128,7 +79,7 @@ __global__ void __launch_bounds__(256)
     if (r < 0) continue;
     uint8_t* tile = image + ((r >> 7) * stages + p.stage) * kMxBytes;
     const int in = (int)r & 127;
-    *reinterpret_cast<uint2*>(tile + mx_code_at(in, p.b) + 8 * p.half) = q;
+    *reinterpret_cast<uint2*>(tile + mx_code_at(in, p.b) + 8 * p.half) = h.codes;
     if ((threadIdx.x & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_at(in, p.b)) = scales;
   }
 }

@@ -13,7 +13,8 @@ kernels are this package's own, through the C-ABI (include/comp_b200.h, where la
 import torch
 
 from .kv import _call, _dtype_id, _on_device, _raw_stream
-from .mx import MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _out_dtype, _rows, _stride
+from .mx import (FUSED_ROWS, MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _few_size, _out_dtype,
+                 _rows, _stride)
 
 MAX_TOP = 32
 
@@ -102,17 +103,20 @@ def _check_plan(name, plan):
         raise TypeError(f"{name}: plan must be a Plan (route, sort), got {type(plan).__name__}")
 
 
-def workspace_size(plan, k):
-    """Bytes of device workspace that linear needs for rows of k values."""
+def workspace_size(plan, w, gather=True):
+    """Bytes of device workspace that linear(x, w, plan, gather) needs."""
     choices = plan.tokens * plan.top
-    return (choices // TILE_ROWS + min(plan.experts, choices)) * -(-k // STAGE) * STAGE_BYTES
+    if (plan.tokens if gather else choices) <= FUSED_ROWS:
+        return _few_size(w, (plan.tokens, plan.top, bool(gather)), "b2q_experts_linear_workspace_size", plan.tokens, plan.top,
+                         plan.experts, 1 if gather else 0, w.rows, w.k)
+    return (choices // TILE_ROWS + min(plan.experts, choices)) * -(-w.k // STAGE) * STAGE_BYTES
 
 
 def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     """Each sorted row, quantized to MXFP4, times its expert's weights w (MXTensor [E][N][K]) -> [T * top][N] of `dtype`
     (default: x's) in sorted order; rows past plan.offsets[E] stay unwritten. x: [T][K], a token's row for each of its choices,
-    or with gather=False the sorted rows [T * top][K]. workspace: a CUDA uint8 tensor of workspace_size(plan, K) bytes, 128-byte
-    aligned (allocated here when None)."""
+    or with gather=False the sorted rows [T * top][K]. workspace: a CUDA uint8 tensor of workspace_size(plan, w, gather)
+    bytes, 128-byte aligned (allocated here when None)."""
     if not isinstance(w, MXTensor):
         raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
     _check_plan("linear", plan)
@@ -130,16 +134,17 @@ def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     did = _out_dtype("linear", dtype)
     x = _rows(x)
     y = _check_out("linear", out, dtype, (choices, n), dev)
-    need = workspace_size(plan, k)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        need = workspace_size(plan, w, gather)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     else:
         _on_device("linear", dev, workspace)
         if not workspace.is_contiguous():
             raise ValueError("linear: workspace must be contiguous")
+        need = workspace.numel() * workspace.element_size()
     _call(dev, "b2q_experts_linear", xid, x.data_ptr(), _stride(x), 1 if gather else 0, w.image.data_ptr(),
           plan._words.data_ptr(), plan.tokens, plan.top, plan.experts, n, k, did, y.data_ptr(), _stride(y),
-          workspace.data_ptr(), workspace.numel() * workspace.element_size(), _raw_stream(dev.index))
+          0 if workspace is None else workspace.data_ptr(), need, _raw_stream(dev.index))
     return y
 
 

@@ -14,10 +14,12 @@ TypeError / ValueError / RuntimeError on what they do not take.
 
 import torch
 
+from . import _lib
 from .kv import DTYPE_ID, _call, _dtype_id, _on_device, _raw_stream
 
 TILE_ROWS, STAGE, STAGE_BYTES = 128, 256, 17408  # an image: 128 rows by 256 values a run of bytes
 MAX_EXPERTS = 1024
+FUSED_ROWS = 16  # products of up to so many rows may quantize them in their own launch
 
 
 def image_bytes(rows, k, experts=1):
@@ -47,6 +49,7 @@ class MXTensor:
         if image.dim() != 1 or image.numel() < need or not image.is_contiguous() or (need and image.data_ptr() % 128):
             raise ValueError(f"MXTensor: the image must be {need} contiguous bytes, 128-byte aligned, got {tuple(image.shape)}")
         self.image, self.rows, self.k, self.experts, self.device = image, rows, k, experts, image.device
+        self._sizes = {}  # workspaces of products with few rows
 
     @property
     def shape(self):
@@ -183,6 +186,15 @@ def matmul(a, w, dtype=torch.bfloat16, out=None):
     return y
 
 
+def _few_size(w, key, name, *args):
+    """The workspace of a product of w with few rows, which may be one launch that needs none."""
+    size = w._sizes.get(key)
+    if size is None:
+        with torch.cuda.device(w.device):
+            size = w._sizes[key] = getattr(_lib.load(), name)(*args)
+    return size
+
+
 def linear(x, w, dtype=None, out=None):
     """x [M][K] (f32, f16 or bf16; any strides), quantized to MXFP4, times w [N][K] -> [M][N] of `dtype` (default: x's)."""
     if not isinstance(w, MXTensor):
@@ -199,8 +211,8 @@ def linear(x, w, dtype=None, out=None):
     did = _out_dtype("linear", dtype)
     x = _rows(x)
     y = _check_out("linear", out, dtype, (m, n), dev)
-    need = image_bytes(m, k)
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    need = image_bytes(m, k) if m > FUSED_ROWS else _few_size(w, m, "b2q_mx_linear_workspace_size", m, n, k)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _call(dev, "b2q_mx_linear", xid, x.data_ptr(), _stride(x), w.image.data_ptr(), m, n, k, did, y.data_ptr(), _stride(y),
-          workspace.data_ptr(), need, _raw_stream(dev.index))
+          workspace.data_ptr() if need else 0, need, _raw_stream(dev.index))
     return y

@@ -408,8 +408,10 @@ int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, in
 int b2q_mx_matmul(const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y, int64_t ldy,
                   b2q_stream_t stream);
 
-/* b2q_mx_quantize of x [M][K] and b2q_mx_matmul with it. workspace: b2q_mx_bytes(1, M, K) bytes of device memory, 128-byte
- * aligned; calls that may overlap on the GPU need one each. */
+/* b2q_mx_quantize of x [M][K] and b2q_mx_matmul with it, in one launch for up to 16 rows (unless K is very long). workspace: device
+ * memory of b2q_mx_linear_workspace_size(M, N, K) bytes (0 for one launch), 128-byte aligned; calls that may overlap on the GPU
+ * need one each. */
+size_t b2q_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K);
 int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y,
                   int64_t ldy, void* workspace, size_t workspace_bytes, b2q_stream_t stream);
 
@@ -435,10 +437,10 @@ int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t ex
 /*
  * Each sorted row times its expert's weights (image w of [experts][N][K]) -> y [tokens * top][N], in sorted order; rows from
  * offsets[experts] on are left unwritten. x is [tokens][K] (gather != 0: a token's row for each of its choices) or the sorted
- * rows [tokens * top][K]; it is quantized to MXFP4 on the way, into the workspace (128-byte aligned; calls that may overlap on
- * the GPU need one each). The plan is one that b2q_experts_route or b2q_experts_sort wrote for the same sizes.
+ * rows [tokens * top][K]; it is quantized to MXFP4 on the way, into the workspace (128-byte aligned; 0 bytes for a few rows; calls
+ * that may overlap on the GPU need one each). The plan is one that b2q_experts_route or b2q_experts_sort wrote for the same sizes.
  */
-size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int64_t K);
+size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int gather, int64_t N, int64_t K);
 int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, const uint8_t* w, const int32_t* plan, int64_t tokens,
                        int64_t top, int64_t experts, int64_t N, int64_t K, int dtype, void* y, int64_t ldy, void* workspace,
                        size_t workspace_bytes, b2q_stream_t stream);

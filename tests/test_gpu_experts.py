@@ -98,7 +98,8 @@ def expert_case(rng, tokens, top, n_experts, n, k, dtype, gather, skip=0, skew=F
 @pytest.mark.parametrize("tokens,top,n_experts,n,k,skip", [
     (1, 1, 1, 1, 32, 0), (1, 8, 64, 256, 512, 0), (1, 2, 4, 300, 2080, 0), (3, 4, 8, 128, 4096, 0), (16, 2, 8, 700, 288, 3),
     (61, 6, 40, 512, 1440, 0), (64, 8, 160, 130, 256, 0), (200, 3, 4, 1000, 544, 5), (300, 2, 2, 260, 1024, 0),
-    (1000, 2, 9, 513, 320, 7), (700, 4, 5, 3500, 96, 0), (5, 1, 1000, 64, 64, 0)])
+    (1000, 2, 9, 513, 320, 7), (700, 4, 5, 3500, 96, 0), (5, 1, 1000, 64, 64, 0), (16, 8, 100, 200, 320, 0), (16, 1, 3, 4000, 96, 4),
+    (2, 8, 9, 130, 5000 // 32 * 32, 0), (13, 9, 16, 20000, 64, 0), (17, 2, 6, 300, 288, 0)])
 def test_linear(cuda, gather, tokens, top, n_experts, n, k, skip):
     rng = np.random.default_rng(tokens + n + k)
     dtype = ("f32", "f16", "bf16")[(tokens + n) % 3]
@@ -132,6 +133,18 @@ def test_popular_experts(cuda, counts, n, k):
     want, mass = ref.experts_linear(ref.values(*ref.quantize(x.numpy())), ref.values(*w), offsets, order, 1)
     check(experts.linear(x.to(cuda), packed(w, cuda), plan), want, mass, k, "f32")
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("n", [100, 40000])
+def test_same_expert_twice(cuda, n):
+    """A token whose choices are all of one expert gets a row for each."""
+    rng = np.random.default_rng(n)
+    ids = np.array([[3, 3, 3], [0, 3, 0], [1, -1, 1]])
+    x, w = torch.from_numpy(rng.standard_normal((3, 96)).astype(np.float32)), planes(rng, (4, n, 96))
+    plan = experts.sort(torch.from_numpy(ids.astype(np.int32)).to(cuda), 4)
+    offsets, _, order = check_plan(plan, ids, 4)
+    want, mass = ref.experts_linear(ref.values(*ref.quantize(x.numpy())), ref.values(*w), offsets, order, 3)
+    check(experts.linear(x.to(cuda), packed(w, cuda), plan)[: offsets[-1]], want[: offsets[-1]], mass[: offsets[-1]], 96, "f32")
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -232,7 +245,8 @@ def test_refusals(cuda):
                        (lambda: experts.linear(x, w, plan, dtype=torch.int8), TypeError),
                        (lambda: experts.linear(x, w, experts.route(torch.zeros((4, 4), device=cuda), 2)), ValueError),
                        (lambda: experts.linear(x, w, plan, out=y.T), ValueError),
-                       (lambda: experts.linear(x, w, plan, workspace=small), ValueError),
+                       (lambda: experts.linear(torch.ones((40, 64), device=cuda), w, experts.route(torch.zeros((40, 3), device=cuda), 2),
+                                               workspace=small), ValueError),
                        (lambda: experts.combine(y[:7], plan), ValueError), (lambda: experts.combine(y.double(), plan), TypeError),
                        (lambda: experts.combine(y, plan, plan.weights.half()), TypeError),
                        (lambda: experts.combine(y, plan, plan.weights[:, :1]), ValueError),

@@ -146,16 +146,19 @@ def test_blocks_of_different_sizes(cuda, m, n, k, spread):
 
 
 @pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("m,n,k", [(1, 513, 96), (17, 384, 1056), (150, 128, 256), (260, 9000, 320)])
+@pytest.mark.parametrize("m,n,k", [(1, 513, 96), (17, 384, 1056), (150, 128, 256), (260, 9000, 320), (1, 1, 32), (1, 1000, 4096),
+                                   (2, 130, 8192), (8, 40000, 288), (9, 300, 2080), (16, 20000, 1056), (16, 128, 5120), (3, 2000, 14336),
+                                   (1, 2000, 28672), (16, 9700, 7168)])
 def test_linear(cuda, dtype, m, n, k):
     rng = np.random.default_rng(m + n)
     x = torch.from_numpy(rng.standard_normal((m, k))).to(DT[dtype])
-    w = planes(rng, (n, k))
-    vx, vw = ref.values(*ref.quantize(x.float().numpy())), ref.values(*w)
+    w = planes(rng, (n, k)) if n * k < 1 << 24 else (rng.integers(0, 256, (n, k // 2), dtype=np.uint8),
+                                                     rng.integers(116, 122, (n, k // 32), dtype=np.uint8))
+    vx, vw = (torch.from_numpy(ref.values(*p)).to(cuda) for p in (ref.quantize(x.float().numpy()), w))
     tw = packed(w, cuda)
     y = mx.linear(x.to(cuda), tw)
-    assert y.dtype == DT[dtype]
-    check(y, vx @ vw.T, np.abs(vx) @ np.abs(vw).T, k, dtype)
+    assert y.dtype == DT[dtype] and device_error() == 0
+    check(y, (vx @ vw.T).cpu().numpy(), (vx.abs() @ vw.abs().T).cpu().numpy(), k, dtype)
     # out: any row stride and alignment; what lies around it stays
     wide = torch.full((m, n + 5), 7.0, dtype=DT[dtype], device=cuda)
     assert mx.linear(x.to(cuda), tw, out=wide[:, 3 : n + 3]).data_ptr() == wide[:, 3:].data_ptr()
@@ -235,11 +238,13 @@ def test_weights_quantized_right_before(cuda):
     for i in range(10):
         wv = torch.randn((4096, 1024), generator=gen, device=cuda)
         x = torch.randn((3, 1024), generator=gen, device=cuda)
-        got, again = mx.linear(x, mx.quantize(wv)), mx.matmul(mx.quantize(x), mx.quantize(wv), dtype=torch.float32)
+        many = x.repeat(30, 1)
+        calls = (lambda w: mx.linear(x, w), lambda w: mx.linear(many, w), lambda w: mx.matmul(mx.quantize(x), w))
+        got = [call(mx.quantize(wv)) for call in calls]
         w = mx.quantize(wv)
         torch.cuda.synchronize()
-        want = mx.linear(x, w)
-        assert torch.equal(got, want) and torch.equal(again, want)
+        for call, y in zip(calls, got):
+            assert torch.equal(call(w), y)
 
 
 def test_refusals(cuda):

@@ -21,15 +21,15 @@ def test_sizes(lib):
         assert lib.b2q_mx_bytes(*bad) == 0 and "b2q_mx_bytes" in _lib.last_error()
     for e, rows, k in ((1, 1, 32), (7, 300, 4096), (2, 128, 256)):
         assert lib.b2q_mx_bytes(e, rows, k) == mx.image_bytes(rows, k, e)
-    for t, top, e, k in ((1, 1, 1, 32), (64, 8, 128, 4096), (1000, 3, 9, 288), (5, 1, 1000, 64)):
-        plan = experts.Plan(t, top, e, torch.device("cpu"))
-        assert lib.b2q_experts_linear_workspace_size(t, top, e, k) == experts.workspace_size(plan, k)
+    assert lib.b2q_mx_linear_workspace_size(17, 300, 288) == 2 * 17408 and lib.b2q_mx_linear_workspace_size(1, 1, 20) == 0
+    for t, top, e, k in ((17, 1, 1, 32), (64, 8, 128, 4096), (1000, 3, 9, 288), (50, 1, 1000, 64)):
+        size = lib.b2q_experts_linear_workspace_size(t, top, e, 1, 64, k)
         # the most tiles that sorted rows can take
         counts = np.zeros(e, dtype=np.int64)
         n = t * top
         counts[: min(e, n)] = 1
         counts[0] += n - counts.sum()
-        assert (-(-counts // 128)).sum() * -(-k // 256) * 17408 <= experts.workspace_size(plan, k)
+        assert (-(-counts // 128)).sum() * -(-k // 256) * 17408 <= size
 
 
 def test_quantize_refusals(lib):
@@ -50,7 +50,7 @@ def test_product_refusals(lib):
     assert f(a=None) == -1 and f(w=None) == -1 and f(y=None) == -1 and f(m=-1) == -1 and f(n=-1) == -1 and f(k=16) == -1
     assert f(dtype=4) == -1 and f(ldy=2) == -1 and f(a=64) == -2 and f(w=64) == -2 and f(y=4098) == -2
     assert f(m=0) == 0 and f(n=0) == 0
-    g = lambda x=4096, ldx=64, w=4096, y=4096, ws=4096, size=17408, m=2, dtype=2: lib.b2q_mx_linear(  # noqa: E731
+    g = lambda x=4096, ldx=64, w=4096, y=4096, ws=4096, size=17408, m=20, dtype=2: lib.b2q_mx_linear(  # noqa: E731
         0, x, ldx, w, m, 3, 64, dtype, y, 3, ws, size, None)
     assert g(x=None) == -1 and g(w=None) == -1 and g(y=None) == -1 and g(ws=None) == -1 and g(size=17407) == -1 and g(dtype=9) == -1
     assert g(x=4100) == -2 and g(ldx=65) == -2 and g(ws=4096 + 16) == -1 and g(m=0, ws=None) == 0
@@ -64,7 +64,7 @@ def test_expert_refusals(lib):
     assert r(plan=None) == -1 and r(plan=4098) == -2 and r(ids=4097) == -2 and r(x=4097) == -2 and r(t=1 << 30) == -4
     s = lambda ids=4096, t=2, top=2, e=8, plan=4096: lib.b2q_experts_sort(ids, t, top, e, plan, None)  # noqa: E731
     assert s(ids=None) == -1 and s(plan=None) == -1 and s(e=0) == -1 and s(top=33) == -1 and s(ids=4098) == -2
-    f = lambda x=4096, ldx=64, w=4096, plan=4096, t=2, n=3, k=64, dtype=0, y=4096, ldy=3, ws=4096, size=1 << 20: (  # noqa: E731
+    f = lambda x=4096, ldx=64, w=4096, plan=4096, t=20, n=3, k=64, dtype=0, y=4096, ldy=3, ws=4096, size=1 << 20: (  # noqa: E731
         lib.b2q_experts_linear(0, x, ldx, 1, w, plan, t, 2, 8, n, k, dtype, y, ldy, ws, size, None))
     assert f(x=None) == -1 and f(w=None) == -1 and f(plan=None) == -1 and f(y=None) == -1 and f(ws=None) == -1 and f(k=40) == -1
     assert f(dtype=3) == -1 and f(ldy=2) == -1 and f(size=17408) == -1 and f(x=4104) == -2 and f(w=4096 + 64) == -2 and f(y=4098) == -2
