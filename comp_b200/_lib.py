@@ -69,6 +69,7 @@ SIGNATURES = {
     "b2q_mx_matmul": (INT, [P, P, I64, I64, I64, INT, P, I64, P]),
     "b2q_mx_linear_workspace_size": (ctypes.c_size_t, [I64, I64, I64]),
     "b2q_mx_linear": (INT, [INT, P, I64, P, I64, I64, I64, INT, P, I64, P, ctypes.c_size_t, P]),
+    "b2q_experts_plan_words": (ctypes.c_size_t, [I64, I64, I64]),
     "b2q_experts_route": (INT, [INT, P, I64, I64, I64, I64, INT, P, P, P, P]),
     "b2q_experts_sort": (INT, [P, I64, I64, I64, P, P]),
     "b2q_experts_linear_workspace_size": (ctypes.c_size_t, [I64, I64, I64, INT, I64, I64]),

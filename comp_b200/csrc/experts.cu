@@ -5,11 +5,11 @@
 //
 // Sort: stable, by counting. The choices (token * top + j) are cut into runs, one a warp; a warp counts its run's experts 32
 // choices at a time (lanes with the same expert find each other with one match), the counts before each warp's run give
-// every choice its place, and a second walk over the run hands the places out. Up to 32 warps are one CTA; longer lists take
-// a cluster of 8, which add their counts through distributed shared memory: one launch either way, no atomics, so that the
-// order is always the same. A small list's router is the same launch.
+// every choice its place, and a second walk over the run hands the places out. A short list is one CTA's work, routing
+// included: one launch, whose choices stay in shared memory. A long one is two: CTAs all over the GPU route and count their
+// tokens, then each adds up what the others before it counted and places its own. The order is the same every time.
 //
-// Combine: a thread adds the same 16 bytes of a token's rows, in order of its choices, in f32: one pass, bound by memory.
+// Combine: a thread adds the same 32 bytes of a token's rows, in order of its choices, in f32: one pass, bound by memory.
 #include <algorithm>
 #include <atomic>
 
@@ -19,74 +19,85 @@ namespace b2q {
 
 namespace {
 
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCluster = 8;
+constexpr int64_t kMostChoices = 1 << 26, kMostPart = 14000;  // in a plan; in a part, whose experts lie in shared memory
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSmallChoices = 4096, kSmallTokens = 128;  // lists of up to so many are sorted, and routed, by one CTA
 
 struct PlanOut {
   int32_t *offsets, *tiles;            // [experts + 1]
   int32_t *pos, *order;                // [choices]
   int32_t *dest, *dest_row;            // [choices] rows of the operand image: by choice, by sorted row
+  int32_t* counts;                     // [parts][experts] of a long list's parts
 };
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Whole numbers in the order of the logits; 0 for -inf and NaN, which are never chosen.
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t b = __float_as_uint(x + 0.f);  // -0 as 0
+// Whole numbers in the order of the logits; 0 for -inf and NaN, which are never chosen. 16-bit logits leave the low 13 bits
+// of theirs free (zeros, or ones below 0): there the number of the expert goes, the lowest highest, so that one maximum finds both.
+template <typename T>
+__device__ __forceinline__ uint32_t order_key(T logit, int e) {
+  const float x = to_float(logit) + 0.f;  // -0 as 0
   if (!(x > -INFINITY)) return 0;
-  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  const uint32_t b = __float_as_uint(x), k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return sizeof(T) == 4 ? k : (k & 0xffffe000u) | (uint32_t)(0x1fff - e);
 }
+template <typename T>
 __device__ __forceinline__ float key_value(uint32_t k) {
-  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+  const bool negative = !(k & 0x80000000u);
+  if (sizeof(T) == 2) k = negative ? k | 0x1fffu : k & 0xffffe000u;
+  return __uint_as_float(negative ? ~k : k ^ 0x80000000u);
 }
 // exp(v - top): the largest counts 1, infinities among them
-__device__ __forceinline__ float exp_below(uint32_t key, uint32_t top) {
-  return key == top ? 1.f : expf(key_value(key) - key_value(top));
-}
+__device__ __forceinline__ float exp_below(float v, float top) { return v == top ? 1.f : expf(v - top); }
 
 // One token by a warp: lane j < top gets the j-th expert (or -1) and its weight.
 template <int V, typename T>
 __device__ __forceinline__ void route_token(const T* logits, int experts, int top, bool normalize, int lane, int* id, float* weight) {
   uint32_t key[V];
-  uint32_t mine = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = v * 32 + lane;
-    key[v] = e < experts ? order_key(to_float(logits[e])) : 0;
-    mine = max(mine, key[v]);
+    key[v] = e < experts ? order_key(logits[e], e) : 0;
   }
-  const uint32_t largest = __reduce_max_sync(0xffffffffu, mine);
+  uint32_t mine = key[0];  // the lane's largest, and (f32) which it is
+  int at = 0;
+  auto largest_of_lane = [&] {
+    mine = key[0], at = 0;
+#pragma unroll
+    for (int v = 1; v < V; ++v)
+      if (key[v] > mine) mine = key[v], at = v;
+  };
+  largest_of_lane();
+  uint32_t m = __reduce_max_sync(0xffffffffu, mine);
+  const float largest = key_value<T>(m);
   float total = 0.f;
   if (!normalize) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) total += key[v] ? exp_below(key[v], largest) : 0.f;
+    for (int v = 0; v < V; ++v) total += key[v] ? exp_below(key_value<T>(key[v]), largest) : 0.f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   int chosen = -1;
   uint32_t chosen_key = 0;
-  for (int j = 0; j < top; ++j) {
-    const uint32_t m = j == 0 ? largest : __reduce_max_sync(0xffffffffu, mine);
-    if (m == 0) break;
-    uint32_t at = 0xffffffffu;
-    if (mine == m) {
-#pragma unroll
-      for (int v = V - 1; v >= 0; --v)
-        if (key[v] == m) at = v * 32 + lane;
+  for (int j = 0; j < top && m != 0; ++j) {
+    int e;
+    if (sizeof(T) == 2) {
+      e = 0x1fff - (int)(m & 0x1fffu);
+    } else {
+      e = (int)__reduce_min_sync(0xffffffffu, mine == m ? (uint32_t)(at * 32 + lane) : 0xffffffffu);
     }
-    at = __reduce_min_sync(0xffffffffu, at);
-    if (lane == j) chosen = (int)at, chosen_key = m;
-    if ((at & 31) == lane) {
-      mine = 0;
+    if (lane == j) chosen = e, chosen_key = m;
+    if ((e & 31) == lane) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (v == (int)(at >> 5)) key[v] = 0;
-        mine = max(mine, key[v]);
-      }
+      for (int v = 0; v < V; ++v)
+        if (v == at) key[v] = 0;
+      largest_of_lane();
     }
+    if (j + 1 < top) m = __reduce_max_sync(0xffffffffu, mine);
   }
-  float w = chosen >= 0 ? exp_below(chosen_key, largest) : 0.f;
+  const float w = chosen >= 0 ? exp_below(key_value<T>(chosen_key), largest) : 0.f;
   if (normalize) {
     total = w;
 #pragma unroll
@@ -96,153 +107,197 @@ __device__ __forceinline__ void route_token(const T* logits, int experts, int to
   *weight = chosen >= 0 ? w / total : 0.f;
 }
 
+struct RouteArgs {
+  const void* logits;
+  int64_t ld;
+  int top;
+  bool normalize;
+  int32_t* ids;    // (without routing: given)
+  float* weights;
+};
+
+// The tokens first .. end - 1 by the CTA's warps.
 template <int V, typename T>
-__device__ __forceinline__ void route_rows(const T* logits, int64_t ld, int64_t tokens, int experts, int top, bool normalize,
-                                           int32_t* ids, float* weights, int64_t first, int64_t step) {
+__device__ __forceinline__ void route_tokens(const RouteArgs& a, int experts, int64_t first, int64_t end, int32_t* kept) {
   const int lane = threadIdx.x & 31;
-  for (int64_t t = first; t < tokens; t += step) {
+  for (int64_t t = first + (threadIdx.x >> 5); t < end; t += blockDim.x >> 5) {
     int id;
     float w;
-    route_token<V>(logits + t * ld, experts, top, normalize, lane, &id, &w);
-    if (lane < top) ids[t * top + lane] = id, weights[t * top + lane] = w;
+    route_token<V>(static_cast<const T*>(a.logits) + t * a.ld, experts, a.top, a.normalize, lane, &id, &w);
+    if (lane < a.top) {
+      a.ids[t * a.top + lane] = id, a.weights[t * a.top + lane] = w;
+      kept[(t - first) * a.top + lane] = id;
+    }
   }
 }
 
-template <int V, typename T>
-__global__ void __launch_bounds__(256)
-    route_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int experts, int top, bool normalize,
-                 int32_t* __restrict__ ids, float* __restrict__ weights) {
-  pdl_wait_then_trigger();
-  route_rows<V>(logits, ld, tokens, experts, top, normalize, ids, weights, (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5),
-                (int64_t)gridDim.x * 8);
+// An expert's number, -1 for none.
+__device__ __forceinline__ int checked(int id, int experts) {
+  if (id >= experts) {
+    atomicCAS(&g_device_error, 0, kErrExpert);
+    return -1;
+  }
+  return id < 0 ? -1 : id;
 }
 
-__device__ __forceinline__ int ld_cluster_int(uint32_t addr, uint32_t rank) {
-  uint32_t there;
-  int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
-  return v;
-}
-__device__ __forceinline__ void sync_cluster(uint32_t ranks) {
-  if (ranks > 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  else
-    __syncthreads();
-}
-
-// The sum of `v` over the threads before this one, and over all (kSortThreads threads).
-__device__ __forceinline__ int sum_before(int v, int* scratch, int* all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int sum = v;
+// The sums of `rows` and `tiles` over the threads before this one, and over all.
+__device__ __forceinline__ void sums_before(int* rows, int* tiles, uint64_t* scratch, int* all_rows, int* all_tiles) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const uint64_t v = (uint64_t)*tiles << 32 | (uint32_t)*rows;
+  uint64_t sum = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, sum, o);
+    const uint64_t u = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += u;
   }
-  __syncthreads();
   if (lane == 31) scratch[warp] = sum;
   __syncthreads();
-  int w = scratch[lane];
+  uint64_t w = lane < warps ? scratch[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, w, o);
+    const uint64_t u = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += u;
   }
-  *all = __shfl_sync(0xffffffffu, w, 31);
-  const int upto = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  return sum - v + (warp ? upto : 0);
+  const uint64_t all = __shfl_sync(0xffffffffu, w, 31), upto = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  sum += (warp ? upto : 0) - v;
+  *rows = (int)(uint32_t)sum, *tiles = (int)(sum >> 32), *all_rows = (int)(uint32_t)all, *all_tiles = (int)(all >> 32);
 }
 
-// V > 0: a single CTA routes first (logits of type T).
-template <int V, typename T>
-__global__ void __launch_bounds__(kSortThreads, 1)
-    sort_kernel(const T* __restrict__ logits, int64_t ld, int top, bool normalize, int32_t* ids, float* weights, int choices,
-                int experts, const PlanOut p) {
-  extern __shared__ int s_count[];  // [warps][experts], then the CTA's totals [experts]
-  __shared__ int s_scratch[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* totals = s_count + kSortWarps * experts;
-  uint32_t rank, ranks;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-  for (int i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) s_count[i] = 0;
-  pdl_wait_then_trigger();
-  if constexpr (V > 0) {
-    route_rows<V>(logits, ld, choices / top, experts, top, normalize, ids, weights, warp, kSortWarps);
-    __threadfence_block();
-  }
-  __syncthreads();
-
-  // this warp's run of choices, and what it counts of each expert
-  const int run = ((choices + (int)ranks * kSortWarps * 32 - 1) / ((int)ranks * kSortWarps * 32)) * 32;
-  const int64_t begin = (int64_t)((int)rank * kSortWarps + warp) * run;
-  const int64_t end = min((int64_t)choices, begin + run);
+// Hands out the places of the CTA's choices first .. end - 1: `before` and `total` are the expert threadIdx.x's choices in
+// earlier parts and in all.  ids(i): choice i's expert or -1. s_count: [warps][experts] zeros, s_move [experts].
+template <typename Ids, typename Total>
+__device__ __forceinline__ void place(Ids ids, Total total_of, int64_t first, int64_t end, int64_t choices, int experts, int* s_count,
+                                      int* s_move, uint64_t* scratch, bool writes_totals, int64_t part, int64_t parts,
+                                      const PlanOut& p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all_warps = blockDim.x >> 5;
+  const int warps = min(all_warps, (int)((end - first + 31) >> 5));  // with runs of their own
+  const int64_t run = warps ? ((end - first + warps * 32 - 1) / (warps * 32)) * 32 : 0;
+  const int64_t begin = min(end, first + warp * run), stop = warp < warps ? min(end, begin + run) : begin;
   int* mine = s_count + warp * experts;
-  auto expert_of = [&](int64_t i) {
-    const int id = i < end ? (V > 0 ? *(volatile const int32_t*)(ids + i) : ids[i]) : -1;
-    if (id >= experts) {
-      atomicCAS(&g_device_error, 0, kErrExpert);
-      return -1;
-    }
-    return id < 0 ? -1 : id;
-  };
-  for (int64_t i = begin; i < end; i += 32) {
-    const int id = expert_of(i + lane);
+  for (int64_t i = begin; i < stop; i += 32) {
+    const int id = i + lane < stop ? ids(i + lane) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, id);
     if (id >= 0 && lane == __ffs(same) - 1) mine[id] += __popc(same);
     __syncwarp();
   }
   __syncthreads();
-
-  // counts before each warp's run; all counts of the CTA
   const int e = threadIdx.x;
-  int total = 0;
+  int before = 0, total = 0;  // this expert's choices in earlier parts, and in all
+  int here = 0;
   if (e < experts) {
-    for (int w = 0; w < kSortWarps; ++w) {
+    for (int w = 0; w < warps; ++w) {
       const int c = s_count[w * experts + e];
-      s_count[w * experts + e] = total;
-      total += c;
-    }
-    totals[e] = total;
-  }
-  sync_cluster(ranks);
-  int before = 0, all = 0;  // counts of this expert in the CTAs before this one, and in all
-  if (e < experts) {
-    for (uint32_t r = 0; r < ranks; ++r) {
-      const int c = ranks > 1 ? ld_cluster_int(smem_addr(totals + e), r) : total;
-      if (r < rank) before += c;
-      all += c;
+      s_count[w * experts + e] = here;
+      here += c;
     }
   }
-  sync_cluster(ranks);  // the others' totals are read before they change, and before a CTA ends
-  int placed, tiles;
-  const int offset = sum_before(all, s_scratch, &placed);
-  const int tile = sum_before((all + kMxRows - 1) / kMxRows, s_scratch, &tiles);
+  total_of(e, here, &before, &total);
+  int offset = total, tile = (total + kMxRows - 1) / kMxRows, placed, tiles;
+  sums_before(&offset, &tile, scratch, &placed, &tiles);
   if (e < experts) {
-    if (rank == 0) p.offsets[e] = offset, p.tiles[e] = tile;
-    for (int w = 0; w < kSortWarps; ++w) s_count[w * experts + e] += offset + before;
-    totals[e] = tile * kMxRows - offset;  // from a sorted row to the image's
+    if (writes_totals) p.offsets[e] = offset, p.tiles[e] = tile;
+    for (int w = 0; w < warps; ++w) s_count[w * experts + e] += offset + before;
+    s_move[e] = tile * kMxRows - offset;  // from a sorted row to the image's
   }
-  if (rank == 0 && threadIdx.x == 0) p.offsets[experts] = placed, p.tiles[experts] = tiles;
+  if (writes_totals && threadIdx.x == 0) p.offsets[experts] = placed, p.tiles[experts] = tiles;
   __syncthreads();
-
-  for (int64_t i = begin; i < end; i += 32) {
+  for (int64_t i = begin; i < stop; i += 32) {
     const int64_t c = i + lane;
-    const int id = expert_of(c);
+    const int id = c < stop ? ids(c) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, id);
     int row = -1, image = -1;
-    if (id >= 0) row = mine[id] + __popc(same & ((1u << lane) - 1)), image = row + totals[id];
+    if (id >= 0) row = mine[id] + __popc(same & ((1u << lane) - 1)), image = row + s_move[id];
     __syncwarp();
     if (id >= 0 && lane == __ffs(same) - 1) mine[id] += __popc(same);
     __syncwarp();
-    if (c < end) {
+    if (c < stop) {
       p.pos[c] = row, p.dest[c] = image;
       if (row >= 0) p.order[row] = (int)c, p.dest_row[row] = image;
     }
   }
-  for (int64_t r = (int64_t)placed + (int)rank * kSortThreads + threadIdx.x; r < choices; r += (int64_t)ranks * kSortThreads)
+  for (int64_t r = placed + part * blockDim.x + threadIdx.x; r < choices; r += parts * blockDim.x)
     p.order[r] = -1, p.dest_row[r] = -1;
+}
+
+// A short list by one CTA. V > 0: routed first (logits of type T).
+template <int V, typename T>
+__global__ void __launch_bounds__(kSortThreads, 1)
+    sort_small_kernel(const RouteArgs a, int choices, int experts, const PlanOut p) {
+  extern __shared__ int s_mem[];  // [choices] ids, [experts] moves, [warps][experts] counts
+  __shared__ uint64_t s_scratch[32];
+  int *s_ids = s_mem, *s_move = s_ids + choices, *s_count = s_move + experts;
+  const int warps = min((int)blockDim.x >> 5, (choices + 31) >> 5);
+  for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) s_count[i] = 0;
+  pdl_wait_then_trigger();
+  if constexpr (V > 0) {
+    route_tokens<V, T>(a, experts, 0, choices / a.top, s_ids);
+  } else {
+    for (int i = threadIdx.x; i < choices; i += blockDim.x) s_ids[i] = checked(a.ids[i], experts);
+  }
+  __syncthreads();
+  place([&](int64_t i) { return s_ids[i]; }, [](int, int here, int* before, int* total) { *total = here; }, 0, choices, choices,
+        experts, s_count, s_move, s_scratch, true, 0, 1, p);
+}
+
+// A long list's parts, `per` tokens each: routed and counted,
+template <int V, typename T>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const RouteArgs a, int64_t tokens, int per, int experts, const PlanOut p) {
+  extern __shared__ int s_mem[];  // [per * top] ids, [experts] counts
+  int *s_ids = s_mem, *s_count = s_ids + per * a.top;
+  for (int i = threadIdx.x; i < experts; i += blockDim.x) s_count[i] = 0;
+  pdl_wait_then_trigger();
+  const int64_t first = (int64_t)blockIdx.x * per, end = min(tokens, first + per);
+  const int n = (int)(end - first) * a.top;
+  if constexpr (V > 0) {
+    route_tokens<V, T>(a, experts, first, end, s_ids);
+  } else {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) s_ids[i] = a.ids[first * a.top + i];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int id = checked(s_ids[i], experts);
+    if (id >= 0) atomicAdd(&s_count[id], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) p.counts[(int64_t)blockIdx.x * experts + e] = s_count[e];
+}
+
+// then placed. As many threads as experts at the least.
+__global__ void __launch_bounds__(kSortThreads, 1)
+    sort_place_kernel(const int32_t* ids, int top, int64_t tokens, int per, int experts, const PlanOut p) {
+  extern __shared__ int s_mem[];  // [per * top] ids, [experts] moves, earlier and all counts, [warps][experts] counts
+  __shared__ uint64_t s_scratch[32];
+  int *s_ids = s_mem, *s_move = s_ids + per * top, *s_before = s_move + experts, *s_total = s_before + experts;
+  int* s_count = s_total + experts;
+  const int64_t first = (int64_t)blockIdx.x * per, end = min(tokens, first + per);
+  const int n = (int)(end - first) * top, warps = min((int)blockDim.x >> 5, (n + 31) >> 5);
+  for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) s_count[i] = 0;
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) s_before[e] = s_total[e] = 0;
+  pdl_wait_then_trigger();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int id = ids[first * top + i];
+    s_ids[i] = id < experts ? id : -1;
+  }
+  __syncthreads();
+  // the parts' counts of an expert are added up by as many threads as there are for it
+  const int parts = gridDim.x, groups = max(1, (int)blockDim.x / experts), group = threadIdx.x / experts;
+  if (group < groups) {
+    const int e = threadIdx.x - group * experts;
+    int before = 0, total = 0;
+#pragma unroll 8
+    for (int q = group; q < parts; q += groups) {
+      const int c = p.counts[(int64_t)q * experts + e];
+      total += c;
+      before += q < (int)blockIdx.x ? c : 0;
+    }
+    atomicAdd(&s_before[e], before), atomicAdd(&s_total[e], total);
+  }
+  __syncthreads();
+  place([&](int64_t i) { return s_ids[i - first * top]; },
+        [&](int e, int, int* before, int* total) {
+          if (e < experts) *before = s_before[e], *total = s_total[e];
+        },
+        first * top, end * top, tokens * top, experts, s_count, s_move, s_scratch, blockIdx.x == 0, blockIdx.x, parts, p);
 }
 
 // Vectors of B bytes of T.
@@ -255,7 +310,11 @@ struct Vec {
   };
   __device__ Vec() {}
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (B == 16) {
+    if constexpr (B == 32) {
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p));
+    } else if constexpr (B == 16) {
       const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
       w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else if constexpr (B == 8) {
@@ -268,7 +327,11 @@ struct Vec {
     }
   }
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (B == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (B == 32)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                   "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    else if constexpr (B == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     else if constexpr (B == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else if constexpr (B == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
     else *p = v[0];
@@ -285,17 +348,18 @@ __global__ void __launch_bounds__(256)
                    const float* __restrict__ weights, int64_t tokens, int top, int vectors, T* __restrict__ out, int64_t ldo) {
   pdl_wait_then_trigger();
   using V = Vec<T, B>;
+  constexpr int kAtOnce = 4;
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t t = item < (1ll << 32) ? (int64_t)((uint32_t)item / (uint32_t)vectors) : item / vectors;
   if (t >= tokens) return;
   const int c = (int)(item - t * vectors) * V::N;
   float sum[V::N] = {};
-  for (int j0 = 0; j0 < top; j0 += 4) {  // four rows' loads at once
-    V v[4];
-    float w[4];
-    int r[4];
+  for (int j0 = 0; j0 < top; j0 += kAtOnce) {  // so many rows' loads at once
+    V v[kAtOnce];
+    float w[kAtOnce];
+    int r[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kAtOnce; ++j) {
       r[j] = j0 + j < top ? pos[t * top + j0 + j] : -1;
       if (r[j] >= rows) r[j] = -1;
       if (r[j] >= 0) {
@@ -304,7 +368,7 @@ __global__ void __launch_bounds__(256)
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kAtOnce; ++j)
       if (r[j] >= 0) {
 #pragma unroll
         for (int i = 0; i < V::N; ++i) sum[i] = fmaf(w[j], to_float(v[j].v[i]), sum[i]);
@@ -322,82 +386,94 @@ int launch_combine(const void* y, int64_t ldy, int64_t rows, const int32_t* pos,
   // the widest vectors that both row strides and bases are whole multiples of
   const uint64_t all = (reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) | (uint64_t)(ldy * sizeof(T)) |
                        (uint64_t)(ldo * sizeof(T)) | (uint64_t)(N * sizeof(T));
-  const int bytes = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+  const int bytes = all % 32 == 0 ? 32 : all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
   const int64_t vectors = N * (int)sizeof(T) / bytes, grid = (tokens * vectors + 255) / 256;
   if (vectors > INT32_MAX || grid > INT32_MAX) return fail(B2Q_ERANGE, "b2q_experts_combine: too many values for one launch");
   auto launch = [&](auto kernel) {
     launch_maybe_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, stream, static_cast<const T*>(y), ldy, rows, pos, weights, tokens,
                      top, (int)vectors, static_cast<T*>(out), ldo);
   };
-  if (bytes == 16) launch(combine_kernel<T, 16>);
+  if (bytes == 32) launch(combine_kernel<T, 32>);
+  else if (bytes == 16) launch(combine_kernel<T, 16>);
   else if (bytes == 8) launch(combine_kernel<T, 8>);
   else if (bytes == 4) launch(combine_kernel<T, 4>);
   else if constexpr (sizeof(T) == 2) launch(combine_kernel<T, 2>);
   return after_launch("experts_combine");
 }
 
-// Lists of up to so many choices are sorted by one CTA, and routed by it.
-constexpr int64_t kSmallChoices = 4096, kSmallTokens = 128;
+// A long list's parts: tokens each, and how many.
+struct Parts {
+  int per, count;
+};
+Parts parts_of(int64_t tokens, int64_t top) {
+  // some 1000 choices a CTA, but no more of them than fill a GPU (the counts are [parts][experts], and every CTA reads them)
+  const int64_t choices = tokens * top;
+  const int64_t want = std::max({(int64_t)1, std::min<int64_t>(choices / 1024, 144), (choices + kMostPart - 1) / kMostPart});
+  const int64_t per = (tokens + want - 1) / want;
+  return {(int)per, (int)((tokens + per - 1) / per)};
+}
 
-template <int V, typename T>
-int launch_sort(const T* logits, int64_t ld, int top, bool normalize, int32_t* ids, float* weights, int64_t choices, int experts,
-                const PlanOut& p, cudaStream_t stream) {
-  const auto kernel = sort_kernel<V, T>;
-  static std::atomic<unsigned long long> done{0};  // devices on which the kernel may take the memory of the most experts
+bool is_small(int64_t tokens, int64_t top, bool routed) {
+  return tokens * top <= kSmallChoices && (!routed || tokens <= kSmallTokens);
+}
+
+// Lets a kernel take up to `most` bytes of shared memory, once a device.
+template <typename Kernel>
+int allow_smem(Kernel kernel, int most, std::atomic<unsigned long long>& done) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSortWarps + 1) * (int)kMaxExperts * 4);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  if (e != cudaSuccess) return fail(B2Q_ECUDA, "experts_sort: %s", cudaGetErrorString(e));
-  const int ranks = choices > kSmallChoices ? kSortCluster : 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ranks);
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = (size_t)(kSortWarps + 1) * experts * 4;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, kernel, logits, ld, top, normalize, ids, weights, (int)choices, experts, p);
+  return e == cudaSuccess ? B2Q_OK : fail(B2Q_ECUDA, "experts: %s", cudaGetErrorString(e));
+}
+
+constexpr int kSortSmem = 220 * 1024;
+static_assert((kMostPart + kMaxTop + kMaxExperts * (3 + kSortWarps)) * 4 <= kSortSmem, "a part's experts and counts");
+
+template <int V, typename T>
+int route_and_sort(const RouteArgs& a, int64_t tokens, int experts, const PlanOut& p, cudaStream_t stream) {
+  const int64_t choices = tokens * a.top;
+  static std::atomic<unsigned long long> done_small{0}, done_count{0}, done_place{0};
+  if (is_small(tokens, a.top, V > 0)) {
+    // warps with runs of 32 choices each, a warp a token, a thread an expert
+    const int warps = std::min<int>(kSortWarps, std::max<int>((int)(choices + 31) / 32, 1));
+    const int need = std::max(std::max(warps, V > 0 ? (int)tokens : 0), (experts + 31) / 32);
+    const int threads = std::min(kSortThreads, need * 32);
+    const size_t smem = (size_t)(choices + experts + std::min<int64_t>(threads / 32, (choices + 31) / 32) * experts) * 4;
+    int rc = allow_smem(sort_small_kernel<V, T>, kSortSmem, done_small);
+    if (rc) return rc;
+    launch_maybe_pdl(sort_small_kernel<V, T>, dim3(1), dim3(threads), smem, stream, a, (int)choices, experts, p);
+    return after_launch("experts_sort");
+  }
+  const Parts q = parts_of(tokens, a.top);
+  const size_t ids = (size_t)q.per * a.top * 4;
+  const size_t smem_count = ids + (size_t)experts * 4, smem_place = ids + (size_t)experts * (3 + kSortWarps) * 4;
+  int rc = allow_smem(sort_count_kernel<V, T>, kSortSmem, done_count);
+  if (!rc) rc = allow_smem(sort_place_kernel, kSortSmem, done_place);
+  if (rc) return rc;
+  launch_maybe_pdl(sort_count_kernel<V, T>, dim3(q.count), dim3(kSortThreads), smem_count, stream, a, tokens, q.per, experts, p);
+  rc = after_launch("experts_count");
+  if (rc) return rc;
+  launch_maybe_pdl(sort_place_kernel, dim3(q.count), dim3(kSortThreads), smem_place, stream, a.ids, a.top, tokens, q.per, experts, p);
   return after_launch("experts_sort");
 }
 
-template <int V, typename T>
-int route_and_sort(const T* logits, int64_t ld, int64_t tokens, int experts, int top, bool normalize, int32_t* ids, float* weights,
-                   const PlanOut& p, cudaStream_t stream) {
-  const int64_t choices = tokens * top;
-  if (tokens <= kSmallTokens) return launch_sort<V>(logits, ld, top, normalize, ids, weights, choices, experts, p, stream);
-  DeviceInfo dev;
-  int rc = device_info(&dev);
-  if (rc) return rc;
-  const unsigned grid = (unsigned)std::min<int64_t>((tokens + 7) / 8, (int64_t)dev.sms * 8);
-  launch_maybe_pdl(route_kernel<V, T>, dim3(grid), dim3(256), 0, stream, logits, ld, tokens, experts, top, normalize, ids, weights);
-  rc = after_launch("experts_route");
-  return rc ? rc : launch_sort<0>(static_cast<const float*>(nullptr), 0, top, false, ids, weights, choices, experts, p, stream);
-}
-
 template <typename T>
-int route_typed(const void* logits, int64_t ld, int64_t tokens, int experts, int top, bool normalize, int32_t* ids, float* weights,
-                const PlanOut& p, cudaStream_t stream) {
-  const T* x = static_cast<const T*>(logits);
-  if (experts <= 32) return route_and_sort<1>(x, ld, tokens, experts, top, normalize, ids, weights, p, stream);
-  if (experts <= 64) return route_and_sort<2>(x, ld, tokens, experts, top, normalize, ids, weights, p, stream);
-  if (experts <= 128) return route_and_sort<4>(x, ld, tokens, experts, top, normalize, ids, weights, p, stream);
-  if (experts <= 256) return route_and_sort<8>(x, ld, tokens, experts, top, normalize, ids, weights, p, stream);
-  if (experts <= 512) return route_and_sort<16>(x, ld, tokens, experts, top, normalize, ids, weights, p, stream);
-  return route_and_sort<32>(x, ld, tokens, experts, top, normalize, ids, weights, p, stream);
+int route_typed(const RouteArgs& a, int64_t tokens, int experts, const PlanOut& p, cudaStream_t stream) {
+  if (experts <= 32) return route_and_sort<1, T>(a, tokens, experts, p, stream);
+  if (experts <= 64) return route_and_sort<2, T>(a, tokens, experts, p, stream);
+  if (experts <= 128) return route_and_sort<4, T>(a, tokens, experts, p, stream);
+  if (experts <= 256) return route_and_sort<8, T>(a, tokens, experts, p, stream);
+  if (experts <= 512) return route_and_sort<16, T>(a, tokens, experts, p, stream);
+  return route_and_sort<32, T>(a, tokens, experts, p, stream);
 }
 
-// The plan's parts in its one allocation: offsets, tiles [experts + 1 each]; pos, order, dest, dest_row [choices each].
+// The plan's parts in its one allocation: offsets, tiles [experts + 1 each]; pos, order, dest, dest_row [choices each]; counts.
 PlanOut plan_parts(int32_t* plan, int64_t choices, int64_t experts) {
   int32_t* lists = plan + 2 * (experts + 1);
-  return {plan, plan + experts + 1, lists, lists + choices, lists + 2 * choices, lists + 3 * choices};
+  return {plan, plan + experts + 1, lists, lists + choices, lists + 2 * choices, lists + 3 * choices, lists + 4 * choices};
 }
 
 int check_plan(const char* who, const int32_t* plan, int64_t tokens, int64_t top, int64_t experts) {
@@ -405,7 +481,7 @@ int check_plan(const char* who, const int32_t* plan, int64_t tokens, int64_t top
     return fail(B2Q_EINVAL, "%s: %lld tokens, %lld choices each (1..%lld)", who, (long long)tokens, (long long)top, (long long)kMaxTop);
   if (experts < 1 || experts > kMaxExperts)
     return fail(B2Q_EINVAL, "%s: %lld experts (1..%lld)", who, (long long)experts, (long long)kMaxExperts);
-  if (tokens > (1ll << 30) / top) return fail(B2Q_ERANGE, "%s: %lld tokens of %lld choices", who, (long long)tokens, (long long)top);
+  if (tokens > kMostChoices / top) return fail(B2Q_ERANGE, "%s: %lld tokens of %lld choices", who, (long long)tokens, (long long)top);
   if (!plan) return fail(B2Q_EINVAL, "%s: plan is NULL", who);
   if (!aligned(plan, 4)) return fail(B2Q_EALIGN, "%s: plan must be 4-byte aligned", who);
   return B2Q_OK;
@@ -421,6 +497,13 @@ using namespace b2q;
 
 extern "C" {
 
+size_t b2q_experts_plan_words(int64_t tokens, int64_t top, int64_t experts) {
+  int32_t any = 0;
+  if (check_plan("b2q_experts_plan_words", &any, tokens, top, experts)) return 0;
+  const int64_t choices = tokens * top;
+  return (size_t)(2 * (experts + 1) + 4 * choices + (is_small(tokens, top, true) ? 0 : parts_of(tokens, top).count * experts));
+}
+
 int b2q_experts_route(int dtype, const void* logits, int64_t ld, int64_t tokens, int64_t experts, int64_t top, int normalize,
                       int32_t* ids, float* weights, int32_t* plan, b2q_stream_t stream) {
   const char* who = "b2q_experts_route";
@@ -433,11 +516,10 @@ int b2q_experts_route(int dtype, const void* logits, int64_t ld, int64_t tokens,
   if (!aligned(logits, mx_dtype_size(dtype)) || !aligned(ids, 4) || !aligned(weights, 4))
     return fail(B2Q_EALIGN, "%s: a pointer is not aligned to its type", who);
   const PlanOut p = plan_parts(plan, tokens * top, experts);
-  if (dtype == B2Q_DTYPE_F32)
-    return route_typed<float>(logits, ld, tokens, (int)experts, (int)top, normalize != 0, ids, weights, p, stream);
-  if (dtype == B2Q_DTYPE_F16)
-    return route_typed<__half>(logits, ld, tokens, (int)experts, (int)top, normalize != 0, ids, weights, p, stream);
-  return route_typed<__nv_bfloat16>(logits, ld, tokens, (int)experts, (int)top, normalize != 0, ids, weights, p, stream);
+  const RouteArgs a = {logits, ld, (int)top, normalize != 0, ids, weights};
+  if (dtype == B2Q_DTYPE_F32) return route_typed<float>(a, tokens, (int)experts, p, stream);
+  if (dtype == B2Q_DTYPE_F16) return route_typed<__half>(a, tokens, (int)experts, p, stream);
+  return route_typed<__nv_bfloat16>(a, tokens, (int)experts, p, stream);
 }
 
 int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t experts, int32_t* plan, b2q_stream_t stream) {
@@ -446,8 +528,8 @@ int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t ex
   if (rc) return rc;
   if (tokens > 0 && !ids) return fail(B2Q_EINVAL, "%s: ids is NULL", who);
   if (!aligned(ids, 4)) return fail(B2Q_EALIGN, "%s: ids must be 4-byte aligned", who);
-  return launch_sort<0>(static_cast<const float*>(nullptr), 0, (int)top, false, const_cast<int32_t*>(ids), nullptr, tokens * top,
-                        (int)experts, plan_parts(plan, tokens * top, experts), stream);
+  const RouteArgs a = {nullptr, 0, (int)top, false, const_cast<int32_t*>(ids), nullptr};
+  return route_and_sort<0, float>(a, tokens, (int)experts, plan_parts(plan, tokens * top, experts), stream);
 }
 
 size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int gather, int64_t N, int64_t K) {

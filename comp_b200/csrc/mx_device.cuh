@@ -88,6 +88,16 @@ __device__ __forceinline__ uint32_t load8(const __nv_bfloat16* p, float (&v)[8])
   return max(m << 16, m & 0xffff0000u);
 }
 
+// 32 bytes at once (the address a multiple of 32): twice the widest load of older GPUs.
+__device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+
+// The scale of a block whose largest magnitude has the bits m (infinities and NaN at the top).
+__device__ __forceinline__ uint32_t mx_scale_of(uint32_t m) { return m >= 0x7f800000u ? 255u : max((int)(m >> 23) - 2, 0); }
+
 // Half a block, values 8h .. 8h + 7 and 16 + 8h .. 16 + 8h + 7 from `p` on (the two nibbles of bytes 8h .. 8h + 7), by one of two
 // neighbouring lanes; finish() gives the block's scale and leaves the codes. All 32 lanes call it.
 struct MxHalf {
@@ -105,17 +115,16 @@ struct MxHalf {
       for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
     }
   }
-  __device__ __forceinline__ uint32_t finish() {
-    const uint32_t m = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-    if (m >= 0x7f800000u) {
-      codes = make_uint2(0, 0);
-      return 255;
-    }
-    const uint32_t s = max((int)(m >> 23) - 2, 0);
+  // (s: the scale; codes of a block that is NaN are zeros)
+  __device__ __forceinline__ void encode(uint32_t s) {
     const float up = __uint_as_float((254 - s) << 23);  // 2^(127 - s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) lo[i] *= up, hi[i] *= up;
-    codes = make_uint2(to_e2m1x8(lo, hi, 0), to_e2m1x8(lo, hi, 4));
+    codes = s == 255 ? make_uint2(0, 0) : make_uint2(to_e2m1x8(lo, hi, 0), to_e2m1x8(lo, hi, 4));
+  }
+  __device__ __forceinline__ uint32_t finish() {
+    const uint32_t s = mx_scale_of(max(largest, __shfl_xor_sync(0xffffffffu, largest, 1)));
+    encode(s);
     return s;
   }
 };

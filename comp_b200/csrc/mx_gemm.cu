@@ -39,7 +39,7 @@ struct MxTile {
   static constexpr uint32_t kScaleCol = 448;                  // scales: two sets, which stages take in turn
   static constexpr uint32_t kScaleSet = 8 + kParts * 8;
   static_assert(kSecond + TN <= kScaleCol && kScaleCol + 2 * kScaleSet <= 512, "tensor memory");
-  static_assert(kSmem <= 227 * 1024 - 8192, "shared memory");  // beside it: the experts' first tiles
+  static_assert(kSmem <= 227 * 1024 - 13 * 1024, "shared memory");  // beside it: the experts' first tiles
 };
 
 constexpr int kThreads = 192;
@@ -74,29 +74,32 @@ struct TileAt {
   bool again;       // other tiles read the same weights
 };
 
+// Where the experts' rows and tiles begin, in shared memory: [experts + 1] rows of y, tiles of TN rows, tiles of the image.
+struct Experts {
+  const int *rows, *tiles, *image;
+};
+
 template <int TN>
-__device__ __forceinline__ TileAt tile_at(const MxGemm& g, const int* first, int t) {
+__device__ __forceinline__ TileAt tile_at(const MxGemm& g, const Experts& x, int t) {
   TileAt r;
-  int e = 0, local = t, count;
-  int64_t rows = g.rows, base = 0, tile0 = 0;
+  int e = 0, local = t, rows = (int)g.rows, count = (rows + TN - 1) / TN, base = 0, tile0 = 0;
   if (g.offsets) {
-    int lo = 0, hi = g.experts;  // the expert whose tiles hold t: first[e] * row_tiles <= t < first[e + 1] * row_tiles
+    int lo = 0, hi = g.experts;  // the expert whose tiles hold t: tiles[e] * row_tiles <= t < tiles[e + 1] * row_tiles
+    const int nth = t / g.row_tiles;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((int64_t)first[mid] * g.row_tiles <= t) lo = mid;
+      if (x.tiles[mid] <= nth) lo = mid;
       else hi = mid;
     }
     e = lo;
-    local = t - first[e] * g.row_tiles;
-    count = first[e + 1] - first[e];
-    base = g.offsets[e], rows = g.offsets[e + 1] - base, tile0 = g.tiles[e];
-  } else {
-    count = (int)((rows + TN - 1) / TN);
+    local = t - x.tiles[e] * g.row_tiles;
+    count = x.tiles[e + 1] - x.tiles[e];
+    base = x.rows[e], rows = x.rows[e + 1] - base, tile0 = x.image[e];
   }
   // the tiles of the same weights follow one another, so that those are read from memory once
   const int rt = local / count, at = (local - rt * count) * TN;
   r.w_tile = (int64_t)e * g.row_tiles + rt, r.x_tile = tile0 + (at >> 7), r.sub = at & 127;
-  r.row0 = base + at, r.n = (int)min((int64_t)TN, rows - at), r.n0 = rt * kMxRows, r.again = count > 1;
+  r.row0 = base + at, r.n = min(TN, rows - at), r.n0 = rt * kMxRows, r.again = count > 1;
   return r;
 }
 
@@ -110,7 +113,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
   __shared__ int s_abort, s_tiles, s_warp[kThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
-  int* first = reinterpret_cast<int*>(smem_raw + C::kSmem);  // [experts + 1] tiles of TN rows before each expert's
+  int* table = reinterpret_cast<int*>(smem_raw + C::kSmem);
+  const Experts experts = {table, table + g.experts + 1, table + 2 * (g.experts + 1)};
   uint32_t rank = 0, ranks = 1;
   if (SPLIT) {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -131,9 +135,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
   if (!g.early) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (g.offsets) {  // sums of the experts' tiles, kThreads experts at a time
     int before = 0;
-    for (int e0 = 0; e0 < g.experts; e0 += kThreads) {
+    for (int e0 = 0; e0 <= g.experts; e0 += kThreads) {
       const int e = e0 + threadIdx.x;
-      const int rows = e < g.experts ? g.offsets[e + 1] - g.offsets[e] : 0, mine = (rows + TN - 1) / TN;
+      const int row = e <= g.experts ? g.offsets[e] : 0, rows = e < g.experts ? g.offsets[e + 1] - row : 0;
+      const int mine = (rows + TN - 1) / TN;
+      if (e <= g.experts) table[e] = row, table[2 * (g.experts + 1) + e] = g.tiles[e];
       int sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -148,11 +154,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
         if (i < warp) sum += s_warp[i];
         all += s_warp[i];
       }
-      if (e < g.experts) first[e] = before + sum - mine;
+      if (e < g.experts) table[g.experts + 1 + e] = before + sum - mine;
       before += all;
       __syncthreads();
     }
-    if (threadIdx.x == 0) first[g.experts] = before, s_tiles = before * g.row_tiles;
+    if (threadIdx.x == 0) table[2 * g.experts + 1] = before, s_tiles = before * g.row_tiles;
   } else if (threadIdx.x == 0) {
     s_tiles = (int)((g.rows + TN - 1) / TN) * g.row_tiles;
   }
@@ -176,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
   uint32_t it = 0, tile_count = 0;  // stages and tiles so far: the barriers' phases
   bool waited = !g.early;
   for (int t = start; t < tiles; t += step) {
-    const TileAt at = tile_at<TN>(g, first, t);
+    const TileAt at = tile_at<TN>(g, experts, t);
     if (warp == 0) {
       if (lane == 0 && ok) {
         const uint64_t once = evict_first_policy();
@@ -310,32 +316,36 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
     }
   }
 
-  // nothing of this CTA's is under way when it ends: its copies have landed and its products are done
-  if (warp == 0 && lane == 0) {
-    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (uint32_t i = it > S ? it - S : 0; i < it; ++i) mbar_wait(smem_addr(&b_full[i % S]), (i / S) & 1, kWaitLimit);
-  }
-  if (warp == 1 && lane == 0) {
-    tc::mma_commit(smem_addr(&b_end));
-    if (!mbar_wait(smem_addr(&b_end), 0, kWaitLimit)) atomicExch(&s_abort, 1);
-  }
+  // Nothing of this CTA's is under way when it ends: the epilogue has seen the last products, and so the last copies, unless a
+  // wait ran out.
+  if (warp == 0 && lane == 0 && !waited) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (threadIdx.x == 0 && s_abort) atomicCAS(&g_device_error, 0, kErrTimeout);
+  if (s_abort) {
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_device_error, 0, kErrTimeout);
+      for (uint32_t i = it > S ? it - S : 0; i < it; ++i) mbar_wait(smem_addr(&b_full[i % S]), (i / S) & 1, kWaitLimit);
+    }
+    if (threadIdx.x == 32) {
+      tc::mma_commit(smem_addr(&b_end));
+      mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
+    }
+    __syncthreads();
+  }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 template <int TN, bool SPLIT>
 int launch_tile(const MxGemm& g, int ctas, int ranks, cudaStream_t stream) {
   using C = MxTile<TN>;
-  const int smem = C::kSmem + (g.offsets ? (g.experts + 1) * 4 : 0);
+  const int smem = C::kSmem + (g.offsets ? (g.experts + 1) * 12 : 0);
   static std::atomic<unsigned long long> done{0};  // devices on which the kernel may take that much
   const auto kernel = mx_gemm_kernel<TN, SPLIT>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem + (kMaxExperts + 1) * 4);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem + (kMaxExperts + 1) * 12);
     if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return fail(B2Q_ECUDA, "mx_gemm: %s", cudaGetErrorString(e));

@@ -5,9 +5,10 @@
 // the scale's inverse, a power of two, is exact; the conversion rounds it once, to nearest even. A block with an infinity
 // or a NaN has s = 255, NaN.
 //
-// All three are one pass, bound by memory. Two threads take a block, values 8h .. 8h + 7 and 16 + 8h .. 16 + 8h + 7 (the two
-// nibbles of bytes 8h .. 8h + 7): 16-byte loads of 16-bit values whose pairs make whole 32-byte sectors, and one 8-byte
-// store each.
+// All three are one pass, bound by memory: a thread a block, values in runs of 32 bytes (a sector) where the rows are
+// aligned to them, else of 16, and 16 bytes of codes.
+#include <type_traits>
+
 #include "mx_device.cuh"
 
 namespace b2q {
@@ -29,49 +30,105 @@ int check_mx_rows(const char* who, const char* name, int dtype, const void* x, i
 
 namespace {
 
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  store4(p, v[0], v[1], v[2], v[3]);
-  store4(p + 4, v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  uint32_t w[4];
+// 16 values from `p` on as f32, and their largest magnitude's bits. WIDE: the address is a multiple of 32 bytes.
+template <bool WIDE, typename T>
+__device__ __forceinline__ uint32_t load16(const T* p, float (&a)[8], float (&b)[8]) {
+  if constexpr (!WIDE) return max(load8(p, a), load8(p + 8, b));
+  uint32_t w[8], m = 0;
+  load32(p, w);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    for (int i = 0; i < 8; ++i) a[i] = __uint_as_float(w[i]), m = max(m, w[i] & 0x7fffffffu);
+    load32(p + 8, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = __uint_as_float(w[i]), m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float* v = (i < 4 ? a : b) + 2 * (i & 3);
+      if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[0] = f.x, v[1] = f.y;
+      } else {
+        v[0] = __uint_as_float(w[i] << 16), v[1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+      m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    }
+    if constexpr (std::is_same_v<T, __half>)
+      return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))));
+    else
+      return max(m << 16, m & 0xffff0000u);
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A thread's place: half block `half` of block b of a stage of a row; 16 threads a stage.
+// 16 values to `p`.
+template <bool WIDE, typename T>
+__device__ __forceinline__ void store16(T* p, const float (&a)[8], const float (&b)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float(&v)[8] = h ? b : a;
+      if constexpr (WIDE)
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + 8 * h), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                     "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+      else
+        store4(p + 8 * h, v[0], v[1], v[2], v[3]), store4(p + 8 * h + 4, v[4], v[5], v[6], v[7]);
+    }
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = (i < 4 ? a : b)[2 * (i & 3)], y = (i < 4 ? a : b)[2 * (i & 3) + 1];
+      if constexpr (std::is_same_v<T, __half>) {
+        w[i] = pack_half2(x, y);
+      } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    if constexpr (WIDE) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                   "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    } else {
+      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(p + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+}
+
+// A thread's place: block b of a stage of a row; 8 threads a stage.
 struct Place {
   int64_t row;
-  int stage, b, half;
+  int stage, b;
 };
 __device__ __forceinline__ Place place_of(int64_t item, int stages) {
-  const int64_t s = item >> 4;
+  const int64_t s = item >> 3;
   const int64_t row = s < (1ll << 31) ? (int64_t)((uint32_t)s / (uint32_t)stages) : s / stages;
-  return {row, (int)(s - row * stages), (int)(item >> 1) & 7, (int)item & 1};
+  return {row, (int)(s - row * stages), (int)item & 7};
 }
 
-template <typename T>
+template <bool WIDE, typename T>
 __global__ void __launch_bounds__(256)
     mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int stages, uint8_t* __restrict__ image,
                        const int32_t* __restrict__ dest, int fan) {
   pdl_wait_then_trigger();
   const Place p = place_of((int64_t)blockIdx.x * 256 + threadIdx.x, stages);
-  const int at = p.stage * kMxStage + p.b * 32 + 8 * p.half;
-  const bool there = p.row < rows && at < K;  // K is a multiple of 32: a whole block is there, or none of it
-  MxHalf h;
-  h.load(x + p.row * ldx + at, there);
-  const uint32_t s = h.finish();
-  uint32_t scales = s << (8 * (p.b & 3));  // the 4 blocks of a word: 8 lanes of the same row
+  const int at = p.stage * kMxStage + p.b * 32;
+  uint32_t m = 0;
+  MxHalf h[2] = {};
+  if (p.row < rows && at < K) {  // K is a multiple of 32: a whole block is there, or none of it
+    const T* src = x + p.row * ldx + at;
+    m = load16<WIDE>(src, h[0].lo, h[1].lo);
+    m = max(m, load16<WIDE>(src + 16, h[0].hi, h[1].hi));
+  }
+  const uint32_t s = mx_scale_of(m);
+  h[0].encode(s), h[1].encode(s);
+  uint32_t scales = s << (8 * (p.b & 3));  // the 4 blocks of a word: 4 lanes of the same row
+  scales |= __shfl_xor_sync(0xffffffffu, scales, 1);
   scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
-  scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
   if (p.row >= rows) return;
   const int64_t first = dest ? p.row * fan : 0;
   for (int j = 0; j < fan; ++j) {
@@ -79,30 +136,32 @@ __global__ void __launch_bounds__(256)
     if (r < 0) continue;
     uint8_t* tile = image + ((r >> 7) * stages + p.stage) * kMxBytes;
     const int in = (int)r & 127;
-    *reinterpret_cast<uint2*>(tile + mx_code_at(in, p.b) + 8 * p.half) = h.codes;
-    if ((threadIdx.x & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_at(in, p.b)) = scales;
+    *reinterpret_cast<uint4*>(tile + mx_code_at(in, p.b)) = make_uint4(h[0].codes.x, h[0].codes.y, h[1].codes.x, h[1].codes.y);
+    if ((p.b & 3) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_at(in, p.b)) = scales;
   }
 }
 
-template <typename T>
+template <bool WIDE, typename T>
 __global__ void __launch_bounds__(256)
     mx_dequantize_kernel(const uint8_t* __restrict__ image, int64_t rows, int K, int stages, T* __restrict__ y, int64_t ldy) {
   pdl_wait_then_trigger();
   const Place p = place_of((int64_t)blockIdx.x * 256 + threadIdx.x, stages);
-  const int at = p.stage * kMxStage + p.b * 32 + 8 * p.half;
+  const int at = p.stage * kMxStage + p.b * 32;
   if (p.row >= rows || at >= K) return;
   const uint8_t* tile = image + ((p.row >> 7) * stages + p.stage) * kMxBytes;
   const int in = (int)p.row & 127;
-  const uint2 q = *reinterpret_cast<const uint2*>(tile + mx_code_at(in, p.b) + 8 * p.half);
+  const uint4 q = *reinterpret_cast<const uint4*>(tile + mx_code_at(in, p.b));
   const float d = mx_scale(tile[mx_scale_at(in, p.b)]);
-  float lo[8], hi[8];
-  from_e2m1x8(q.x, lo, hi, 0);
-  from_e2m1x8(q.y, lo, hi, 4);
+  float lo[2][8], hi[2][8];
+  from_e2m1x8(q.x, lo[0], hi[0], 0);
+  from_e2m1x8(q.y, lo[0], hi[0], 4);
+  from_e2m1x8(q.z, lo[1], hi[1], 0);
+  from_e2m1x8(q.w, lo[1], hi[1], 4);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) lo[i] *= d, hi[i] *= d;
+  for (int i = 0; i < 8; ++i) lo[0][i] *= d, hi[0][i] *= d, lo[1][i] *= d, hi[1][i] *= d;
   T* dst = y + p.row * ldy + at;
-  store8(dst, lo);
-  store8(dst + 16, hi);
+  store16<WIDE>(dst, lo[0], lo[1]);
+  store16<WIDE>(dst + 16, hi[0], hi[1]);
 }
 
 // Planes [experts][rows] of codes and scales into an image whose experts begin at whole tiles; rows beyond the last are zeros.
@@ -142,17 +201,19 @@ int launch_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int6
                        int fan, cudaStream_t stream) {
   const int stages = (int)mx_stages(K);
   unsigned grid;
-  int rc = grid_of("b2q_mx_quantize", rows * stages * 16, &grid);
+  int rc = grid_of("b2q_mx_quantize", rows * stages * 8, &grid);
   if (rc || rows == 0) return rc;
+  const bool wide = aligned(x, 32) && (rows == 1 || ldx * mx_dtype_size(dtype) % 32 == 0);
+  auto launch = [&](auto kernel, auto* p) {
+    launch_maybe_pdl(kernel, dim3(grid), dim3(256), 0, stream, p, ldx, rows, (int)K, stages, image, dest, fan);
+  };
   if (dtype == B2Q_DTYPE_F32)
-    launch_maybe_pdl(mx_quantize_kernel<float>, grid, 256, 0, stream, static_cast<const float*>(x), ldx, rows, (int)K, stages,
-                     image, dest, fan);
+    launch(wide ? mx_quantize_kernel<true, float> : mx_quantize_kernel<false, float>, static_cast<const float*>(x));
   else if (dtype == B2Q_DTYPE_F16)
-    launch_maybe_pdl(mx_quantize_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(x), ldx, rows, (int)K, stages,
-                     image, dest, fan);
+    launch(wide ? mx_quantize_kernel<true, __half> : mx_quantize_kernel<false, __half>, static_cast<const __half*>(x));
   else
-    launch_maybe_pdl(mx_quantize_kernel<__nv_bfloat16>, grid, 256, 0, stream, static_cast<const __nv_bfloat16*>(x), ldx, rows,
-                     (int)K, stages, image, dest, fan);
+    launch(wide ? mx_quantize_kernel<true, __nv_bfloat16> : mx_quantize_kernel<false, __nv_bfloat16>,
+           static_cast<const __nv_bfloat16*>(x));
   return after_launch("mx_quantize");
 }
 
@@ -192,15 +253,19 @@ int b2q_mx_dequantize(const uint8_t* image, int64_t rows, int64_t K, int dtype, 
     return fail(B2Q_EALIGN, "%s: y and its row stride must be 16-byte aligned, the image 128-byte", who);
   const int stages = (int)mx_stages(K);
   unsigned grid;
-  rc = grid_of(who, rows * stages * 16, &grid);
+  rc = grid_of(who, rows * stages * 8, &grid);
   if (rc) return rc;
+  const bool wide = aligned(y, 32) && (rows == 1 || ldy * mx_dtype_size(dtype) % 32 == 0);
+  auto launch = [&](auto kernel, auto* p) {
+    launch_maybe_pdl(kernel, dim3(grid), dim3(256), 0, stream, image, rows, (int)K, stages, p, ldy);
+  };
   if (dtype == B2Q_DTYPE_F32)
-    launch_maybe_pdl(mx_dequantize_kernel<float>, grid, 256, 0, stream, image, rows, (int)K, stages, static_cast<float*>(y), ldy);
+    launch(wide ? mx_dequantize_kernel<true, float> : mx_dequantize_kernel<false, float>, static_cast<float*>(y));
   else if (dtype == B2Q_DTYPE_F16)
-    launch_maybe_pdl(mx_dequantize_kernel<__half>, grid, 256, 0, stream, image, rows, (int)K, stages, static_cast<__half*>(y), ldy);
+    launch(wide ? mx_dequantize_kernel<true, __half> : mx_dequantize_kernel<false, __half>, static_cast<__half*>(y));
   else
-    launch_maybe_pdl(mx_dequantize_kernel<__nv_bfloat16>, grid, 256, 0, stream, image, rows, (int)K, stages,
-                     static_cast<__nv_bfloat16*>(y), ldy);
+    launch(wide ? mx_dequantize_kernel<true, __nv_bfloat16> : mx_dequantize_kernel<false, __nv_bfloat16>,
+           static_cast<__nv_bfloat16*>(y));
   return after_launch("mx_dequantize");
 }
 

@@ -12,6 +12,7 @@ kernels are this package's own, through the C-ABI (include/comp_b200.h, where la
 
 import torch
 
+from . import _lib
 from .kv import _call, _dtype_id, _on_device, _raw_stream
 from .mx import (FUSED_ROWS, MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _few_size, _out_dtype,
                  _rows, _stride)
@@ -28,7 +29,9 @@ class Plan:
         choices = tokens * top
         self.tokens, self.top, self.experts, self.device = tokens, top, experts, dev
         self.ids = self.weights = None
-        self._words = torch.empty(2 * (experts + 1) + 4 * choices, dtype=torch.int32, device=dev)
+        words = 2 * (experts + 1) + 4 * choices if tokens <= 128 and choices <= 4096 else \
+            _lib.load().b2q_experts_plan_words(tokens, top, experts)
+        self._words = torch.empty(words, dtype=torch.int32, device=dev)
 
     @property
     def offsets(self):
@@ -50,7 +53,7 @@ def _check_sizes(name, tokens, top, experts):
         raise ValueError(f"{name}: {experts} experts (1..{MAX_EXPERTS})")
     if not 1 <= top <= MAX_TOP:
         raise ValueError(f"{name}: {top} choices a token (1..{MAX_TOP})")
-    if tokens * top > 1 << 30:
+    if tokens * top > 1 << 26:
         raise ValueError(f"{name}: {tokens} tokens of {top} choices")
 
 

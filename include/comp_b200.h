@@ -417,12 +417,12 @@ int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int
 
 /*
  * The plan of a layer of experts: which of `experts` (1..1024) the `top` (1..32) choices of each token go to, sorted by
- * expert, and within one by token * top + choice. int32, one allocation of 2 (experts + 1) + 4 tokens * top words:
+ * expert, and within one by token * top + choice (2^26 choices at most). int32, one allocation of b2q_experts_plan_words words:
  *   offsets [experts + 1]    the sorted rows where each expert's begin
  *   tiles   [experts + 1]    the same in tiles of 128 rows, every expert from a whole tile on
  *   pos     [tokens * top]   the sorted row of each choice (-1: it goes nowhere)
  *   order   [tokens * top]   the choice of each sorted row (-1 from offsets[experts] on)
- *   dest, dest_row           rows of the operand image, by choice and by sorted row
+ *   dest, dest_row           rows of the operand image, by choice and by sorted row; then counts of a long list's parts
  *
  * b2q_experts_route: ids i32 [tokens][top] are the experts with the largest logits [tokens][experts] (dtype, row stride ld),
  * in falling order, the lowest index first among equals. -inf and NaN are never chosen: where fewer are left, id -1 and weight 0.
@@ -430,6 +430,7 @@ int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int
  * b2q_experts_sort: the plan of given ids i32 [tokens][top]; negative ids go nowhere, and so do ids beyond the experts, which
  * set the device error word to 5. A token may choose an expert twice.
  */
+size_t b2q_experts_plan_words(int64_t tokens, int64_t top, int64_t experts);
 int b2q_experts_route(int dtype, const void* logits, int64_t ld, int64_t tokens, int64_t experts, int64_t top, int normalize,
                       int32_t* ids, float* weights, int32_t* plan, b2q_stream_t stream);
 int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t experts, int32_t* plan, b2q_stream_t stream);

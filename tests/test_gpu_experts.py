@@ -60,11 +60,13 @@ def test_route_strides(cuda):
     x = torch.randn((200, 300), device=cuda)
     for v in (x[:, 7:90], x[::3, :64], x.T[:150, :100], x[:1].expand(9, 300)):
         a, b = experts.route(v, 4), experts.route(v.contiguous(), 4)
-        assert torch.equal(a.ids, b.ids) and torch.equal(a._words, b._words) and torch.equal(a.weights, b.weights)
+        for name in ("ids", "weights", "offsets", "pos", "order"):
+            assert torch.equal(getattr(a, name), getattr(b, name))
 
 
 @pytest.mark.parametrize("tokens,top,n", [(0, 1, 3), (1, 1, 1), (1, 8, 64), (7, 3, 5), (64, 8, 128), (1024, 4, 1000), (1025, 4, 17),
-                                          (4097, 1, 2), (3000, 10, 160), (20000, 8, 1024), (131072, 1, 7)])
+                                          (4097, 1, 2), (3000, 10, 160), (20000, 8, 1024), (131072, 1, 7),
+                                          (128, 32, 600), (4096, 1, 33), (600, 32, 1000), (300000, 8, 64)])
 def test_sort(cuda, tokens, top, n):
     rng = np.random.default_rng(tokens)
     ids = rng.integers(-1 if tokens % 2 else 0, n, (tokens, top))

@@ -32,6 +32,15 @@ def test_sizes(lib):
         assert (-(-counts // 128)).sum() * -(-k // 256) * 17408 <= size
 
 
+def test_plan_words(lib):
+    for t, top, e in ((0, 1, 1), (1, 8, 64), (128, 32, 1024), (129, 1, 5), (4097, 1, 5), (16384, 8, 256), (1 << 23, 8, 1024)):
+        words = lib.b2q_experts_plan_words(t, top, e)
+        plain = 2 * (e + 1) + 4 * t * top
+        assert words == plain if t <= 128 and t * top <= 4096 else words > plain and (words - plain) % e == 0
+    for bad in ((-1, 1, 1), (1, 0, 1), (1, 33, 64), (1, 1, 0), (1, 1, 1025), (1 << 26, 2, 4)):
+        assert lib.b2q_experts_plan_words(*bad) == 0 and "b2q_experts_plan_words" in _lib.last_error()
+
+
 def test_quantize_refusals(lib):
     q = lambda dtype=0, x=4096, ldx=64, rows=2, k=64, image=4096: lib.b2q_mx_quantize(dtype, x, ldx, rows, k, image, None)  # noqa: E731
     assert q(dtype=3) == -1 and q(x=None) == -1 and q(image=None) == -1 and q(rows=-1) == -1 and q(k=48) == -1 and q(ldx=32) == -1
@@ -61,7 +70,7 @@ def test_expert_refusals(lib):
         dtype, x, ld, t, e, top, 1, ids, w, plan, None)
     assert r(dtype=5) == -1 and r(x=None) == -1 and r(ld=7) == -1 and r(t=-1) == -1 and r(e=0) == -1 and r(e=1025, ld=2000) == -1
     assert r(top=0) == -1 and r(top=9) == -1 and r(top=33, e=64, ld=64) == -1 and r(ids=None) == -1 and r(w=None) == -1
-    assert r(plan=None) == -1 and r(plan=4098) == -2 and r(ids=4097) == -2 and r(x=4097) == -2 and r(t=1 << 30) == -4
+    assert r(plan=None) == -1 and r(plan=4098) == -2 and r(ids=4097) == -2 and r(x=4097) == -2 and r(t=1 << 26) == -4
     s = lambda ids=4096, t=2, top=2, e=8, plan=4096: lib.b2q_experts_sort(ids, t, top, e, plan, None)  # noqa: E731
     assert s(ids=None) == -1 and s(plan=None) == -1 and s(e=0) == -1 and s(top=33) == -1 and s(ids=4098) == -2
     f = lambda x=4096, ldx=64, w=4096, plan=4096, t=20, n=3, k=64, dtype=0, y=4096, ldy=3, ws=4096, size=1 << 20: (  # noqa: E731
