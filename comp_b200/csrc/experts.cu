@@ -5,9 +5,9 @@
 //
 // Sort: stable, by counting. The choices (token * top + j) are cut into runs, one a warp; a warp counts its run's experts 32
 // choices at a time (lanes with the same expert find each other with one match), the counts before each warp's run give
-// every choice its place, and a second walk over the run hands the places out. A short list is one CTA's work, routing
-// included: one launch, whose choices stay in shared memory. A long one is two: CTAs all over the GPU route and count their
-// tokens, then each adds up what the others before it counted and places its own. The order is the same every time.
+// every choice its place, and a second walk over the run hands the places out. A short list is one launch: a cluster routes
+// it and its first CTA, to which the others send their choices, places it. A long one is two: CTAs all over the GPU route and
+// count their tokens, then each adds up what the others before it counted and places its own. The order is always the same.
 //
 // Combine: a thread adds the same 32 bytes of a token's rows, in order of its choices, in f32: one pass, bound by memory.
 #include <algorithm>
@@ -21,6 +21,7 @@ namespace {
 
 constexpr int64_t kMostChoices = 1 << 26, kMostPart = 14000;  // in a plan; in a part, whose experts lie in shared memory
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kRun = 64;  // choices a warp counts, and places, at the least
 constexpr int kSmallChoices = 4096, kSmallTokens = 128;  // lists of up to so many are sorted, and routed, by one CTA
 
 struct PlanOut {
@@ -116,19 +117,37 @@ struct RouteArgs {
   float* weights;
 };
 
-// The tokens first .. end - 1 by the CTA's warps.
-template <int V, typename T>
-__device__ __forceinline__ void route_tokens(const RouteArgs& a, int experts, int64_t first, int64_t end, int32_t* kept) {
+// The tokens first, first + step, .. below end by this warp; keep(choice, expert) besides what is stored.
+template <int V, typename T, typename Keep>
+__device__ __forceinline__ void route_tokens(const RouteArgs& a, int experts, int64_t first, int64_t end, int64_t step, Keep keep) {
   const int lane = threadIdx.x & 31;
-  for (int64_t t = first + (threadIdx.x >> 5); t < end; t += blockDim.x >> 5) {
+  for (int64_t t = first; t < end; t += step) {
     int id;
     float w;
     route_token<V>(static_cast<const T*>(a.logits) + t * a.ld, experts, a.top, a.normalize, lane, &id, &w);
     if (lane < a.top) {
       a.ids[t * a.top + lane] = id, a.weights[t * a.top + lane] = w;
-      kept[(t - first) * a.top + lane] = id;
+      keep(t * a.top + lane, id);
     }
   }
+}
+
+__device__ __forceinline__ uint32_t cluster_address(uint32_t addr, uint32_t rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_ranks() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
 }
 
 // An expert's number, -1 for none.
@@ -170,7 +189,7 @@ __device__ __forceinline__ void place(Ids ids, Total total_of, int64_t first, in
                                       int* s_move, uint64_t* scratch, bool writes_totals, int64_t part, int64_t parts,
                                       const PlanOut& p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, all_warps = blockDim.x >> 5;
-  const int warps = min(all_warps, (int)((end - first + 31) >> 5));  // with runs of their own
+  const int warps = min(all_warps, (int)((end - first + kRun - 1) / kRun));  // with runs of their own
   const int64_t run = warps ? ((end - first + warps * 32 - 1) / (warps * 32)) * 32 : 0;
   const int64_t begin = min(end, first + warp * run), stop = warp < warps ? min(end, begin + run) : begin;
   int* mine = s_count + warp * experts;
@@ -219,47 +238,72 @@ __device__ __forceinline__ void place(Ids ids, Total total_of, int64_t first, in
     p.order[r] = -1, p.dest_row[r] = -1;
 }
 
-// A short list by one CTA. V > 0: routed first (logits of type T).
+// A short list. V > 0: the CTAs of a cluster route it (logits of type T); the first of them places it.
 template <int V, typename T>
 __global__ void __launch_bounds__(kSortThreads, 1)
     sort_small_kernel(const RouteArgs a, int choices, int experts, const PlanOut p) {
   extern __shared__ int s_mem[];  // [choices] ids, [experts] moves, [warps][experts] counts
   __shared__ uint64_t s_scratch[32];
   int *s_ids = s_mem, *s_move = s_ids + choices, *s_count = s_move + experts;
-  const int warps = min((int)blockDim.x >> 5, (choices + 31) >> 5);
-  for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) s_count[i] = 0;
+  const int warps = min((int)blockDim.x >> 5, (choices + kRun - 1) / kRun);
+  const uint32_t rank = cluster_rank(), ranks = cluster_ranks();
+  if (V > 0) cluster_arrive();
+  if (rank == 0)
+    for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) s_count[i] = 0;
   pdl_wait_then_trigger();
   if constexpr (V > 0) {
-    route_tokens<V, T>(a, experts, 0, choices / a.top, s_ids);
+    const uint32_t first = cluster_address(smem_addr(s_ids), 0);
+    cluster_wait();
+    route_tokens<V, T>(a, experts, rank * (blockDim.x >> 5) + (threadIdx.x >> 5), choices / a.top, ranks * (blockDim.x >> 5),
+                       [&](int64_t c, int id) {
+                         asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(first + (uint32_t)c * 4), "r"(id) : "memory");
+                       });
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
   } else {
     for (int i = threadIdx.x; i < choices; i += blockDim.x) s_ids[i] = checked(a.ids[i], experts);
+    __syncthreads();
   }
-  __syncthreads();
   place([&](int64_t i) { return s_ids[i]; }, [](int, int here, int* before, int* total) { *total = here; }, 0, choices, choices,
         experts, s_count, s_move, s_scratch, true, 0, 1, p);
 }
 
-// A long list's parts, `per` tokens each: routed and counted,
+// A long list's parts, `per` tokens each: routed and counted, each by the CTAs of a cluster,
 template <int V, typename T>
-__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const RouteArgs a, int64_t tokens, int per, int experts, const PlanOut p) {
-  extern __shared__ int s_mem[];  // [per * top] ids, [experts] counts
-  int *s_ids = s_mem, *s_count = s_ids + per * a.top;
+__global__ void __launch_bounds__(512) sort_count_kernel(const RouteArgs a, int64_t tokens, int per, int experts, const PlanOut p) {
+  extern __shared__ int s_count[];  // [experts]
   for (int i = threadIdx.x; i < experts; i += blockDim.x) s_count[i] = 0;
   pdl_wait_then_trigger();
-  const int64_t first = (int64_t)blockIdx.x * per, end = min(tokens, first + per);
-  const int n = (int)(end - first) * a.top;
+  __syncthreads();
+  const uint32_t rank = cluster_rank(), ranks = cluster_ranks();
+  const int64_t part = blockIdx.x / ranks, first = part * per, end = min(tokens, first + per);
+  auto count = [&](int64_t, int id) {
+    if (id >= 0) atomicAdd(&s_count[id], 1);  // (whole numbers: in any order)
+  };
   if constexpr (V > 0) {
-    route_tokens<V, T>(a, experts, first, end, s_ids);
+    route_tokens<V, T>(a, experts, first + rank * (blockDim.x >> 5) + (threadIdx.x >> 5), end, ranks * (blockDim.x >> 5), count);
   } else {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) s_ids[i] = a.ids[first * a.top + i];
+    for (int64_t i = first * a.top + rank * blockDim.x + threadIdx.x; i < end * a.top; i += ranks * blockDim.x)
+      count(i, checked(a.ids[i], experts));
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int id = checked(s_ids[i], experts);
-    if (id >= 0) atomicAdd(&s_count[id], 1);
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += blockDim.x) p.counts[(int64_t)blockIdx.x * experts + e] = s_count[e];
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0)
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+      int sum = s_count[e];
+      for (uint32_t r = 1; r < ranks; ++r) {
+        int c;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(cluster_address(smem_addr(s_count + e), r)) : "memory");
+        sum += c;
+      }
+      p.counts[part * experts + e] = sum;
+    }
+  __syncwarp();
+  cluster_arrive();  // the others' counts are read before they end
+  cluster_wait();
 }
 
 // then placed. As many threads as experts at the least.
@@ -270,7 +314,7 @@ __global__ void __launch_bounds__(kSortThreads, 1)
   int *s_ids = s_mem, *s_move = s_ids + per * top, *s_before = s_move + experts, *s_total = s_before + experts;
   int* s_count = s_total + experts;
   const int64_t first = (int64_t)blockIdx.x * per, end = min(tokens, first + per);
-  const int n = (int)(end - first) * top, warps = min((int)blockDim.x >> 5, (n + 31) >> 5);
+  const int n = (int)(end - first) * top, warps = min((int)blockDim.x >> 5, (n + kRun - 1) / kRun);
   for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) s_count[i] = 0;
   for (int e = threadIdx.x; e < experts; e += blockDim.x) s_before[e] = s_total[e] = 0;
   pdl_wait_then_trigger();
@@ -284,7 +328,7 @@ __global__ void __launch_bounds__(kSortThreads, 1)
   if (group < groups) {
     const int e = threadIdx.x - group * experts;
     int before = 0, total = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int q = group; q < parts; q += groups) {
       const int c = p.counts[(int64_t)q * experts + e];
       total += c;
@@ -406,9 +450,9 @@ struct Parts {
   int per, count;
 };
 Parts parts_of(int64_t tokens, int64_t top) {
-  // some 1000 choices a CTA, but no more of them than fill a GPU (the counts are [parts][experts], and every CTA reads them)
+  // some 1000 choices or 128 tokens a CTA, but no more of them than fill a GPU (the counts are [parts][experts], and every CTA reads them)
   const int64_t choices = tokens * top;
-  const int64_t want = std::max({(int64_t)1, std::min<int64_t>(choices / 1024, 144), (choices + kMostPart - 1) / kMostPart});
+  const int64_t want = std::max({(int64_t)1, std::min<int64_t>(std::max(choices / 1024, tokens / 128), 144), (choices + kMostPart - 1) / kMostPart});
   const int64_t per = (tokens + want - 1) / want;
   return {(int)per, (int)((tokens + per - 1) / per)};
 }
@@ -429,32 +473,50 @@ int allow_smem(Kernel kernel, int most, std::atomic<unsigned long long>& done) {
   return e == cudaSuccess ? B2Q_OK : fail(B2Q_ECUDA, "experts: %s", cudaGetErrorString(e));
 }
 
+template <typename... KArgs, typename... Args>
+int launch_cluster(const char* who, void (*kernel)(KArgs...), int grid, int ranks, int threads, size_t smem, cudaStream_t stream,
+                   Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  return after_launch(who);
+}
+
 constexpr int kSortSmem = 220 * 1024;
 static_assert((kMostPart + kMaxTop + kMaxExperts * (3 + kSortWarps)) * 4 <= kSortSmem, "a part's experts and counts");
 
 template <int V, typename T>
 int route_and_sort(const RouteArgs& a, int64_t tokens, int experts, const PlanOut& p, cudaStream_t stream) {
   const int64_t choices = tokens * a.top;
-  static std::atomic<unsigned long long> done_small{0}, done_count{0}, done_place{0};
+  static std::atomic<unsigned long long> done_small{0}, done_place{0};
   if (is_small(tokens, a.top, V > 0)) {
-    // warps with runs of 32 choices each, a warp a token, a thread an expert
-    const int warps = std::min<int>(kSortWarps, std::max<int>((int)(choices + 31) / 32, 1));
-    const int need = std::max(std::max(warps, V > 0 ? (int)tokens : 0), (experts + 31) / 32);
-    const int threads = std::min(kSortThreads, need * 32);
-    const size_t smem = (size_t)(choices + experts + std::min<int64_t>(threads / 32, (choices + 31) / 32) * experts) * 4;
+    // A warp a run and a thread an expert in the CTA that places; routing, a cluster of up to 8 with some 8 tokens each (one
+    // CTA takes 64 tokens of 128 experts, 8 choices each, in 7 us, 4 of them the issue of its instructions).
+    const int ranks = V == 0 ? 1 : tokens > 32 ? 8 : tokens > 8 ? 4 : 1;
+    const int runs = (int)(choices + kRun - 1) / kRun, routing = V > 0 ? (int)(tokens + ranks - 1) / ranks : 8;
+    const int threads = std::min(kSortThreads, std::max({runs, routing, (experts + 31) / 32, 1}) * 32);
+    const size_t smem = (size_t)(choices + experts + std::min(threads / 32, runs) * experts) * 4;
     int rc = allow_smem(sort_small_kernel<V, T>, kSortSmem, done_small);
     if (rc) return rc;
-    launch_maybe_pdl(sort_small_kernel<V, T>, dim3(1), dim3(threads), smem, stream, a, (int)choices, experts, p);
-    return after_launch("experts_sort");
+    return launch_cluster("experts_sort", sort_small_kernel<V, T>, ranks, ranks, threads, smem, stream, a, (int)choices, experts, p);
   }
   const Parts q = parts_of(tokens, a.top);
-  const size_t ids = (size_t)q.per * a.top * 4;
-  const size_t smem_count = ids + (size_t)experts * 4, smem_place = ids + (size_t)experts * (3 + kSortWarps) * 4;
-  int rc = allow_smem(sort_count_kernel<V, T>, kSortSmem, done_count);
-  if (!rc) rc = allow_smem(sort_place_kernel, kSortSmem, done_place);
+  const size_t smem_place = ((size_t)q.per * a.top + (size_t)experts * (3 + kSortWarps)) * 4;
+  int rc = allow_smem(sort_place_kernel, kSortSmem, done_place);
   if (rc) return rc;
-  launch_maybe_pdl(sort_count_kernel<V, T>, dim3(q.count), dim3(kSortThreads), smem_count, stream, a, tokens, q.per, experts, p);
-  rc = after_launch("experts_count");
+  const int ranks = V > 0 ? 4 : 1;
+  rc = launch_cluster("experts_count", sort_count_kernel<V, T>, q.count * ranks, ranks, 512, (size_t)experts * 4, stream, a, tokens, q.per,
+                      experts, p);
   if (rc) return rc;
   launch_maybe_pdl(sort_place_kernel, dim3(q.count), dim3(kSortThreads), smem_place, stream, a.ids, a.top, tokens, q.per, experts, p);
   return after_launch("experts_sort");

@@ -111,9 +111,13 @@ struct MxHalf {
       largest = load8(p, lo);
       largest = max(largest, load8(p + 16, hi));
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
+      clear();
     }
+  }
+  __device__ __forceinline__ void clear() {
+    largest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
   }
   // (s: the scale; codes of a block that is NaN are zeros)
   __device__ __forceinline__ void encode(uint32_t s) {

@@ -19,7 +19,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "mx_tc.cuh"
+#include "mx_tiles.cuh"
 
 namespace b2q {
 
@@ -50,57 +50,12 @@ __device__ __forceinline__ void arrive_bar(uint32_t bar) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t there;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-  return v;
-}
 // 32 consecutive columns of this thread's lane
 __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&a)[16], uint32_t (&b)[16]) {
   tc::tmem_ld16_nowait(taddr, a);
   tc::tmem_ld16_nowait(taddr + 16, b);
   tc::tmem_wait_ld_regs(a);
   tc::regs_ready(b);
-}
-
-// A tile: its weight rows, its rows of y, and where its rows of x lie in the image.
-struct TileAt {
-  int64_t w_tile;   // 128-row tile of the weight image
-  int64_t x_tile;   // 128-row tile of the image of x that holds its first row
-  int64_t row0;     // first row of y
-  int sub, n, n0;   // first row within x_tile, rows, first column of y
-  bool again;       // other tiles read the same weights
-};
-
-// Where the experts' rows and tiles begin, in shared memory: [experts + 1] rows of y, tiles of TN rows, tiles of the image.
-struct Experts {
-  const int *rows, *tiles, *image;
-};
-
-template <int TN>
-__device__ __forceinline__ TileAt tile_at(const MxGemm& g, const Experts& x, int t) {
-  TileAt r;
-  int e = 0, local = t, rows = (int)g.rows, count = (rows + TN - 1) / TN, base = 0, tile0 = 0;
-  if (g.offsets) {
-    int lo = 0, hi = g.experts;  // the expert whose tiles hold t: tiles[e] * row_tiles <= t < tiles[e + 1] * row_tiles
-    const int nth = t / g.row_tiles;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (x.tiles[mid] <= nth) lo = mid;
-      else hi = mid;
-    }
-    e = lo;
-    local = t - x.tiles[e] * g.row_tiles;
-    count = x.tiles[e + 1] - x.tiles[e];
-    base = x.rows[e], rows = x.rows[e + 1] - base, tile0 = x.image[e];
-  }
-  // the tiles of the same weights follow one another, so that those are read from memory once
-  const int rt = local / count, at = (local - rt * count) * TN;
-  r.w_tile = (int64_t)e * g.row_tiles + rt, r.x_tile = tile0 + (at >> 7), r.sub = at & 127;
-  r.row0 = base + at, r.n = min(TN, rows - at), r.n0 = rt * kMxRows, r.again = count > 1;
-  return r;
 }
 
 template <int TN, bool SPLIT>
@@ -114,7 +69,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
   int* table = reinterpret_cast<int*>(smem_raw + C::kSmem);
-  const Experts experts = {table, table + g.experts + 1, table + 2 * (g.experts + 1)};
   uint32_t rank = 0, ranks = 1;
   if (SPLIT) {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -133,35 +87,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (!g.early) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (g.offsets) {  // sums of the experts' tiles, kThreads experts at a time
-    int before = 0;
-    for (int e0 = 0; e0 <= g.experts; e0 += kThreads) {
-      const int e = e0 + threadIdx.x;
-      const int row = e <= g.experts ? g.offsets[e] : 0, rows = e < g.experts ? g.offsets[e + 1] - row : 0;
-      const int mine = (rows + TN - 1) / TN;
-      if (e <= g.experts) table[e] = row, table[2 * (g.experts + 1) + e] = g.tiles[e];
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      if (lane == 31) s_warp[warp] = sum;
-      __syncthreads();
-      int all = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) {
-        if (i < warp) sum += s_warp[i];
-        all += s_warp[i];
-      }
-      if (e < g.experts) table[g.experts + 1 + e] = before + sum - mine;
-      before += all;
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) table[2 * g.experts + 1] = before, s_tiles = before * g.row_tiles;
-  } else if (threadIdx.x == 0) {
-    s_tiles = (int)((g.rows + TN - 1) / TN) * g.row_tiles;
-  }
+  const int units = g.row_tiles;
+  const Experts experts = count_tiles<TN, kThreads>(g, table, s_warp, &s_tiles, units);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -174,71 +101,77 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   bool ok = true;
-  auto wait_one = [&](uint64_t* bar, uint32_t phase) {
-    if (ok && !mbar_wait(smem_addr(bar), phase & 1, kWaitLimit)) ok = false, atomicExch(&s_abort, 1);
+  // a wait that ran out ends the role's work: every later one is skipped
+  auto wait_warp = [&](uint64_t* bar, uint32_t phase) {
+    if (ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_addr(bar), phase & 1, kWaitLimit));
+      if (!ok) atomicExch(&s_abort, 1);
+    }
     return ok;
   };
 
   uint32_t it = 0, tile_count = 0;  // stages and tiles so far: the barriers' phases
   bool waited = !g.early;
   for (int t = start; t < tiles; t += step) {
-    const TileAt at = tile_at<TN>(g, experts, t);
+    const TileAt at = tile_at<TN>(g, experts, t, units);
     if (warp == 0) {
-      if (lane == 0 && ok) {
-        const uint64_t once = evict_first_policy();
-        uint64_t keep;
-        asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
-        const uint64_t w_policy = at.again ? keep : once;
-        const int parts = (at.n + 127) >> 7;
-        // of the rows' codes no more than the products read (which is up to 8 rows more, left from other stages)
-        const uint32_t codes = (uint32_t)((at.n + 7) & ~7) * 128, bytes = kMxBytes + codes + parts * 1024;
-        const uint8_t* w = g.w + at.w_tile * g.stages * kMxBytes;
-        const uint8_t* x = g.x + at.x_tile * g.stages * kMxBytes;
-        auto copy_x = [&](uint32_t stage, uint32_t bar, int k) {
-          const uint8_t* src = x + (int64_t)k * kMxBytes;
-          for (int i = 0; i < parts; ++i, src += (int64_t)g.stages * kMxBytes) {
-            bulk_g2s(stage + kMxBytes + i * kMxCodes, src + at.sub * 128, min(codes - i * kMxCodes, (uint32_t)kMxCodes), bar, keep);
-            bulk_g2s(stage + kMxBytes + C::kXCodes + i * 1024, src + kMxCodes, 1024, bar, keep);
-          }
-        };
-        int k = k0;
-        if (!waited) {  // the weights of the first stages do not depend on the preceding kernel
-          const int ahead = min(S, k1 - k0);
+      const uint64_t once = evict_first_policy();
+      uint64_t keep;
+      asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
+      const uint64_t w_policy = at.again ? keep : once;
+      const int parts = (at.n + 127) >> 7;
+      // of the rows' codes no more than the products read (which is up to 8 rows more, left from other stages)
+      const uint32_t codes = (uint32_t)((at.n + 7) & ~7) * 128, bytes = kMxBytes + codes + parts * 1024;
+      const uint8_t* w = g.w + ((int64_t)at.e * units + at.rt) * g.stages * kMxBytes;
+      const uint8_t* x = g.x + (int64_t)at.x_tile * g.stages * kMxBytes;
+      auto copy_x = [&](uint32_t stage, uint32_t bar, int k) {
+        const uint8_t* src = x + (int64_t)k * kMxBytes;
+        for (int i = 0; i < parts; ++i, src += (int64_t)g.stages * kMxBytes) {
+          bulk_g2s(stage + kMxBytes + i * kMxCodes, src + at.sub * 128, min(codes - i * kMxCodes, (uint32_t)kMxCodes), bar, keep);
+          bulk_g2s(stage + kMxBytes + C::kXCodes + i * 1024, src + kMxCodes, 1024, bar, keep);
+        }
+      };
+      int k = k0;
+      if (!waited) {  // the weights of the first stages do not depend on the preceding kernel
+        const int ahead = min(S, k1 - k0);
+        if (elect_one())
           for (int i = 0; i < ahead; ++i) {
             const uint32_t bar = smem_addr(&b_full[i]);
             mbar_expect_tx(bar, bytes);
             bulk_g2s(ring + i * C::kStageBytes, w + (int64_t)(k0 + i) * kMxBytes, kMxBytes, bar, w_policy);
           }
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          waited = true;
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        waited = true;
+        if (elect_one())
           for (int i = 0; i < ahead; ++i) copy_x(ring + i * C::kStageBytes, smem_addr(&b_full[i]), k0 + i);
-          it = ahead, k = k0 + ahead;
-        }
-        for (; k < k1; ++k, ++it) {
-          const uint32_t s = it % S, bar = smem_addr(&b_full[s]), stage = ring + s * C::kStageBytes;
-          if (it >= S && !wait_one(&b_empty[s], it / S - 1)) break;
+        it = ahead, k = k0 + ahead;
+      }
+      for (; k < k1; ++k, ++it) {
+        const uint32_t s = it % S, bar = smem_addr(&b_full[s]), stage = ring + s * C::kStageBytes;
+        if (it >= S && !wait_warp(&b_empty[s], it / S - 1)) break;
+        if (elect_one()) {
           mbar_expect_tx(bar, bytes);
           bulk_g2s(stage, w + (int64_t)k * kMxBytes, kMxBytes, bar, w_policy);
           copy_x(stage, bar, k);
         }
+        __syncwarp();
       }
-      __syncwarp();
     } else if (warp == 1) {
-      if (lane == 0 && ok) {
-        const uint32_t buf = tile_count & 1, acc = tmem + buf * C::kSecond;
-        // 256 columns: the previous tile's epilogue has read the columns that both share; else: the last but one is done
-        if (TN == 256 ? tile_count >= 1 : tile_count >= 2) {
-          const uint32_t before = tile_count - (TN == 256 ? 1 : 2);
-          wait_one(&b_free[before & 1], before >> 1);
-        }
+      const uint32_t buf = tile_count & 1, acc = tmem + buf * C::kSecond;
+      // 256 columns: the previous tile's epilogue has read the columns that both share; else: the last but one is done
+      if (TN == 256 ? tile_count >= 1 : tile_count >= 2) {
+        const uint32_t before = tile_count - (TN == 256 ? 1 : 2);
+        wait_warp(&b_free[before & 1], before >> 1);
+      }
+      tc::fence_after();
+      const int n = (at.n + 15) & ~15;
+      const uint32_t desc[2] = {instr_desc_mxf4(n, 0), instr_desc_mxf4(n, 1)};
+      const uint32_t column = TN == 64 ? (uint32_t)at.sub >> 5 : 0;  // where the tile's scales begin: 0 or 2
+      for (int k = k0; k < k1; ++k, ++it) {
+        const uint32_t s = it % S, stage = ring + s * C::kStageBytes;
+        if (!wait_warp(&b_full[s], it / S)) break;
         tc::fence_after();
-        const int n = (at.n + 15) & ~15;
-        const uint32_t desc[2] = {instr_desc_mxf4(n, 0), instr_desc_mxf4(n, 1)};
-        const uint32_t column = TN == 64 ? (uint32_t)at.sub >> 5 : 0;  // where the tile's scales begin: 0 or 2
-        for (int k = k0; k < k1 && ok; ++k, ++it) {
-          const uint32_t s = it % S, stage = ring + s * C::kStageBytes;
-          if (!wait_one(&b_full[s], it / S)) break;
-          tc::fence_after();
+        if (elect_one()) {
           const uint32_t sw = tmem + C::kScaleCol + (it & 1) * C::kScaleSet, sx = sw + 8;
           const uint32_t x_scales = stage + kMxBytes + C::kXCodes;
 #pragma unroll
@@ -254,18 +187,15 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
             mma_mxf4(acc, da + j * 2, db + j * 2, desc[j & 1], sw + (j >> 1) * 4, sx + (j >> 1) * 4 * C::kParts + column,
                      k > k0 || j > 0);
           tc::mma_commit(smem_addr(&b_empty[s]));
+          if (k == k1 - 1) tc::mma_commit(smem_addr(&b_acc[buf]));
         }
-        tc::mma_commit(smem_addr(&b_acc[buf]));
+        __syncwarp();
       }
-      __syncwarp();
     } else {
       const uint32_t buf = tile_count & 1, lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t acc = tmem + lanes + buf * C::kSecond;
-      const int in = (warp & 3) * 32 + lane, n = at.n0 + in;
-      if (ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_addr(&b_acc[buf]), (tile_count >> 1) & 1, kWaitLimit));
-        if (!ok) atomicExch(&s_abort, 1);
-      }
+      const int in = (warp & 3) * 32 + lane, n = at.rt * kMxRows + in;
+      wait_warp(&b_acc[buf], tile_count >> 1);
       tc::fence_after();
       if (ok) {
         // in the order in which the next tile's products need the columns: the first accumulator's last 64 first
@@ -286,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
               for (int c = 0; c < 32; ++c)
                 asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + c * 512), "r"(v[c >> 4][c & 15]) : "memory");
             } else if (n < g.N) {
-              const int64_t to = (at.row0 + c0) * g.ldy + n;
+              const int64_t to = (int64_t)(at.row0 + c0) * g.ldy + n;
 #pragma unroll
               for (int c = 0; c < 32; ++c)
                 if (c0 + c < at.n) store_as(g.y, to + c * g.ldy, g.dtype, __uint_as_float(v[c >> 4][c & 15]));
@@ -303,12 +233,24 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
     if constexpr (SPLIT) {
       cluster_sync();
       if (warp >= 2) {
-        const int in = (warp - 2) * 32 + lane, n = at.n0 + in;
+        const int in = (warp - 2) * 32 + lane, n = at.rt * kMxRows + in;
         const int c1 = (int)(at.n * (rank + 1) / ranks);
-        for (int c = (int)(at.n * rank / ranks); c < c1; ++c) {
-          float sum = 0.f;
-          for (uint32_t r = 0; r < ranks; ++r) sum += ld_cluster(ring + (c * 128 + in) * 4, r);
-          if (n < g.N && !s_abort) store_as(g.y, (at.row0 + c) * g.ldy + n, g.dtype, sum);
+        for (int c = (int)(at.n * rank / ranks); c < c1; c += 8) {  // eight columns' loads are under way at a time
+          float sum[8] = {};
+          for (uint32_t r = 0; r < ranks; ++r) {
+            float part[8];
+            uint32_t there;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(ring + (c * 128 + in) * 4), "r"(r));
+#pragma unroll
+            for (int i = 0; i < 8; ++i)  // (past the last column: inside the ring still)
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[i]) : "r"(there + i * 512) : "memory");
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += part[i];
+          }
+          if (n < g.N && !s_abort)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (c + i < c1) store_as(g.y, (int64_t)(at.row0 + c + i) * g.ldy + n, g.dtype, sum[i]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring's next stages come through the other proxy
@@ -318,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
 
   // Nothing of this CTA's is under way when it ends: the epilogue has seen the last products, and so the last copies, unless a
   // wait ran out.
-  if (warp == 0 && lane == 0 && !waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (warp == 0 && !waited) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc::fence_before();
   __syncthreads();
   tc::fence_after();

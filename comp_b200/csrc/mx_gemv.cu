@@ -1,10 +1,14 @@
-// MXFP4 products of up to 16 rows (the next tokens of a few sequences), quantizing the rows on the way: one launch.
+// MXFP4 products of up to 4 rows (the next tokens of a few sequences), quantizing the rows on the way: one launch.
 //
 // What counts here is the stream of weights, 17/32 byte a value, and what a launch costs before and after it. As in mx_gemm.cu
 // a CTA's tile is 128 weight rows, whose stages of 256 values of K one thread copies into a ring and another one multiplies;
 // but all rows of x stay in shared memory, and their scales in tensor memory, for as long as the CTA lives: eight warps quantize
-// them there while the first weights are on their way. Before it waits for the preceding kernel a CTA asks for its first
-// weights to be brought into L2; that is only a hint, so that it does no harm where the preceding kernel writes them.
+// them there while the first weights are on their way. (Asking for those to be brought into L2 before waiting for the
+// preceding kernel, a hint that could do no harm, was slower: 8192 x 8192 10.9 us, 9.7 without.)
+//
+// Every CTA reads all rows as they are given, four times the bytes of their codes, from the same lines of L2: 0.5 us a row.
+// Measured against quantizing first and multiplying then, us: 8192 x 8192 with 1 / 2 / 4 / 8 / 16 rows 9.7 / 10.5 / 11.7 / 14.2 / 19.4
+// and 11.9 / 12.1 / 12.1 / 12.2 / 12.2; 4096 x 4096 5.4 / 5.6 / 5.8 / 7.0 / 8.9 and 7.5 / 7.7 / 7.8 / 7.9 / 7.9. So up to 4.
 //
 // A layer of experts needs no gathering: every expert that has rows is multiplied with all rows of x (the unit's other side
 // is 16 rows at the least), and of the results only those that its choices ask for are stored.
@@ -22,7 +26,8 @@ namespace {
 
 constexpr int kThreads = 320;                   // copying, multiplying, then 8 warps that quantize, 4 of which store
 constexpr int kMaxRing = 8;
-constexpr int kMaxChoices = 128;                // rows of y that a layer of experts makes of the up to 16 of x
+constexpr int kMaxRows = 4, kXStage = 8 * 128;  // rows of x; bytes of a stage of them, a whole group of 8
+constexpr int kMaxChoices = 128;                // rows of y that a layer of experts makes of them
 constexpr uint32_t kScaleW = 32, kScaleX = 48;  // columns: accumulators 2 x 16, weight scales 2 x 8, then 4 a stage of x
 
 struct Gemv {
@@ -34,7 +39,6 @@ struct Gemv {
   int rows, K, N, row_tiles, stages, experts, dtype;
   int top;      // choices a token where x has a row a token, else 0
   int ring;     // stages of weights in shared memory
-  int rows8;    // rows of x there, in whole groups of 8
   int columns;  // of tensor memory
 };
 
@@ -51,9 +55,9 @@ __device__ __forceinline__ GemvTile gemv_tile(const Gemv& g, const int* used, co
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
-  extern __shared__ uint8_t smem_raw[];  // ring [ring][kMxBytes], x codes [stages][rows8 * 128], x scales [stages][512]
+  extern __shared__ uint8_t smem_raw[];  // ring [ring][kMxBytes], x codes [stages + 1][kXStage], x scales [stages][512]
   __shared__ uint64_t b_full[kMaxRing], b_empty[kMaxRing], b_acc[2], b_free[2], b_x, b_part, b_end;
-  __shared__ float s_part[16][kMxRows];  // the parts of the rows of x whose sums this CTA makes: [row / ranks * ranks + rank]
+  __shared__ float s_part[8][kMxRows];  // the parts of the rows of x whose sums this CTA makes: [row / ranks * ranks + rank]
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_count, s_used[kMaxChoices], s_offsets[kMaxChoices + 1];
   __shared__ uint8_t s_token[kMaxChoices];  // the row of x of each row of y
@@ -65,8 +69,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   const int k0 = (int)((int64_t)g.stages * rank / ranks), k1 = (int)((int64_t)g.stages * (rank + 1) / ranks), nk = k1 - k0;
   const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
   uint8_t* x_mem = smem_raw + (ring - smem_addr(smem_raw)) + g.ring * kMxBytes;
-  // (the products read 16 rows: with rows8 = 8 the next stage's for the second half, after the last stage a gap of 8)
-  const int x_bytes = (nk * g.rows8 + 16 - g.rows8) * 128;
+  // (the products read 16 rows: the next stage's for the second half, after the last stage a gap)
+  const int x_bytes = (nk + 1) * kXStage;
   const uint32_t x_codes = ring + g.ring * kMxBytes, x_scales = x_codes + x_bytes;
 
   if (warp == 0 && lane == 0) {
@@ -75,10 +79,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     mbar_init(smem_addr(&b_x), 256), mbar_init(smem_addr(&b_part), 1), mbar_init(smem_addr(&b_end), 1);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (!g.offsets && start < g.row_tiles) {
-      const uint8_t* w = g.w + ((int64_t)start * g.stages + k0) * kMxBytes;
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(w), "r"(min(nk, 16) * kMxBytes) : "memory");
-    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
@@ -109,10 +109,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   const uint32_t tmem = s_tmem;
   const int tiles = g.offsets ? s_count * g.row_tiles : g.row_tiles;
   bool ok = true;
-  auto wait_one = [&](uint64_t* bar, uint32_t phase) {
-    if (ok && !mbar_wait(smem_addr(bar), phase & 1, kWaitLimit)) ok = false, atomicExch(&s_abort, 1);
-    return ok;
-  };
   auto wait_warp = [&](uint64_t* bar, uint32_t phase) {
     if (ok) {
       ok = __all_sync(0xffffffffu, mbar_wait(smem_addr(bar), phase & 1, kWaitLimit));
@@ -122,69 +118,80 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   };
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t once = evict_first_policy();
-      uint32_t s = 0, round = 0;
-      for (int t = start; t < tiles && ok; t += step) {
-        const GemvTile at = gemv_tile(g, s_used, s_offsets, t);
-        const uint8_t* w = g.w + (at.w_tile * g.stages + k0) * kMxBytes;
-        for (int k = 0; k < nk; ++k, w += kMxBytes) {
-          if (round && !wait_one(&b_empty[s], round - 1)) break;
+    const uint64_t once = evict_first_policy();
+    uint32_t s = 0, round = 0;
+    for (int t = start; t < tiles && ok; t += step) {
+      const GemvTile at = gemv_tile(g, s_used, s_offsets, t);
+      const uint8_t* w = g.w + (at.w_tile * g.stages + k0) * kMxBytes;
+      for (int k = 0; k < nk; ++k, w += kMxBytes) {
+        if (round && !wait_warp(&b_empty[s], round - 1)) break;
+        if (elect_one()) {
           const uint32_t bar = smem_addr(&b_full[s]);
           mbar_expect_tx(bar, kMxBytes);
           bulk_g2s(ring + s * kMxBytes, w, kMxBytes, bar, once);
-          if (++s == (uint32_t)g.ring) s = 0, ++round;
         }
+        __syncwarp();
+        if (++s == (uint32_t)g.ring) s = 0, ++round;
       }
-      // (after a wait that ran out: what is still under way lands before the CTA ends)
-      if (!ok)
-        for (uint32_t i = 0; i < (uint32_t)g.ring; ++i)
-          if (round || i < s) mbar_wait(smem_addr(&b_full[i]), (i < s ? round : round - 1) & 1, kWaitLimit);
     }
+    // (after a wait that ran out: what is still under way lands before the CTA ends)
+    if (!ok)
+      for (uint32_t i = 0; i < (uint32_t)g.ring; ++i)
+        if (round || i < s) mbar_wait(smem_addr(&b_full[i]), (i < s ? round : round - 1) & 1, kWaitLimit);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && start < tiles) {
+    if (start < tiles) {
       const uint32_t desc[2] = {instr_desc_mxf4(16, 0), instr_desc_mxf4(16, 1)};
-      wait_one(&b_x, 0);
-      for (int k = 0; k < nk && ok; ++k) copy_scales(tmem + kScaleX + 4 * k, x_scales + k * 512);
+      wait_warp(&b_x, 0);
+      tc::fence_after();
+      if (ok && elect_one())
+        for (int k = 0; k < nk; ++k) copy_scales(tmem + kScaleX + 4 * k, x_scales + k * 512);
+      __syncwarp();
       uint32_t s = 0, round = 0, it = 0, count = 0;
       for (int t = start; t < tiles && ok; t += step, ++count) {
         const uint32_t buf = count & 1, acc = tmem + buf * 16;
-        if (count >= 2) wait_one(&b_free[buf], (count >> 1) - 1);
+        if (count >= 2) wait_warp(&b_free[buf], (count >> 1) - 1);
         tc::fence_after();
-        for (int k = 0; k < nk && ok; ++k, ++it) {
-          if (!wait_one(&b_full[s], round)) break;
+        for (int k = 0; k < nk; ++k, ++it) {
+          if (!wait_warp(&b_full[s], round)) break;
           tc::fence_after();
-          const uint32_t stage = ring + s * kMxBytes, sw = tmem + kScaleW + (it & 1) * 8, sx = tmem + kScaleX + 4 * k;
-          copy_scales(sw, stage + kMxCodes);
-          copy_scales(sw + 4, stage + kMxCodes + 512);
-          const uint64_t da = desc_swizzled(stage), db = desc_swizzled(x_codes + k * g.rows8 * 128);
+          if (elect_one()) {
+            const uint32_t stage = ring + s * kMxBytes, sw = tmem + kScaleW + (it & 1) * 8, sx = tmem + kScaleX + 4 * k;
+            copy_scales(sw, stage + kMxCodes);
+            copy_scales(sw + 4, stage + kMxCodes + 512);
+            const uint64_t da = desc_swizzled(stage), db = desc_swizzled(x_codes + k * kXStage);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_mxf4(acc, da + j * 2, db + j * 2, desc[j & 1], sw + (j >> 1) * 4, sx + (j >> 1) * 2, k > 0 || j > 0);
-          tc::mma_commit(smem_addr(&b_empty[s]));
+            for (int j = 0; j < 4; ++j)
+              mma_mxf4(acc, da + j * 2, db + j * 2, desc[j & 1], sw + (j >> 1) * 4, sx + (j >> 1) * 2, k > 0 || j > 0);
+            tc::mma_commit(smem_addr(&b_empty[s]));
+            if (k == nk - 1) tc::mma_commit(smem_addr(&b_acc[buf]));
+          }
+          __syncwarp();
           if (++s == (uint32_t)g.ring) s = 0, ++round;
         }
-        tc::mma_commit(smem_addr(&b_acc[buf]));
       }
     }
     __syncwarp();
   } else {
-    // quantize: two threads a block, as in mx_quant.cu
-    const int t0 = threadIdx.x - 64, items = g.rows * nk * 16;
-    for (int i = t0; i - lane < items; i += 256) {
-      const int row = i / (nk * 16), in = i - row * nk * 16, k = in >> 4, b = (in >> 1) & 7, half = in & 1;
-      const int at = (k0 + k) * kMxStage + b * 32 + 8 * half;
-      MxHalf q;
-      q.load(static_cast<const T*>(g.x) + row * g.ldx + at, i < items && at < g.K);
-      uint32_t scales = q.finish() << (8 * (b & 3));
-      scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
-      scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
-      if (i < items) {
-        *reinterpret_cast<uint2*>(x_mem + k * g.rows8 * 128 + mx_code_at(row, b) + 8 * half) = q.codes;
-        // a stage's scales: row r is lane r, blocks 0..3 in column 0, blocks 4..7 in column 2
-        if ((threadIdx.x & 7) == 0)
-          *reinterpret_cast<uint32_t*>(x_mem + x_bytes + k * 512 + row * 16 + (b >> 2) * 8) = scales;
+    // quantize: two threads a block; `per` threads a row, or all for each of several rows at a time
+    const int t0 = threadIdx.x - 64, per = nk * 16, together = max(1, 256 / per), mine = per < 256 ? t0 / per : 0;
+    const int last = mine < together ? per : 0;
+    int in = t0 - mine * per;
+    for (int trip = 0; trip < (per + 255) / 256; ++trip, in += 256) {
+      const int k = in >> 4, b = (in >> 1) & 7, half = in & 1, at = (k0 + k) * kMxStage + b * 32 + 8 * half;
+      for (int r0 = 0; r0 < g.rows; r0 += together) {
+        const int row = r0 + mine;
+        const bool there = row < g.rows && in < last;
+        MxHalf q;
+        q.load(static_cast<const T*>(g.x) + row * g.ldx + at, there && at < g.K);
+        uint32_t scales = q.finish() << (8 * (b & 3));
+        scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
+        scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+        if (there) {
+          *reinterpret_cast<uint2*>(x_mem + k * kXStage + mx_code_at(row, b) + 8 * half) = q.codes;
+          // a stage's scales: row r is lane r, blocks 0..3 in column 0, blocks 4..7 in column 2
+          if ((in & 7) == 0) *reinterpret_cast<uint32_t*>(x_mem + x_bytes + k * 512 + row * 16 + (b >> 2) * 8) = scales;
+        }
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the tensor cores read them
@@ -215,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
           const int row = at.row0 + i, x_row = g.offsets ? s_token[row] : row;
           uint32_t mine = v[0];
 #pragma unroll
-          for (int c = 1; c < 16; ++c) mine = c == x_row ? v[c] : mine;
+          for (int c = 1; c < kMaxRows; ++c) mine = c == x_row ? v[c] : mine;
           store_as(g.y, (int64_t)row * g.ldy + n, g.dtype, __uint_as_float(mine));
         }
       continue;
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     if (threadIdx.x == 64) mbar_expect_tx(smem_addr(&b_part), (uint32_t)owned * ranks * kMxRows * 4);
     if (stores && ok) {
 #pragma unroll
-      for (int c = 0; c < 16; ++c)
+      for (int c = 0; c < kMaxRows; ++c)
         if (c < g.rows) {
           const uint32_t owner = (uint32_t)c % ranks, slot = (uint32_t)c / ranks * ranks + rank;
           uint32_t to, bar;
@@ -262,25 +269,24 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
 }
 
 struct GemvPlan {
-  int ranks, nk, ring, rows8;
+  int ranks, nk, ring;
   size_t smem;
 };
 
 // Whether and how the kernel takes `rows` rows of x: CTAs in a cluster, the most stages one has, stages of its ring.
 bool plan_gemv(int64_t rows, int64_t used, int64_t row_tiles, int64_t stages, int sms, GemvPlan* p) {
-  if (rows < 1 || rows > 16) return false;
+  if (rows < 1 || rows > kMaxRows) return false;
   int ranks = 1;
   while (ranks < 8 && used * row_tiles * ranks * 2 <= sms && stages >= ranks * 4) ranks *= 2;
   const int64_t nk = (stages + ranks - 1) / ranks;
-  const int rows8 = rows <= 8 ? 8 : 16;
   if (nk > (512 - (int)kScaleX) / 4) return false;
-  const size_t x = (size_t)nk * (rows8 * 128 + 512) + (16 - rows8) * 128 + 1024;  // 1024: the ring is aligned to that
+  const size_t x = (size_t)(nk + 1) * kXStage + nk * 512 + 1024;  // 1024: the ring is aligned to that
   // a ring that leaves room for the next kernel's CTA beside this one, or else for all that an SM has
   const size_t half = 104 * 1024, all = 214 * 1024;
   size_t ring = x + 4 * kMxBytes <= half ? (half - x) / kMxBytes : x + 3 * kMxBytes <= all ? (all - x) / kMxBytes : 0;
   if (ring == 0) return false;
   ring = std::min<size_t>(std::min<size_t>(ring, kMaxRing), std::max<int64_t>(nk, 2));
-  *p = {ranks, (int)nk, (int)ring, rows8, x + ring * kMxBytes};
+  *p = {ranks, (int)nk, (int)ring, x + ring * kMxBytes};
   return true;
 }
 
@@ -328,7 +334,7 @@ int launch_mx_gemv(const MxGemv& a, cudaStream_t stream) {
   const int64_t used = std::min<int64_t>(a.offsets ? a.choices : 1, a.experts), row_tiles = mx_tiles(a.N), stages = mx_stages(a.K);
   if (!plan_gemv(a.rows, used, row_tiles, stages, dev.sms, &p)) return fail(B2Q_ERANGE, "mx_gemv: more rows than the kernel takes");
   const Gemv g = {a.w, a.x, a.y, a.offsets, a.order, a.ldx, a.ldy, (int)a.rows, (int)a.K, (int)a.N, (int)row_tiles, (int)stages,
-                  (int)a.experts, a.dtype, a.top, p.ring, p.rows8, kScaleX + 4 * p.nk <= 256 ? 256 : 512};
+                  (int)a.experts, a.dtype, a.top, p.ring, kScaleX + 4 * p.nk <= 256 ? 256 : 512};
   // with several CTAs a tile every tile has a cluster of its own
   const int64_t ctas = std::min<int64_t>(used * row_tiles, dev.sms / p.ranks);
   if (a.x_dtype == B2Q_DTYPE_F32) return launch_gemv<float>(g, p, (int)ctas, stream);

@@ -38,7 +38,7 @@ struct MxGemm {
 };
 int launch_mx_gemm(const MxGemm& g, cudaStream_t stream);
 
-// Up to 16 rows of x, quantized by the kernel itself.
+// Up to 4 rows of x, quantized by the kernel itself.
 struct MxGemv {
   const uint8_t* w;
   const void* x;

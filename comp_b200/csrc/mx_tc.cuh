@@ -7,6 +7,15 @@
 
 namespace b2q {
 
+// One lane of a converged warp, told in the way that lets the compiler see that it is one: tensor-core instructions take
+// their operands from uniform registers, and behind a branch on the lane's number each issues ten times as slowly (a stage's
+// six scale copies and four products 900 cycles, so 220).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // K-major operand with the 128-byte swizzle: 8 rows every 1024 bytes
 __device__ __forceinline__ uint64_t desc_swizzled(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3fff) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);

@@ -13,39 +13,51 @@ kernels are this package's own, through the C-ABI (include/comp_b200.h, where la
 import torch
 
 from . import _lib
-from .kv import _call, _dtype_id, _on_device, _raw_stream
-from .mx import (FUSED_ROWS, MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _few_size, _out_dtype,
-                 _rows, _stride)
+from .kv import _dtype_id, _on_device
+from .mx import (FUSED_ROWS, MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _enter, _few_size,
+                 _out_dtype, _rows, _stride)
 
 MAX_TOP = 32
 
 
 class Plan:
-    """Choices (token * top + j) sorted by expert. int32 tensors: offsets [experts + 1] (the sorted rows where each expert's
-    begin), pos [tokens][top] (each choice's sorted row, -1: it goes nowhere), order [tokens * top] (each sorted row's choice, -1
-    past the last). From route also ids int32 and weights f32 [tokens][top]."""
+    """Choices (token * top + j) sorted by expert. int32 tensors: ids [tokens][top] (each choice's expert, -1: none), offsets
+    [experts + 1] (the sorted rows where each expert's begin), pos [tokens][top] (each choice's sorted row, -1: it goes nowhere),
+    order [tokens * top] (each sorted row's choice, -1 past the last); weights f32 [tokens][top] (from route, else None). All lie in
+    one allocation, whose parts are made tensors when they are asked for."""
 
-    def __init__(self, tokens, top, experts, dev):
+    def __init__(self, tokens, top, experts, like, ids=None):
         choices = tokens * top
-        self.tokens, self.top, self.experts, self.device = tokens, top, experts, dev
-        self.ids = self.weights = None
+        self.tokens, self.top, self.experts, self.device = tokens, top, experts, like.device
         words = 2 * (experts + 1) + 4 * choices if tokens <= 128 and choices <= 4096 else \
             _lib.load().b2q_experts_plan_words(tokens, top, experts)
-        self._words = torch.empty(words, dtype=torch.int32, device=dev)
+        self._ids, self._routed = ids, words if ids is None else 0  # (routed: ids and weights follow the plan's own words)
+        self._words = like.new_empty(words + 2 * choices if ids is None else words, dtype=torch.int32)
+
+    def _part(self, at, rows=True):
+        if rows:
+            return self._words.as_strided((self.tokens, self.top), (self.top, 1), at)
+        return self._words.as_strided((self.tokens * self.top,), (1,), at)
+
+    @property
+    def ids(self):
+        return self._part(self._routed) if self._ids is None else self._ids
+
+    @property
+    def weights(self):
+        return self._part(self._routed + self.tokens * self.top).view(torch.float32) if self._ids is None else None
 
     @property
     def offsets(self):
-        return self._words[: self.experts + 1]
+        return self._words.as_strided((self.experts + 1,), (1,))
 
     @property
     def pos(self):
-        at = 2 * (self.experts + 1)
-        return self._words[at : at + self.tokens * self.top].view(self.tokens, self.top)
+        return self._part(2 * (self.experts + 1))
 
     @property
     def order(self):
-        at, n = 2 * (self.experts + 1), self.tokens * self.top
-        return self._words[at + n : at + 2 * n]
+        return self._part(2 * (self.experts + 1) + self.tokens * self.top, rows=False)
 
 
 def _check_sizes(name, tokens, top, experts):
@@ -74,11 +86,11 @@ def route(logits, top, normalize=True):
     s0, s1 = logits.stride()
     if (s1 != 1 and experts > 1) or (tokens > 1 and s0 < experts):
         logits = logits.clone(memory_format=torch.contiguous_format)
-    plan = Plan(tokens, top, experts, dev)
-    plan.ids = torch.empty((tokens, top), dtype=torch.int32, device=dev)
-    plan.weights = torch.empty((tokens, top), dtype=torch.float32, device=dev)
-    _call(dev, "b2q_experts_route", did, logits.data_ptr(), _stride(logits), tokens, experts, top, 1 if normalize else 0,
-          plan.ids.data_ptr(), plan.weights.data_ptr(), plan._words.data_ptr(), _raw_stream(dev.index))
+    plan = Plan(tokens, top, experts, logits)
+    words = plan._words.data_ptr()
+    ids = words + 4 * plan._routed
+    _enter(dev, _lib.load().b2q_experts_route, did, logits.data_ptr(), _stride(logits), tokens, experts, top, 1 if normalize else 0,
+           ids, ids + 4 * tokens * top, words)
     return plan
 
 
@@ -95,9 +107,8 @@ def sort(ids, experts):
     tokens, top = ids.shape
     _check_sizes("sort", tokens, top, experts)
     ids = ids.contiguous()
-    plan = Plan(tokens, top, experts, dev)
-    plan.ids = ids
-    _call(dev, "b2q_experts_sort", ids.data_ptr(), tokens, top, experts, plan._words.data_ptr(), _raw_stream(dev.index))
+    plan = Plan(tokens, top, experts, ids, ids)
+    _enter(dev, _lib.load().b2q_experts_sort, ids.data_ptr(), tokens, top, experts, plan._words.data_ptr())
     return plan
 
 
@@ -133,22 +144,26 @@ def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     choices = plan.tokens * plan.top
     if x.dim() != 2 or x.shape != (plan.tokens if gather else choices, k):
         raise ValueError(f"linear: x {tuple(x.shape)}, expected [{plan.tokens if gather else choices}][{k}]")
-    dtype = x.dtype if dtype is None else dtype
+    if dtype is None:
+        dtype = x.dtype
     did = _out_dtype("linear", dtype)
-    x = _rows(x)
-    y = _check_out("linear", out, dtype, (choices, n), dev)
+    x, x_at, ldx = _rows(x)
+    if out is None:
+        out = x.new_empty((choices, n), dtype=dtype)
+        at, ldy = out.data_ptr(), n
+    else:
+        at, ldy = _check_out("linear", out, dtype, (choices, n), dev)
     if workspace is None:
         need = workspace_size(plan, w, gather)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        workspace = x.new_empty(need, dtype=torch.uint8) if need else None
     else:
         _on_device("linear", dev, workspace)
         if not workspace.is_contiguous():
             raise ValueError("linear: workspace must be contiguous")
         need = workspace.numel() * workspace.element_size()
-    _call(dev, "b2q_experts_linear", xid, x.data_ptr(), _stride(x), 1 if gather else 0, w.image.data_ptr(),
-          plan._words.data_ptr(), plan.tokens, plan.top, plan.experts, n, k, did, y.data_ptr(), _stride(y),
-          0 if workspace is None else workspace.data_ptr(), need, _raw_stream(dev.index))
-    return y
+    _enter(dev, _lib.load().b2q_experts_linear, xid, x_at, ldx, 1 if gather else 0, w.image.data_ptr(), plan._words.data_ptr(),
+           plan.tokens, plan.top, plan.experts, n, k, did, at, ldy, 0 if workspace is None else workspace.data_ptr(), need)
+    return out
 
 
 def combine(y, plan, weights=None, out=None):
@@ -169,10 +184,16 @@ def combine(y, plan, weights=None, out=None):
         if weights.shape != (plan.tokens, plan.top):
             raise ValueError(f"combine: weights {tuple(weights.shape)}, expected ({plan.tokens}, {plan.top})")
         weights = weights.contiguous()
-    if (n > 1 and y.stride(1) != 1) or (choices > 1 and y.stride(0) < n):
-        y = y.clone(memory_format=torch.contiguous_format)
-    o = _check_out("combine", out, y.dtype, (plan.tokens, n), dev)
-    _call(dev, "b2q_experts_combine", did, y.data_ptr(), _stride(y), plan._words.data_ptr(),
-          0 if weights is None else weights.data_ptr(), plan.tokens, plan.top, plan.experts, n, o.data_ptr(), _stride(o),
-          _raw_stream(dev.index))
-    return o
+    ldy = n
+    if not y.is_contiguous():
+        if (n > 1 and y.stride(1) != 1) or (choices > 1 and y.stride(0) < n):
+            y = y.clone(memory_format=torch.contiguous_format)
+        ldy = _stride(y)
+    if out is None:
+        out = y.new_empty((plan.tokens, n))
+        at, ldo = out.data_ptr(), n
+    else:
+        at, ldo = _check_out("combine", out, y.dtype, (plan.tokens, n), dev)
+    _enter(dev, _lib.load().b2q_experts_combine, did, y.data_ptr(), ldy, plan._words.data_ptr(),
+           0 if weights is None else weights.data_ptr(), plan.tokens, plan.top, plan.experts, n, at, ldo)
+    return out

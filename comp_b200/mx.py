@@ -15,16 +15,35 @@ TypeError / ValueError / RuntimeError on what they do not take.
 import torch
 
 from . import _lib
-from .kv import DTYPE_ID, _call, _dtype_id, _on_device, _raw_stream
+from .kv import DTYPE_ID, _dtype_id, _on_device, _raw_stream
+
+# A token's step is many calls of a few microseconds on the GPU: what a call costs on the host counts. So the functions
+# look at the common case first (contiguous, aligned), make tensors from tensors, and enter the library once.
+_current_device = torch._C._cuda_getDevice
 
 TILE_ROWS, STAGE, STAGE_BYTES = 128, 256, 17408  # an image: 128 rows by 256 values a run of bytes
 MAX_EXPERTS = 1024
-FUSED_ROWS = 16  # products of up to so many rows may quantize them in their own launch
+FUSED_ROWS = 4  # products of up to so many rows may quantize them in their own launch
 
 
 def image_bytes(rows, k, experts=1):
     """Bytes of the image of `experts` operands of [rows][k]."""
     return experts * -(-rows // TILE_ROWS) * -(-k // STAGE) * STAGE_BYTES
+
+
+def _enter(dev, entry, *args):
+    """The library's entry on dev and its current stream (the last argument)."""
+    if _current_device() == dev.index:
+        rc = entry(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _raw_stream(dev.index))
+    if rc:
+        raise (ValueError if rc in (-1, -2, -4) else _error(rc))(_lib.last_error())
+
+
+def _error(code):
+    return lambda text: _lib.B2QError(code, text)
 
 
 def _check_k(name, k):
@@ -51,6 +70,13 @@ class MXTensor:
         self.image, self.rows, self.k, self.experts, self.device = image, rows, k, experts, image.device
         self._sizes = {}  # workspaces of products with few rows
 
+    @classmethod
+    def _made(cls, image, rows, k, experts=None):
+        self = cls.__new__(cls)
+        self.image, self.rows, self.k, self.experts, self.device = image, rows, k, experts, image.device
+        self._sizes = {}
+        return self
+
     @property
     def shape(self):
         return (self.rows, self.k) if self.experts is None else (self.experts, self.rows, self.k)
@@ -70,11 +96,16 @@ def _cuda(name, t):
 
 
 def _rows(t):
-    """t with unit column stride and 16-byte aligned base and rows that do not overlap (a copy only when needed)."""
+    """(t, its address, its row stride): unit column stride, a 16-byte aligned base and rows that do not overlap (a copy only
+    when needed)."""
+    at, (m, k) = t.data_ptr(), t.shape
+    if t.is_contiguous() and not at & 15:
+        return t, at, k
     s0, s1 = t.stride()
-    if (s1 != 1 and t.shape[1] > 1) or t.data_ptr() % 16 or (t.shape[0] > 1 and (s0 * t.element_size() % 16 or s0 < t.shape[1])):
+    if s1 != 1 or at & 15 or (m > 1 and (s0 * t.element_size() & 15 or s0 < k)):
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        return t, t.data_ptr(), k
+    return t, at, s0 if m > 1 else k
 
 
 def _stride(t):
@@ -91,10 +122,10 @@ def quantize(x):
         raise ValueError(f"quantize: x {tuple(x.shape)}, expected [M][K]")
     m, k = x.shape
     _check_k("quantize", k)
-    x = _rows(x)
-    t = MXTensor(torch.empty(image_bytes(m, k), dtype=torch.uint8, device=dev), m, k)
-    _call(dev, "b2q_mx_quantize", did, x.data_ptr(), _stride(x), m, k, t.image.data_ptr(), _raw_stream(dev.index))
-    return t
+    x, at, ldx = _rows(x)
+    image = x.new_empty(image_bytes(m, k), dtype=torch.uint8)
+    _enter(dev, _lib.load().b2q_mx_quantize, did, at, ldx, m, k, image.data_ptr())
+    return MXTensor._made(image, m, k)
 
 
 def dequantize(t, dtype=torch.float32):
@@ -105,11 +136,12 @@ def dequantize(t, dtype=torch.float32):
     if did is None:
         raise TypeError(f"dequantize: dtype {dtype}, expected float32, float16 or bfloat16")
     dev = t.device
-    y = torch.empty(t.shape, dtype=dtype, device=dev)
-    for e in range(t.experts or 1):
-        out = y if t.experts is None else y[e]
-        at = t.image.data_ptr() + e * image_bytes(t.rows, t.k)
-        _call(dev, "b2q_mx_dequantize", at, t.rows, t.k, did, out.data_ptr(), t.k, _raw_stream(dev.index))
+    y = t.image.new_empty(t.shape, dtype=dtype)
+    at, to, entry = t.image.data_ptr(), y.data_ptr(), _lib.load().b2q_mx_dequantize
+    for _ in range(t.experts or 1):
+        _enter(dev, entry, at, t.rows, t.k, did, to, t.k)
+        at += image_bytes(t.rows, t.k)
+        to += t.rows * t.k * y.element_size()
     return y
 
 
@@ -130,10 +162,9 @@ def pack(codes, scales):
     codes, scales = codes.contiguous(), scales.contiguous()
     if codes.data_ptr() % 16:
         codes = codes.clone()
-    t = MXTensor(torch.empty(image_bytes(n, k, experts or 1), dtype=torch.uint8, device=dev), n, k, experts)
-    _call(dev, "b2q_mx_pack", codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, t.image.data_ptr(),
-          _raw_stream(dev.index))
-    return t
+    image = codes.new_empty(image_bytes(n, k, experts or 1))
+    _enter(dev, _lib.load().b2q_mx_pack, codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, image.data_ptr())
+    return MXTensor._made(image, n, k, experts)
 
 
 def from_ggml(blocks, n, k, experts=None):
@@ -151,14 +182,12 @@ def from_ggml(blocks, n, k, experts=None):
 
 
 def _check_out(name, out, dtype, shape, dev):
-    """An output tensor given or made: unit column stride, rows that do not overlap."""
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
+    """The address and row stride of a given output: unit column stride, rows that do not overlap."""
     _on_device(name, dev, out)
     if out.dtype != dtype or out.shape != shape or (shape[1] > 1 and out.stride(1) != 1) or \
             (shape[0] > 1 and out.stride(0) < shape[1]):
         raise ValueError(f"{name}: out must be a {dtype} {shape} tensor with unit column stride on {dev}")
-    return out
+    return out.data_ptr(), _stride(out)
 
 
 def _out_dtype(name, dtype):
@@ -180,10 +209,13 @@ def matmul(a, w, dtype=torch.bfloat16, out=None):
         raise ValueError(f"matmul: a {a.shape} on {a.device} and w {w.shape} on {w.device}")
     did = _out_dtype("matmul", dtype)
     dev = a.device
-    y = _check_out("matmul", out, dtype, (a.rows, w.rows), dev)
-    _call(dev, "b2q_mx_matmul", a.image.data_ptr(), w.image.data_ptr(), a.rows, w.rows, a.k, did, y.data_ptr(), _stride(y),
-          _raw_stream(dev.index))
-    return y
+    if out is None:
+        out = a.image.new_empty((a.rows, w.rows), dtype=dtype)
+        at, ldy = out.data_ptr(), w.rows
+    else:
+        at, ldy = _check_out("matmul", out, dtype, (a.rows, w.rows), dev)
+    _enter(dev, _lib.load().b2q_mx_matmul, a.image.data_ptr(), w.image.data_ptr(), a.rows, w.rows, a.k, did, at, ldy)
+    return out
 
 
 def _few_size(w, key, name, *args):
@@ -207,12 +239,17 @@ def linear(x, w, dtype=None, out=None):
     if x.dim() != 2 or x.shape[1] != k:
         raise ValueError(f"linear: x {tuple(x.shape)}, expected [M][{k}]")
     m = x.shape[0]
-    dtype = x.dtype if dtype is None else dtype
+    if dtype is None:
+        dtype = x.dtype
     did = _out_dtype("linear", dtype)
-    x = _rows(x)
-    y = _check_out("linear", out, dtype, (m, n), dev)
+    x, x_at, ldx = _rows(x)
+    if out is None:
+        out = x.new_empty((m, n), dtype=dtype)
+        at, ldy = out.data_ptr(), n
+    else:
+        at, ldy = _check_out("linear", out, dtype, (m, n), dev)
     need = image_bytes(m, k) if m > FUSED_ROWS else _few_size(w, m, "b2q_mx_linear_workspace_size", m, n, k)
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, "b2q_mx_linear", xid, x.data_ptr(), _stride(x), w.image.data_ptr(), m, n, k, did, y.data_ptr(), _stride(y),
-          workspace.data_ptr() if need else 0, need, _raw_stream(dev.index))
-    return y
+    workspace = x.new_empty(need, dtype=torch.uint8) if need else None
+    _enter(dev, _lib.load().b2q_mx_linear, xid, x_at, ldx, w.image.data_ptr(), m, n, k, did, at, ldy,
+           workspace.data_ptr() if need else 0, need)
+    return out

@@ -408,7 +408,7 @@ int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, in
 int b2q_mx_matmul(const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y, int64_t ldy,
                   b2q_stream_t stream);
 
-/* b2q_mx_quantize of x [M][K] and b2q_mx_matmul with it, in one launch for up to 16 rows (unless K is very long). workspace: device
+/* b2q_mx_quantize of x [M][K] and b2q_mx_matmul with it, in one launch for up to 4 rows (unless K is very long). workspace: device
  * memory of b2q_mx_linear_workspace_size(M, N, K) bytes (0 for one launch), 128-byte aligned; calls that may overlap on the GPU
  * need one each. */
 size_t b2q_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K);
