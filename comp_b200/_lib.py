@@ -63,8 +63,8 @@ SIGNATURES = {
     "b2q_attention_workspace_size": (ctypes.c_size_t, [P, P]),
     "b2q_attention": (INT, [P, P, P, ctypes.c_size_t, P]),
     "b2q_mx_bytes": (ctypes.c_size_t, [I64, I64, I64]),
-    "b2q_mx_quantize": (INT, [INT, P, I64, I64, I64, P, P]),
-    "b2q_mx_dequantize": (INT, [P, I64, I64, INT, P, I64, P]),
+    "b2q_mx_quantize": (INT, [INT, P, I64, I64, I64, I64, P, P]),
+    "b2q_mx_dequantize": (INT, [P, I64, I64, I64, INT, P, I64, P]),
     "b2q_mx_pack": (INT, [P, P, I64, I64, I64, P, P]),
     "b2q_mx_matmul": (INT, [P, P, I64, I64, I64, INT, P, I64, P]),
     "b2q_mx_linear_workspace_size": (ctypes.c_size_t, [I64, I64, I64]),

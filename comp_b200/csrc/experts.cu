@@ -629,7 +629,7 @@ int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, cons
   if (!workspace || workspace_bytes < need || !aligned(workspace, 128))
     return fail(B2Q_EINVAL, "%s: workspace of %zu bytes, 128-byte aligned, needed (%zu given)", who, need, workspace_bytes);
   uint8_t* image = static_cast<uint8_t*>(workspace);
-  rc = launch_mx_quantize(x_dtype, x, ldx, rows, K, image, gather ? p.dest : p.dest_row, gather ? (int)top : 1, stream);
+  rc = launch_mx_quantize(x_dtype, x, ldx, rows, rows, K, image, gather ? p.dest : p.dest_row, gather ? (int)top : 1, stream);
   if (rc) return rc;
   const MxGemm g = {w, image, y, p.offsets, p.tiles, ldy, choices, (int)N, (int)mx_tiles(N), (int)mx_stages(K), (int)experts,
                     dtype, 1};

@@ -322,7 +322,7 @@ int launch_mx_gemm(const MxGemm& g, cudaStream_t stream) {
   const int64_t tiles = used * ((each + tn - 1) / tn) * g.row_tiles;
   // every tile that there can be: each expert's last one may be all but empty
   const int64_t most = ((g.rows + tn - 1) / tn + (g.offsets ? used : 0)) * g.row_tiles;
-  if (most > INT32_MAX) return fail(B2Q_ERANGE, "mx_gemm: too many tiles");
+  if (most > INT32_MAX / 2) return fail(B2Q_ERANGE, "mx_gemm: too many tiles");
   int ranks = 1;
   while (ranks < 8 && tiles * ranks * 2 <= dev.sms && g.stages >= ranks * 4 && tn <= 128) ranks *= 2;
   const int ctas = (int)std::min<int64_t>(most, dev.sms / ranks);
@@ -394,7 +394,7 @@ int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int
   if (!workspace || workspace_bytes < need || !aligned(workspace, 128))
     return fail(B2Q_EINVAL, "%s: workspace of %zu bytes, 128-byte aligned, needed (%zu given)", who, need, workspace_bytes);
   uint8_t* image = static_cast<uint8_t*>(workspace);
-  rc = launch_mx_quantize(x_dtype, x, ldx, M, K, image, nullptr, 1, stream);
+  rc = launch_mx_quantize(x_dtype, x, ldx, M, M, K, image, nullptr, 1, stream);
   if (rc) return rc;
   const MxGemm g = {w, image, y, nullptr, nullptr, ldy, M, (int)N, (int)mx_tiles(N), (int)mx_stages(K), 1, dtype, 1};
   return launch_mx_gemm(g, stream);

@@ -275,7 +275,7 @@ struct GemvPlan {
 
 // Whether and how the kernel takes `rows` rows of x: CTAs in a cluster, the most stages one has, stages of its ring.
 bool plan_gemv(int64_t rows, int64_t used, int64_t row_tiles, int64_t stages, int sms, GemvPlan* p) {
-  if (rows < 1 || rows > kMaxRows) return false;
+  if (rows < 1 || rows > kMaxRows || used * row_tiles > INT32_MAX / 2) return false;
   int ranks = 1;
   while (ranks < 8 && used * row_tiles * ranks * 2 <= sms && stages >= ranks * 4) ranks *= 2;
   const int64_t nk = (stages + ranks - 1) / ranks;

@@ -23,9 +23,10 @@ inline int mx_dtype_size(int dtype) { return dtype == B2Q_DTYPE_F32 ? 4 : 2; }
 int check_mx_shape(const char* who, int64_t rows, int64_t K);
 int check_mx_rows(const char* who, const char* name, int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K);
 
-// Quantizes x into an image: row r goes to the image rows dest[r * fan + j], j < fan (negative: nowhere; null: to row r).
-int launch_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, uint8_t* image, const int32_t* dest,
-                       int fan, cudaStream_t stream);
+// Quantizes x into an image: row r goes to the image rows dest[r * fan + j], j < fan (negative: nowhere), or without dest to its
+// place among operands of `each` rows.
+int launch_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t each, int64_t K, uint8_t* image,
+                       const int32_t* dest, int fan, cudaStream_t stream);
 
 struct MxGemm {
   const uint8_t *w, *x;    // images: the weights of all experts, one after the other; the rows

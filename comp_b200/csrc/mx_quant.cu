@@ -14,7 +14,7 @@
 namespace b2q {
 
 int check_mx_shape(const char* who, int64_t rows, int64_t K) {
-  if (rows < 0 || rows > INT32_MAX) return fail(B2Q_EINVAL, "%s: %lld rows", who, (long long)rows);
+  if (rows < 0 || rows > INT32_MAX - 1024) return fail(B2Q_EINVAL, "%s: %lld rows", who, (long long)rows);
   if (K < 32 || K % 32 || K > INT32_MAX / 2)
     return fail(B2Q_EINVAL, "%s: K=%lld is not a positive multiple of 32", who, (long long)K);
   return B2Q_OK;
@@ -110,10 +110,17 @@ __device__ __forceinline__ Place place_of(int64_t item, int stages) {
   return {row, (int)(s - row * stages), (int)item & 7};
 }
 
+// The image's row of row r of operands of `each` rows, which begin at whole tiles.
+__device__ __forceinline__ int64_t image_row(int64_t r, int64_t each) {
+  if (r < each) return r;
+  const int64_t e = r / each;
+  return e * ((each + kMxRows - 1) / kMxRows * kMxRows) + (r - e * each);
+}
+
 template <bool WIDE, typename T>
 __global__ void __launch_bounds__(256)
-    mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int stages, uint8_t* __restrict__ image,
-                       const int32_t* __restrict__ dest, int fan) {
+    mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int64_t each, int K, int stages,
+                       uint8_t* __restrict__ image, const int32_t* __restrict__ dest, int fan) {
   pdl_wait_then_trigger();
   const Place p = place_of((int64_t)blockIdx.x * 256 + threadIdx.x, stages);
   const int at = p.stage * kMxStage + p.b * 32;
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(256)
   if (p.row >= rows) return;
   const int64_t first = dest ? p.row * fan : 0;
   for (int j = 0; j < fan; ++j) {
-    const int64_t r = dest ? dest[first + j] : p.row;
+    const int64_t r = dest ? dest[first + j] : image_row(p.row, each);
     if (r < 0) continue;
     uint8_t* tile = image + ((r >> 7) * stages + p.stage) * kMxBytes;
     const int in = (int)r & 127;
@@ -143,13 +150,15 @@ __global__ void __launch_bounds__(256)
 
 template <bool WIDE, typename T>
 __global__ void __launch_bounds__(256)
-    mx_dequantize_kernel(const uint8_t* __restrict__ image, int64_t rows, int K, int stages, T* __restrict__ y, int64_t ldy) {
+    mx_dequantize_kernel(const uint8_t* __restrict__ image, int64_t rows, int64_t each, int K, int stages, T* __restrict__ y,
+                         int64_t ldy) {
   pdl_wait_then_trigger();
   const Place p = place_of((int64_t)blockIdx.x * 256 + threadIdx.x, stages);
   const int at = p.stage * kMxStage + p.b * 32;
   if (p.row >= rows || at >= K) return;
-  const uint8_t* tile = image + ((p.row >> 7) * stages + p.stage) * kMxBytes;
-  const int in = (int)p.row & 127;
+  const int64_t r = image_row(p.row, each);
+  const uint8_t* tile = image + ((r >> 7) * stages + p.stage) * kMxBytes;
+  const int in = (int)r & 127;
   const uint4 q = *reinterpret_cast<const uint4*>(tile + mx_code_at(in, p.b));
   const float d = mx_scale(tile[mx_scale_at(in, p.b)]);
   float lo[2][8], hi[2][8];
@@ -188,6 +197,11 @@ __global__ void __launch_bounds__(256)
   dst[mx_scale_at(in, b)] = d;
 }
 
+int check_experts(const char* who, int64_t experts) {
+  if (experts >= 1 && experts <= kMaxExperts) return B2Q_OK;
+  return fail(B2Q_EINVAL, "%s: %lld experts (1..%lld)", who, (long long)experts, (long long)kMaxExperts);
+}
+
 int grid_of(const char* who, int64_t items, unsigned* grid) {
   const int64_t n = (items + 255) / 256;
   if (n > INT32_MAX) return fail(B2Q_ERANGE, "%s: too many values for one launch", who);
@@ -197,15 +211,15 @@ int grid_of(const char* who, int64_t items, unsigned* grid) {
 
 }  // namespace
 
-int launch_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, uint8_t* image, const int32_t* dest,
-                       int fan, cudaStream_t stream) {
+int launch_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t each, int64_t K, uint8_t* image,
+                       const int32_t* dest, int fan, cudaStream_t stream) {
   const int stages = (int)mx_stages(K);
   unsigned grid;
   int rc = grid_of("b2q_mx_quantize", rows * stages * 8, &grid);
   if (rc || rows == 0) return rc;
   const bool wide = aligned(x, 32) && (rows == 1 || ldx * mx_dtype_size(dtype) % 32 == 0);
   auto launch = [&](auto kernel, auto* p) {
-    launch_maybe_pdl(kernel, dim3(grid), dim3(256), 0, stream, p, ldx, rows, (int)K, stages, image, dest, fan);
+    launch_maybe_pdl(kernel, dim3(grid), dim3(256), 0, stream, p, ldx, rows, each, (int)K, stages, image, dest, fan);
   };
   if (dtype == B2Q_DTYPE_F32)
     launch(wide ? mx_quantize_kernel<true, float> : mx_quantize_kernel<false, float>, static_cast<const float*>(x));
@@ -225,27 +239,29 @@ extern "C" {
 
 size_t b2q_mx_bytes(int64_t experts, int64_t rows, int64_t K) {
   if (check_mx_shape("b2q_mx_bytes", rows, K)) return 0;
-  if (experts < 1 || experts > kMaxExperts) {
-    fail(B2Q_EINVAL, "b2q_mx_bytes: %lld experts (1..%lld)", (long long)experts, (long long)kMaxExperts);
-    return 0;
-  }
+  if (check_experts("b2q_mx_bytes", experts)) return 0;
   return (size_t)experts * mx_tiles(rows) * mx_stages(K) * kMxBytes;
 }
 
-int b2q_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, uint8_t* image, b2q_stream_t stream) {
+int b2q_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t experts, int64_t rows, int64_t K, uint8_t* image,
+                    b2q_stream_t stream) {
   const char* who = "b2q_mx_quantize";
   int rc = check_mx_shape(who, rows, K);
-  if (!rc) rc = check_mx_rows(who, "x", dtype, x, ldx, rows, K);
+  if (!rc) rc = check_experts(who, experts);
+  if (!rc) rc = check_mx_rows(who, "x", dtype, x, ldx, experts * rows, K);
   if (rc || rows == 0) return rc;
   if (!image) return fail(B2Q_EINVAL, "%s: image is NULL", who);
-  if (!aligned(x, 16) || (rows > 1 && ldx * mx_dtype_size(dtype) % 16) || !aligned(image, 128))
+  if (!aligned(x, 16) || (experts * rows > 1 && ldx * mx_dtype_size(dtype) % 16) || !aligned(image, 128))
     return fail(B2Q_EALIGN, "%s: x and its row stride must be 16-byte aligned, the image 128-byte", who);
-  return launch_mx_quantize(dtype, x, ldx, rows, K, image, nullptr, 1, stream);
+  return launch_mx_quantize(dtype, x, ldx, experts * rows, rows, K, image, nullptr, 1, stream);
 }
 
-int b2q_mx_dequantize(const uint8_t* image, int64_t rows, int64_t K, int dtype, void* y, int64_t ldy, b2q_stream_t stream) {
+int b2q_mx_dequantize(const uint8_t* image, int64_t experts, int64_t each, int64_t K, int dtype, void* y, int64_t ldy,
+                      b2q_stream_t stream) {
   const char* who = "b2q_mx_dequantize";
-  int rc = check_mx_shape(who, rows, K);
+  int rc = check_mx_shape(who, each, K);
+  if (!rc) rc = check_experts(who, experts);
+  const int64_t rows = rc ? 0 : experts * each;
   if (!rc) rc = check_mx_rows(who, "y", dtype, y, ldy, rows, K);
   if (rc || rows == 0) return rc;
   if (!image) return fail(B2Q_EINVAL, "%s: image is NULL", who);
@@ -257,7 +273,7 @@ int b2q_mx_dequantize(const uint8_t* image, int64_t rows, int64_t K, int dtype, 
   if (rc) return rc;
   const bool wide = aligned(y, 32) && (rows == 1 || ldy * mx_dtype_size(dtype) % 32 == 0);
   auto launch = [&](auto kernel, auto* p) {
-    launch_maybe_pdl(kernel, dim3(grid), dim3(256), 0, stream, image, rows, (int)K, stages, p, ldy);
+    launch_maybe_pdl(kernel, dim3(grid), dim3(256), 0, stream, image, rows, each, (int)K, stages, p, ldy);
   };
   if (dtype == B2Q_DTYPE_F32)
     launch(wide ? mx_dequantize_kernel<true, float> : mx_dequantize_kernel<false, float>, static_cast<float*>(y));
@@ -273,10 +289,8 @@ int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, in
                 b2q_stream_t stream) {
   const char* who = "b2q_mx_pack";
   int rc = check_mx_shape(who, rows, K);
-  if (rc) return rc;
-  if (experts < 1 || experts > kMaxExperts)
-    return fail(B2Q_EINVAL, "%s: %lld experts (1..%lld)", who, (long long)experts, (long long)kMaxExperts);
-  if (rows == 0) return B2Q_OK;
+  if (!rc) rc = check_experts(who, experts);
+  if (rc || rows == 0) return rc;
   if (!codes || !scales || !image) return fail(B2Q_EINVAL, "%s: null pointer", who);
   if (!aligned(codes, 16) || !aligned(image, 128))
     return fail(B2Q_EALIGN, "%s: codes must be 16-byte aligned, the image 128-byte", who);

@@ -129,7 +129,7 @@ def workspace_size(plan, w, gather=True):
 def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     """Each sorted row, quantized to MXFP4, times its expert's weights w (MXTensor [E][N][K]) -> [T * top][N] of `dtype`
     (default: x's) in sorted order; rows past plan.offsets[E] stay unwritten. x: [T][K], a token's row for each of its choices,
-    or with gather=False the sorted rows [T * top][K]. workspace: a CUDA uint8 tensor of workspace_size(plan, w, gather)
+    or with gather=False the sorted rows [T * top][K]. out: the tensor for the result (it shares no memory with x). workspace: a CUDA uint8 tensor of workspace_size(plan, w, gather)
     bytes, 128-byte aligned (allocated here when None)."""
     if not isinstance(w, MXTensor):
         raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
@@ -168,7 +168,8 @@ def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
 
 def combine(y, plan, weights=None, out=None):
     """Sorted rows y [T * top][N] back to their tokens -> [T][N] of y's type: the sum of weights[t][j] (f32 [T][top]; None: 1) times
-    y[pos[t][j]], in f32 and in order of j. A choice that goes nowhere adds nothing."""
+    y[pos[t][j]], in f32 and in order of j. A choice that goes nowhere adds nothing.
+    out: the tensor for the result (it shares no memory with y)."""
     _check_plan("combine", plan)
     dev = plan.device
     _on_device("combine", dev, y)

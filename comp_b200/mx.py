@@ -51,15 +51,21 @@ def _check_k(name, k):
         raise ValueError(f"{name}: K={k} is not a positive multiple of the MXFP4 block (32)")
 
 
+def _check_experts(name, experts):
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise ValueError(f"{name}: {experts} experts (1..{MAX_EXPERTS})")
+
+
 class MXTensor:
-    """An MXFP4 operand [rows][k], or [experts][rows][k], as its image: uint8, 128-byte aligned (include/comp_b200.h)."""
+    """An MXFP4 operand [rows][k], or [experts][rows][k], as its image: uint8, 128-byte aligned, as quantize, pack and from_ggml
+    make it (include/comp_b200.h)."""
 
     def __init__(self, image, rows, k, experts=None):
         _check_k("MXTensor", k)
         if rows < 0:
             raise ValueError(f"MXTensor: {rows} rows")
-        if experts is not None and not 1 <= experts <= MAX_EXPERTS:
-            raise ValueError(f"MXTensor: {experts} experts (1..{MAX_EXPERTS})")
+        if experts is not None:
+            _check_experts("MXTensor", experts)
         if not isinstance(image, torch.Tensor) or image.device.type != "cuda":
             raise RuntimeError("comp_b200.MXTensor: the image must be a CUDA tensor (this backend has no CPU path)")
         if image.dtype != torch.uint8:
@@ -113,35 +119,34 @@ def _stride(t):
 
 
 def quantize(x):
-    """x [M][K] (f32, f16 or bf16; any strides) -> MXTensor. Each block of 32 values along K takes the power of two that brings
-    its largest magnitude to 4 .. 8; values are rounded to nearest even and cut off at 6. Blocks with an infinity or a NaN
-    are NaN."""
+    """x [M][K], or [experts][M][K] (f32, f16 or bf16; any strides) -> MXTensor. Each block of 32 values along K takes the power
+    of two that brings its largest magnitude to 4 .. 8; values are rounded to nearest even and cut off at 6. Blocks with an
+    infinity or a NaN are NaN."""
     dev = _cuda("quantize", x)
     did = _dtype_id("quantize: x", x)
-    if x.dim() != 2:
-        raise ValueError(f"quantize: x {tuple(x.shape)}, expected [M][K]")
+    experts = None
+    if x.dim() == 3:
+        experts = x.shape[0]
+        _check_experts("quantize", experts)
+        x = x.flatten(0, 1)
+    elif x.dim() != 2:
+        raise ValueError(f"quantize: x {tuple(x.shape)}, expected [M][K] or [experts][M][K]")
     m, k = x.shape
     _check_k("quantize", k)
+    each = m if experts is None else m // experts
     x, at, ldx = _rows(x)
-    image = x.new_empty(image_bytes(m, k), dtype=torch.uint8)
-    _enter(dev, _lib.load().b2q_mx_quantize, did, at, ldx, m, k, image.data_ptr())
-    return MXTensor._made(image, m, k)
+    image = x.new_empty(image_bytes(each, k, experts or 1), dtype=torch.uint8)
+    _enter(dev, _lib.load().b2q_mx_quantize, did, at, ldx, experts or 1, each, k, image.data_ptr())
+    return MXTensor._made(image, each, k, experts)
 
 
 def dequantize(t, dtype=torch.float32):
     """The values of an MXTensor, each rounded once to `dtype`: [rows][k], or [experts][rows][k]."""
     if not isinstance(t, MXTensor):
         raise TypeError(f"dequantize: expected an MXTensor, got {type(t).__name__}")
-    did = DTYPE_ID.get(dtype)
-    if did is None:
-        raise TypeError(f"dequantize: dtype {dtype}, expected float32, float16 or bfloat16")
-    dev = t.device
+    did = _out_dtype("dequantize", dtype)
     y = t.image.new_empty(t.shape, dtype=dtype)
-    at, to, entry = t.image.data_ptr(), y.data_ptr(), _lib.load().b2q_mx_dequantize
-    for _ in range(t.experts or 1):
-        _enter(dev, entry, at, t.rows, t.k, did, to, t.k)
-        at += image_bytes(t.rows, t.k)
-        to += t.rows * t.k * y.element_size()
+    _enter(t.device, _lib.load().b2q_mx_dequantize, t.image.data_ptr(), t.experts or 1, t.rows, t.k, did, y.data_ptr(), t.k)
     return y
 
 
@@ -157,8 +162,8 @@ def pack(codes, scales):
     n, k = codes.shape[-2], codes.shape[-1] * 2
     _check_k("pack", k)
     experts = codes.shape[0] if codes.dim() == 3 else None
-    if experts is not None and not 1 <= experts <= MAX_EXPERTS:
-        raise ValueError(f"pack: {experts} experts (1..{MAX_EXPERTS})")
+    if experts is not None:
+        _check_experts("pack", experts)
     codes, scales = codes.contiguous(), scales.contiguous()
     if codes.data_ptr() % 16:
         codes = codes.clone()
@@ -199,7 +204,7 @@ def _out_dtype(name, dtype):
 
 def matmul(a, w, dtype=torch.bfloat16, out=None):
     """MXTensors a [M][K] and w [N][K] -> a w^T [M][N]: exact products, f32 sums, rounded once to `dtype`. out: the tensor for
-    the result (any row stride)."""
+    the result (any row stride; it shares no memory with the operands)."""
     for t, name in ((a, "a"), (w, "w")):
         if not isinstance(t, MXTensor):
             raise TypeError(f"matmul: {name} must be an MXTensor, got {type(t).__name__}")
@@ -228,7 +233,8 @@ def _few_size(w, key, name, *args):
 
 
 def linear(x, w, dtype=None, out=None):
-    """x [M][K] (f32, f16 or bf16; any strides), quantized to MXFP4, times w [N][K] -> [M][N] of `dtype` (default: x's)."""
+    """x [M][K] (f32, f16 or bf16; any strides), quantized to MXFP4, times w [N][K] -> [M][N] of `dtype` (default: x's).
+    out: the tensor for the result (any row stride; it shares no memory with x)."""
     if not isinstance(w, MXTensor):
         raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
     if w.experts is not None:

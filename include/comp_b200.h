@@ -387,14 +387,17 @@ int b2q_attention(const b2q_kv_cache* cache, const b2q_attention_args* args, voi
 size_t b2q_mx_bytes(int64_t experts, int64_t rows, int64_t K);
 
 /*
- * Quantizes x [rows][K] (dtype B2Q_DTYPE_*, row stride ldx elements, 16-byte aligned in base and row stride) into an image:
- * per block s = max(0, floor(log2 max|x|) + 125), values x / 2^(s - 127) rounded to nearest even, those above 6 cut off to 6.
- * A block with an infinity or a NaN is NaN (s = 255, codes 0); one of zeros has s = 0. Asynchronous on `stream`.
+ * Quantizes x [experts * rows][K] (dtype B2Q_DTYPE_*, row stride ldx elements, 16-byte aligned in base and row stride) into an
+ * image of `experts` operands: per block s = max(0, floor(log2 max|x|) + 125), values x / 2^(s - 127) rounded to nearest even,
+ * those above 6 cut off to 6. A block with an infinity or a NaN is NaN (s = 255, codes 0); one of zeros has s = 0. Asynchronous
+ * on `stream`.
  */
-int b2q_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t K, uint8_t* image, b2q_stream_t stream);
+int b2q_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t experts, int64_t rows, int64_t K, uint8_t* image,
+                    b2q_stream_t stream);
 
-/* The values of an image, each rounded once to dtype, into y [rows][K] (16-byte aligned in base and row stride). */
-int b2q_mx_dequantize(const uint8_t* image, int64_t rows, int64_t K, int dtype, void* y, int64_t ldy, b2q_stream_t stream);
+/* The values of an image, each rounded once to dtype, into y [experts * rows][K] (16-byte aligned in base and row stride). */
+int b2q_mx_dequantize(const uint8_t* image, int64_t experts, int64_t rows, int64_t K, int dtype, void* y, int64_t ldy,
+                      b2q_stream_t stream);
 
 /* Planes codes [experts][rows][K/2] (16-byte aligned) and scales [experts][rows][K/32], contiguous, into an image. */
 int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, int64_t rows, int64_t K, uint8_t* image,
@@ -403,7 +406,8 @@ int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, in
 /*
  * y[m][n] = sum over blocks of 2^(sa - 127) 2^(sw - 127) * sum over the block of a w: images a of [M][K] and w of [N][K], y
  * [M][N] of dtype with row stride ldy. Products are exact, sums are f32 (the tensor cores', in an order that depends on M, N
- * and K alone), rounded once to dtype. A NaN block makes its row (of a) or column (of w) NaN.
+ * and K alone), rounded once to dtype. A NaN block makes its row (of a) or column (of w) NaN. y shares no memory with the
+ * operands (here, below and of x).
  */
 int b2q_mx_matmul(const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y, int64_t ldy,
                   b2q_stream_t stream);

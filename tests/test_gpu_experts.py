@@ -5,6 +5,8 @@ by half a unit of the difference (2^-24 of at most 104, where exp is 0), the sum
 (2^-21 + 104 * 2^-24 + n * 2^-24) of the weight, and 2^-149 where it is next to 0. Products: see test_gpu_mx. A combined sum of n
 rows is off by n * 2^-24 * mass before its own rounding."""
 
+import os
+
 import numpy as np
 import pytest
 import torch
@@ -215,6 +217,14 @@ def test_layer(cuda, tokens):
         graph.replay()
         assert torch.equal(got, layer(x.roll(i, 1), logits.roll(i, 1), tu, td, top))
     assert device_error() == 0
+
+
+def test_example(cuda):
+    import runpy
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    main = runpy.run_path(os.path.join(root, "examples", "expert_layer.py"))["main"]
+    assert main(["--hidden", "512", "--inner", "192", "--experts", "12", "--top", "3", "--prompt", "40", "--steps", "3"]) == 0
 
 
 def test_no_tokens(cuda):

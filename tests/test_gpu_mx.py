@@ -187,6 +187,21 @@ def test_no_rows(cuda):
     assert mx.matmul(w, none).shape == (40, 0) and mx.linear(torch.ones((3, 64), device=cuda), none).shape == (3, 0)
 
 
+@pytest.mark.parametrize("dtype", DT)
+def test_experts_in_one_tensor(cuda, dtype):
+    """Operands of experts begin at whole tiles, whatever their rows."""
+    rng = np.random.default_rng(6)
+    for shape in ((1, 5, 32), (3, 1, 96), (4, 128, 64), (3, 200, 288), (1024, 2, 32)):
+        x = torch.from_numpy(rng.standard_normal(shape)).to(DT[dtype])
+        want = ref.values(*ref.quantize(x.float().numpy()))
+        t = mx.quantize(x.to(cuda))
+        assert t.shape == shape and t.nbytes == t.image.numel()
+        assert np.array_equal(mx.dequantize(t).double().cpu().numpy(), want)
+        assert torch.equal(mx.dequantize(packed(ref.quantize(x.float().numpy()), cuda)).double().cpu(), torch.from_numpy(want))
+    t = mx.quantize(torch.randn((96, 3, 8), device=cuda).permute(1, 2, 0))  # any strides
+    assert t.shape == (3, 8, 96)
+
+
 def test_from_ggml(cuda):
     rng = np.random.default_rng(2)
     codes, scales = planes(rng, (3, 50, 96))
@@ -196,6 +211,35 @@ def test_from_ggml(cuda):
     assert np.array_equal(mx.dequantize(t).double().cpu().numpy(), ref.values(codes, scales))
     one = mx.from_ggml(torch.from_numpy(blocks[1].reshape(-1)).to(cuda), 50, 96)
     assert torch.equal(mx.dequantize(one), mx.dequantize(t)[1])
+
+
+def test_gguf(cuda, tmp_path):
+    """A weight and a layer of experts through a GGUF file, against gguf-py's own reading of the blocks."""
+    gguf = pytest.importorskip("gguf")
+    from comp_b200 import gguf_io
+
+    rng = np.random.default_rng(4)
+    one, many = planes(rng, (40, 96), 5.0), planes(rng, (3, 20, 64), 5.0)
+    kind = gguf.GGMLQuantizationType.MXFP4
+    path = str(tmp_path / "w.gguf")
+    w = gguf.GGUFWriter(path, "test")
+    blocks = {}
+    for name, (codes, scales) in (("one", one), ("many", many)):
+        b = np.concatenate([scales[..., None], codes.reshape(*scales.shape, 16)], -1)
+        blocks[name] = b.reshape(*scales.shape[:-1], -1)
+        w.add_tensor(name, blocks[name], raw_dtype=kind)
+    w.add_tensor("plain", np.zeros((4, 32), dtype=np.float32))
+    w.write_header_to_file(), w.write_kv_data_to_file(), w.write_tensors_to_file(), w.close()
+    for name, (codes, scales) in (("one", one), ("many", many)):
+        t = gguf_io.load_mx(path, name, device=cuda)
+        assert t.shape == (*scales.shape[:-1], scales.shape[-1] * 32)
+        got = mx.dequantize(t).cpu().numpy()
+        assert np.array_equal(got.astype(np.float64), ref.values(codes, scales))
+        assert np.array_equal(got, gguf.dequantize(blocks[name], kind))
+    with pytest.raises(ValueError):
+        gguf_io.load_mx(path, "plain", device=cuda)
+    with pytest.raises(KeyError):
+        gguf_io.load_mx(path, "none", device=cuda)
 
 
 @pytest.mark.parametrize("m", [1, 70, 300])

@@ -42,13 +42,14 @@ def test_plan_words(lib):
 
 
 def test_quantize_refusals(lib):
-    q = lambda dtype=0, x=4096, ldx=64, rows=2, k=64, image=4096: lib.b2q_mx_quantize(dtype, x, ldx, rows, k, image, None)  # noqa: E731
+    q = lambda dtype=0, x=4096, ldx=64, rows=2, k=64, image=4096, e=1: lib.b2q_mx_quantize(dtype, x, ldx, e, rows, k, image, None)  # noqa: E731
     assert q(dtype=3) == -1 and q(x=None) == -1 and q(image=None) == -1 and q(rows=-1) == -1 and q(k=48) == -1 and q(ldx=32) == -1
+    assert q(e=0) == -1 and q(e=1025) == -1 and q(e=2, rows=1, ldx=32) == -1
     assert q(x=4100) == -2 and q(ldx=66) == -2 and q(image=4096 + 64) == -2 and q(dtype=1, ldx=68) == -2
     assert q(rows=0, x=None, image=None) == 0
-    d = lambda image=4096, rows=2, k=64, dtype=0, y=4096, ldy=64: lib.b2q_mx_dequantize(image, rows, k, dtype, y, ldy, None)  # noqa: E731
+    d = lambda image=4096, rows=2, k=64, dtype=0, y=4096, ldy=64, e=1: lib.b2q_mx_dequantize(image, e, rows, k, dtype, y, ldy, None)  # noqa: E731
     assert d(image=None) == -1 and d(y=None) == -1 and d(dtype=-1) == -1 and d(k=0) == -1 and d(ldy=63) == -1
-    assert d(y=4104) == -2 and d(ldy=65) == -2 and d(rows=0) == 0
+    assert d(y=4104) == -2 and d(ldy=65) == -2 and d(rows=0) == 0 and d(e=0) == -1
     p = lambda codes=4096, scales=4096, e=1, rows=2, k=64, image=4096: lib.b2q_mx_pack(codes, scales, e, rows, k, image, None)  # noqa: E731
     assert p(codes=None) == -1 and p(scales=None) == -1 and p(image=None) == -1 and p(e=0) == -1 and p(e=1025) == -1 and p(k=20) == -1
     assert p(codes=4100) == -2 and p(image=64) == -2 and p(rows=0) == 0
