@@ -216,10 +216,17 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
               for (int c = 0; c < 32; ++c)
                 asm volatile("st.shared.u32 [%0], %1;" ::"r"(mine + c * 512), "r"(v[c >> 4][c & 15]) : "memory");
             } else if (n < g.N) {
-              const int64_t to = (int64_t)(at.row0 + c0) * g.ldy + n;
+              with_type(g.y, g.dtype, [&](auto* y) {
+                auto* to = y + (int64_t)(at.row0 + c0) * g.ldy + n;
+                if (c0 + 32 <= at.n) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (c0 + c < at.n) store_as(g.y, to + c * g.ldy, g.dtype, __uint_as_float(v[c >> 4][c & 15]));
+                  for (int c = 0; c < 32; ++c, to += g.ldy) store_one(to, __uint_as_float(v[c >> 4][c & 15]));
+                } else {
+#pragma unroll
+                  for (int c = 0; c < 32; ++c, to += g.ldy)
+                    if (c0 + c < at.n) store_one(to, __uint_as_float(v[c >> 4][c & 15]));
+                }
+              });
             }
           }
         }
@@ -248,9 +255,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
             for (int i = 0; i < 8; ++i) sum[i] += part[i];
           }
           if (n < g.N && !s_abort)
+            with_type(g.y, g.dtype, [&](auto* y) {
+              auto* to = y + (int64_t)(at.row0 + c) * g.ldy + n;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (c + i < c1) store_as(g.y, (int64_t)(at.row0 + c + i) * g.ldy + n, g.dtype, sum[i]);
+              for (int i = 0; i < 8; ++i, to += g.ldy)
+                if (c + i < c1) store_one(to, sum[i]);
+            });
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring's next stages come through the other proxy
@@ -309,6 +319,34 @@ int launch_tile(const MxGemm& g, int ctas, int ranks, cudaStream_t stream) {
 
 }  // namespace
 
+// Rows of x a tile, and CTAs that share its K.
+struct Shape {
+  int tn, ranks;
+};
+
+// The shape that takes least time by what rounds of tiles take, us. Measured on layers of 1000 to 14336 rows, K of 1024 to 8192,
+// with 16 to 2048 rows of x and all shapes: a stage of a tile with n rows takes 0.28 (n = 64), 0.33 (128), 0.45 (256); its
+// epilogue 2, 2.6, 4, beside the next tile's products; joining parts of K 1 + n / 50. Chosen / the next best, us: 8192 x 8192 with 64
+// rows 13.3 (K in 2) / 15.1 (whole), with 256 rows 17.2 (128 a tile) / 19.5 (256), with 512 rows 21.2 (256) / 30.7 (128); 4096 x
+// 4096 with 256 rows 10.2 (64) / 11.2 (128). Clusters of 8 wait for as many free SMs of a kind: 2048 x 8192 with 16 rows 14.8, K in 4
+// parts 8.4.
+static Shape choose_shape(int64_t used, int64_t each, int64_t row_tiles, int64_t stages, int sms) {
+  Shape best = {64, 1};
+  double least = 1e30;
+  for (int tn : {64, 128, 256})
+    for (int ranks : {1, 2, 4}) {
+      const int64_t tiles = used * ((each + tn - 1) / tn) * row_tiles;
+      if (ranks > 1 && (tn == 256 || tiles * ranks > sms || stages < 2 * ranks)) continue;
+      const double n = (double)std::min<int64_t>(each, tn);
+      const double stage = n <= 64 ? 0.28 : n <= 128 ? 0.28 + (n - 64) * 0.0008 : 0.33 + (n - 128) * 0.00094;
+      const double work = (double)((stages + ranks - 1) / ranks) * stage, after = 1.3 + n / 96;
+      const double rounds = (double)((tiles + sms / ranks - 1) / (sms / ranks));
+      const double time = (rounds - 1) * std::max(work, after) + work + after + (ranks > 1 ? 1 + n / 50 : 0);
+      if (time < least) least = time, best = {tn, ranks};
+    }
+  return best;
+}
+
 int launch_mx_gemm(const MxGemm& g, cudaStream_t stream) {
   if (g.rows == 0 || g.N == 0) return B2Q_OK;
   DeviceInfo dev;
@@ -317,14 +355,11 @@ int launch_mx_gemm(const MxGemm& g, cudaStream_t stream) {
   // rows an expert has on average, of the experts that can have any
   const int64_t used = g.offsets ? std::min<int64_t>(g.experts, g.rows) : 1;
   const int64_t each = (g.rows + used - 1) / used;
-  int tn = each <= 64 ? 64 : each <= 128 ? 128 : 256;
-  while (tn > 64 && used * ((each + tn - 1) / tn) * g.row_tiles < dev.sms) tn /= 2;
-  const int64_t tiles = used * ((each + tn - 1) / tn) * g.row_tiles;
+  const Shape shape = choose_shape(used, each, g.row_tiles, g.stages, dev.sms);
+  const int tn = shape.tn, ranks = shape.ranks;
   // every tile that there can be: each expert's last one may be all but empty
   const int64_t most = ((g.rows + tn - 1) / tn + (g.offsets ? used : 0)) * g.row_tiles;
   if (most > INT32_MAX / 2) return fail(B2Q_ERANGE, "mx_gemm: too many tiles");
-  int ranks = 1;
-  while (ranks < 8 && tiles * ranks * 2 <= dev.sms && g.stages >= ranks * 4 && tn <= 128) ranks *= 2;
   const int ctas = (int)std::min<int64_t>(most, dev.sms / ranks);
   switch (tn) {
     case 64: return ranks > 1 ? launch_tile<64, true>(g, ctas, ranks, stream) : launch_tile<64, false>(g, ctas, 1, stream);

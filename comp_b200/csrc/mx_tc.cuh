@@ -41,6 +41,16 @@ __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uin
       "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
       : "memory");
 }
+__device__ __forceinline__ void store_one(float* y, float v) { *y = v; }
+__device__ __forceinline__ void store_one(__half* y, float v) { *y = __float2half_rn(v); }
+__device__ __forceinline__ void store_one(__nv_bfloat16* y, float v) { *y = __float2bfloat16_rn(v); }
+// f(y as its type): the type is looked at once for all that f stores
+template <typename F>
+__device__ __forceinline__ void with_type(void* y, int dtype, F f) {
+  if (dtype == B2Q_DTYPE_BF16) f(static_cast<__nv_bfloat16*>(y));
+  else if (dtype == B2Q_DTYPE_F16) f(static_cast<__half*>(y));
+  else f(static_cast<float*>(y));
+}
 __device__ __forceinline__ void store_as(void* y, int64_t at, int dtype, float v) {
   if (dtype == B2Q_DTYPE_BF16)
     static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
