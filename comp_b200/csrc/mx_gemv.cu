@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     }
     __syncwarp();
   } else {
-    // quantize: two threads a block; `per` threads a row, or all for each of several rows at a time
+    // quantizing: two threads a block; `per` threads a row, or all for each of several rows at a time
     const int t0 = threadIdx.x - 64, per = nk * 16, together = max(1, 256 / per), mine = per < 256 ? t0 / per : 0;
     const int last = mine < together ? per : 0;
     int in = t0 - mine * per;
@@ -277,7 +277,7 @@ struct GemvPlan {
 bool plan_gemv(int64_t rows, int64_t used, int64_t row_tiles, int64_t stages, int sms, GemvPlan* p) {
   if (rows < 1 || rows > kMaxRows || used * row_tiles > INT32_MAX / 2) return false;
   int ranks = 1;
-  while (ranks < 8 && used * row_tiles * ranks * 2 <= sms && stages >= ranks * 4) ranks *= 2;
+  while (ranks < 8 && used * row_tiles * ranks * 2 <= sms && stages >= ranks * 2) ranks *= 2;
   const int64_t nk = (stages + ranks - 1) / ranks;
   if (nk > (512 - (int)kScaleX) / 4) return false;
   const size_t x = (size_t)(nk + 1) * kXStage + nk * 512 + 1024;  // 1024: the ring is aligned to that
