@@ -13,9 +13,9 @@ kernels are this package's own, through the C-ABI (include/comp_b200.h, where la
 import torch
 
 from . import _lib
-from .kv import _dtype_id, _on_device
+from .kv import DTYPE_ID, _dtype_id
 from .mx import (FUSED_ROWS, MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _enter, _few_size,
-                 _out_dtype, _rows, _stride)
+                 _out_dtype, _rows, _same, _stride)
 
 MAX_TOP = 32
 
@@ -28,11 +28,16 @@ class Plan:
 
     def __init__(self, tokens, top, experts, like, ids=None):
         choices = tokens * top
-        self.tokens, self.top, self.experts, self.device = tokens, top, experts, like.device
+        self.tokens, self.top, self.experts = tokens, top, experts
         words = 2 * (experts + 1) + 4 * choices if tokens <= 128 and choices <= 4096 else \
             _lib.load().b2q_experts_plan_words(tokens, top, experts)
         self._ids, self._routed = ids, words if ids is None else 0  # (routed: ids and weights follow the plan's own words)
         self._words = like.new_empty(words + 2 * choices if ids is None else words, dtype=torch.int32)
+        self._at, self._index = self._words.data_ptr(), self._words.get_device()
+
+    @property
+    def device(self):
+        return self._words.device
 
     def _part(self, at, rows=True):
         if rows:
@@ -73,8 +78,10 @@ def route(logits, top, normalize=True):
     """logits [T][E] (f32, f16 or bf16) -> Plan of the `top` largest of each token: plan.ids (falling; the lowest index first
     among equals) and plan.weights, their softmax over the chosen, or (normalize=False) over all E. -inf and NaN are never
     chosen: a token with fewer others has ids -1, of weight 0, that go nowhere."""
-    dev = _cuda("route", logits)
-    did = _dtype_id("route: logits", logits)
+    index = _cuda("route", logits)
+    did = DTYPE_ID.get(logits.dtype)
+    if did is None:
+        _dtype_id("route: logits", logits)
     if logits.dim() != 2:
         raise ValueError(f"route: logits {tuple(logits.shape)}, expected [T][E]")
     if not isinstance(top, int):
@@ -83,21 +90,24 @@ def route(logits, top, normalize=True):
     _check_sizes("route", tokens, top, experts)
     if top > experts:
         raise ValueError(f"route: {top} choices of {experts} experts")
-    s0, s1 = logits.stride()
-    if (s1 != 1 and experts > 1) or (tokens > 1 and s0 < experts):
-        logits = logits.clone(memory_format=torch.contiguous_format)
+    ld = experts
+    if not logits.is_contiguous():
+        s0, s1 = logits.stride()
+        if (s1 != 1 and experts > 1) or (tokens > 1 and s0 < experts):
+            logits = logits.clone(memory_format=torch.contiguous_format)
+        ld = _stride(logits)
     plan = Plan(tokens, top, experts, logits)
-    words = plan._words.data_ptr()
+    words = plan._at
     ids = words + 4 * plan._routed
-    _enter(dev, _lib.load().b2q_experts_route, did, logits.data_ptr(), _stride(logits), tokens, experts, top, 1 if normalize else 0,
-           ids, ids + 4 * tokens * top, words)
+    _enter(index, _lib.load().b2q_experts_route, did, logits.data_ptr(), ld, tokens, experts, top, 1 if normalize else 0, ids,
+           ids + 4 * tokens * top, words)
     return plan
 
 
 def sort(ids, experts):
     """ids int32 [T][top], the experts of each token -> Plan. Negative ids go nowhere (experts held elsewhere, padding); so do
     ids beyond the experts, which set the device error word to 5."""
-    dev = _cuda("sort", ids)
+    index = _cuda("sort", ids)
     if ids.dtype != torch.int32:
         raise TypeError(f"sort: ids dtype {ids.dtype}, expected torch.int32")
     if ids.dim() != 2:
@@ -108,7 +118,7 @@ def sort(ids, experts):
     _check_sizes("sort", tokens, top, experts)
     ids = ids.contiguous()
     plan = Plan(tokens, top, experts, ids, ids)
-    _enter(dev, _lib.load().b2q_experts_sort, ids.data_ptr(), tokens, top, experts, plan._words.data_ptr())
+    _enter(index, _lib.load().b2q_experts_sort, ids.data_ptr(), tokens, top, experts, plan._at)
     return plan
 
 
@@ -136,33 +146,37 @@ def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     _check_plan("linear", plan)
     if w.experts != plan.experts:
         raise ValueError(f"linear: w {w.shape}, expected [{plan.experts}][N][K]")
-    dev, n, k = w.device, w.rows, w.k
-    if plan.device != dev:
-        raise RuntimeError(f"comp_b200.linear: tensors on different devices ({dev} and {plan.device})")
-    _on_device("linear", dev, x)
-    xid = _dtype_id("linear: x", x)
-    choices = plan.tokens * plan.top
-    if x.dim() != 2 or x.shape != (plan.tokens if gather else choices, k):
-        raise ValueError(f"linear: x {tuple(x.shape)}, expected [{plan.tokens if gather else choices}][{k}]")
-    if dtype is None:
-        dtype = x.dtype
-    did = _out_dtype("linear", dtype)
+    index, n, k, tokens, top = w._index, w.rows, w.k, plan.tokens, plan.top
+    if plan._index != index:
+        raise RuntimeError(f"comp_b200.linear: tensors on different devices ({w.device} and {plan.device})")
+    _same("linear", index, x)
+    given = x.dtype
+    xid = DTYPE_ID.get(given)
+    if xid is None:
+        _dtype_id("linear: x", x)
+    choices = tokens * top
+    if x.shape != (tokens if gather else choices, k):
+        raise ValueError(f"linear: x {tuple(x.shape)}, expected [{tokens if gather else choices}][{k}]")
+    if dtype is None or dtype is given:
+        dtype, did = given, xid
+    else:
+        did = _out_dtype("linear", dtype)
     x, x_at, ldx = _rows(x)
     if out is None:
-        out = x.new_empty((choices, n), dtype=dtype)
+        out = x.new_empty((choices, n)) if did == xid else x.new_empty((choices, n), dtype=dtype)
         at, ldy = out.data_ptr(), n
     else:
-        at, ldy = _check_out("linear", out, dtype, (choices, n), dev)
+        at, ldy = _check_out("linear", out, dtype, (choices, n), index)
     if workspace is None:
         need = workspace_size(plan, w, gather)
         workspace = x.new_empty(need, dtype=torch.uint8) if need else None
     else:
-        _on_device("linear", dev, workspace)
+        _same("linear", index, workspace)
         if not workspace.is_contiguous():
             raise ValueError("linear: workspace must be contiguous")
         need = workspace.numel() * workspace.element_size()
-    _enter(dev, _lib.load().b2q_experts_linear, xid, x_at, ldx, 1 if gather else 0, w.image.data_ptr(), plan._words.data_ptr(),
-           plan.tokens, plan.top, plan.experts, n, k, did, at, ldy, 0 if workspace is None else workspace.data_ptr(), need)
+    _enter(index, _lib.load().b2q_experts_linear, xid, x_at, ldx, 1 if gather else 0, w._at, plan._at, tokens, top, plan.experts, n, k,
+           did, at, ldy, 0 if workspace is None else workspace.data_ptr(), need)
     return out
 
 
@@ -171,30 +185,34 @@ def combine(y, plan, weights=None, out=None):
     y[pos[t][j]], in f32 and in order of j. A choice that goes nowhere adds nothing.
     out: the tensor for the result (it shares no memory with y)."""
     _check_plan("combine", plan)
-    dev = plan.device
-    _on_device("combine", dev, y)
-    did = _dtype_id("combine: y", y)
-    choices = plan.tokens * plan.top
-    if y.dim() != 2 or y.shape[0] != choices:
-        raise ValueError(f"combine: y {tuple(y.shape)}, expected [{choices}][N]")
-    n = y.shape[1]
+    index, tokens, top = plan._index, plan.tokens, plan.top
+    _same("combine", index, y)
+    did = DTYPE_ID.get(y.dtype)
+    if did is None:
+        _dtype_id("combine: y", y)
+    shape, choices = y.shape, tokens * top
+    if len(shape) != 2 or shape[0] != choices:
+        raise ValueError(f"combine: y {tuple(shape)}, expected [{choices}][N]")
+    n = shape[1]
+    w_at = 0
     if weights is not None:
-        _on_device("combine", dev, weights)
-        if weights.dtype != torch.float32:
+        _same("combine", index, weights)
+        if weights.dtype is not torch.float32:
             raise TypeError(f"combine: weights dtype {weights.dtype}, expected torch.float32")
-        if weights.shape != (plan.tokens, plan.top):
-            raise ValueError(f"combine: weights {tuple(weights.shape)}, expected ({plan.tokens}, {plan.top})")
-        weights = weights.contiguous()
+        if weights.shape != (tokens, top):
+            raise ValueError(f"combine: weights {tuple(weights.shape)}, expected ({tokens}, {top})")
+        if not weights.is_contiguous():
+            weights = weights.contiguous()
+        w_at = weights.data_ptr()
     ldy = n
     if not y.is_contiguous():
         if (n > 1 and y.stride(1) != 1) or (choices > 1 and y.stride(0) < n):
             y = y.clone(memory_format=torch.contiguous_format)
         ldy = _stride(y)
     if out is None:
-        out = y.new_empty((plan.tokens, n))
+        out = y.new_empty((tokens, n))
         at, ldo = out.data_ptr(), n
     else:
-        at, ldo = _check_out("combine", out, y.dtype, (plan.tokens, n), dev)
-    _enter(dev, _lib.load().b2q_experts_combine, did, y.data_ptr(), ldy, plan._words.data_ptr(),
-           0 if weights is None else weights.data_ptr(), plan.tokens, plan.top, plan.experts, n, at, ldo)
+        at, ldo = _check_out("combine", out, y.dtype, (tokens, n), index)
+    _enter(index, _lib.load().b2q_experts_combine, did, y.data_ptr(), ldy, plan._at, w_at, tokens, top, plan.experts, n, at, ldo)
     return out

@@ -31,13 +31,13 @@ def image_bytes(rows, k, experts=1):
     return experts * -(-rows // TILE_ROWS) * -(-k // STAGE) * STAGE_BYTES
 
 
-def _enter(dev, entry, *args):
-    """The library's entry on dev and its current stream (the last argument)."""
-    if _current_device() == dev.index:
-        rc = entry(*args, _raw_stream(dev.index))
+def _enter(index, entry, *args):
+    """The library's entry on device `index` and its current stream (the last argument)."""
+    if _current_device() == index:
+        rc = entry(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = entry(*args, _raw_stream(dev.index))
+        with torch.cuda.device(index):
+            rc = entry(*args, _raw_stream(index))
     if rc:
         raise (ValueError if rc in (-1, -2, -4) else _error(rc))(_lib.last_error())
 
@@ -73,15 +73,22 @@ class MXTensor:
         need = image_bytes(rows, k, experts or 1)
         if image.dim() != 1 or image.numel() < need or not image.is_contiguous() or (need and image.data_ptr() % 128):
             raise ValueError(f"MXTensor: the image must be {need} contiguous bytes, 128-byte aligned, got {tuple(image.shape)}")
-        self.image, self.rows, self.k, self.experts, self.device = image, rows, k, experts, image.device
-        self._sizes = {}  # workspaces of products with few rows
+        self._set(image, rows, k, experts)
 
     @classmethod
     def _made(cls, image, rows, k, experts=None):
         self = cls.__new__(cls)
-        self.image, self.rows, self.k, self.experts, self.device = image, rows, k, experts, image.device
-        self._sizes = {}
+        self._set(image, rows, k, experts)
         return self
+
+    def _set(self, image, rows, k, experts):
+        self.image, self.rows, self.k, self.experts = image, rows, k, experts
+        self._at, self._index = image.data_ptr(), image.get_device()
+        self._sizes = {}  # workspaces of products with few rows
+
+    @property
+    def device(self):
+        return self.image.device
 
     @property
     def shape(self):
@@ -96,18 +103,25 @@ class MXTensor:
 
 
 def _cuda(name, t):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    """The number of a CUDA tensor's device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f"comp_b200.{name}: tensors must be CUDA tensors (this backend has no CPU path)")
-    return t.device
+    return t.get_device()
+
+
+def _same(name, index, t):
+    """Raises unless t is a tensor on CUDA device `index`."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        _on_device(name, torch.device("cuda", index), t)
 
 
 def _rows(t):
     """(t, its address, its row stride): unit column stride, a 16-byte aligned base and rows that do not overlap (a copy only
     when needed)."""
-    at, (m, k) = t.data_ptr(), t.shape
+    at = t.data_ptr()
     if t.is_contiguous() and not at & 15:
-        return t, at, k
-    s0, s1 = t.stride()
+        return t, at, t.shape[1]
+    (m, k), (s0, s1) = t.shape, t.stride()
     if s1 != 1 or at & 15 or (m > 1 and (s0 * t.element_size() & 15 or s0 < k)):
         t = t.clone(memory_format=torch.contiguous_format)
         return t, t.data_ptr(), k
@@ -122,8 +136,10 @@ def quantize(x):
     """x [M][K], or [experts][M][K] (f32, f16 or bf16; any strides) -> MXTensor. Each block of 32 values along K takes the power
     of two that brings its largest magnitude to 4 .. 8; values are rounded to nearest even and cut off at 6. Blocks with an
     infinity or a NaN are NaN."""
-    dev = _cuda("quantize", x)
-    did = _dtype_id("quantize: x", x)
+    index = _cuda("quantize", x)
+    did = DTYPE_ID.get(x.dtype)
+    if did is None:
+        _dtype_id("quantize: x", x)
     experts = None
     if x.dim() == 3:
         experts = x.shape[0]
@@ -136,7 +152,7 @@ def quantize(x):
     each = m if experts is None else m // experts
     x, at, ldx = _rows(x)
     image = x.new_empty(image_bytes(each, k, experts or 1), dtype=torch.uint8)
-    _enter(dev, _lib.load().b2q_mx_quantize, did, at, ldx, experts or 1, each, k, image.data_ptr())
+    _enter(index, _lib.load().b2q_mx_quantize, did, at, ldx, experts or 1, each, k, image.data_ptr())
     return MXTensor._made(image, each, k, experts)
 
 
@@ -146,15 +162,15 @@ def dequantize(t, dtype=torch.float32):
         raise TypeError(f"dequantize: expected an MXTensor, got {type(t).__name__}")
     did = _out_dtype("dequantize", dtype)
     y = t.image.new_empty(t.shape, dtype=dtype)
-    _enter(t.device, _lib.load().b2q_mx_dequantize, t.image.data_ptr(), t.experts or 1, t.rows, t.k, did, y.data_ptr(), t.k)
+    _enter(t._index, _lib.load().b2q_mx_dequantize, t._at, t.experts or 1, t.rows, t.k, did, y.data_ptr(), t.k)
     return y
 
 
 def pack(codes, scales):
     """Planes codes uint8 [N][K/2] (in a block of 16 bytes byte i = value i in the low nibble, value i + 16 in the high one) and
     scales uint8 [N][K/32], or with a leading axis of experts -> MXTensor."""
-    dev = _cuda("pack", codes)
-    _on_device("pack", dev, scales)
+    index = _cuda("pack", codes)
+    _same("pack", index, scales)
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError(f"pack: codes {codes.dtype} and scales {scales.dtype}, expected torch.uint8")
     if codes.dim() not in (2, 3) or codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * scales.shape[-1]:
@@ -168,7 +184,7 @@ def pack(codes, scales):
     if codes.data_ptr() % 16:
         codes = codes.clone()
     image = codes.new_empty(image_bytes(n, k, experts or 1))
-    _enter(dev, _lib.load().b2q_mx_pack, codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, image.data_ptr())
+    _enter(index, _lib.load().b2q_mx_pack, codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, image.data_ptr())
     return MXTensor._made(image, n, k, experts)
 
 
@@ -186,12 +202,12 @@ def from_ggml(blocks, n, k, experts=None):
     return pack(b[..., 1:].flatten(-2), b[..., 0])
 
 
-def _check_out(name, out, dtype, shape, dev):
+def _check_out(name, out, dtype, shape, index):
     """The address and row stride of a given output: unit column stride, rows that do not overlap."""
-    _on_device(name, dev, out)
+    _same(name, index, out)
     if out.dtype != dtype or out.shape != shape or (shape[1] > 1 and out.stride(1) != 1) or \
             (shape[0] > 1 and out.stride(0) < shape[1]):
-        raise ValueError(f"{name}: out must be a {dtype} {shape} tensor with unit column stride on {dev}")
+        raise ValueError(f"{name}: out must be a {dtype} {shape} tensor with unit column stride on cuda:{index}")
     return out.data_ptr(), _stride(out)
 
 
@@ -210,16 +226,16 @@ def matmul(a, w, dtype=torch.bfloat16, out=None):
             raise TypeError(f"matmul: {name} must be an MXTensor, got {type(t).__name__}")
         if t.experts is not None:
             raise ValueError(f"matmul: {name} {t.shape} has experts (comp_b200.experts.linear)")
-    if a.k != w.k or a.device != w.device:
+    index = w._index
+    if a.k != w.k or a._index != index:
         raise ValueError(f"matmul: a {a.shape} on {a.device} and w {w.shape} on {w.device}")
     did = _out_dtype("matmul", dtype)
-    dev = a.device
     if out is None:
         out = a.image.new_empty((a.rows, w.rows), dtype=dtype)
         at, ldy = out.data_ptr(), w.rows
     else:
-        at, ldy = _check_out("matmul", out, dtype, (a.rows, w.rows), dev)
-    _enter(dev, _lib.load().b2q_mx_matmul, a.image.data_ptr(), w.image.data_ptr(), a.rows, w.rows, a.k, did, at, ldy)
+        at, ldy = _check_out("matmul", out, dtype, (a.rows, w.rows), index)
+    _enter(index, _lib.load().b2q_mx_matmul, a._at, w._at, a.rows, w.rows, a.k, did, at, ldy)
     return out
 
 
@@ -239,23 +255,30 @@ def linear(x, w, dtype=None, out=None):
         raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
     if w.experts is not None:
         raise ValueError(f"linear: w {w.shape} has experts (comp_b200.experts.linear)")
-    dev, k, n = w.device, w.k, w.rows
-    _on_device("linear", dev, x)
-    xid = _dtype_id("linear: x", x)
-    if x.dim() != 2 or x.shape[1] != k:
-        raise ValueError(f"linear: x {tuple(x.shape)}, expected [M][{k}]")
-    m = x.shape[0]
-    if dtype is None:
-        dtype = x.dtype
-    did = _out_dtype("linear", dtype)
+    index, k, n = w._index, w.k, w.rows
+    _same("linear", index, x)
+    given = x.dtype
+    xid = DTYPE_ID.get(given)
+    if xid is None:
+        _dtype_id("linear: x", x)
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError(f"linear: x {tuple(shape)}, expected [M][{k}]")
+    m = shape[0]
+    if dtype is None or dtype is given:
+        dtype, did = given, xid
+    else:
+        did = _out_dtype("linear", dtype)
     x, x_at, ldx = _rows(x)
     if out is None:
-        out = x.new_empty((m, n), dtype=dtype)
+        out = x.new_empty((m, n)) if did == xid else x.new_empty((m, n), dtype=dtype)
         at, ldy = out.data_ptr(), n
     else:
-        at, ldy = _check_out("linear", out, dtype, (m, n), dev)
+        at, ldy = _check_out("linear", out, dtype, (m, n), index)
     need = image_bytes(m, k) if m > FUSED_ROWS else _few_size(w, m, "b2q_mx_linear_workspace_size", m, n, k)
-    workspace = x.new_empty(need, dtype=torch.uint8) if need else None
-    _enter(dev, _lib.load().b2q_mx_linear, xid, x_at, ldx, w.image.data_ptr(), m, n, k, did, at, ldy,
-           workspace.data_ptr() if need else 0, need)
+    if need:
+        workspace = x.new_empty(need, dtype=torch.uint8)
+        _enter(index, _lib.load().b2q_mx_linear, xid, x_at, ldx, w._at, m, n, k, did, at, ldy, workspace.data_ptr(), need)
+    else:
+        _enter(index, _lib.load().b2q_mx_linear, xid, x_at, ldx, w._at, m, n, k, did, at, ldy, 0, 0)
     return out
