@@ -67,8 +67,13 @@ __device__ __forceinline__ void route_token(const T* logits, int experts, int to
   auto largest_of_lane = [&] {
     mine = key[0], at = 0;
 #pragma unroll
-    for (int v = 1; v < V; ++v)
-      if (key[v] > mine) mine = key[v], at = v;
+    for (int v = 1; v < V; ++v) {
+      if constexpr (sizeof(T) == 2) {
+        mine = max(mine, key[v]);
+      } else {
+        if (key[v] > mine) mine = key[v], at = v;
+      }
+    }
   };
   largest_of_lane();
   uint32_t m = __reduce_max_sync(0xffffffffu, mine);
@@ -93,7 +98,7 @@ __device__ __forceinline__ void route_token(const T* logits, int experts, int to
     if ((e & 31) == lane) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (v == at) key[v] = 0;
+        if (sizeof(T) == 2 ? key[v] == m : v == at) key[v] = 0;  // (16-bit: no key is there twice)
       largest_of_lane();
     }
     if (j + 1 < top) m = __reduce_max_sync(0xffffffffu, mine);
