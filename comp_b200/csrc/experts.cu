@@ -397,13 +397,15 @@ __global__ void __launch_bounds__(256)
                    const float* __restrict__ weights, int64_t tokens, int top, int vectors, T* __restrict__ out, int64_t ldo) {
   pdl_wait_then_trigger();
   using V = Vec<T, B>;
-  constexpr int kAtOnce = 4;
+  // Rows whose loads are under way together: other warps hide the rest. 65536 rows of 4096 bf16 with 1 / 2 / 4 / 8: 100 / 99 / 109 /
+  // 174 us; 16384 of 4096 f32 51 / 57 / 63 / 105.
+  constexpr int kAtOnce = sizeof(T) == 4 ? 1 : 2;
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t t = item < (1ll << 32) ? (int64_t)((uint32_t)item / (uint32_t)vectors) : item / vectors;
   if (t >= tokens) return;
   const int c = (int)(item - t * vectors) * V::N;
   float sum[V::N] = {};
-  for (int j0 = 0; j0 < top; j0 += kAtOnce) {  // so many rows' loads at once
+  for (int j0 = 0; j0 < top; j0 += kAtOnce) {
     V v[kAtOnce];
     float w[kAtOnce];
     int r[kAtOnce];
