@@ -1,5 +1,5 @@
 """MXFP4 and layers of experts, restated in numpy and 64 bits: quantization by its definition, planes, products, routing, the
-sort by expert and the way back. The checker of comp_b200.mx and comp_b200.experts."""
+sort by expert and the way back: what the tests of comp_b200.mx and comp_b200.experts compare with."""
 
 import numpy as np
 

@@ -51,6 +51,20 @@ def test_results_past_32_bits(cuda):
     assert device_error() == 0
 
 
+@pytest.mark.parametrize("m,n,k", [(2, 10_000, 29_696), (4, 20_000, 27_904), (1, 130, 61_440), (3, 19_000, 16_384), (300, 500, 61_440)])
+def test_long_sums(cuda, m, n, k):
+    """Rows so long that one launch has no room for them, and just short enough; against 64 bits on the operands' own values
+    (bound as in test_gpu_mx: K / 32 sums of blocks, each off by at most 2^-23 of the magnitudes so far)."""
+    gen = torch.Generator(device=cuda).manual_seed(k)
+    x, w = (torch.randn(s, generator=gen, device=cuda) for s in ((m, k), (n, k)))
+    w = mx.quantize(w)
+    y = mx.linear(x, w)
+    va, vw = mx.dequantize(mx.quantize(x)).double(), mx.dequantize(w).double()
+    want, mass = va @ vw.T, va.abs() @ vw.abs().T
+    assert bool(((y.double() - want).abs() <= (k / 32 + 8) * 2.0**-23 * mass + 2.0**-24 * want.abs()).all())
+    assert device_error() == 0
+
+
 def test_combine_past_32_bits(cuda):
     tokens, top, n = 150_001, 2, 8192  # 2.46e9 values
     y = _rows(tokens * top, n, cuda)
