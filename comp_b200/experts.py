@@ -29,7 +29,7 @@ class Plan:
     def __init__(self, tokens, top, experts, like, ids=None):
         choices = tokens * top
         self.tokens, self.top, self.experts = tokens, top, experts
-        words = 2 * (experts + 1) + 4 * choices if tokens <= 128 and choices <= 4096 else \
+        words = 2 * (experts + 1) + 4 * choices if tokens <= 128 and choices <= 1024 else \
             _lib.load().b2q_experts_plan_words(tokens, top, experts)
         self._ids, self._routed = ids, words if ids is None else 0  # (routed: ids and weights follow the plan's own words)
         self._words = like.new_empty(words + 2 * choices if ids is None else words, dtype=torch.int32)

@@ -33,10 +33,10 @@ def test_sizes(lib):
 
 
 def test_plan_words(lib):
-    for t, top, e in ((0, 1, 1), (1, 8, 64), (128, 32, 1024), (129, 1, 5), (4097, 1, 5), (16384, 8, 256), (1 << 23, 8, 1024)):
+    for t, top, e in ((0, 1, 1), (1, 8, 64), (128, 8, 1024), (128, 9, 64), (1, 32, 1024), (129, 1, 5), (4097, 1, 5), (16384, 8, 256), (1 << 23, 8, 1024)):
         words = lib.b2q_experts_plan_words(t, top, e)
         plain = 2 * (e + 1) + 4 * t * top
-        assert words == plain if t <= 128 and t * top <= 4096 else words > plain and (words - plain) % e == 0
+        assert words == plain if t <= 128 and t * top <= 1024 else words > plain and (words - plain) % e == 0
     for bad in ((-1, 1, 1), (1, 0, 1), (1, 33, 64), (1, 1, 0), (1, 1, 1025), (1 << 26, 2, 4)):
         assert lib.b2q_experts_plan_words(*bad) == 0 and "b2q_experts_plan_words" in _lib.last_error()
 
