@@ -16,6 +16,11 @@
 //     first one's end, and those are read first.
 // Few tiles (narrow layers, few rows) leave most of the GPU idle: then the CTAs of a cluster split K between them, and add
 // their parts in order of rank through distributed shared memory, so that results do not depend on timing.
+//
+// What bounds it: a stage of 256 rows writes 51 KB into shared memory and the products read 49 KB of it, 790 cycles at 128 bytes a
+// cycle, where the products alone would take 512; measured 745 to 820, at 1.6 to 1.7 GHz under the power limit: 4096 x 14336 x
+// 4096 103 us (4.7 PFLOP/s), 118 in a long run; 8192 x 8192 x 8192 209 us (5.3). With few rows the weights' stream: 64 tokens of 8
+// among 128 experts of 4096 x 2048 97 us (5.8 TB/s).
 #include <algorithm>
 #include <atomic>
 
