@@ -34,6 +34,12 @@ class AttentionArgs(ctypes.Structure):
                 ("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
 
 
+# The argument blocks of the MXFP4 and expert calls, field by field (include/comp_b200.h), as struct.Struct(...).pack makes them.
+MX_LINEAR_ARGS = "@4P6q2i"
+EXPERTS_ROUTE_ARGS = "@4P4q2i"
+EXPERTS_LINEAR_ARGS = "@5P8q3i4x"
+EXPERTS_COMBINE_ARGS = "@4P6qi4x"
+
 # name -> (restype, argtypes); every symbol include/comp_b200.h declares
 SIGNATURES = {
     "b2q_version": (ctypes.c_char_p, []),
@@ -68,13 +74,13 @@ SIGNATURES = {
     "b2q_mx_pack": (INT, [P, P, I64, I64, I64, P, P]),
     "b2q_mx_matmul": (INT, [P, P, I64, I64, I64, INT, P, I64, P]),
     "b2q_mx_linear_workspace_size": (ctypes.c_size_t, [I64, I64, I64]),
-    "b2q_mx_linear": (INT, [INT, P, I64, P, I64, I64, I64, INT, P, I64, P, ctypes.c_size_t, P]),
+    "b2q_mx_linear": (INT, [P, P]),
     "b2q_experts_plan_words": (ctypes.c_size_t, [I64, I64, I64]),
-    "b2q_experts_route": (INT, [INT, P, I64, I64, I64, I64, INT, P, P, P, P]),
+    "b2q_experts_route": (INT, [P, P]),
     "b2q_experts_sort": (INT, [P, I64, I64, I64, P, P]),
     "b2q_experts_linear_workspace_size": (ctypes.c_size_t, [I64, I64, I64, INT, I64, I64]),
-    "b2q_experts_linear": (INT, [INT, P, I64, INT, P, P, I64, I64, I64, I64, I64, INT, P, I64, P, ctypes.c_size_t, P]),
-    "b2q_experts_combine": (INT, [INT, P, I64, P, P, I64, I64, I64, I64, P, I64, P]),
+    "b2q_experts_linear": (INT, [P, P]),
+    "b2q_experts_combine": (INT, [P, P]),
     "b2q_set_tuning": (INT, [INT, INT, INT]),
     "b2q_set_pipeline": (INT, [INT, INT]),
     "b2q_set_warps": (INT, [INT]),

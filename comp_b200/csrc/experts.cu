@@ -577,9 +577,10 @@ size_t b2q_experts_plan_words(int64_t tokens, int64_t top, int64_t experts) {
   return (size_t)(2 * (experts + 1) + 4 * choices + (is_small(tokens, top, true) ? 0 : parts_of(tokens, top).count * experts));
 }
 
-int b2q_experts_route(int dtype, const void* logits, int64_t ld, int64_t tokens, int64_t experts, int64_t top, int normalize,
-                      int32_t* ids, float* weights, int32_t* plan, b2q_stream_t stream) {
+int b2q_experts_route(const b2q_experts_route_args* args, b2q_stream_t stream) {
   const char* who = "b2q_experts_route";
+  if (!args) return fail(B2Q_EINVAL, "%s: null arguments", who);
+  const auto [logits, ids, weights, plan, ld, tokens, experts, top, dtype, normalize] = *args;
   int rc = check_plan(who, plan, tokens, top, experts);
   if (rc) return rc;
   if (dtype < B2Q_DTYPE_F32 || dtype > B2Q_DTYPE_BF16) return fail(B2Q_EINVAL, "%s: unknown dtype %d", who, dtype);
@@ -615,10 +616,10 @@ size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t ex
   return (size_t)tiles * mx_stages(K) * kMxBytes;
 }
 
-int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, const uint8_t* w, const int32_t* plan, int64_t tokens,
-                       int64_t top, int64_t experts, int64_t N, int64_t K, int dtype, void* y, int64_t ldy, void* workspace,
-                       size_t workspace_bytes, b2q_stream_t stream) {
+int b2q_experts_linear(const b2q_experts_linear_args* args, b2q_stream_t stream) {
   const char* who = "b2q_experts_linear";
+  if (!args) return fail(B2Q_EINVAL, "%s: null arguments", who);
+  const auto [x, w, plan, y, workspace, ldx, tokens, top, experts, N, K, ldy, workspace_bytes, x_dtype, dtype, gather] = *args;
   int rc = check_plan(who, plan, tokens, top, experts);
   const int64_t choices = rc ? 0 : tokens * top;
   if (!rc) rc = check_mx_shape(who, N, K);
@@ -647,9 +648,10 @@ int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, cons
   return launch_mx_gemm(g, stream);
 }
 
-int b2q_experts_combine(int dtype, const void* y, int64_t ldy, const int32_t* plan, const float* weights, int64_t tokens,
-                        int64_t top, int64_t experts, int64_t N, void* out, int64_t ldo, b2q_stream_t stream) {
+int b2q_experts_combine(const b2q_experts_combine_args* args, b2q_stream_t stream) {
   const char* who = "b2q_experts_combine";
+  if (!args) return fail(B2Q_EINVAL, "%s: null arguments", who);
+  const auto [y, plan, weights, out, ldy, tokens, top, experts, N, ldo, dtype] = *args;
   int rc = check_plan(who, plan, tokens, top, experts);
   if (rc) return rc;
   if (dtype < B2Q_DTYPE_F32 || dtype > B2Q_DTYPE_BF16) return fail(B2Q_EINVAL, "%s: unknown dtype %d", who, dtype);

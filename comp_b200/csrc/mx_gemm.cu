@@ -417,9 +417,10 @@ size_t b2q_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K) {
   return mx_gemv_takes(M, 1, 1, N, K) ? 0 : b2q_mx_bytes(1, M, K);
 }
 
-int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y,
-                  int64_t ldy, void* workspace, size_t workspace_bytes, b2q_stream_t stream) {
+int b2q_mx_linear(const b2q_mx_linear_args* args, b2q_stream_t stream) {
   const char* who = "b2q_mx_linear";
+  if (!args) return fail(B2Q_EINVAL, "%s: null arguments", who);
+  const auto [x, w, y, workspace, ldx, M, N, K, ldy, workspace_bytes, x_dtype, dtype] = *args;
   int rc = check_mx_shape(who, M, K);
   if (!rc) rc = check_mx_shape(who, N, K);
   if (!rc) rc = check_mx_rows(who, "x", x_dtype, x, ldx, M, K);

@@ -10,14 +10,19 @@ Nothing synchronizes: how many rows an expert has stays on the device, and all o
 kernels are this package's own, through the C-ABI (include/comp_b200.h, where layouts and formulas stand).
 """
 
+import struct
+
 import torch
 
 from . import _lib
 from .kv import DTYPE_ID, _dtype_id
 from .mx import (FUSED_ROWS, MAX_EXPERTS, STAGE, STAGE_BYTES, TILE_ROWS, MXTensor, _check_out, _cuda, _enter, _few_size,
-                 _out_dtype, _rows, _same, _stride)
+                 _out_dtype, _rows, _same, _scratch, _stride)
 
 MAX_TOP = 32
+_pack_route = struct.Struct(_lib.EXPERTS_ROUTE_ARGS).pack
+_pack_linear = struct.Struct(_lib.EXPERTS_LINEAR_ARGS).pack
+_pack_combine = struct.Struct(_lib.EXPERTS_COMBINE_ARGS).pack
 
 
 class Plan:
@@ -99,8 +104,8 @@ def route(logits, top, normalize=True):
     plan = Plan(tokens, top, experts, logits)
     words = plan._at
     ids = words + 4 * plan._routed
-    _enter(index, _lib.load().b2q_experts_route, did, logits.data_ptr(), ld, tokens, experts, top, 1 if normalize else 0, ids,
-           ids + 4 * tokens * top, words)
+    _enter(index, _lib.load().b2q_experts_route, _pack_route(logits.data_ptr(), ids, ids + 4 * tokens * top, words, ld, tokens,
+                                                             experts, top, did, 1 if normalize else 0))
     return plan
 
 
@@ -169,14 +174,15 @@ def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
         at, ldy = _check_out("linear", out, dtype, (choices, n), index)
     if workspace is None:
         need = workspace_size(plan, w, gather)
-        workspace = x.new_empty(need, dtype=torch.uint8) if need else None
+        workspace = _scratch(index, need, x) if need else None
     else:
         _same("linear", index, workspace)
         if not workspace.is_contiguous():
             raise ValueError("linear: workspace must be contiguous")
         need = workspace.numel() * workspace.element_size()
-    _enter(index, _lib.load().b2q_experts_linear, xid, x_at, ldx, 1 if gather else 0, w._at, plan._at, tokens, top, plan.experts, n, k,
-           did, at, ldy, 0 if workspace is None else workspace.data_ptr(), need)
+    _enter(index, _lib.load().b2q_experts_linear,
+           _pack_linear(x_at, w._at, plan._at, at, 0 if workspace is None else workspace.data_ptr(), ldx, tokens, top, plan.experts, n,
+                        k, ldy, need, xid, did, 1 if gather else 0))
     return out
 
 
@@ -214,5 +220,6 @@ def combine(y, plan, weights=None, out=None):
         at, ldo = out.data_ptr(), n
     else:
         at, ldo = _check_out("combine", out, y.dtype, (tokens, n), index)
-    _enter(index, _lib.load().b2q_experts_combine, did, y.data_ptr(), ldy, plan._at, w_at, tokens, top, plan.experts, n, at, ldo)
+    _enter(index, _lib.load().b2q_experts_combine,
+           _pack_combine(y.data_ptr(), plan._at, w_at, at, ldy, tokens, top, plan.experts, n, ldo, did))
     return out

@@ -12,6 +12,9 @@ TypeError / ValueError / RuntimeError on what they do not take.
     y = mx.linear(x, w)                        # x [M][k] -> y [M][n] of x's type
 """
 
+import struct
+import threading
+
 import torch
 
 from . import _lib
@@ -20,6 +23,22 @@ from .kv import DTYPE_ID, _dtype_id, _on_device, _raw_stream
 # A token's step is many calls of a few microseconds on the GPU: what a call costs on the host counts. So the functions
 # look at the common case first (contiguous, aligned), make tensors from tensors, and enter the library once.
 _current_device = torch._C._cuda_getDevice
+_pack_linear = struct.Struct(_lib.MX_LINEAR_ARGS).pack
+
+# Scratch of a call that is launched on the default stream, whose calls never overlap: each thread keeps up to 4 MB of it a
+# device (threads may come between one another's two launches). Other streams, captured ones among them, get their own a call.
+_kept = threading.local()
+KEPT_BYTES = 4 << 20
+
+
+def _scratch(index, need, like):
+    """A tensor of `need` bytes at least, for use on the current stream of device `index`, which is like's."""
+    if need > KEPT_BYTES or _raw_stream(index):
+        return like.new_empty(need, dtype=torch.uint8)
+    kept = _kept.__dict__.get(index)
+    if kept is None or kept.numel() < need:
+        kept = _kept.__dict__[index] = like.new_empty(min(KEPT_BYTES, 2 * need), dtype=torch.uint8)
+    return kept
 
 TILE_ROWS, STAGE, STAGE_BYTES = 128, 256, 17408  # an image: 128 rows by 256 values a run of bytes
 MAX_EXPERTS = 1024
@@ -74,12 +93,6 @@ class MXTensor:
         if image.dim() != 1 or image.numel() < need or not image.is_contiguous() or (need and image.data_ptr() % 128):
             raise ValueError(f"MXTensor: the image must be {need} contiguous bytes, 128-byte aligned, got {tuple(image.shape)}")
         self._set(image, rows, k, experts)
-
-    @classmethod
-    def _made(cls, image, rows, k, experts=None):
-        self = cls.__new__(cls)
-        self._set(image, rows, k, experts)
-        return self
 
     def _set(self, image, rows, k, experts):
         self.image, self.rows, self.k, self.experts = image, rows, k, experts
@@ -140,20 +153,22 @@ def quantize(x):
     did = DTYPE_ID.get(x.dtype)
     if did is None:
         _dtype_id("quantize: x", x)
-    experts = None
-    if x.dim() == 3:
-        experts = x.shape[0]
+    shape, experts = x.shape, None
+    if len(shape) == 3:
+        experts, m, k = shape
         _check_experts("quantize", experts)
         x = x.flatten(0, 1)
-    elif x.dim() != 2:
-        raise ValueError(f"quantize: x {tuple(x.shape)}, expected [M][K] or [experts][M][K]")
-    m, k = x.shape
+    elif len(shape) == 2:
+        m, k = shape
+    else:
+        raise ValueError(f"quantize: x {tuple(shape)}, expected [M][K] or [experts][M][K]")
     _check_k("quantize", k)
-    each = m if experts is None else m // experts
     x, at, ldx = _rows(x)
-    image = x.new_empty(image_bytes(each, k, experts or 1), dtype=torch.uint8)
-    _enter(index, _lib.load().b2q_mx_quantize, did, at, ldx, experts or 1, each, k, image.data_ptr())
-    return MXTensor._made(image, each, k, experts)
+    image = x.new_empty(image_bytes(m, k, experts or 1), dtype=torch.uint8)
+    t = MXTensor.__new__(MXTensor)
+    t._set(image, m, k, experts)
+    _enter(index, _lib.load().b2q_mx_quantize, did, at, ldx, experts or 1, m, k, t._at)
+    return t
 
 
 def dequantize(t, dtype=torch.float32):
@@ -184,8 +199,10 @@ def pack(codes, scales):
     if codes.data_ptr() % 16:
         codes = codes.clone()
     image = codes.new_empty(image_bytes(n, k, experts or 1))
-    _enter(index, _lib.load().b2q_mx_pack, codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, image.data_ptr())
-    return MXTensor._made(image, n, k, experts)
+    t = MXTensor.__new__(MXTensor)
+    t._set(image, n, k, experts)
+    _enter(index, _lib.load().b2q_mx_pack, codes.data_ptr(), scales.data_ptr(), experts or 1, n, k, t._at)
+    return t
 
 
 def from_ggml(blocks, n, k, experts=None):
@@ -276,9 +293,7 @@ def linear(x, w, dtype=None, out=None):
     else:
         at, ldy = _check_out("linear", out, dtype, (m, n), index)
     need = image_bytes(m, k) if m > FUSED_ROWS else _few_size(w, m, "b2q_mx_linear_workspace_size", m, n, k)
-    if need:
-        workspace = x.new_empty(need, dtype=torch.uint8)
-        _enter(index, _lib.load().b2q_mx_linear, xid, x_at, ldx, w._at, m, n, k, did, at, ldy, workspace.data_ptr(), need)
-    else:
-        _enter(index, _lib.load().b2q_mx_linear, xid, x_at, ldx, w._at, m, n, k, did, at, ldy, 0, 0)
+    workspace = _scratch(index, need, x) if need else None
+    _enter(index, _lib.load().b2q_mx_linear,
+           _pack_linear(x_at, w._at, at, workspace.data_ptr() if need else 0, ldx, m, n, k, ldy, need, xid, did))
     return out

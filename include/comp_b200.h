@@ -415,9 +415,18 @@ int b2q_mx_matmul(const uint8_t* a, const uint8_t* w, int64_t M, int64_t N, int6
 /* b2q_mx_quantize of x [M][K] and b2q_mx_matmul with it, in one launch for up to 4 rows (unless K is very long). workspace: device
  * memory of b2q_mx_linear_workspace_size(M, N, K) bytes (0 for one launch), 128-byte aligned; calls that may overlap on the GPU
  * need one each. */
+typedef struct {
+  const void* x;
+  const uint8_t* w;
+  void* y;
+  void* workspace;
+  int64_t ldx, M, N, K, ldy;
+  size_t workspace_bytes;
+  int32_t x_dtype, dtype;
+} b2q_mx_linear_args;
+
 size_t b2q_mx_linear_workspace_size(int64_t M, int64_t N, int64_t K);
-int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int64_t M, int64_t N, int64_t K, int dtype, void* y,
-                  int64_t ldy, void* workspace, size_t workspace_bytes, b2q_stream_t stream);
+int b2q_mx_linear(const b2q_mx_linear_args* args, b2q_stream_t stream);
 
 /*
  * The plan of a layer of experts: which of `experts` (1..1024) the `top` (1..32) choices of each token go to, sorted by
@@ -435,8 +444,16 @@ int b2q_mx_linear(int x_dtype, const void* x, int64_t ldx, const uint8_t* w, int
  * set the device error word to 5. A token may choose an expert twice.
  */
 size_t b2q_experts_plan_words(int64_t tokens, int64_t top, int64_t experts);
-int b2q_experts_route(int dtype, const void* logits, int64_t ld, int64_t tokens, int64_t experts, int64_t top, int normalize,
-                      int32_t* ids, float* weights, int32_t* plan, b2q_stream_t stream);
+typedef struct {
+  const void* logits;
+  int32_t* ids;
+  float* weights;
+  int32_t* plan;
+  int64_t ld, tokens, experts, top;
+  int32_t dtype, normalize;
+} b2q_experts_route_args;
+
+int b2q_experts_route(const b2q_experts_route_args* args, b2q_stream_t stream);
 int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t experts, int32_t* plan, b2q_stream_t stream);
 
 /*
@@ -445,15 +462,32 @@ int b2q_experts_sort(const int32_t* ids, int64_t tokens, int64_t top, int64_t ex
  * rows [tokens * top][K]; it is quantized to MXFP4 on the way, into the workspace (128-byte aligned; 0 bytes for a few rows; calls
  * that may overlap on the GPU need one each). The plan is one that b2q_experts_route or b2q_experts_sort wrote for the same sizes.
  */
+typedef struct {
+  const void* x;
+  const uint8_t* w;
+  const int32_t* plan;
+  void* y;
+  void* workspace;
+  int64_t ldx, tokens, top, experts, N, K, ldy;
+  size_t workspace_bytes;
+  int32_t x_dtype, dtype, gather;
+} b2q_experts_linear_args;
+
 size_t b2q_experts_linear_workspace_size(int64_t tokens, int64_t top, int64_t experts, int gather, int64_t N, int64_t K);
-int b2q_experts_linear(int x_dtype, const void* x, int64_t ldx, int gather, const uint8_t* w, const int32_t* plan, int64_t tokens,
-                       int64_t top, int64_t experts, int64_t N, int64_t K, int dtype, void* y, int64_t ldy, void* workspace,
-                       size_t workspace_bytes, b2q_stream_t stream);
+int b2q_experts_linear(const b2q_experts_linear_args* args, b2q_stream_t stream);
 
 /* out[t] = sum over j of weights[t][j] * y[pos[t][j]] (f32, in order of j, rounded once; weights NULL: 1): sorted rows y
  * [tokens * top][N] back to their tokens, out [tokens][N]; both of dtype. A choice that goes nowhere adds nothing. */
-int b2q_experts_combine(int dtype, const void* y, int64_t ldy, const int32_t* plan, const float* weights, int64_t tokens,
-                        int64_t top, int64_t experts, int64_t N, void* out, int64_t ldo, b2q_stream_t stream);
+typedef struct {
+  const void* y;
+  const int32_t* plan;
+  const float* weights;
+  void* out;
+  int64_t ldy, tokens, top, experts, N, ldo;
+  int32_t dtype;
+} b2q_experts_combine_args;
+
+int b2q_experts_combine(const b2q_experts_combine_args* args, b2q_stream_t stream);
 
 /* Benchmark/tuning hook (process-wide): force rows per group (1, 2, 4), chunks per thread and grid size of the
  * GEMV schedule; 0 restores the planner's choice. Results do not depend on it (except the f32 summation order). */

@@ -75,6 +75,30 @@ def test_combine_past_32_bits(cuda):
         assert torch.allclose(out[t].double(), want, rtol=2.0**-8, atol=1e-30)
 
 
+def test_threads_on_the_default_stream(cuda):
+    """Threads whose calls come between one another's launches: each has scratch of its own, of any size in turn."""
+    import threading
+
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    w = mx.quantize(torch.randn((700, 1024), generator=gen, device=cuda))
+    xs = [[torch.randn((m, 1024), generator=gen, device=cuda) for m in (5 + i, 300, 20, 9000, 130)] for i in range(4)]
+    want = [[mx.linear(x, w) for x in row] for row in xs]
+    got = [[] for _ in xs]
+
+    def work(i):
+        for _ in range(30):
+            got[i].append([mx.linear(x, w) for x in xs[i]])
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, rounds in enumerate(got):
+        assert len(rounds) == 30 and all(torch.equal(a, b) for r in rounds for a, b in zip(r, want[i]))
+
+
 @pytest.mark.parametrize("tokens", [1, 40, 700])
 def test_layers_on_two_streams(cuda, tokens):
     """The same weights used by two streams at once, each call with memory of its own."""

@@ -1,12 +1,18 @@
 """MXFP4 and layers of experts without a GPU: the C-ABI's refusals (checked before any launch) and the oracle against second
 statements of its parts."""
 
+import struct
+
 import numpy as np
 import pytest
 import torch
 
 from comp_b200 import _lib, experts, mx
 from oracle import mx as ref
+
+
+def pack(form, *values):
+    return struct.pack(form, *(0 if v is None else v for v in values))
 
 
 @pytest.fixture(scope="module")
@@ -61,26 +67,28 @@ def test_product_refusals(lib):
     assert f(dtype=4) == -1 and f(ldy=2) == -1 and f(a=64) == -2 and f(w=64) == -2 and f(y=4098) == -2
     assert f(m=0) == 0 and f(n=0) == 0
     g = lambda x=4096, ldx=64, w=4096, y=4096, ws=4096, size=17408, m=20, dtype=2: lib.b2q_mx_linear(  # noqa: E731
-        0, x, ldx, w, m, 3, 64, dtype, y, 3, ws, size, None)
+        pack(_lib.MX_LINEAR_ARGS, x, w, y, ws, ldx, m, 3, 64, 3, size, 0, dtype), None)
+    assert lib.b2q_mx_linear(None, None) == -1
     assert g(x=None) == -1 and g(w=None) == -1 and g(y=None) == -1 and g(ws=None) == -1 and g(size=17407) == -1 and g(dtype=9) == -1
     assert g(x=4100) == -2 and g(ldx=65) == -2 and g(ws=4096 + 16) == -1 and g(m=0, ws=None) == 0
 
 
 def test_expert_refusals(lib):
     r = lambda dtype=0, x=4096, ld=8, t=2, e=8, top=2, ids=4096, w=4096, plan=4096: lib.b2q_experts_route(  # noqa: E731
-        dtype, x, ld, t, e, top, 1, ids, w, plan, None)
+        pack(_lib.EXPERTS_ROUTE_ARGS, x, ids, w, plan, ld, t, e, top, dtype, 1), None)
     assert r(dtype=5) == -1 and r(x=None) == -1 and r(ld=7) == -1 and r(t=-1) == -1 and r(e=0) == -1 and r(e=1025, ld=2000) == -1
     assert r(top=0) == -1 and r(top=9) == -1 and r(top=33, e=64, ld=64) == -1 and r(ids=None) == -1 and r(w=None) == -1
     assert r(plan=None) == -1 and r(plan=4098) == -2 and r(ids=4097) == -2 and r(x=4097) == -2 and r(t=1 << 26) == -4
     s = lambda ids=4096, t=2, top=2, e=8, plan=4096: lib.b2q_experts_sort(ids, t, top, e, plan, None)  # noqa: E731
     assert s(ids=None) == -1 and s(plan=None) == -1 and s(e=0) == -1 and s(top=33) == -1 and s(ids=4098) == -2
     f = lambda x=4096, ldx=64, w=4096, plan=4096, t=20, n=3, k=64, dtype=0, y=4096, ldy=3, ws=4096, size=1 << 20: (  # noqa: E731
-        lib.b2q_experts_linear(0, x, ldx, 1, w, plan, t, 2, 8, n, k, dtype, y, ldy, ws, size, None))
+        lib.b2q_experts_linear(pack(_lib.EXPERTS_LINEAR_ARGS, x, w, plan, y, ws, ldx, t, 2, 8, n, k, ldy, size, 0, dtype, 1), None))
     assert f(x=None) == -1 and f(w=None) == -1 and f(plan=None) == -1 and f(y=None) == -1 and f(ws=None) == -1 and f(k=40) == -1
     assert f(dtype=3) == -1 and f(ldy=2) == -1 and f(size=17408) == -1 and f(x=4104) == -2 and f(w=4096 + 64) == -2 and f(y=4098) == -2
     assert f(t=0, ws=None) == 0 and f(n=0) == 0
     c = lambda dtype=0, y=4096, ldy=4, plan=4096, w=4096, n=4, out=4096, ldo=4: lib.b2q_experts_combine(  # noqa: E731
-        dtype, y, ldy, plan, w, 2, 2, 8, n, out, ldo, None)
+        pack(_lib.EXPERTS_COMBINE_ARGS, y, plan, w, out, ldy, 2, 2, 8, n, ldo, dtype), None)
+    assert all(f(None, None) == -1 for f in (lib.b2q_experts_route, lib.b2q_experts_linear, lib.b2q_experts_combine))
     assert c(dtype=3) == -1 and c(y=None) == -1 and c(out=None) == -1 and c(plan=None) == -1 and c(ldy=3) == -1 and c(ldo=3) == -1
     assert c(n=-1) == -1 and c(y=4098) == -2 and c(w=4098) == -2 and c(n=0) == 0
 
