@@ -243,8 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
         }
     }
     __syncwarp();
-    // no CTA ends before all have sent their parts
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has sent its parts
     if (stores && owned > 0 && wait_warp(&b_part, 0) && n < g.N)
       for (int i = 0; i < owned; ++i) {
         const int x_row = (int)rank + i * (int)ranks;
@@ -253,6 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
         for (int row = at.row0; row < at.row0 + at.count; ++row)
           if ((g.offsets ? s_token[row] : row) == x_row) store_as(g.y, (int64_t)row * g.ldy + n, g.dtype, sum);
       }
+    __syncwarp();
+    // no CTA ends before all have sent theirs (parts for one that gave up waiting find its memory)
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   tc::fence_before();
   __syncthreads();
