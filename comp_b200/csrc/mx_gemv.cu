@@ -36,7 +36,7 @@ struct Gemv {
   void* y;
   const int32_t *offsets, *order;  // of a plan; null: one expert, whose row of y is the row of x
   int64_t ldx, ldy;
-  int rows, K, N, row_tiles, stages, experts, dtype;
+  int rows, K, N, row_tiles, stages, experts, choices, dtype;
   int top;      // choices a token where x has a row a token, else 0
   int ring;     // stages of weights in shared memory
   int columns;  // of tensor memory
@@ -86,20 +86,26 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (g.offsets && warp == 2) {  // the experts that have rows, and where those begin
+  if (g.offsets && warp == 2) {  // the experts that have rows, and where those begin: 128 experts' loads at a time
     int n = 0;
-    for (int e0 = 0; e0 < g.experts; e0 += 32) {
-      const int e = e0 + lane;
-      const int a = e < g.experts ? g.offsets[e] : 0, b = e < g.experts ? g.offsets[e + 1] : 0;
-      const uint32_t some = __ballot_sync(0xffffffffu, b > a);
-      const int at = n + __popc(some & ((1u << lane) - 1));
-      if (b > a && at < kMaxChoices) s_used[at] = e, s_offsets[at] = a, s_offsets[at + 1] = b;
-      n += __popc(some);
+    for (int e0 = 0; e0 < g.experts; e0 += 128) {
+      int at[5];
+#pragma unroll
+      for (int u = 0; u < 5; ++u) at[u] = g.offsets[min(e0 + u * 32 + lane, g.experts)];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + u * 32 + lane, after = __shfl_down_sync(0xffffffffu, at[u], 1),
+                  over = __shfl_sync(0xffffffffu, at[u + 1], 0);
+        const int begin = at[u], end = lane < 31 ? after : over;
+        const uint32_t some = __ballot_sync(0xffffffffu, end > begin);
+        const int i = n + __popc(some & ((1u << lane) - 1));
+        if (end > begin && i < kMaxChoices) s_used[i] = e, s_offsets[i] = begin, s_offsets[i + 1] = end;
+        n += __popc(some);
+      }
     }
     if (lane == 0) s_count = min(n, kMaxChoices);
   } else if (g.offsets && warp == 3) {
-    const int n = g.offsets[g.experts];
-    for (int r = lane; r < kMaxChoices; r += 32) s_token[r] = r >= n ? 0 : g.top ? g.order[r] / g.top : r;
+    for (int r = lane; r < g.choices; r += 32) s_token[r] = g.top ? max(g.order[r], 0) / g.top : r;  // (-1: nobody's row)
   }
   tc::fence_before();
   __syncthreads();
@@ -336,7 +342,7 @@ int launch_mx_gemv(const MxGemv& a, cudaStream_t stream) {
   const int64_t used = std::min<int64_t>(a.offsets ? a.choices : 1, a.experts), row_tiles = mx_tiles(a.N), stages = mx_stages(a.K);
   if (!plan_gemv(a.rows, used, row_tiles, stages, dev.sms, &p)) return fail(B2Q_ERANGE, "mx_gemv: more rows than the kernel takes");
   const Gemv g = {a.w, a.x, a.y, a.offsets, a.order, a.ldx, a.ldy, (int)a.rows, (int)a.K, (int)a.N, (int)row_tiles, (int)stages,
-                  (int)a.experts, a.dtype, a.top, p.ring, kScaleX + 4 * p.nk <= 256 ? 256 : 512};
+                  (int)a.experts, (int)a.choices, a.dtype, a.top, p.ring, kScaleX + 4 * p.nk <= 256 ? 256 : 512};
   // with several CTAs a tile every tile has a cluster of its own
   const int64_t ctas = std::min<int64_t>(used * row_tiles, dev.sms / p.ranks);
   if (a.x_dtype == B2Q_DTYPE_F32) return launch_gemv<float>(g, p, (int)ctas, stream);
