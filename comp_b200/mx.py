@@ -25,10 +25,15 @@ from .kv import DTYPE_ID, _dtype_id, _on_device, _raw_stream
 _current_device = torch._C._cuda_getDevice
 _pack_linear = struct.Struct(_lib.MX_LINEAR_ARGS).pack
 
-# Scratch of a call that is launched on the default stream, whose calls never overlap: each thread keeps up to 4 MB of it a
-# device (threads may come between one another's two launches). Other streams, captured ones among them, get their own a call.
-_kept = threading.local()
+TILE_ROWS, STAGE, STAGE_BYTES = 128, 256, 17408  # an image: 128 rows by 256 values a run of bytes
+MAX_EXPERTS = 1024
+FUSED_ROWS = 4  # products of up to so many rows may quantize them in their own launch
+
+# Scratch of a call that is launched on the default stream, where one call's kernels write it only once the call before has
+# ended: each thread keeps up to 4 MB of it a device (another thread's launches may come between a call's two). Other streams,
+# captured ones among them, get theirs call by call.
 KEPT_BYTES = 4 << 20
+_kept = threading.local()
 
 
 def _scratch(index, need, like):
@@ -39,10 +44,6 @@ def _scratch(index, need, like):
     if kept is None or kept.numel() < need:
         kept = _kept.__dict__[index] = like.new_empty(min(KEPT_BYTES, 2 * need), dtype=torch.uint8)
     return kept
-
-TILE_ROWS, STAGE, STAGE_BYTES = 128, 256, 17408  # an image: 128 rows by 256 values a run of bytes
-MAX_EXPERTS = 1024
-FUSED_ROWS = 4  # products of up to so many rows may quantize them in their own launch
 
 
 def image_bytes(rows, k, experts=1):
