@@ -40,6 +40,14 @@ class Plan:
         self._words = like.new_empty(words + 2 * choices if ids is None else words, dtype=torch.int32)
         self._at, self._index = self._words.data_ptr(), self._words.get_device()
 
+    def __getstate__(self):
+        return {name: v for name, v in self.__dict__.items() if name not in ("_at", "_index")}
+
+    def __setstate__(self, state):  # a copy's words lie elsewhere
+        self.__dict__.update(state)
+        self._index = _cuda("Plan", self._words)
+        self._at = self._words.data_ptr()
+
     @property
     def device(self):
         return self._words.device
@@ -127,13 +135,22 @@ def sort(ids, experts):
     return plan
 
 
-def _check_plan(name, plan):
+def _check_pair(name, plan, w):
+    if not isinstance(w, MXTensor):
+        raise TypeError(f"{name}: w must be an MXTensor, got {type(w).__name__}")
     if not isinstance(plan, Plan):
         raise TypeError(f"{name}: plan must be a Plan (route, sort), got {type(plan).__name__}")
+    if w.experts != plan.experts:
+        raise ValueError(f"{name}: w {w.shape}, expected [{plan.experts}][N][K]")
 
 
 def workspace_size(plan, w, gather=True):
     """Bytes of device workspace that linear(x, w, plan, gather) needs."""
+    _check_pair("workspace_size", plan, w)
+    return _workspace_size(plan, w, gather)
+
+
+def _workspace_size(plan, w, gather):
     choices = plan.tokens * plan.top
     if (plan.tokens if gather else choices) <= FUSED_ROWS:
         return _few_size(w, (plan.tokens, plan.top, bool(gather)), "b2q_experts_linear_workspace_size", plan.tokens, plan.top,
@@ -144,13 +161,9 @@ def workspace_size(plan, w, gather=True):
 def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     """Each sorted row, quantized to MXFP4, times its expert's weights w (MXTensor [E][N][K]) -> [T * top][N] of `dtype`
     (default: x's) in sorted order; rows past plan.offsets[E] stay unwritten. x: [T][K], a token's row for each of its choices,
-    or with gather=False the sorted rows [T * top][K]. out: the tensor for the result (it shares no memory with x). workspace: a CUDA uint8 tensor of workspace_size(plan, w, gather)
-    bytes, 128-byte aligned (allocated here when None)."""
-    if not isinstance(w, MXTensor):
-        raise TypeError(f"linear: w must be an MXTensor, got {type(w).__name__}")
-    _check_plan("linear", plan)
-    if w.experts != plan.experts:
-        raise ValueError(f"linear: w {w.shape}, expected [{plan.experts}][N][K]")
+    or with gather=False the sorted rows [T * top][K]. out: the tensor for the result (it shares no memory with x). workspace: a
+    CUDA uint8 tensor of workspace_size(plan, w, gather) bytes, 128-byte aligned (allocated here when None)."""
+    _check_pair("linear", plan, w)
     index, n, k, tokens, top = w._index, w.rows, w.k, plan.tokens, plan.top
     if plan._index != index:
         raise RuntimeError(f"comp_b200.linear: tensors on different devices ({w.device} and {plan.device})")
@@ -173,7 +186,7 @@ def linear(x, w, plan, gather=True, dtype=None, out=None, workspace=None):
     else:
         at, ldy = _check_out("linear", out, dtype, (choices, n), index)
     if workspace is None:
-        need = workspace_size(plan, w, gather)
+        need = _workspace_size(plan, w, gather)
         workspace = _scratch(index, need, x) if need else None
     else:
         _same("linear", index, workspace)
@@ -190,7 +203,8 @@ def combine(y, plan, weights=None, out=None):
     """Sorted rows y [T * top][N] back to their tokens -> [T][N] of y's type: the sum of weights[t][j] (f32 [T][top]; None: 1) times
     y[pos[t][j]], in f32 and in order of j. A choice that goes nowhere adds nothing.
     out: the tensor for the result (it shares no memory with y)."""
-    _check_plan("combine", plan)
+    if not isinstance(plan, Plan):
+        raise TypeError(f"combine: plan must be a Plan (route, sort), got {type(plan).__name__}")
     index, tokens, top = plan._index, plan.tokens, plan.top
     _same("combine", index, y)
     did = DTYPE_ID.get(y.dtype)

@@ -96,13 +96,20 @@ class MXTensor:
         self._set(image, rows, k, experts)
 
     def _set(self, image, rows, k, experts):
-        self.image, self.rows, self.k, self.experts = image, rows, k, experts
+        self._image, self.rows, self.k, self.experts = image, rows, k, experts
         self._at, self._index = image.data_ptr(), image.get_device()
         self._sizes = {}  # workspaces of products with few rows
 
+    def __reduce__(self):  # a copy's image lies elsewhere
+        return MXTensor, (self._image, self.rows, self.k, self.experts)
+
+    @property
+    def image(self):
+        return self._image
+
     @property
     def device(self):
-        return self.image.device
+        return self._image.device
 
     @property
     def shape(self):
@@ -177,7 +184,7 @@ def dequantize(t, dtype=torch.float32):
     if not isinstance(t, MXTensor):
         raise TypeError(f"dequantize: expected an MXTensor, got {type(t).__name__}")
     did = _out_dtype("dequantize", dtype)
-    y = t.image.new_empty(t.shape, dtype=dtype)
+    y = t._image.new_empty(t.shape, dtype=dtype)
     _enter(t._index, _lib.load().b2q_mx_dequantize, t._at, t.experts or 1, t.rows, t.k, did, y.data_ptr(), t.k)
     return y
 
@@ -249,7 +256,7 @@ def matmul(a, w, dtype=torch.bfloat16, out=None):
         raise ValueError(f"matmul: a {a.shape} on {a.device} and w {w.shape} on {w.device}")
     did = _out_dtype("matmul", dtype)
     if out is None:
-        out = a.image.new_empty((a.rows, w.rows), dtype=dtype)
+        out = a._image.new_empty((a.rows, w.rows), dtype=dtype)
         at, ldy = out.data_ptr(), w.rows
     else:
         at, ldy = _check_out("matmul", out, dtype, (a.rows, w.rows), index)
