@@ -16,6 +16,8 @@
 //     first one's end, and those are read first.
 // Few tiles (narrow layers, few rows) leave most of the GPU idle: then the CTAs of a cluster split K between them, and add
 // their parts in order of rank through distributed shared memory, so that results do not depend on timing.
+// (They hold tensor memory while they wait for one another, which is safe only because none of them ever waits for any: beside
+// its 205 KB of shared memory and more an SM has no room for another kernel that takes tensor memory, whose least is 28.)
 //
 // What bounds it: a stage of 256 rows writes 51 KB into shared memory and the products read 49 KB of it, 790 cycles at 128 bytes a
 // cycle, where the products alone would take 512; measured 745 to 820, at 1.6 to 1.7 GHz under the power limit: 4096 x 14336 x
@@ -45,6 +47,7 @@ struct MxTile {
   static constexpr uint32_t kScaleSet = 8 + kParts * 8;
   static_assert(kSecond + TN <= kScaleCol && kScaleCol + 2 * kScaleSet <= 512, "tensor memory");
   static_assert(kSmem <= 227 * 1024 - 13 * 1024, "shared memory");  // beside it: the experts' table
+  static_assert(kSmem >= 200 * 1024, "one CTA with tensor memory an SM");  // of 228 KB: the others' take 28 at the least
 };
 
 constexpr int kThreads = 192;

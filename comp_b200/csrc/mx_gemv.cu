@@ -15,6 +15,11 @@
 //
 // Where there are fewer tiles than SMs the CTAs of a cluster split K: each sends the columns of its part to the CTAs that own
 // them (distributed shared memory, counted in bytes by the owner's barrier), which add them in order of rank.
+//
+// Tensor memory is taken when a CTA begins, and a CTA that finds none free waits for others of its SM, whose kernels may be any.
+// A cluster starts as a whole, but nothing says that all of its CTAs find tensor memory. So that calls on several streams cannot
+// wait for one another in a ring, no CTA waits for another one of its cluster while it holds tensor memory: each tells the
+// others that it has begun before it asks for any, and gives it back as soon as its accumulator is in registers.
 #include <algorithm>
 #include <atomic>
 
@@ -25,10 +30,9 @@ namespace b2q {
 namespace {
 
 constexpr int kThreads = 320;                   // copying, multiplying, then 8 warps that quantize, 4 of which store
-constexpr int kMaxRing = 8;
-constexpr int kMaxRows = 4, kXStage = 8 * 128;  // rows of x; bytes of a stage of them, a whole group of 8
-constexpr int kMaxChoices = 128;                // rows of y that a layer of experts makes of them
-constexpr uint32_t kScaleW = 32, kScaleX = 48;  // columns: accumulators 2 x 16, weight scales 2 x 8, then 4 a stage of x
+constexpr int kMaxRing = kGemvRing, kMaxRows = kGemvRows, kXStage = kGemvXStage;
+constexpr int kMaxChoices = 128;  // rows of y that a layer of experts makes of them
+constexpr uint32_t kScaleW = kGemvScaleW, kScaleX = kGemvScaleX;
 
 struct Gemv {
   const uint8_t* w;
@@ -80,6 +84,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncwarp();
+  // barriers are ready (waited for before the first parts): told before asking for tensor memory
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
                  "r"(g.columns));
@@ -110,7 +117,6 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // barriers are ready: waited for before the first parts
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = s_tmem;
   const int tiles = g.offsets ? s_count * g.row_tiles : g.row_tiles;
@@ -205,11 +211,30 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   }
 
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const bool stores = warp >= 2 && warp < 6;
+  // The storing warps have read their last accumulator: tensor memory is given back.
+  bool held = true;
+  auto give_back = [&] {
+    held = false;
+    if (stores) {
+      tc::fence_before();
+      asm volatile("bar.arrive 1, 160;" ::: "memory");
+    } else if (warp == 1) {
+      asm volatile("bar.sync 1, 160;" ::: "memory");
+      tc::fence_after();
+      if (__shfl_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort), 0)) {  // products may be under way: they end first
+        if (elect_one()) tc::mma_commit(smem_addr(&b_end));
+        __syncwarp();
+        mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
+        __syncwarp();
+      }
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns));
+    }
+  };
   uint32_t count = 0;
   for (int t = start; t < tiles; t += step, ++count) {  // (once where CTAs share a tile: there are clusters enough)
     const GemvTile at = gemv_tile(g, s_used, s_offsets, t);
     const int in = (warp & 3) * 32 + lane, n = at.n0 + in;
-    const bool stores = warp >= 2 && warp < 6;
     uint32_t v[16];
     if (stores) {
       const uint32_t buf = count & 1;
@@ -249,7 +274,16 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
         }
     }
     __syncwarp();
+    give_back();
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has sent its parts
+    // Another CTA's parts may be late for as long as other kernels hold the tensor memory that it waits for: a wait that runs out
+    // is followed by one for the cluster, after which all have sent theirs.
+    bool all_sent = false;
+    if (stores && owned > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_addr(&b_part), 0, kWaitLimit))) {
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      all_sent = true;
+    }
     if (stores && owned > 0 && wait_warp(&b_part, 0) && n < g.N)
       for (int i = 0; i < owned; ++i) {
         const int x_row = (int)rank + i * (int)ranks;
@@ -260,42 +294,12 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
       }
     __syncwarp();
     // no CTA ends before all have sent theirs (parts for one that gave up waiting find its memory)
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (!all_sent) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  tc::fence_before();
+  __syncwarp();
+  if (held) give_back();
   __syncthreads();
-  tc::fence_after();
-  if (s_abort) {  // products may be under way still: they end before their tensor memory is given back
-    if (threadIdx.x == 32) {
-      atomicCAS(&g_device_error, 0, kErrTimeout);
-      tc::mma_commit(smem_addr(&b_end));
-      mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
-    }
-    __syncthreads();
-  }
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.columns));
-}
-
-struct GemvPlan {
-  int ranks, nk, ring;
-  size_t smem;
-};
-
-// Whether and how the kernel takes `rows` rows of x: CTAs in a cluster, the most stages one has, stages of its ring.
-bool plan_gemv(int64_t rows, int64_t used, int64_t row_tiles, int64_t stages, int sms, GemvPlan* p) {
-  if (rows < 1 || rows > kMaxRows || used * row_tiles > INT32_MAX / 2) return false;
-  int ranks = 1;
-  while (ranks < 8 && used * row_tiles * ranks * 2 <= sms && stages >= ranks * 2) ranks *= 2;
-  const int64_t nk = (stages + ranks - 1) / ranks;
-  if (nk > (512 - (int)kScaleX) / 4) return false;
-  const size_t x = (size_t)(nk + 1) * kXStage + nk * 512 + 1024;  // 1024: the ring is aligned to that
-  // a ring that leaves room for the next kernel's CTA beside this one, or else for all that an SM has
-  const size_t half = 104 * 1024, all = 214 * 1024;
-  size_t ring = x + 4 * kMxBytes <= half ? (half - x) / kMxBytes : x + 3 * kMxBytes <= all ? (all - x) / kMxBytes : 0;
-  if (ring == 0) return false;
-  ring = std::min<size_t>(std::min<size_t>(ring, kMaxRing), std::max<int64_t>(nk, 2));
-  *p = {ranks, (int)nk, (int)ring, x + ring * kMxBytes};
-  return true;
+  if (s_abort && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
 }
 
 template <typename T>
@@ -305,7 +309,7 @@ int launch_gemv(const Gemv& g, const GemvPlan& p, int ctas, cudaStream_t stream)
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1))) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 214 * 1024);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemvSmem);
     if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return fail(B2Q_ECUDA, "mx_gemv: %s", cudaGetErrorString(e));
@@ -342,7 +346,7 @@ int launch_mx_gemv(const MxGemv& a, cudaStream_t stream) {
   const int64_t used = std::min<int64_t>(a.offsets ? a.choices : 1, a.experts), row_tiles = mx_tiles(a.N), stages = mx_stages(a.K);
   if (!plan_gemv(a.rows, used, row_tiles, stages, dev.sms, &p)) return fail(B2Q_ERANGE, "mx_gemv: more rows than the kernel takes");
   const Gemv g = {a.w, a.x, a.y, a.offsets, a.order, a.ldx, a.ldy, (int)a.rows, (int)a.K, (int)a.N, (int)row_tiles, (int)stages,
-                  (int)a.experts, (int)a.choices, a.dtype, a.top, p.ring, kScaleX + 4 * p.nk <= 256 ? 256 : 512};
+                  (int)a.experts, (int)a.choices, a.dtype, a.top, p.ring, p.columns};
   // with several CTAs a tile every tile has a cluster of its own
   const int64_t ctas = std::min<int64_t>(used * row_tiles, dev.sms / p.ranks);
   if (a.x_dtype == B2Q_DTYPE_F32) return launch_gemv<float>(g, p, (int)ctas, stream);

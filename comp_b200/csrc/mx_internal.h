@@ -1,14 +1,10 @@
-// Host-side internals shared by the MXFP4 and expert translation units: the operand image, argument checks, launchers.
+// Host-side internals shared by the MXFP4 and expert translation units: argument checks, launchers.
 #pragma once
 
 #include "b2q_internal.h"
+#include "mx_plan.h"
 
 namespace b2q {
-
-// An operand image: tiles of 128 rows by stages of 256 values. A stage of a tile is one run of 17408 bytes: 128 rows of 128
-// bytes of codes, then the scales of its 8 blocks a row (see mx_device.cuh).
-constexpr int kMxRows = 128, kMxStage = 256;
-constexpr int kMxCodes = kMxRows * kMxStage / 2, kMxScales = kMxRows * kMxStage / 32, kMxBytes = kMxCodes + kMxScales;
 
 constexpr int kErrExpert = 5;  // device error word: an expert's number beyond the experts
 
