@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     return ok;
   };
 
+  uint32_t issued = 0;  // stages asked for (warp 0)
   if (warp == 0) {
     const uint64_t once = evict_first_policy();
     uint32_t s = 0, round = 0;
@@ -143,13 +144,10 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
           bulk_g2s(ring + s * kMxBytes, w, kMxBytes, bar, once);
         }
         __syncwarp();
+        ++issued;
         if (++s == (uint32_t)g.ring) s = 0, ++round;
       }
     }
-    // (after a wait that ran out: what is still under way lands before the CTA ends)
-    if (!ok)
-      for (uint32_t i = 0; i < (uint32_t)g.ring; ++i)
-        if (round || i < s) mbar_wait(smem_addr(&b_full[i]), (i < s ? round : round - 1) & 1, kWaitLimit);
     __syncwarp();
   } else if (warp == 1) {
     if (start < tiles) {
@@ -299,7 +297,11 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   __syncwarp();
   if (held) give_back();
   __syncthreads();
-  if (s_abort && threadIdx.x == 0) atomicCAS(&g_device_error, 0, kErrTimeout);
+  if (s_abort && threadIdx.x == 0) {  // whichever wait ran out: copies that are under way land before the CTA ends
+    atomicCAS(&g_device_error, 0, kErrTimeout);
+    for (uint32_t i = first_under_way(issued, g.ring); i < issued; ++i)
+      mbar_wait(smem_addr(&b_full[i % g.ring]), i / g.ring & 1, kWaitLimit);
+  }
 }
 
 template <typename T>

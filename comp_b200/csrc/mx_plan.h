@@ -20,6 +20,10 @@ constexpr int kGemvRows = 4, kGemvXStage = 8 * 128;     // rows of x; bytes of a
 constexpr uint32_t kGemvScaleW = 32, kGemvScaleX = 48;  // columns: accumulators 2 x 16, weight scales 2 x 8, then 4 a stage of x
 constexpr size_t kGemvSmem = 214 * 1024;
 
+// A ring's stages are numbered as they are asked for: stage i lies in slot i % ring, and its arrival is phase i / ring of the slot's
+// barrier. Of `issued` stages the ones from here on, a slot's last each, may be under way still.
+constexpr uint32_t first_under_way(uint32_t issued, uint32_t ring) { return issued > ring ? issued - ring : 0; }
+
 struct GemvPlan {
   int ranks, nk, ring;  // CTAs in a cluster, the most stages one has, stages of its ring
   int columns;          // of tensor memory

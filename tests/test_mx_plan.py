@@ -16,6 +16,7 @@ extern "C" int plan(int64_t rows, int64_t used, int64_t row_tiles, int64_t stage
   out[0] = p.ranks, out[1] = p.nk, out[2] = p.ring, out[3] = p.columns, out[4] = (int64_t)p.smem;
   return 1;
 }
+extern "C" unsigned under_way(unsigned issued, unsigned ring) { return b2q::first_under_way(issued, ring); }
 """
 
 SM_SMEM, RESERVED, COLUMNS, STAGE = 228 * 1024, 1024, 512, 17408
@@ -34,6 +35,7 @@ def plan(tmp_path_factory):
         out = (ctypes.c_int64 * 5)()
         return dict(zip(("ranks", "nk", "ring", "columns", "smem"), out)) if lib.plan(rows, used, row_tiles, stages, sms, out) else None
 
+    call.under_way = lib.under_way
     return call
 
 
@@ -72,3 +74,18 @@ def test_few_tiles_share_k(plan):
 
 def test_refused(plan):
     assert plan(0, 1, 1, 1) is None and plan(5, 1, 1, 1) is None and plan(1, 1, 148, 116) is None and plan(1, 1, 1 << 30, 1) is None
+
+
+@pytest.mark.parametrize("ring", [2, 3, 5, 8])
+def test_copies_waited_for_at_the_end(plan, ring):
+    """Barriers as the hardware keeps them (a wait for a parity ends when the phase of that parity has ended), stages asked for in
+    turn while the last ones have not been seen by anyone: the waits cover every stage that may be under way, and end."""
+    for issued in range(0, 4 * ring + 2):
+        waits = {(i % ring, i // ring & 1) for i in range(plan.under_way(issued, ring), issued)}
+        assert len(waits) == min(issued, ring)
+        ended = [0] * ring  # phases that have ended, a slot: all but the last stage's of it are known to have
+        for i in range(issued):
+            ended[i % ring] += i + ring < issued
+        for slot in range(min(issued, ring)):
+            running = ended[slot] & 1  # the parity of the phase under way: what the slot's wait has to be for
+            assert (slot, running) in waits and (slot, running ^ 1) not in waits
