@@ -288,8 +288,9 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemm_kernel(const MxGemm g) {
       atomicCAS(&g_device_error, 0, kErrTimeout);
       for (uint32_t i = it > S ? it - S : 0; i < it; ++i) mbar_wait(smem_addr(&b_full[i % S]), (i / S) & 1, kWaitLimit);
     }
-    if (threadIdx.x == 32) {
-      tc::mma_commit(smem_addr(&b_end));
+    if (warp == 1) {  // (a commit is for the products of the lane that makes it: the one that is elected for them)
+      if (elect_one()) tc::mma_commit(smem_addr(&b_end));
+      __syncwarp();
       mbar_wait(smem_addr(&b_end), 0, kWaitLimit);
     }
     __syncthreads();
