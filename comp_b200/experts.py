@@ -29,15 +29,16 @@ class Plan:
     """Choices (token * top + j) sorted by expert. int32 tensors: ids [tokens][top] (each choice's expert, -1: none), offsets
     [experts + 1] (the sorted rows where each expert's begin), pos [tokens][top] (each choice's sorted row, -1: it goes nowhere),
     order [tokens * top] (each sorted row's choice, -1 past the last); weights f32 [tokens][top] (from route, else None). All lie in
-    one allocation, whose parts are made tensors when they are asked for."""
+    one allocation, whose parts are made tensors when they are asked for; ids of a plan from sort are worked out from its other
+    parts then (the tensor that sort was given is the caller's, and may hold the next step's)."""
 
-    def __init__(self, tokens, top, experts, like, ids=None):
+    def __init__(self, tokens, top, experts, like, routed):
         choices = tokens * top
         self.tokens, self.top, self.experts = tokens, top, experts
         words = 2 * (experts + 1) + 4 * choices if tokens <= 128 and choices <= 1024 else \
             _lib.load().b2q_experts_plan_words(tokens, top, experts)
-        self._ids, self._routed = ids, words if ids is None else 0  # (routed: ids and weights follow the plan's own words)
-        self._words = like.new_empty(words + 2 * choices if ids is None else words, dtype=torch.int32)
+        self._routed = words if routed else 0  # (ids and weights follow the plan's own words)
+        self._words = like.new_empty(words + 2 * choices if routed else words, dtype=torch.int32)
         self._at, self._index = self._words.data_ptr(), self._words.get_device()
 
     def __getstate__(self):
@@ -59,11 +60,14 @@ class Plan:
 
     @property
     def ids(self):
-        return self._part(self._routed) if self._ids is None else self._ids
+        if self._routed:
+            return self._part(self._routed)
+        pos = self.pos  # a choice's expert is the one among whose rows its own lies
+        return torch.where(pos < 0, -1, torch.searchsorted(self.offsets[1:], pos, right=True, out_int32=True))
 
     @property
     def weights(self):
-        return self._part(self._routed + self.tokens * self.top).view(torch.float32) if self._ids is None else None
+        return self._part(self._routed + self.tokens * self.top).view(torch.float32) if self._routed else None
 
     @property
     def offsets(self):
@@ -109,7 +113,7 @@ def route(logits, top, normalize=True):
         if (s1 != 1 and experts > 1) or (tokens > 1 and s0 < experts):
             logits = logits.clone(memory_format=torch.contiguous_format)
         ld = _stride(logits)
-    plan = Plan(tokens, top, experts, logits)
+    plan = Plan(tokens, top, experts, logits, True)
     words = plan._at
     ids = words + 4 * plan._routed
     _enter(index, _lib.load().b2q_experts_route, _pack_route(logits.data_ptr(), ids, ids + 4 * tokens * top, words, ld, tokens,
@@ -130,7 +134,7 @@ def sort(ids, experts):
     tokens, top = ids.shape
     _check_sizes("sort", tokens, top, experts)
     ids = ids.contiguous()
-    plan = Plan(tokens, top, experts, ids, ids)
+    plan = Plan(tokens, top, experts, ids, False)
     _enter(index, _lib.load().b2q_experts_sort, ids.data_ptr(), tokens, top, experts, plan._at)
     return plan
 
