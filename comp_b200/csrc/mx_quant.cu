@@ -198,9 +198,12 @@ __global__ void __launch_bounds__(256)
   dst[mx_scale_at(in, b)] = d;
 }
 
-int check_experts(const char* who, int64_t experts) {
-  if (experts >= 1 && experts <= kMaxExperts) return B2Q_OK;
-  return fail(B2Q_EINVAL, "%s: %lld experts (1..%lld)", who, (long long)experts, (long long)kMaxExperts);
+int check_experts(const char* who, int64_t experts, int64_t rows, int64_t K) {
+  if (experts < 1 || experts > kMaxExperts)
+    return fail(B2Q_EINVAL, "%s: %lld experts (1..%lld)", who, (long long)experts, (long long)kMaxExperts);
+  if (experts * mx_tiles(rows) * mx_stages(K) > INT64_MAX / kMxBytes)
+    return fail(B2Q_ERANGE, "%s: %lld x %lld x %lld values are past 64-bit sizes", who, (long long)experts, (long long)rows, (long long)K);
+  return B2Q_OK;
 }
 
 int grid_of(const char* who, int64_t items, unsigned* grid) {
@@ -240,7 +243,7 @@ extern "C" {
 
 size_t b2q_mx_bytes(int64_t experts, int64_t rows, int64_t K) {
   if (check_mx_shape("b2q_mx_bytes", rows, K)) return 0;
-  if (check_experts("b2q_mx_bytes", experts)) return 0;
+  if (check_experts("b2q_mx_bytes", experts, rows, K)) return 0;
   return (size_t)experts * mx_tiles(rows) * mx_stages(K) * kMxBytes;
 }
 
@@ -248,7 +251,7 @@ int b2q_mx_quantize(int dtype, const void* x, int64_t ldx, int64_t experts, int6
                     b2q_stream_t stream) {
   const char* who = "b2q_mx_quantize";
   int rc = check_mx_shape(who, rows, K);
-  if (!rc) rc = check_experts(who, experts);
+  if (!rc) rc = check_experts(who, experts, rows, K);
   if (!rc) rc = check_mx_rows(who, "x", dtype, x, ldx, experts * rows, K);
   if (rc || rows == 0) return rc;
   if (!image) return fail(B2Q_EINVAL, "%s: image is NULL", who);
@@ -261,7 +264,7 @@ int b2q_mx_dequantize(const uint8_t* image, int64_t experts, int64_t each, int64
                       b2q_stream_t stream) {
   const char* who = "b2q_mx_dequantize";
   int rc = check_mx_shape(who, each, K);
-  if (!rc) rc = check_experts(who, experts);
+  if (!rc) rc = check_experts(who, experts, each, K);
   const int64_t rows = rc ? 0 : experts * each;
   if (!rc) rc = check_mx_rows(who, "y", dtype, y, ldy, rows, K);
   if (rc || rows == 0) return rc;
@@ -290,7 +293,7 @@ int b2q_mx_pack(const uint8_t* codes, const uint8_t* scales, int64_t experts, in
                 b2q_stream_t stream) {
   const char* who = "b2q_mx_pack";
   int rc = check_mx_shape(who, rows, K);
-  if (!rc) rc = check_experts(who, experts);
+  if (!rc) rc = check_experts(who, experts, rows, K);
   if (rc || rows == 0) return rc;
   if (!codes || !scales || !image) return fail(B2Q_EINVAL, "%s: null pointer", who);
   if (!aligned(codes, 16) || !aligned(image, 128))
