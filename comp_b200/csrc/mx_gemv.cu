@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
   tc::fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  const int tiles = g.offsets ? s_count * g.row_tiles : g.row_tiles;
+  int tiles = g.offsets ? s_count * g.row_tiles : g.row_tiles;
+  if (ranks > 1) tiles = min(tiles, step);  // a cluster has one tile at the most (a plan of other sizes might name more)
   bool ok = true;
   auto wait_warp = [&](uint64_t* bar, uint32_t phase) {
     if (ok) {
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) mx_gemv_kernel(const Gemv g) {
     }
   };
   uint32_t count = 0;
-  for (int t = start; t < tiles; t += step, ++count) {  // (once where CTAs share a tile: there are clusters enough)
+  for (int t = start; t < tiles; t += step, ++count) {  // (once where CTAs share a tile)
     const GemvTile at = gemv_tile(g, s_used, s_offsets, t);
     const int in = (warp & 3) * 32 + lane, n = at.n0 + in;
     uint32_t v[16];
