@@ -22,7 +22,9 @@
 // What bounds it: a stage of 256 rows writes 51 KB into shared memory and the products read 49 KB of it, 790 cycles at 128 bytes a
 // cycle, where the products alone would take 512; measured 745 to 820, at 1.6 to 1.7 GHz under the power limit: 4096 x 14336 x
 // 4096 103 us (4.7 PFLOP/s), 118 in a long run; 8192 x 8192 x 8192 209 us (5.3). With few rows the weights' stream: 64 tokens of 8
-// among 128 experts of 4096 x 2048 97 us (5.8 TB/s).
+// among 128 experts of 4096 x 2048 97 us (5.8 TB/s). In between the steps that follow one another: 8192 x 8192 with 16 / 64 / 256 rows
+// 11.7 / 13.8 / 17.9 us, where the weights take 5.5: the quantizer's launch 2.5, 128 of 148 SMs at work (64 row tiles, K or
+// the rows of x in two), the join of the parts of K 1 + n / 50.
 #include <algorithm>
 #include <atomic>
 
@@ -340,6 +342,8 @@ struct Shape {
 // rows 13.3 (K in 2) / 15.1 (whole), with 256 rows 17.2 (128 a tile) / 19.5 (256), with 512 rows 21.2 (256) / 30.7 (128); 4096 x
 // 4096 with 256 rows 10.2 (64) / 11.2 (128). Clusters of 8 wait for as many free SMs of a kind: 2048 x 8192 with 16 rows 14.8, K in 4
 // parts 8.4.
+// Experts: by the average, so that no size has to be known on the host. 4096 tokens, 4 of 32 experts of 4096 x 4096, with at the most
+// 578 / 2754 / 4029 rows an expert: 154 / 158 / 150 us; 512 tokens with 84 / 173 / 512: 69 / 73 / 63.
 static Shape choose_shape(int64_t used, int64_t each, int64_t row_tiles, int64_t stages, int sms) {
   Shape best = {64, 1};
   double least = 1e30;

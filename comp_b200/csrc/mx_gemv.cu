@@ -4,11 +4,12 @@
 // a CTA's tile is 128 weight rows, whose stages of 256 values of K one thread copies into a ring and another one multiplies;
 // but all rows of x stay in shared memory, and their scales in tensor memory, for as long as the CTA lives: eight warps quantize
 // them there while the first weights are on their way. (Asking for those to be brought into L2 before waiting for the
-// preceding kernel, a hint that could do no harm, was slower: 8192 x 8192 10.9 us, 9.7 without.)
+// preceding kernel, a hint that could do no harm, was 1.2 us slower at 8192 x 8192.)
 //
 // Every CTA reads all rows as they are given, four times the bytes of their codes, from the same lines of L2: 0.5 us a row.
-// Measured against quantizing first and multiplying then, us: 8192 x 8192 with 1 / 2 / 4 / 8 / 16 rows 9.7 / 10.5 / 11.7 / 14.2 / 19.4
-// and 11.9 / 12.1 / 12.1 / 12.2 / 12.2; 4096 x 4096 5.4 / 5.6 / 5.8 / 7.0 / 8.9 and 7.5 / 7.7 / 7.8 / 7.9 / 7.9. So up to 4.
+// Measured with 1 / 2 / 4 rows against quantizing first and multiplying then (5 rows; 16 take 0.1 more), us, weights from memory:
+// 8192 x 8192 9.2 / 10.1 / 11.3 and 11.6; 14336 x 4096 8.4 / 9.2 / 10.1 and 10.2; 4096 x 14336 8.4 / 9.4 / 10.4 and 11.4; 4096 x 4096
+// 4.9 / 5.1 / 5.3 and 7.2; 2000 x 1024 3.4 / 3.6 / 3.8 and 4.9. So up to 4: at 0.5 us a row wide layers are worse off with more.
 //
 // A layer of experts needs no gathering: every expert that has rows is multiplied with all rows of x (the unit's other side
 // is 16 rows at the least), and of the results only those that its choices ask for are stored.

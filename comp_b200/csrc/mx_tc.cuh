@@ -8,7 +8,7 @@
 namespace b2q {
 
 // One lane of a converged warp, told in the way that lets the compiler see that it is one: tensor-core instructions take
-// their operands from uniform registers, and behind a branch on the lane's number each issues ten times as slowly (a stage's
+// their operands from uniform registers, and behind a branch on the lane's number each issues some four times as slowly (a stage's
 // six scale copies and four products 900 cycles, so 220).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
